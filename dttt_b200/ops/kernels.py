@@ -783,3 +783,44 @@ def gdn_chunk_bwd(k, v, beta, log_alpha, S0, gS):
     _check(_lib.lib().dttt_gdn_chunk_bwd(_p(k), _p(v), _p(beta), _p(log_alpha), _p(states), _p(gS), _p(dk), _p(dv), _p(db), _p(dla), _p(dS0),
                                          B, C, nh, D, _stream()), "gdn_chunk_bwd")
     return dk.sum(0), dv, db.sum(0), dla.sum(0), dS0
+
+
+# =============================================================================== decoding family
+_d = _ct.c_double
+_lib.register("dttt_sample_ranks", _i, [_i])
+_lib.register("dttt_sample", _i, [_vp, _i, _ll, _i, _ll, _ll, _i, _vp, _vp, _d, _vp, _i, _vp, _d, _vp, _d, _vp, _i, _vp, _vp, _vp, _vp])
+_lib.register("dttt_unmask", _i, [_vp] * 8 + [_f, _i] + [_vp] * 4 + [_i, _i, _vp])
+_SYMBOL.update(sampling="dttt_sample")
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+SAMPLE_VOCAB_MAX = 8 * 49152           # a row's f32 slices in the shared memory of eight CTAs
+UNMASK_SLOTS_MAX = 32768               # a row's order keys in the shared memory of one CTA
+
+
+def sample(x, u, bias, temperature, top_k, top_p, min_p, priority):
+    """``x [outer, inner, V]`` (contiguous along V, any strides of the rows), ``u [outer, inner]``, ``bias [outer, V]`` or None; a
+    parameter is a number or a contiguous tensor ``[outer, inner]`` (f32; int32 for ``top_k``).  ``(tokens, logp, priority)``
+    ``[outer, inner]``; ``priority`` 0 logp (the same tensor) | 1 margin | 2 entropy."""
+    outer, inner, V = x.shape
+    tokens = torch.empty(outer, inner, dtype=torch.int64, device=x.device)
+    logp = torch.empty(outer, inner, dtype=torch.float32, device=x.device)
+    prio = torch.empty_like(logp) if priority else None
+    if tokens.numel():
+        num = lambda p, off: (off, p) if torch.is_tensor(p) else (p, None)
+        (t, t_row), (k, k_row), (p, p_row), (m, m_row) = num(temperature, 1.0), num(top_k, 0), num(top_p, 1.0), num(min_p, 0.0)
+        with torch.cuda.device(x.device):
+            _check(_lib.lib().dttt_sample(_p(x), _LOGIT_TYPES[x.dtype], outer * inner, inner, x.stride(0), x.stride(1), V, _p(u), _p(bias),
+                                          float(t), _p(t_row), int(k), _p(k_row), float(p), _p(p_row), float(m), _p(m_row), priority,
+                                          _p(tokens), _p(logp), _p(prio), _stream()), "sample")
+    return tokens, logp, logp if prio is None else prio
+
+
+def unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure):
+    """Contiguous ``[B, C]`` tensors (``quota [B]``); ``(ids, known, held, where)`` after the commit."""
+    B, C = ids.shape
+    ids_out, known_out, held_out, where = torch.empty_like(ids), torch.empty_like(known), torch.empty_like(held), torch.empty_like(known)
+    if ids.numel():
+        with torch.cuda.device(ids.device):
+            _check(_lib.lib().dttt_unmask(_p(ids), _p(known), _p(held), _p(tokens), _p(logp), _p(priority), _p(quota), _p(allowed),
+                                          0.0 if sure is None else float(sure), 0 if sure is None else 1, _p(ids_out), _p(known_out),
+                                          _p(held_out), _p(where), B, C, _stream()), "unmask")
+    return ids_out, known_out, held_out, where

@@ -147,3 +147,54 @@ def gdn_update_sequential(k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, 
         err = vt - torch.einsum("...hvk,...hk->...hv", Sd, kt)
         S = Sd + beta[..., t, :, None, None].float() * torch.einsum("...hv,...hk->...hvk", err, kt)
     return S
+
+
+# ------------------------------------------------------------------ decoding a block
+def sample_tokens(x: torch.Tensor, u: torch.Tensor, bias: Optional[torch.Tensor], temperature: torch.Tensor, top_k: torch.Tensor,
+                  top_p: torch.Tensor, min_p: torch.Tensor, priority: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``ops.sampling.sample_tokens`` on ``x [..., V]`` with every parameter a tensor of the rows' shape (f64; ``top_k`` int64).
+    The masses are summed in 64 bits: a draw may fall next to the border between two tokens."""
+    V = x.shape[-1]
+    x = x.float() if bias is None else x.float() + bias.view(bias.shape[0], *[1] * (x.dim() - 2), V)
+    m = x.amax(-1, keepdim=True)
+    void = ~torch.isfinite(m[..., 0])                                  # NaN or +inf somewhere, or nothing above -inf
+    x, m = torch.where(void[..., None], 0.0, x), torch.where(void[..., None], 0.0, m)
+    e = torch.exp(x.double() - m.double())
+    z = e.sum(-1)
+    best = torch.where(x == m, torch.arange(V, device=x.device), V).amin(-1)
+    greedy = ~(temperature > 0)
+    w = torch.exp((x.double() - m.double()) / temperature.clamp(1e-6, 1e6).nan_to_num(1.0)[..., None])
+    order = torch.sort(x, dim=-1, descending=True, stable=True).indices
+    ws = w.gather(-1, order)
+    keep = ws >= min_p.clamp(max=1.0)[..., None]
+    k = torch.where((top_k > 0) & (top_k < V), top_k, V)
+    inside = torch.arange(V, device=x.device) < k[..., None]
+    ws = torch.where(inside, ws, 0.0)
+    cut = ~(top_p >= 1)[..., None] & (ws.cumsum(-1) - ws >= top_p.clamp(min=0.0)[..., None] * ws.sum(-1, keepdim=True))
+    cut[..., 0] = False
+    w = w * torch.zeros_like(keep).scatter(-1, order, (keep & inside & ~cut))
+    cum = w.cumsum(-1)
+    drawn = torch.searchsorted(cum, u.double().clamp(0, 1)[..., None] * cum[..., -1:], right=True)[..., 0]
+    last = torch.where(w > 0, torch.arange(V, device=x.device), 0).amax(-1)
+    tokens = torch.where(greedy, best, torch.minimum(drawn, last))
+    lp = x.gather(-1, tokens[..., None])[..., 0].double() - m[..., 0].double() - torch.log(z)
+    if priority == "margin":
+        top = e.topk(min(2, V), -1).values / z[..., None]
+        pr = top[..., 0] - (top[..., 1] if V > 1 else 0.0)
+    elif priority == "entropy":
+        pr = torch.xlogy(e, e).sum(-1) / z - torch.log(z)
+    else:
+        pr = lp
+    nan = torch.where(void, float("nan"), 0.0)
+    return torch.where(void, -1, tokens), (lp + nan).float(), (pr + nan).float()
+
+
+def unmask(ids, known, held, tokens, logp, priority, quota, allowed=None, sure=None):
+    """``ops.sampling.unmask``: the rank of a slot is its position when its row is sorted by descending priority."""
+    shut = known if allowed is None else (known | ~allowed)
+    p = torch.where(shut, torch.full_like(priority, float("-inf")), priority)
+    rank = torch.argsort(torch.argsort(-p, dim=-1, stable=True), dim=-1)
+    where = (rank < quota[:, None]) & ~shut
+    if sure is not None:
+        where = where | ((logp >= sure) & ~known)
+    return torch.where(where, tokens, ids), known | where, torch.where(where, logp, held), where
