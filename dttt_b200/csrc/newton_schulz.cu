@@ -1,0 +1,452 @@
+// Newton-Schulz orthogonalisation of batches of matrices on the tensor cores.
+//
+//   x_0 = g / |g|_F                                     g [rows, cols], d the smaller side
+//   G_k = x_k x_k^T  (x_k^T x_k when rows > cols)       [d, d]
+//   P_k = b G_k + c G_k G_k                             [d, d], symmetric
+//   x_{k+1} = a x_k + P_k x_k  (a x_k + x_k P_k)        y = x_steps in bf16
+//
+// y is a polynomial of the matrix times g / |g|; its derivative is taken with the polynomial and the norm held constant (the map
+// is then linear and self-adjoint), so the backward applies the same a r + P_k r in reverse order to the cotangent.
+//
+// Operands are f16, not bf16: the same tensor-core rate with three more bits.  Five iterations multiply small singular values by
+// up to 3.4 each, and what the roundings of x and P leave in those directions grows with them: 1.2e-2 of the result with bf16
+// operands, 1.5e-3 with f16 (Gaussian and gradient-like matrices; the bf16 result itself rounds by 1.7e-3).  Everything that
+// is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12 for
+// those, 2^5 for the cotangent, which may grow 3.4445-fold per iteration.  Sums are f32 (tensor memory), the norms f64.
+//
+// Every product is C = alpha A B + beta D on CTA pairs: 256 x 256 tiles, tcgen05.mma.cta_group::2, plain per-CTA TMA loads.
+#include "host_check.h"
+#include "ptx_sm100.cuh"
+
+#include <cuda_fp16.h>
+
+#include <cstring>
+#include <mutex>
+
+namespace dttt {
+namespace ns {
+
+constexpr int BM = 128;        // rows of A per CTA (256 per pair)
+constexpr int BN = 256;        // output columns per pair; each CTA loads BN / 2 of them
+constexpr int BK = 64;
+constexpr int UMMA_K = 16;
+constexpr int STAGES = 6;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr int B_BYTES = (BN / 2) * BK * 2;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int SMEM_TOTAL = STAGES * STAGE_BYTES + 1024 + 1024;
+
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+constexpr float X_SCALE = 4096.f;           // of x, G and P
+constexpr float R_SCALE = 32.f;             // of the cotangent
+
+enum { OUT_F16 = 0, OUT_BF16 = 1, OUT_F32 = 2 };
+
+struct Params {
+  int M, N, K, batch;
+  int a_mn_major, b_mn_major;
+  float alpha, beta;
+  const __half* D;             // or null; same shape as C
+  long long ldd, d_batch;
+  void* C;
+  int out;
+  long long ldc, c_batch;
+  const double* num;           // per-batch factors of the output, or null
+  const double* den;
+  int* status;
+  int tiles_m, tiles_n;
+};
+
+__device__ __forceinline__ void tile_coords(int tile, const Params& p, int& b, int& tm, int& tn) {
+  const int per_batch = p.tiles_m * p.tiles_n;
+  b = tile / per_batch;
+  const int t = tile - b * per_batch;
+  constexpr int GROUP = 8;                                     // bands of 8 pair rows, n fastest inside a band
+  const int band = t / (GROUP * p.tiles_n);
+  const int first_m = band * GROUP;
+  const int rows = min(GROUP, p.tiles_m - first_m);
+  const int r = t - band * GROUP * p.tiles_n;
+  tm = first_m + (r % rows);
+  tn = r / rows;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);      // the leader's count both CTAs' bytes
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 2;                          // the leader's: both CTAs' epilogues have drained it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_word = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const int num_tiles = p.batch * p.tiles_m * p.tiles_n;
+  const int kblocks = (p.K + BK - 1) / BK;
+  constexpr uint32_t TMEM_COLS = 2 * BN;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 256); }
+    *abort_word = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&mapA);
+    tma_prefetch_desc(&mapB);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < num_tiles && ok; tile += n_pairs) {
+        int b, tm, tn;
+        tile_coords(tile, p, b, tm, tn);
+        const int m0 = tm * 2 * BM + (int)rank * BM;
+        const int n0 = tn * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % STAGES;
+          const uint32_t ph = (it / STAGES) & 1;
+          if (!mbar_wait_bounded(&empty[s], ph ^ 1, abort_word, p.status, ERR_WAIT_EMPTY)) { ok = false; break; }
+          uint8_t* sA = smem + s * STAGE_BYTES;
+          uint8_t* sB = sA + A_BYTES;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * STAGE_BYTES);
+          const uint32_t bar = mapa_u32(&full[s], 0);
+          const int k0 = kb * BK;
+          if (!p.a_mn_major) {
+            tma_load_3d_pair(sA, &mapA, bar, k0, m0, b);
+          } else {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load_3d_pair(sA + j * (BK * 128), &mapA, bar, m0 + j * 64, k0, b);
+          }
+          if (!p.b_mn_major) {
+            tma_load_3d_pair(sB, &mapB, bar, k0, n0, b);
+          } else {
+#pragma unroll
+            for (int j = 0; j < (BN / 2) / 64; ++j) tma_load_3d_pair(sB + j * (BK * 128), &mapB, bar, n0 + j * 64, k0, b);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = make_idesc_f16(2 * BM, BN, p.a_mn_major, p.b_mn_major);
+      const uint32_t a_lbo = p.a_mn_major ? BK * 128 : 16, b_lbo = p.b_mn_major ? BK * 128 : 16;
+      const uint32_t a_kstep = p.a_mn_major ? UMMA_K * 128 : UMMA_K * 2;
+      const uint32_t b_kstep = p.b_mn_major ? UMMA_K * 128 : UMMA_K * 2;
+      uint32_t it = 0, local_tile = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < num_tiles && ok; tile += n_pairs, ++local_tile) {
+        const int acc = local_tile & 1;
+        const uint32_t acc_ph = (local_tile >> 1) & 1;
+        if (!mbar_wait_bounded(&acc_empty[acc], acc_ph ^ 1, abort_word, p.status, ERR_WAIT_TMEM_EMPTY)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % STAGES;
+          const uint32_t ph = (it / STAGES) & 1;
+          if (!mbar_wait_bounded(&full[s], ph, abort_word, p.status, ERR_WAIT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sA = smem_u32(smem + s * STAGE_BYTES);
+          const uint32_t sB = sA + A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_f16_pair(d_tmem, make_smem_desc(sA + k * a_kstep, a_lbo, 1024), make_smem_desc(sB + k * b_kstep, b_lbo, 1024), idesc,
+                          (kb | k) ? 1u : 0u);
+          umma_commit_pair(&empty[s], 3);
+        }
+        if (ok) umma_commit_pair(&acc_full[acc], 3);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    uint32_t local_tile = 0;
+    for (int tile = pair_id; tile < num_tiles; tile += n_pairs, ++local_tile) {
+      int b, tm, tn;
+      tile_coords(tile, p, b, tm, tn);
+      const int acc = local_tile & 1;
+      const uint32_t acc_ph = (local_tile >> 1) & 1;
+      int got = 1;
+      if (lane == 0) got = mbar_wait_bounded(&acc_full[acc], acc_ph, abort_word, p.status, ERR_WAIT_TMEM_FULL) ? 1 : 0;
+      got = __shfl_sync(0xffffffffu, got, 0);
+      if (!got) break;
+      tc_fence_after();
+      const int row = tm * 2 * BM + (int)rank * BM + quarter * 32 + lane;
+      const uint32_t taddr = tmem_base + acc * BN + ((uint32_t)(quarter * 32) << 16);
+      float alpha = p.alpha, beta = p.beta;
+      if (p.num || p.den) {
+        const double den = p.den ? p.den[b] : 1.0;
+        const float f = den == 0.0 ? 0.f : (float)((p.num ? p.num[b] : 1.0) / den);      // a zero matrix has a zero derivative
+        alpha *= f; beta *= f;
+      }
+      const __half* drow = p.D ? p.D + (long long)b * p.d_batch + (long long)row * p.ldd : nullptr;
+      const long long crow = (long long)b * p.c_batch + (long long)row * p.ldc;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32(taddr + c, r);
+        tmem_ld_wait();
+        const int col = tn * BN + c;
+        const int nc = row < p.M ? min(32, p.N - col) : 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          if (j < nc) {
+            float v = __uint_as_float(r[j]) * alpha;
+            if (drow) v = fmaf(beta, __half2float(drow[col + j]), v);
+            if (p.out == OUT_F16) reinterpret_cast<__half*>(p.C)[crow + col + j] = __float2half_rn(v);
+            else if (p.out == OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p.C)[crow + col + j] = __float2bfloat16(v);
+            else reinterpret_cast<float*>(p.C)[crow + col + j] = v;
+          }
+        }
+        __syncwarp();                                          // the next load is one of the whole warp
+      }
+      tc_fence_before();
+      mbar_arrive_remote(mapa_u32(&acc_empty[acc], 0));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ norms and the f16 copy
+constexpr int NORM_BLOCKS = 128;            // partial sums per matrix
+
+template <class T> __device__ __forceinline__ float load_f32(const T* p) { return (float)*p; }
+template <> __device__ __forceinline__ float load_f32<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0;
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += part[i];
+  return s;
+}
+
+// partial[b][j]: the squares of one of NORM_BLOCKS interleaved pieces of matrix b, in 64 bits
+template <class T>
+__global__ void __launch_bounds__(256) ns_squares_kernel(const T* __restrict__ g, long long n, double* __restrict__ partial) {
+  const T* x = g + (long long)blockIdx.y * n;
+  double s = 0;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    const double v = (double)load_f32(x + i);
+    s += v * v;
+  }
+  s = block_sum(s);
+  if (threadIdx.x == 0) partial[(long long)blockIdx.y * NORM_BLOCKS + blockIdx.x] = s;
+}
+
+// x [rows, ld] = f16(scale g / |g|), norm[b] = |g|
+template <class T>
+__global__ void __launch_bounds__(256) ns_cast_kernel(const T* __restrict__ g, int rows, int cols, const double* __restrict__ partial,
+                                                     float scale, __half* __restrict__ x, int ld, double* __restrict__ norm) {
+  const int b = blockIdx.y;
+  const double v = (int)threadIdx.x < NORM_BLOCKS ? partial[(long long)b * NORM_BLOCKS + threadIdx.x] : 0.0;
+  const double whole = sqrt(block_sum(v));
+  if (blockIdx.x == 0 && threadIdx.x == 0) norm[b] = whole;
+  const double f = whole == 0.0 ? 0.0 : (double)scale / whole;
+  const T* src = g + (long long)b * rows * cols;
+  __half* dst = x + (long long)b * rows * ld;
+  const long long n = (long long)rows * cols;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    const long long r = i / cols;
+    dst[r * ld + (i - r * cols)] = __float2half_rn((float)((double)load_f32(src + i) * f));
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// A stored f16 matrix [rows, cols] per batch entry, rows `ld` apart.
+struct Mat {
+  const void* ptr;
+  int rows, cols;
+  long long ld;
+};
+
+// `mn`: the operand's rows run along the contraction (its M or N index is contiguous); the box is then 64 x BK, else BK x 128.
+static int make_map(CUtensorMap* map, const Mat& m, int batch, bool mn) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return 101;
+  cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)batch};
+  cuuint64_t strides[2] = {(cuuint64_t)m.ld * 2, (cuuint64_t)m.ld * m.rows * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)(mn ? BK : 128), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  if (int c = check_map(m.ptr, 3, dims, strides, 2)) return c;
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(m.ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 200 + (int)r;
+}
+
+static int prepare_device(int* n_sm) {
+  static std::mutex mu;
+  static unsigned long long attr_mask = 0;
+  static int sms[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 301;
+  static thread_local int bound_dev = -1;
+  if (bound_dev != dev) { cudaSetDevice(dev); cudaFree(0); bound_dev = dev; }      // the encoder needs a current context
+  std::lock_guard<std::mutex> lock(mu);
+  if (!(attr_mask >> dev & 1ull)) {
+    if (cudaFuncSetAttribute(ns_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL) != cudaSuccess) return 302;
+    cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    attr_mask |= 1ull << dev;
+  }
+  *n_sm = sms[dev] > 1 ? sms[dev] : 148;
+  return 0;
+}
+
+struct Out {
+  void* C;
+  int kind;
+  long long ld;
+  const double *num, *den;
+};
+
+// C [M, N] = alpha op(A) op(B) + beta D over the batch
+static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, const Mat& B, bool b_mn, float alpha, float beta, const Mat* D,
+                   const Out& o, int* status, int n_sm, cudaStream_t stream) {
+  CUtensorMap mapA, mapB;
+  if (int r = make_map(&mapA, A, batch, a_mn)) return r;
+  if (int r = make_map(&mapB, B, batch, b_mn)) return r;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.M = M; p.N = N; p.K = K; p.batch = batch; p.a_mn_major = a_mn; p.b_mn_major = b_mn; p.alpha = alpha; p.beta = beta;
+  if (D) { p.D = (const __half*)D->ptr; p.ldd = D->ld; p.d_batch = D->ld * D->rows; }
+  p.C = o.C; p.out = o.kind; p.ldc = o.ld; p.c_batch = o.ld * M; p.num = o.num; p.den = o.den; p.status = status;
+  p.tiles_m = (M + 2 * BM - 1) / (2 * BM);
+  p.tiles_n = (N + BN - 1) / BN;
+  const long long tiles = (long long)batch * p.tiles_m * p.tiles_n;
+  if (tiles > 0x3fffffff) return 303;
+  const int pairs = (int)(tiles < n_sm / 2 ? tiles : n_sm / 2);
+  ns_product_kernel<<<2 * pairs, 192, SMEM_TOTAL, stream>>>(mapA, mapB, p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 1000 + (int)e;
+}
+
+// r (f16, scale S) -> a r + P r: into f16 or, at the end, into the caller's tensor
+static int apply(int batch, int rows, int cols, const Mat& r, const Mat& P, float alpha, float beta, const Out& o, int* status, int n_sm,
+                 cudaStream_t stream) {
+  if (rows <= cols) return product(batch, rows, cols, rows, P, false, r, true, alpha, beta, &r, o, status, n_sm, stream);
+  return product(batch, rows, cols, cols, r, false, P, false, alpha, beta, &r, o, status, n_sm, stream);
+}
+
+static int cast(const void* g, int f32, int batch, int rows, int cols, double* partial, float scale, void* x, int ld, double* norm,
+                cudaStream_t stream) {
+  const long long n = (long long)rows * cols;
+  const dim3 gs(NORM_BLOCKS, batch);
+  const long long want = (n + 1023) / 1024;
+  const dim3 gc((unsigned int)(want < 592 ? want : 592), batch);
+  if (f32) {
+    ns_squares_kernel<float><<<gs, 256, 0, stream>>>((const float*)g, n, partial);
+    ns_cast_kernel<float><<<gc, 256, 0, stream>>>((const float*)g, rows, cols, partial, scale, (__half*)x, ld, norm);
+  } else {
+    ns_squares_kernel<__nv_bfloat16><<<gs, 256, 0, stream>>>((const __nv_bfloat16*)g, n, partial);
+    ns_cast_kernel<__nv_bfloat16><<<gc, 256, 0, stream>>>((const __nv_bfloat16*)g, rows, cols, partial, scale, (__half*)x, ld, norm);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 1000 + (int)e;
+}
+
+}  // namespace ns
+}  // namespace dttt
+
+// Bytes of the scratch area for `batch` matrices [rows, cols] (256-byte aligned base): two f16 copies, one d x d f16 matrix, the
+// partial sums and one norm (the cotangent's) per matrix.
+extern "C" long long dttt_newton_schulz_scratch(int batch, int rows, int cols) {
+  const long long ld = (cols + 7) / 8 * 8, d = rows < cols ? rows : cols, ldd = (d + 7) / 8 * 8;
+  auto up = [](long long v) { return (v + 255) / 256 * 256; };
+  return 2 * up(batch * rows * ld * 2) + up(batch * d * ldd * 2) + up(batch * dttt::ns::NORM_BLOCKS * 8ll) + up(batch * 8ll);
+}
+
+// g [batch, rows, cols] (f32 or bf16, contiguous) -> y bf16.  polys: f16 [steps or 1, batch, d, ceil8(d)]; with keep every step's
+// P_k stays there for the backward, else one slot is used again and again.  norms: f64 [batch].
+extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, int cols, int steps, void* scratch, void* polys, int keep,
+                                  double* norms, void* y, int* status, cudaStream_t stream) {
+  using namespace dttt::ns;
+  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || batch > 65535) return -2;
+  int n_sm;
+  if (int r = prepare_device(&n_sm)) return r;
+  const int ld = (cols + 7) / 8 * 8, d = rows < cols ? rows : cols, ldd = (d + 7) / 8 * 8;
+  auto up = [](long long v) { return (v + 255) / 256 * 256; };
+  uint8_t* s = (uint8_t*)scratch;
+  const long long xb = up((long long)batch * rows * ld * 2);
+  void* xs[2] = {s, s + xb};
+  void* gram = s + 2 * xb;
+  double* partial = (double*)((uint8_t*)gram + up((long long)batch * d * ldd * 2));
+  if (int r = cast(g, f32, batch, rows, cols, partial, X_SCALE, xs[0], ld, norms, stream)) return r;
+  const bool wide = rows <= cols;
+  for (int k = 0; k < steps; ++k) {
+    const Mat X = {xs[k & 1], rows, cols, ld}, G = {gram, d, d, ldd};
+    const Mat P = {(uint8_t*)polys + (keep ? (long long)k * batch * d * ldd * 2 : 0), d, d, ldd};
+    const Out og = {gram, OUT_F16, ldd, nullptr, nullptr}, op = {const_cast<void*>(P.ptr), OUT_F16, ldd, nullptr, nullptr};
+    if (int r = product(batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, status, n_sm, stream)) return r;
+    if (int r = product(batch, d, d, d, G, false, G, false, NS_C / X_SCALE, NS_B, &G, op, status, n_sm, stream)) return r;
+    const bool last = k == steps - 1;
+    const float f = last ? 1.f / X_SCALE : 1.f;
+    const Out ox = {last ? y : xs[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : ld, nullptr, nullptr};
+    if (int r = apply(batch, rows, cols, X, P, f / X_SCALE, f * NS_A, ox, status, n_sm, stream)) return r;
+  }
+  return 0;
+}
+
+// r [batch, rows, cols] (f32 or bf16) -> out (f32 or bf16) = prod_k (a I + P_k) r / norms, the P_k of a forward with keep.
+extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, int rows, int cols, int steps, void* scratch, const void* polys,
+                                        const double* norms, void* out, int out_f32, int* status, cudaStream_t stream) {
+  using namespace dttt::ns;
+  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || batch > 65535) return -2;
+  int n_sm;
+  if (int r = prepare_device(&n_sm)) return r;
+  const int ld = (cols + 7) / 8 * 8, d = rows < cols ? rows : cols, ldd = (d + 7) / 8 * 8;
+  auto up = [](long long v) { return (v + 255) / 256 * 256; };
+  uint8_t* s = (uint8_t*)scratch;
+  const long long xb = up((long long)batch * rows * ld * 2);
+  void* xs[2] = {s, s + xb};
+  double* partial = (double*)(s + 2 * xb + up((long long)batch * d * ldd * 2));
+  double* own = (double*)((uint8_t*)partial + up((long long)batch * NORM_BLOCKS * 8));
+  if (int r = cast(r_in, f32, batch, rows, cols, partial, R_SCALE, xs[0], ld, own, stream)) return r;
+  for (int i = 0; i < steps; ++i) {
+    const Mat X = {xs[i & 1], rows, cols, ld};
+    const Mat P = {(const uint8_t*)polys + (long long)(steps - 1 - i) * batch * d * ldd * 2, d, d, ldd};
+    const bool last = i == steps - 1;
+    const float f = last ? 1.f / R_SCALE : 1.f;
+    const Out o = {last ? out : xs[(i + 1) & 1], last ? (out_f32 ? OUT_F32 : OUT_BF16) : OUT_F16, last ? cols : ld, last ? own : nullptr,
+                   last ? norms : nullptr};
+    if (int r = apply(batch, rows, cols, X, P, f / X_SCALE, f * NS_A, o, status, n_sm, stream)) return r;
+  }
+  return 0;
+}

@@ -403,7 +403,7 @@ def main(argv=None) -> None:
     ap.add_argument("--inner_mask_ratio", type=float, default=0.75)
     ap.add_argument("--inner_views", type=int, default=g("inner_views", 1))
     ap.add_argument("--inner_mask_span", type=float, default=0.0)
-    ap.add_argument("--inner_update", default="sgd", choices=["sgd", "sign", "muon2"])
+    ap.add_argument("--inner_update", default="sgd", choices=["sgd", "sign", "muon2", "muon5"])
     ap.add_argument("--inner_mask_mode", default=g("inner_mask_mode", "random"), choices=["random", "rare", "docaware"])
     ap.add_argument("--inner_target_frac", type=float, default=g("inner_target_frac", 0.5))
     ap.add_argument("--inner_task", default=g("inner_task", "mask"), choices=["mask", "causal", "split"])

@@ -824,3 +824,42 @@ def unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure):
                                           0.0 if sure is None else float(sure), 0 if sure is None else 1, _p(ids_out), _p(known_out),
                                           _p(held_out), _p(where), B, C, _stream()), "unmask")
     return ids_out, known_out, held_out, where
+
+
+# =============================================================================== Newton-Schulz family
+_lib.register("dttt_newton_schulz_scratch", _ll, [_i, _i, _i])
+_lib.register("dttt_newton_schulz", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp])
+_lib.register("dttt_newton_schulz_apply", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp])
+_SYMBOL.update(newton_schulz="dttt_newton_schulz")
+
+
+def newton_schulz(g, steps, keep):
+    """``g [B, rows, cols]`` (f32 or bf16, contiguous) -> ``(y bf16, norms [B] f64, polys)``; ``polys`` (f16 ``[steps, B, d, ceil8(d)]``)
+    holds every iteration's polynomial matrix with ``keep``, else scratch."""
+    global LAUNCHES
+    B, rows, cols = g.shape
+    d = min(rows, cols)
+    with torch.cuda.device(g.device):
+        y = torch.empty(B, rows, cols, dtype=torch.bfloat16, device=g.device)
+        norms = torch.empty(B, dtype=torch.float64, device=g.device)
+        polys = torch.empty(steps if keep else 1, B, d, -(-d // 8) * 8, dtype=torch.float16, device=g.device)
+        scratch = torch.empty(int(_lib.lib().dttt_newton_schulz_scratch(B, rows, cols)), dtype=torch.uint8, device=g.device)
+        _check(_lib.lib().dttt_newton_schulz(_p(g), int(g.dtype == torch.float32), B, rows, cols, steps, _p(scratch), _p(polys), int(keep),
+                                             _p(norms), _p(y), _p(_lib.status_tensor(g.device)), _stream()), "newton_schulz")
+    LAUNCHES += 1 + 3 * steps
+    return y, norms, polys
+
+
+def newton_schulz_apply(r, norms, polys, out_dtype):
+    """The linear map of a kept forward applied to ``r [B, rows, cols]`` (f32 or bf16, contiguous)."""
+    global LAUNCHES
+    B, rows, cols = r.shape
+    steps = polys.shape[0]
+    with torch.cuda.device(r.device):
+        out = torch.empty(B, rows, cols, dtype=out_dtype, device=r.device)
+        scratch = torch.empty(int(_lib.lib().dttt_newton_schulz_scratch(B, rows, cols)), dtype=torch.uint8, device=r.device)
+        _check(_lib.lib().dttt_newton_schulz_apply(_p(r), int(r.dtype == torch.float32), B, rows, cols, steps, _p(scratch), _p(polys),
+                                                   _p(norms), _p(out), int(out_dtype == torch.float32), _p(_lib.status_tensor(r.device)),
+                                                   _stream()), "newton_schulz_apply")
+    LAUNCHES += 1 + steps
+    return out

@@ -1,0 +1,83 @@
+"""Newton-Schulz orthogonalisation of an update, the direction of the ``muon5`` write (``ttt.inner.direction``).
+
+``newton_schulz(g)`` drives the singular values of every matrix of ``g [..., rows, cols]`` toward one: from
+``x = g / |g|_F``, ``steps`` times ``x <- a x + (b G + c G G) x`` with ``G = x x^T`` on the smaller side and the coefficients of
+the inner step (reference ``src/ttt/inner_loop.py:350-397``, which runs two iterations in bf16).  On a CUDA device the products
+run on the tensor cores with f16 operands and f32 sums (``csrc/newton_schulz.cu``); elsewhere in f32.
+
+The result is the linear map ``g -> M g / |g|`` with a symmetric polynomial ``M`` of the matrix; as in the reference, ``M`` (and the
+norm, which the rescaling of the direction cancels) is held constant by the derivative, so the backward applies the same map
+to the cotangent, and so does the backward's own backward.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import reference as ref
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    t = t if t.dtype in (torch.float32, torch.bfloat16) else t.float()
+    return t.reshape(-1, *t.shape[-2:]).contiguous()
+
+
+class _Apply(torch.autograd.Function):
+    """``r -> M r / |g|`` with what a forward kept of ``g``; linear and self-adjoint."""
+
+    @staticmethod
+    def forward(ctx, r, norms, polys, dtype):
+        ctx.kept, ctx.dtype = (norms, polys), r.dtype
+        if not r.is_cuda:
+            return ref.newton_schulz_apply(r, norms, polys).to(dtype)
+        from . import kernels
+        out_dtype = torch.float32 if dtype == torch.float32 else torch.bfloat16
+        return kernels.newton_schulz_apply(_flat(r), norms, polys, out_dtype).view(r.shape).to(dtype)
+
+    @staticmethod
+    def backward(ctx, c):
+        return _Apply.apply(c, *ctx.kept, ctx.dtype), None, None, None
+
+
+class _NewtonSchulz(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, steps):
+        y, *ctx.kept = _run(g, steps, True)
+        ctx.dtype = g.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        return _Apply.apply(gy, *ctx.kept, ctx.dtype), None
+
+
+def _run(g: torch.Tensor, steps: int, keep: bool):
+    if not g.is_cuda:
+        y, norms, polys = ref.newton_schulz(g, steps)
+        return y.to(torch.bfloat16), norms, polys
+    from . import kernels
+    if not kernels.available("newton_schulz"):
+        raise RuntimeError("newton_schulz: the kernels are not in the loaded library")
+    y, norms, polys = kernels.newton_schulz(_flat(g), steps, keep)
+    return y.view(g.shape), norms, polys
+
+
+def newton_schulz(g: torch.Tensor, steps: int = 5) -> torch.Tensor:
+    """The orthogonalised direction of every matrix of ``g [..., rows, cols]`` (f32 or bf16), in bf16.
+
+    The norms are taken in 64 bits, so any finite scale of ``g`` will do; a zero matrix gives zeros (and a zero derivative), one
+    that holds NaN or infinities gives NaN.  On a CUDA device operands round to f16: singular values below about 2^-11 of the
+    largest come out with the noise of those roundings, and the derivative has the accuracy of bf16 whatever the type of ``g``.
+    At most 65535 matrices a call."""
+    if g.dim() < 2 or g.shape[-1] == 0 or g.shape[-2] == 0:
+        raise ValueError(f"newton_schulz: g {tuple(g.shape)}, [..., rows, cols] with non-empty matrices is wanted")
+    if g.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"newton_schulz: g of {g.dtype} (float32 or bfloat16)")
+    if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= 32:
+        raise ValueError(f"newton_schulz: steps = {steps!r}, a number from 1 to 32 is wanted")
+    if g.numel() // (g.shape[-1] * g.shape[-2]) > 65535:
+        raise ValueError(f"newton_schulz: {g.numel() // (g.shape[-1] * g.shape[-2])} matrices, at most 65535 are taken in one call")
+    if g.numel() == 0:
+        return g.to(torch.bfloat16)
+    if torch.is_grad_enabled() and g.requires_grad:
+        return _NewtonSchulz.apply(g, steps)
+    return _run(g, steps, False)[0]

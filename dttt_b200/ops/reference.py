@@ -198,3 +198,31 @@ def unmask(ids, known, held, tokens, logp, priority, quota, allowed=None, sure=N
     if sure is not None:
         where = where | ((logp >= sure) & ~known)
     return torch.where(where, tokens, ids), known | where, torch.where(where, logp, held), where
+
+
+# ------------------------------------------------------------------ Newton-Schulz orthogonalisation
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(g: torch.Tensor, steps: int, dtype: torch.dtype = torch.float32):
+    """``ops.newton_schulz.newton_schulz`` without the rounding of the result: ``(y, norms [..., 1, 1], polys)``, with ``polys`` the
+    ``b G + c G G`` of every iteration (on the smaller side)."""
+    a, b, c = NEWTON_SCHULZ
+    g = g.to(dtype)
+    norms = torch.linalg.matrix_norm(g.double(), dim=(-2, -1), keepdim=True)
+    x = torch.where(norms == 0, 0.0, g.double() / norms).to(dtype)
+    wide = x.shape[-2] <= x.shape[-1]
+    polys = []
+    for _ in range(steps):
+        gram = x @ x.mT if wide else x.mT @ x
+        polys.append(b * gram + c * (gram @ gram))
+        x = a * x + (polys[-1] @ x if wide else x @ polys[-1])
+    return x, norms, polys
+
+
+def newton_schulz_apply(r: torch.Tensor, norms: torch.Tensor, polys) -> torch.Tensor:
+    """The linear map of ``newton_schulz`` with its polynomials and norms held constant (its own adjoint)."""
+    x = torch.where(norms == 0, 0.0, r.double() / norms).to(polys[0].dtype)
+    for p in reversed(polys):
+        x = NEWTON_SCHULZ[0] * x + (p @ x if x.shape[-2] <= x.shape[-1] else x @ p)
+    return x

@@ -376,7 +376,7 @@ class TrainConfig:
         _need(c.inner_view_mode != "complement" or c.inner_views in (1, 2),
               "inner_views must be 1 or 2 with complementary views (use inner_view_mode strata for more)")
         _need(c.inner_view_mode != "strata" or c.inner_views >= 2, "inner_view_mode strata needs inner_views >= 2")
-        _need(c.inner_update in ("sgd", "sign", "muon2"), f"inner_update {c.inner_update!r} (sgd | sign | muon2)")
+        _need(c.inner_update in ("sgd", "sign", "muon2", "muon5"), f"inner_update {c.inner_update!r} (sgd | sign | muon2 | muon5)")
         _need(c.inner_mask_mode in ("random", "rare", "docaware"),
               f"inner_mask_mode {c.inner_mask_mode!r} (random | rare | docaware)")
         _need(0.0 < c.inner_update_frac <= 1.0, "inner_update_frac in (0, 1]")

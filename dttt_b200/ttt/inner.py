@@ -1,7 +1,7 @@
 """The write: one clipped gradient step on the per-sequence fast weight per chunk.
 
     g      = grad_W  mean_{i in targets} CE( suffix(h_inner; W)_i , target_i )     per sequence
-    u      = direction(g)                     sgd | sign | muon2, rescaled to ||g||
+    u      = direction(g)                     sgd | sign | muon2 | muon5, rescaled to ||g||
     u     <- u * min(1, clip / ||u||)         ONE norm over all 3 F matrices of a sequence
     W_l   <- W_l - eta_l u_l - lambda_l (W_l - W0_l)                                 in f32
 
@@ -24,6 +24,7 @@ import torch
 from ..ops import ce as CE
 from ..ops import functional as Fn
 from ..ops.attention import own_mask_matrix
+from ..ops.newton_schulz import newton_schulz
 
 FastW = List[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]]
 
@@ -319,6 +320,8 @@ def direction(g: List[torch.Tensor], rule: str) -> List[torch.Tensor]:
         u = [x * torch.rsqrt(x.pow(2) + 1e-12) for x in g]
     elif rule == "muon2":
         u = [orthogonalise(x, 2) for x in g]
+    elif rule == "muon5":
+        u = [newton_schulz(x, 5) for x in g]
     else:
         raise ValueError(f"inner_update {rule!r}")
     ratio = seq_norm(g) / seq_norm(u)

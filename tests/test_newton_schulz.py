@@ -1,0 +1,90 @@
+"""Newton-Schulz directions on the CPU: the singular values, the derivative of the linear map, the write rule, refusals."""
+import pytest
+import torch
+
+from util import loss_and_grads, loss_config, make_engine
+from dttt_b200.ops import reference as ref
+from dttt_b200.ops.newton_schulz import newton_schulz
+from dttt_b200.ttt import inner as IN
+
+A, B, C = ref.NEWTON_SCHULZ
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (5, 5), (4, 9), (9, 4), (2, 3, 6, 4), (1, 7), (7, 1)])
+@pytest.mark.parametrize("steps", [1, 2, 5])
+def test_singular_values_follow_the_polynomial(shape, steps):
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(1)) * 1e-4
+    u, s, vt = torch.linalg.svd(g.double(), full_matrices=False)
+    s = s / s.pow(2).sum(-1, keepdim=True).sqrt()
+    for _ in range(steps):
+        s = A * s + B * s ** 3 + C * s ** 5
+    want = u @ (s[..., None] * vt)
+    y = newton_schulz(g, steps)
+    assert y.dtype == torch.bfloat16 and y.shape == g.shape
+    # bf16 rounds by 2^-9 of a value below 2^(e+1); f32 products of at most 9 terms, amplified at most 3.4445^5 = 485 times
+    assert ((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 485 * 2.0 ** -21 * want.abs().max()).all()
+
+
+def test_derivative_is_the_held_linear_map():
+    gen = torch.Generator().manual_seed(2)
+    g = torch.randn(3, 6, 4, generator=gen).requires_grad_(True)
+    gy = torch.randn(3, 6, 4, generator=gen)
+    _, norms, polys = ref.newton_schulz(g.detach(), 3, torch.float64)
+    eye = torch.eye(4, dtype=torch.float64)
+    m = torch.eye(4, dtype=torch.float64)
+    for p in polys:
+        m = (A * eye + p) @ m
+    want = gy.double() @ m / norms
+    y = newton_schulz(g, 3)
+    got, = torch.autograd.grad(y, g, gy.to(torch.bfloat16), create_graph=False)
+    assert got.dtype == torch.float32
+    # the cotangent rounds to bf16 (2^-8) and the f32 products of four terms err far below that
+    assert (got.double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()
+    # differences of the held map: it is linear, so a step of any size gives the derivative
+    step = lambda r: ref.newton_schulz_apply(r.double(), norms, polys)
+    d = torch.randn(3, 6, 4, generator=gen)
+    slope = step(g.detach().double() + 0.5 * d.double()) - step(g.detach().double() - 0.5 * d.double())
+    assert torch.allclose((slope * gy.double()).sum(), (want * d.double()).sum(), rtol=1e-9)
+
+
+def test_derivative_twice_is_the_same_map():
+    g = torch.randn(2, 3, 5).requires_grad_(True)
+    gy = torch.randn(2, 3, 5).to(torch.bfloat16).requires_grad_(True)
+    gx, = torch.autograd.grad(newton_schulz(g, 2), g, gy, create_graph=True)
+    c = torch.randn(2, 3, 5)
+    back, = torch.autograd.grad(gx, gy, c)
+    _, norms, polys = ref.newton_schulz(g.detach(), 2)
+    assert torch.allclose(back.float(), ref.newton_schulz_apply(c, norms, polys), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_zero_scale_and_special_values():
+    assert newton_schulz(torch.zeros(2, 3, 4)).eq(0).all()
+    z = torch.zeros(3, 4, requires_grad=True)
+    assert torch.autograd.grad(newton_schulz(z), z, torch.ones(3, 4, dtype=torch.bfloat16))[0].eq(0).all()
+    g = torch.randn(3, 4)
+    assert newton_schulz(g * 2.0 ** 100).equal(newton_schulz(g)) and newton_schulz(g * 2.0 ** -100).equal(newton_schulz(g))
+    g[0, 0] = float("inf")
+    assert newton_schulz(g).isnan().all()
+    assert newton_schulz(torch.zeros(0, 3, 4)).shape == (0, 3, 4)
+
+
+@pytest.mark.parametrize("g,steps,word", [(torch.zeros(4), 5, "rows, cols"), (torch.zeros(3, 0), 5, "rows, cols"),
+                                          (torch.zeros(3, 3, dtype=torch.float64), 5, "float64"), (torch.zeros(3, 3), 0, "steps"),
+                                          (torch.zeros(3, 3), 2.0, "steps"), (torch.zeros(3, 3), True, "steps"),
+                                          (torch.zeros(3, 3), 33, "steps"), (torch.zeros(65536, 1, 1), 1, "65535")])
+def test_refusals(g, steps, word):
+    with pytest.raises(ValueError, match=word):
+        newton_schulz(g, steps)
+
+
+def test_the_write_rule_keeps_the_gradient_norm_and_trains():
+    gen = torch.Generator().manual_seed(3)
+    g = [torch.randn(2, 6, 9, generator=gen), torch.randn(2, 9, 6, generator=gen)]
+    u = IN.direction(g, "muon5")
+    assert torch.allclose(IN.seq_norm(u), IN.seq_norm(g), rtol=1e-5)
+    s = torch.linalg.svdvals(u[0])
+    assert (s.amax(-1) / s.amin(-1) < 2).all()                      # five iterations: all singular values within [0.68, 1.21]
+    eng = make_engine(inner_update="muon5")
+    loss, grads, _ = loss_and_grads(eng, torch.randint(0, 120, (2, 32), generator=gen), loss_config(eng.tc))
+    assert loss == loss and all(torch.isfinite(v).all() for v in grads.values())
+    assert grads["fast_weight.gate.weight"].abs().sum() > 0

@@ -1,0 +1,162 @@
+"""The Newton-Schulz kernels against the 64-bit statement.
+
+Bound of the result, relative in the 2-norm: the bf16 result rounds by at most 2^-9 of every value.  Inside, x, G and P round to f16
+(at most 2^-12 relative each, 2^-11.5 in the mean square of three independent roundings) in each of the steps, and what a step
+leaves grows by at most 3.4445 per further step in the directions that the matrix has; relative to a result that grows alike
+it adds up: steps * 3.4445 * 3 * 2^-12 <= 1.3e-2 for five steps as a worst case; independent roundings average over at
+least d terms, which makes it a sum of squares: sqrt(steps * 3) * 3.4445 * 2^-12 = 3.3e-3.  With the result's own: 5.2e-3.
+The derivative applies steps products with the same P and f16 roundings: the same bound."""
+import pytest
+import torch
+
+from dttt_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+BOUND = 5.2e-3
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    from dttt_b200.ops import _lib
+    torch.cuda.synchronize()
+    _lib.check_status()
+
+
+def make(shape, dtype, seed=0, scale=1e-3):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    t = 2 * min(shape[-2:])
+    h = torch.randn(*shape[:-2], t, shape[-2], generator=gen, device="cuda")
+    d = torch.randn(*shape[:-2], t, shape[-1], generator=gen, device="cuda") * torch.rand(*shape[:-2], t, 1, generator=gen, device="cuda")
+    return (h.mT @ d * scale).to(dtype), torch.randn(*shape, generator=gen, device="cuda").to(torch.bfloat16)
+
+
+def off(a, b):
+    return ((a.double() - b.double()).norm() / b.double().norm()).item()
+
+
+SHAPES = [(8, 8), (64, 64), (1, 65, 127), (3, 128, 256), (2, 256, 128), (5, 100, 36), (257, 256), (256, 257), (2, 509, 1283), (1283, 509),
+          (2, 2, 130, 700), (512, 2048), (1024, 1000), (12, 96, 96), (768, 64), (17, 4096)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("steps", [1, 2, 5])
+def test_direction_and_derivative(shape, dtype, steps):
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    g, gy = make(shape, dtype, sum(shape))
+    want, norms, polys = ref.newton_schulz(g, steps, torch.float64)
+    y = newton_schulz(g, steps)
+    assert y.dtype == torch.bfloat16 and y.shape == g.shape and off(y, want) <= BOUND
+    leaf = g.clone().requires_grad_(True)
+    out = newton_schulz(leaf, steps)
+    assert out.equal(y)
+    got, = torch.autograd.grad(out, leaf, gy)
+    assert got.dtype == dtype and off(got, ref.newton_schulz_apply(gy, norms, polys)) <= BOUND
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 9), (9, 1), (3, 5), (2, 3), (7, 33)])
+def test_tiny_matrices(shape):
+    """With a handful of roundings nothing averages out: the worst case above, 1.3e-2 and the result's rounding."""
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    for steps in (1, 5):
+        g, gy = make(shape, torch.float32, 3)
+        leaf = g.clone().requires_grad_(True)
+        want, norms, polys = ref.newton_schulz(g, steps, torch.float64)
+        y = newton_schulz(leaf, steps)
+        assert off(y, want) <= 1.5e-2
+        assert off(torch.autograd.grad(y, leaf, gy)[0], ref.newton_schulz_apply(gy, norms, polys)) <= 1.5e-2
+
+
+def test_derivative_against_differences():
+    """The map is linear in g once its matrix is held: a difference of the 64-bit map along a direction is the derivative."""
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    g, gy = make((200, 320), torch.bfloat16, 4)
+    _, norms, polys = ref.newton_schulz(g, 5, torch.float64)
+    leaf = g.clone().requires_grad_(True)
+    got, = torch.autograd.grad(newton_schulz(leaf), leaf, gy)
+    for seed in (1, 2):
+        _, d = make((200, 320), torch.bfloat16, seed)
+        step = lambda e: ref.newton_schulz_apply(g.double() + e * d.double(), norms, polys)
+        slope = ((step(0.5) - step(-0.5)) * gy.double()).sum()
+        mine = (got.double() * d.double()).sum()
+        assert abs(mine - slope) <= BOUND * got.double().norm() * d.double().norm()
+
+
+def test_twice_differentiable_scale_zero_and_special_values():
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    g, gy = make((3, 150, 90), torch.float32, 5)
+    leaf, cot = g.clone().requires_grad_(True), gy.clone().requires_grad_(True)
+    gx, = torch.autograd.grad(newton_schulz(leaf, 3), leaf, cot, create_graph=True)
+    c, _ = make((3, 150, 90), torch.float32, 6)
+    back, = torch.autograd.grad(gx, cot, c)
+    _, norms, polys = ref.newton_schulz(g, 3, torch.float64)
+    assert back.dtype == torch.bfloat16 and off(back, ref.newton_schulz_apply(c, norms, polys)) <= BOUND
+    assert newton_schulz(g * 2.0 ** 90).equal(newton_schulz(g)) and newton_schulz(g * 2.0 ** -90).equal(newton_schulz(g))
+    z = g.clone()
+    z[1] = 0
+    z[2, 3, 4] = float("nan")
+    leaf = z.requires_grad_(True)
+    y = newton_schulz(leaf)
+    assert y[0].equal(newton_schulz(g[0])) and y[1].eq(0).all() and y[2].isnan().all()
+    gx, = torch.autograd.grad(y, leaf, gy)
+    assert gx[1].eq(0).all() and gx[0].isfinite().all()
+
+
+def test_concentrated_cotangent_and_spectrum():
+    """One entry of the cotangent alone, and a matrix whose singular values span three decades (the noise of the f16 roundings,
+    3 * 2^-12 of the largest value per step, is amplified like the smallest ones: up to 485 times)."""
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    g, gy = make((128, 384), torch.float32, 7)
+    one = torch.zeros_like(gy)
+    one[5, 7] = 1e4
+    leaf = g.clone().requires_grad_(True)
+    got, = torch.autograd.grad(newton_schulz(leaf), leaf, one)
+    _, norms, polys = ref.newton_schulz(g, 5, torch.float64)
+    assert got.isfinite().all() and off(got, ref.newton_schulz_apply(one, norms, polys)) <= BOUND
+    u, _, vt = torch.linalg.svd(g, full_matrices=False)
+    sharp = u @ (torch.logspace(0, -3, 128, device="cuda")[:, None] * vt)
+    assert newton_schulz(sharp).isfinite().all()
+    assert off(newton_schulz(sharp), ref.newton_schulz(sharp, 5, torch.float64)[0]) <= 485 * 3 * 2.0 ** -12 / 5
+
+
+def test_views_repeats_streams_graphs_and_empty():
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    g, gy = make((4, 300, 200), torch.bfloat16, 8)
+    first = newton_schulz(g)
+    assert all(newton_schulz(g).equal(first) for _ in range(3))
+    assert newton_schulz(g.mT.contiguous().mT).equal(first) and newton_schulz(g[1:3]).equal(first[1:3])
+    cut = g[:, 3:290, 5:150]
+    assert newton_schulz(cut).equal(newton_schulz(cut.contiguous()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = newton_schulz(g)
+    torch.cuda.current_stream().wait_stream(side)
+    assert other.equal(first) and newton_schulz(g[:0]).shape == (0, 300, 200)
+    # forward and backward in one graph, replayed on other values; the leaf has no eager graph alive
+    leaf = g.clone().requires_grad_(True)
+    cot = gy.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = newton_schulz(leaf)
+        gx, = torch.autograd.grad(y, leaf, cot)
+    g2, gy2 = make((4, 300, 200), torch.bfloat16, 9)
+    with torch.no_grad():
+        leaf.copy_(g2)
+    cot.copy_(gy2)
+    graph.replay()
+    want = g2.clone().requires_grad_(True)
+    y2 = newton_schulz(want)
+    assert y.equal(y2) and gx.equal(torch.autograd.grad(y2, want, gy2)[0])
+
+
+def test_the_write_rule_on_the_kernels():
+    """The direction that the inner step takes: norms over a sequence's matrices kept, every matrix near-orthogonal."""
+    from dttt_b200.ttt import inner as IN
+    g = [make((2, 256, 512), torch.bfloat16, 1)[0], make((2, 512, 256), torch.float32, 2)[0]]
+    u = IN.direction(g, "muon5")
+    assert torch.allclose(IN.seq_norm(u), IN.seq_norm(g), rtol=1e-3)
+    for t in u:
+        s = torch.linalg.svdvals(t.float())
+        assert (s.amax(-1) / s.amin(-1) < 2.5).all()
