@@ -34,7 +34,8 @@ constexpr int STAGES = 6;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int B_BYTES = (BN / 2) * BK * 2;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int SMEM_TOTAL = STAGES * STAGE_BYTES + 1024 + 1024;
+constexpr int STAGING_BYTES = 4 * 4096;                        // epilogue: 32 rows x 128 bytes per warp
+constexpr int SMEM_TOTAL = STAGES * STAGE_BYTES + 1024 + STAGING_BYTES + 1024;
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float X_SCALE = 4096.f;           // of x, G and P
@@ -54,13 +55,25 @@ struct Params {
   const double* num;           // per-batch factors of the output, or null
   const double* den;
   int* status;
+  int symmetric;               // C is symmetric: tiles on and below the diagonal, those below are stored a second time transposed
   int tiles_m, tiles_n;
 };
 
+__host__ __device__ inline int tiles_per_matrix(const Params& p) {
+  return p.symmetric ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+}
+
 __device__ __forceinline__ void tile_coords(int tile, const Params& p, int& b, int& tm, int& tn) {
-  const int per_batch = p.tiles_m * p.tiles_n;
+  const int per_batch = tiles_per_matrix(p);
   b = tile / per_batch;
   const int t = tile - b * per_batch;
+  if (p.symmetric) {
+    tm = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while (tm * (tm + 1) / 2 > t) --tm;                        // the root may round across a whole number
+    while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
+    tn = t - tm * (tm + 1) / 2;
+    return;
+  }
   constexpr int GROUP = 8;                                     // bands of 8 pair rows, n fastest inside a band
   const int band = t / (GROUP * p.tiles_n);
   const int first_m = band * GROUP;
@@ -68,6 +81,91 @@ __device__ __forceinline__ void tile_coords(int tile, const Params& p, int& b, i
   const int r = t - band * GROUP * p.tiles_n;
   tm = first_m + (r % rows);
   tn = r / rows;
+}
+
+// ------------------------------------------------------------------ the epilogue's pieces
+// A warp handles 32 rows x 64 columns of 16-bit values at a time.  Global memory sees whole 128-byte lines, eight lanes to a row;
+// the threads see a row each (as tcgen05.ld delivers the accumulator).  A 4 KB staging area with 16-byte pieces XOR-swizzled
+// by row turns one into the other.  `rows`, `cols`: what is left of the matrix from here on (may be negative); stored f16 matrices
+// have rows of a multiple of 8, so a piece is there or not as a whole, and what is in the padding is never read.
+__device__ __forceinline__ void load_rows(const __half* d, long long ld, int rows, int cols, int lane, uint4 (&v)[8]) {
+  const int piece = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rr = i * 4 + (lane >> 3);
+    v[i] = d && rr < rows && piece * 8 < cols ? __ldg(reinterpret_cast<const uint4*>(d + rr * ld + piece * 8)) : make_uint4(0, 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void stage_in(uint8_t* stg, int lane, const uint4 (&v)[8]) {
+  const int piece = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rr = i * 4 + (lane >> 3);
+    *reinterpret_cast<uint4*>(stg + rr * 128 + ((piece ^ (rr & 7)) * 16)) = v[i];
+  }
+}
+template <class T2> __device__ __forceinline__ T2 pack2(float a, float b);
+template <> __device__ __forceinline__ __half2 pack2<__half2>(float a, float b) { return __floats2half2_rn(a, b); }
+template <> __device__ __forceinline__ __nv_bfloat162 pack2<__nv_bfloat162>(float a, float b) { return __floats2bfloat162_rn(a, b); }
+template <class T2>
+__device__ __forceinline__ void stage_out(uint8_t* stg, int lane, const uint32_t (&r)[64]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint4 v;
+    T2* h = reinterpret_cast<T2*>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = pack2<T2>(__uint_as_float(r[8 * q + 2 * e]), __uint_as_float(r[8 * q + 2 * e + 1]));
+    *reinterpret_cast<uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16)) = v;
+  }
+}
+__device__ __forceinline__ void flush_lines(const uint8_t* stg, int lane, uint16_t* out, long long ld, int rows, int cols) {
+  const int piece = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rr = i * 4 + (lane >> 3);
+    const uint4 v = *reinterpret_cast<const uint4*>(stg + rr * 128 + ((piece ^ (rr & 7)) * 16));
+    if (rr < rows && piece * 8 < cols) *reinterpret_cast<uint4*>(out + rr * ld + piece * 8) = v;
+  }
+}
+// rows that start at any element: 32 neighbouring elements per instruction
+__device__ __forceinline__ void flush_ragged(const uint8_t* stg, int lane, uint16_t* out, long long ld, int rows, int cols) {
+#pragma unroll 4
+  for (int rr = 0; rr < 32; ++rr) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = h * 32 + lane;
+      const uint16_t v = *reinterpret_cast<const uint16_t*>(stg + rr * 128 + (((j >> 3) ^ (rr & 7)) * 16) + (j & 7) * 2);
+      if (rr < rows && j < cols) out[rr * ld + j] = v;
+    }
+  }
+}
+__device__ __forceinline__ void store_f32(float* out, long long ld, int rows, int cols, int lane, const uint32_t (&r)[64]) {
+  if (lane >= rows) return;
+  float* o = out + lane * ld;
+  if ((ld & 3) == 0) {
+#pragma unroll
+    for (int j = 0; j < 64; j += 4)
+      if (j < cols) *reinterpret_cast<float4*>(o + j) = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
+                                                                    __uint_as_float(r[j + 3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 64; ++j)
+      if (j < cols) o[j] = __uint_as_float(r[j]);
+  }
+}
+// The piece's transpose: column j of the 64 becomes a row.  Neighbouring lanes (rows 2i, 2i + 1 of the piece) trade one value per
+// pair of columns, so that each stores two neighbours: an instruction writes 64 bytes of two rows.
+__device__ __forceinline__ void store_transposed(__half* out, long long ld, int rows, int cols, int lane, const uint32_t (&r)[64]) {
+  const bool odd = lane & 1;
+  const int at = lane & ~1;
+#pragma unroll
+  for (int j = 0; j < 64; j += 2) {
+    const float mine = __uint_as_float(odd ? r[j + 1] : r[j]);
+    const float theirs = __shfl_xor_sync(0xffffffffu, __uint_as_float(odd ? r[j] : r[j + 1]), 1);
+    const __half2 v = odd ? __floats2half2_rn(theirs, mine) : __floats2half2_rn(mine, theirs);
+    const int jr = j + odd;
+    if (jr < rows && at < cols) *reinterpret_cast<__half2*>(out + jr * ld + at) = v;
+  }
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
@@ -84,7 +182,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-  const int num_tiles = p.batch * p.tiles_m * p.tiles_n;
+  const int num_tiles = p.batch * tiles_per_matrix(p);
   const int kblocks = (p.K + BK - 1) / BK;
   constexpr uint32_t TMEM_COLS = 2 * BN;
 
@@ -179,39 +277,63 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
       tile_coords(tile, p, b, tm, tn);
       const int acc = local_tile & 1;
       const uint32_t acc_ph = (local_tile >> 1) & 1;
-      int got = 1;
-      if (lane == 0) got = mbar_wait_bounded(&acc_full[acc], acc_ph, abort_word, p.status, ERR_WAIT_TMEM_FULL) ? 1 : 0;
-      got = __shfl_sync(0xffffffffu, got, 0);
-      if (!got) break;
-      tc_fence_after();
-      const int row = tm * 2 * BM + (int)rank * BM + quarter * 32 + lane;
-      const uint32_t taddr = tmem_base + acc * BN + ((uint32_t)(quarter * 32) << 16);
+      const int row0 = tm * 2 * BM + (int)rank * BM + quarter * 32, n0 = tn * BN;
+      const int rows = p.M - row0;                             // of this warp's 32 (may be negative)
       float alpha = p.alpha, beta = p.beta;
       if (p.num || p.den) {
         const double den = p.den ? p.den[b] : 1.0;
         const float f = den == 0.0 ? 0.f : (float)((p.num ? p.num[b] : 1.0) / den);      // a zero matrix has a zero derivative
         alpha *= f; beta *= f;
       }
-      const __half* drow = p.D ? p.D + (long long)b * p.d_batch + (long long)row * p.ldd : nullptr;
-      const long long crow = (long long)b * p.c_batch + (long long)row * p.ldc;
+      const __half* d0 = p.D ? p.D + (long long)b * p.d_batch + (long long)row0 * p.ldd + n0 : nullptr;
+      uint4 dnext[8];                                          // 64 columns of D, eight lanes to a row's 128 bytes
+      load_rows(d0, p.ldd, rows, (int)p.ldd - n0, lane, dnext);
+      int got = 1;
+      if (lane == 0) got = mbar_wait_bounded(&acc_full[acc], acc_ph, abort_word, p.status, ERR_WAIT_TMEM_FULL) ? 1 : 0;
+      got = __shfl_sync(0xffffffffu, got, 0);
+      if (!got) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + acc * BN + ((uint32_t)(quarter * 32) << 16);
+      uint8_t* stg = smem + STAGES * STAGE_BYTES + 1024 + quarter * 4096;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32(taddr + c, r);
+      for (int c = 0; c < BN; c += 64) {
+        uint32_t r[64];
+        tmem_ld_32x32(taddr + c, reinterpret_cast<uint32_t(&)[32]>(r[0]));
+        tmem_ld_32x32(taddr + c + 32, reinterpret_cast<uint32_t(&)[32]>(r[32]));
+        if (d0) {
+          stage_in(stg, lane, dnext);
+          if (c + 64 < BN) load_rows(d0 + c + 64, p.ldd, rows, (int)p.ldd - n0 - c - 64, lane, dnext);
+          __syncwarp();
+        }
         tmem_ld_wait();
-        const int col = tn * BN + c;
-        const int nc = row < p.M ? min(32, p.N - col) : 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (j < nc) {
-            float v = __uint_as_float(r[j]) * alpha;
-            if (drow) v = fmaf(beta, __half2float(drow[col + j]), v);
-            if (p.out == OUT_F16) reinterpret_cast<__half*>(p.C)[crow + col + j] = __float2half_rn(v);
-            else if (p.out == OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p.C)[crow + col + j] = __float2bfloat16(v);
-            else reinterpret_cast<float*>(p.C)[crow + col + j] = v;
+        for (int q = 0; q < 8; ++q) {
+          uint4 dv = make_uint4(0, 0, 0, 0);
+          if (d0) dv = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16));
+          const __half2* dh = reinterpret_cast<const __half2*>(&dv);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 df = __half22float2(dh[e]);
+            r[8 * q + 2 * e] = __float_as_uint(fmaf(beta, df.x, alpha * __uint_as_float(r[8 * q + 2 * e])));
+            r[8 * q + 2 * e + 1] = __float_as_uint(fmaf(beta, df.y, alpha * __uint_as_float(r[8 * q + 2 * e + 1])));
           }
         }
-        __syncwarp();                                          // the next load is one of the whole warp
+        __syncwarp();
+        if (p.out == OUT_F32) {
+          store_f32(reinterpret_cast<float*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c, p.ldc, rows, p.N - n0 - c, lane, r);
+          __syncwarp();                                        // the next load is one of the whole warp
+        } else {
+          if (p.out == OUT_F16) stage_out<__half2>(stg, lane, r);
+          else stage_out<__nv_bfloat162>(stg, lane, r);
+          __syncwarp();
+          uint16_t* out = reinterpret_cast<uint16_t*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c;
+          if ((p.ldc & 7) == 0) flush_lines(stg, lane, out, p.ldc, rows, (int)p.ldc - n0 - c);
+          else flush_ragged(stg, lane, out, p.ldc, rows, p.N - n0 - c);
+          if (p.symmetric && tm != tn)
+            store_transposed(reinterpret_cast<__half*>(p.C) + (long long)b * p.c_batch + (long long)(n0 + c) * p.ldc + row0, p.ldc, p.N - n0 - c,
+                             (int)p.ldc - row0, lane, r);
+          __syncwarp();
+        }
       }
       tc_fence_before();
       mbar_arrive_remote(mapa_u32(&acc_empty[acc], 0));
@@ -337,9 +459,9 @@ struct Out {
   const double *num, *den;
 };
 
-// C [M, N] = alpha op(A) op(B) + beta D over the batch
+// C [M, N] = alpha op(A) op(B) + beta D over the batch (symmetric: C and D are, and only f16)
 static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, const Mat& B, bool b_mn, float alpha, float beta, const Mat* D,
-                   const Out& o, int* status, int n_sm, cudaStream_t stream) {
+                   const Out& o, bool symmetric, int* status, int n_sm, cudaStream_t stream) {
   CUtensorMap mapA, mapB;
   if (int r = make_map(&mapA, A, batch, a_mn)) return r;
   if (int r = make_map(&mapB, B, batch, b_mn)) return r;
@@ -348,9 +470,10 @@ static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, cons
   p.M = M; p.N = N; p.K = K; p.batch = batch; p.a_mn_major = a_mn; p.b_mn_major = b_mn; p.alpha = alpha; p.beta = beta;
   if (D) { p.D = (const __half*)D->ptr; p.ldd = D->ld; p.d_batch = D->ld * D->rows; }
   p.C = o.C; p.out = o.kind; p.ldc = o.ld; p.c_batch = o.ld * M; p.num = o.num; p.den = o.den; p.status = status;
+  p.symmetric = symmetric;
   p.tiles_m = (M + 2 * BM - 1) / (2 * BM);
   p.tiles_n = (N + BN - 1) / BN;
-  const long long tiles = (long long)batch * p.tiles_m * p.tiles_n;
+  const long long tiles = (long long)batch * tiles_per_matrix(p);
   if (tiles > 0x3fffffff) return 303;
   const int pairs = (int)(tiles < n_sm / 2 ? tiles : n_sm / 2);
   ns_product_kernel<<<2 * pairs, 192, SMEM_TOTAL, stream>>>(mapA, mapB, p);
@@ -361,8 +484,8 @@ static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, cons
 // r (f16, scale S) -> a r + P r: into f16 or, at the end, into the caller's tensor
 static int apply(int batch, int rows, int cols, const Mat& r, const Mat& P, float alpha, float beta, const Out& o, int* status, int n_sm,
                  cudaStream_t stream) {
-  if (rows <= cols) return product(batch, rows, cols, rows, P, false, r, true, alpha, beta, &r, o, status, n_sm, stream);
-  return product(batch, rows, cols, cols, r, false, P, false, alpha, beta, &r, o, status, n_sm, stream);
+  if (rows <= cols) return product(batch, rows, cols, rows, P, false, r, true, alpha, beta, &r, o, false, status, n_sm, stream);
+  return product(batch, rows, cols, cols, r, false, P, false, alpha, beta, &r, o, false, status, n_sm, stream);
 }
 
 static int cast(const void* g, int f32, int batch, int rows, int cols, double* partial, float scale, void* x, int ld, double* norm,
@@ -414,8 +537,8 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
     const Mat X = {xs[k & 1], rows, cols, ld}, G = {gram, d, d, ldd};
     const Mat P = {(uint8_t*)polys + (keep ? (long long)k * batch * d * ldd * 2 : 0), d, d, ldd};
     const Out og = {gram, OUT_F16, ldd, nullptr, nullptr}, op = {const_cast<void*>(P.ptr), OUT_F16, ldd, nullptr, nullptr};
-    if (int r = product(batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, status, n_sm, stream)) return r;
-    if (int r = product(batch, d, d, d, G, false, G, false, NS_C / X_SCALE, NS_B, &G, op, status, n_sm, stream)) return r;
+    if (int r = product(batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, true, status, n_sm, stream)) return r;
+    if (int r = product(batch, d, d, d, G, false, G, false, NS_C / X_SCALE, NS_B, &G, op, true, status, n_sm, stream)) return r;
     const bool last = k == steps - 1;
     const float f = last ? 1.f / X_SCALE : 1.f;
     const Out ox = {last ? y : xs[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : ld, nullptr, nullptr};
