@@ -35,6 +35,7 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 256;
+constexpr int TAB = 32, COPIES = 16;
 constexpr int SLICE_MAX = 49152;            // elements of a slice at most (192 KB)
 constexpr int SLICE_GOOD = 16384;           // a slice up to which three CTAs fit an SM
 
@@ -100,9 +101,12 @@ struct Shared {
   double z, ent;
   float second;
   int at_max, first_max;
-  u64 mass;
+  u64 whole, mass;                          // of the slice; of what is kept of it
+  unsigned int octaves_here[BINS];
   unsigned int count[2][BINS];              // histograms of the threshold search, alternating between rounds
   u64 hmass[2][BINS];
+  unsigned int above_count[2];
+  u64 above_mass[2];
   // this CTA alone
   float fred[WARPS];
   double dred[2][WARPS];
@@ -111,20 +115,52 @@ struct Shared {
   u64 tot_mass[BINS];
   unsigned int tot_count[BINS];
   unsigned int below_count[BINS];           // of the CTAs with a lower rank
+  unsigned int octaves[BINS];               // of all CTAs
+  uint32_t range[2];
+  u64 tot_above_count, tot_above_mass;
   int pick_bin, idx_star;
   u64 pick_above_count, pick_above_mass;
+  double tab[TAB * COPIES];
 };
 
-// (x - m) / T as a mass of `scale` = 2^S units
+// exp((x - m) / T) as a mass of 2^S units, rounded to nearest.  Table-driven (Tang's scheme, from the mathematics): with
+// z = 32 log2(e) (x - m) / T = n + r, |r| <= 1/2, it is 2^(n >> 5) 2^((n & 31) / 32) 2^(r / 32); the last factor by its Taylor series to
+// the fifth order (|r| ln2 / 32 <= 0.0109: truncated by 2.3e-15).  The table holds 16 copies of its 32 values, one per pair of
+// banks, so that the lookups of a half warp never collide.  Half the FP64 instructions of the library's exp, and no conversion back:
+// adding 1.5 2^(52 - S) leaves the rounded mass in the low bits.
 struct Weigher {
-  double m, inv_t, scale;
-  __device__ __forceinline__ u64 operator()(float x) const { return (u64)__double2ll_rn(exp(((double)x - m) * inv_t) * scale); }
+  double c, mc, magic;                      // z = x c + mc
+  float least;                              // below it the mass rounds to 0
+  const double* tab;                        // this thread's copy
+  __device__ __forceinline__ u64 operator()(float x) const {
+    constexpr double SHIFT = 6755399441055744.0;                   // 1.5 2^52: the sum's low word is the rounded integer
+    constexpr double L = 0.02166084939249829;                      // ln2 / 32
+    const double z = fma((double)x, c, mc);
+    const double t = z + SHIFT;
+    const int n = __double2loint(t);
+    const double r = z - (t - SHIFT);
+    double q = L * L * L * L * L / 120;
+    q = fma(q, r, L * L * L * L / 24);
+    q = fma(q, r, L * L * L / 6);
+    q = fma(q, r, L * L / 2);
+    q = fma(q, r, L);
+    q = fma(q, r, 1.0);
+    const double v = q * tab[(n & (TAB - 1)) * COPIES];
+    const double f = __hiloint2double(__double2hiint(v) + ((n >> 5) << 20), __double2loint(v)) + magic;
+    return x >= least ? (u64)(__double_as_longlong(f) - __double_as_longlong(magic)) : 0;
+  }
 };
+
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k <= 0x007fffffu) return -INFINITY;                          // -inf and what has no value
+  if (k >= 0xff800000u) return INFINITY;
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
 
 struct Cut {
-  uint32_t k0, k1;                          // keys above k1 are kept; of those in [k0, k1] the first `ties` by index
+  float lo, hi;                             // values above hi are kept; of those in [lo, hi] the first `ties` by index
   u64 ties, mass;                           // mass: of everything kept
-  u64 before;                               // elements of [k0, k1] in CTAs with a lower rank
+  u64 before;                               // elements of [lo, hi] in CTAs with a lower rank
   u64 here;                                 // ... and in this one
 };
 
@@ -135,49 +171,128 @@ __device__ __forceinline__ Segment split(int a, int b, int parts, int i) {      
   return {s, min(b, s + len)};
 }
 
-// The shortest prefix of the row (value descending, index ascending) whose count (MASS false) or mass (MASS true) reaches
-// `target`: 256-way search over the order keys, one pass over the slice and one cluster barrier per round.
+// Octaves of the tempered mass: bin j of the counts holds the elements whose (m - x) / T log2(e) rounds to j / 8; the last one is
+// not counted.  The rounding is monotone in x, so bins are ranges of the order, and an element's mass is known within 9 %.
+constexpr float PER_OCTAVE = 8.f;
+__device__ __forceinline__ int octave_bin(float x, float m, float scale) {
+  return __float_as_int(fminf((m - x) * scale, (float)(BINS - 1)) + 8388608.f) - 0x4b000000;
+}
+
+// Sums the counts of all CTAs (thread i: bin i), and the running totals of the elements above.
+__device__ __forceinline__ void gather_counts(Shared& sh, int buf, bool mass) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
+  for (int i = threadIdx.x; i < BINS; i += THREADS) {
+    unsigned int c = 0, below = 0;
+    u64 m = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const Shared* p = cluster.map_shared_rank(&sh, r);
+      if (r == me) below = c;
+      c += p->count[buf][i];
+      if (mass) m += p->hmass[buf][i];
+    }
+    sh.tot_count[i] = c; sh.tot_mass[i] = m; sh.below_count[i] = below;
+  }
+  if (threadIdx.x == THREADS - 1) {
+    u64 c = 0, m = 0;
+    for (int r = 0; r < ranks; ++r) { const Shared* p = cluster.map_shared_rank(&sh, r); c += p->above_count[buf]; m += p->above_mass[buf]; }
+    sh.tot_above_count = c; sh.tot_above_mass = m;
+  }
+  __syncthreads();
+}
+
+// From the octave counts, the range of values that has to hold the last element of the prefix whose count or mass reaches
+// `target`.  Warp 0 computes it, from the top bin down, with every element's mass between those of its bin's borders (1e-4 is far
+// more than the rounding of the bins can shift them); the borders are widened by more than the rounding of m - x.
 template <bool MASS>
-__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, u64 target, bool want_mass, int& round) {
+__device__ __forceinline__ void first_range(Shared& sh, float m, float scale, double unit, int V, u64 target) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    constexpr int EACH = BINS / 32;
+    double lo = 0, hi = 0;
+    for (int j = 0; j < EACH; ++j) {
+      const int b = lane * EACH + j;
+      const double c = (double)sh.octaves[b];
+      lo += MASS ? c * exp2f(-(b + 0.5f) / PER_OCTAVE) : c;
+      hi += MASS ? c * exp2f(-fmaxf(b - 0.5f, 0.f) / PER_OCTAVE) : c;
+    }
+    double slo = lo, shi = hi;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double a = __shfl_up_sync(0xffffffffu, slo, o), b = __shfl_up_sync(0xffffffffu, shi, o);
+      if (lane >= o) { slo += a; shi += b; }
+    }
+    slo -= lo; shi -= hi;
+    const double goal = MASS ? (double)target * unit : (double)target, slack = MASS ? (double)V * unit : 0.0;
+    int first = BINS - 1, last = BINS - 1;
+    for (int j = 0; j < EACH; ++j) {
+      const int b = lane * EACH + j;
+      const double c = (double)sh.octaves[b];
+      slo += MASS ? c * exp2f(-(b + 0.5f) / PER_OCTAVE) : c;
+      shi += MASS ? c * exp2f(-fmaxf(b - 0.5f, 0.f) / PER_OCTAVE) : c;
+      if (first == BINS - 1 && (MASS ? shi * 1.0001 + slack : shi) >= goal) first = b;
+      if (last == BINS - 1 && (MASS ? slo * 0.9999 - slack : slo) >= goal) last = b;
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    last = __reduce_min_sync(0xffffffffu, last);
+    if (lane == 0) {
+      const double near = fmax(first - 0.5, 0.0) / scale, far = (last + 0.5) / scale, eps = fabs((double)m) * 1e-6;
+      sh.range[0] = last == BINS - 1 ? 0u : order_key(__double2float_rd((double)m - far * (1 + 1e-5) - eps) + 0.f);
+      sh.range[1] = first == 0 ? 0xffffffffu : order_key(__double2float_ru((double)m - near * (1 - 1e-5) + eps) + 0.f);
+    }
+  }
+  __syncthreads();
+}
+
+// The shortest prefix of the row (value descending, index ascending) whose count (MASS false) or mass (MASS true) reaches
+// `target`: 256-way search over the order keys from the range above; a pass over the slice and a cluster barrier per round.  Only
+// elements of the range and, in the first round, those above it cost more than a comparison.
+template <bool MASS>
+__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, double unit, int V, u64 target,
+                        bool want_mass, int& round) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Segment seg = split(0, n, WARPS, warp);
-  uint32_t k0 = 0, k1 = 0xffffffffu;
+  first_range<MASS>(sh, m, scale, unit, V, target);
+  uint32_t k0 = sh.range[0], k1 = sh.range[1];
   u64 above_c = 0, above_m = 0;
+  bool fresh = true;                                               // what lies above the range is not known yet
   for (;;) {
     const int buf = round & 1;
     ++round;
     int shift = 0;
     while ((k1 - k0) >> shift >= BINS) ++shift;
+    const float lo = key_value(k0), hi = key_value(k1);
     for (int i = tid; i < BINS; i += THREADS) { sh.count[buf][i] = 0; sh.hmass[buf][i] = 0; }
+    if (tid == 0) { sh.above_count[buf] = 0; sh.above_mass[buf] = 0; }
     __syncthreads();
+    unsigned int ac = 0;
+    u64 am = 0;
     for (int i = seg.a + lane; i < seg.b; i += 32) {
-      const uint32_t k = order_key(xs[i]);
-      if (k >= k0 && k <= k1) {
-        const uint32_t bin = (k - k0) >> shift;
-        atomicAdd(&sh.count[buf][bin], 1u);
-        if (MASS || want_mass) atomicAdd(&sh.hmass[buf][bin], w(xs[i]));
+      const float x = xs[i];
+      if (x >= lo) {
+        if (x > hi) {
+          if (fresh) { ++ac; if (MASS || want_mass) am += w(x); }
+        } else {
+          const uint32_t bin = (order_key(x) - k0) >> shift;
+          atomicAdd(&sh.count[buf][bin], 1u);
+          if (MASS || want_mass) atomicAdd(&sh.hmass[buf][bin], w(x));
+        }
       }
+    }
+    if (fresh) {
+      ac = __reduce_add_sync(0xffffffffu, ac);
+      am = warp_sum(am);
+      if (lane == 0 && ac) { atomicAdd(&sh.above_count[buf], ac); atomicAdd(&sh.above_mass[buf], am); }
     }
     cluster.sync();
-    const int ranks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
-    for (int i = tid; i < BINS; i += THREADS) {
-      unsigned int c = 0, below = 0;
-      u64 m = 0;
-      for (int r = 0; r < ranks; ++r) {
-        const Shared* p = cluster.map_shared_rank(&sh, r);
-        if (r == me) below = c;
-        c += p->count[buf][i];
-        m += p->hmass[buf][i];
-      }
-      sh.tot_count[i] = c; sh.tot_mass[i] = m; sh.below_count[i] = below;
-    }
-    __syncthreads();
+    gather_counts(sh, buf, true);
+    if (fresh) { above_c = sh.tot_above_count; above_m = sh.tot_above_mass; fresh = false; }
     if (warp == 0) {
       // lane 0 holds the highest bins: running totals from the top
-      u64 c = 0, m = 0;
-      for (int j = 0; j < BINS / 32; ++j) { const int b = BINS - 1 - (lane * (BINS / 32) + j); c += sh.tot_count[b]; m += sh.tot_mass[b]; }
-      u64 pc = above_c + warp_scan(c, lane) - c, pm = above_m + warp_scan(m, lane) - m;      // before this lane's bins
+      u64 c = 0, ms = 0;
+      for (int j = 0; j < BINS / 32; ++j) { const int b = BINS - 1 - (lane * (BINS / 32) + j); c += sh.tot_count[b]; ms += sh.tot_mass[b]; }
+      u64 pc = above_c + warp_scan(c, lane) - c, pm = above_m + warp_scan(ms, lane) - ms;      // before this lane's bins
       int found = -1;
       u64 fc = 0, fm = 0;
       for (int j = 0; j < BINS / 32; ++j) {
@@ -187,21 +302,21 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, u6
         pc += sh.tot_count[b]; pm += sh.tot_mass[b];
       }
       const unsigned int any = __ballot_sync(0xffffffffu, found >= 0);
-      if (any && lane == __ffs(any) - 1) { sh.pick_bin = found; sh.pick_above_count = fc; sh.pick_above_mass = fm; }
+      if (lane == (any ? __ffs(any) - 1 : 0)) { sh.pick_bin = max(found, 0); sh.pick_above_count = fc; sh.pick_above_mass = fm; }
     }
     __syncthreads();
-    const uint32_t bin = sh.pick_bin;
+    const uint32_t bin = (uint32_t)sh.pick_bin;
     above_c = sh.pick_above_count; above_m = sh.pick_above_mass;
     const u64 cnt = sh.tot_count[bin], mass = sh.tot_mass[bin];
-    const uint32_t lo = k0 + (bin << shift), hi = lo + ((1u << shift) - 1u);
-    const uint32_t top = k1;
-    k0 = lo; k1 = min(hi, top);
+    const uint32_t low = k0 + (bin << shift);
+    k1 = min(low + ((1u << shift) - 1u), k1);
+    k0 = low;
     if (shift == 0 || cnt == 1) {
       Cut c;
-      c.k0 = k0; c.k1 = k1;
+      c.lo = key_value(k0); c.hi = key_value(k1);
       c.before = sh.below_count[bin]; c.here = sh.count[buf][bin];
       if (MASS) {
-        const u64 each = mass / cnt;                              // equal keys: equal masses
+        const u64 each = mass / cnt;                              // equal values: equal masses
         c.ties = (target - above_m + each - 1) / each;
         c.mass = above_m + c.ties * each;
       } else {
@@ -215,8 +330,60 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, u6
   }
 }
 
+// One pass over the slice for everything that needs every element: the untempered sum of exponentials, what the priority needs,
+// the tempered masses (per warp, MASS) and the octave counts (HIST).
+template <bool MASS, bool HIST, int PRI>
+__device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment seg, float m, float scale, const Weigher& w) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float z = 0, ent = 0, second = -INFINITY;
+  int at_max = 0;
+  u64 mass = 0;
+#pragma unroll 4
+  for (int i = seg.a + lane; i < seg.b; i += 32) {
+    const float x = xs[i], d = x - m, e = __expf(d);
+    z += e;
+    if (PRI == PRI_ENTROPY) ent += e * fmaxf(d, -1e4f);
+    if (PRI == PRI_MARGIN) { at_max += x == m; second = x < m ? fmaxf(second, x) : second; }
+    if (MASS) mass += w(x);
+    if (HIST) {
+      const int b = octave_bin(x, m, scale);
+      if (b < BINS - 1) atomicAdd(&sh.octaves_here[b], 1u);
+    }
+  }
+  const double zs = warp_sum((double)z);
+  if (lane == 0) sh.dred[0][warp] = zs;
+  if (PRI == PRI_ENTROPY) { const double v = warp_sum((double)ent); if (lane == 0) sh.dred[1][warp] = v; }
+  if (PRI == PRI_MARGIN) {
+    second = warp_max(second);
+    at_max = __reduce_add_sync(0xffffffffu, at_max);
+    if (lane == 0) { sh.fred[warp] = second; sh.ired[warp] = at_max; }
+  }
+  if (MASS) { mass = warp_sum(mass); if (lane == 0) sh.ured[warp] = mass; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double a = 0, b = 0;
+    float s = -INFINITY;
+    int k = 0;
+    u64 ms = 0;
+    for (int i = 0; i < WARPS; ++i) {
+      a += sh.dred[0][i];
+      if (PRI == PRI_ENTROPY) b += sh.dred[1][i];
+      if (PRI == PRI_MARGIN) { s = fmaxf(s, sh.fred[i]); k += sh.ired[i]; }
+      if (MASS) ms += sh.ured[i];
+    }
+    sh.z = a; sh.ent = b; sh.second = s; sh.at_max = k; sh.whole = ms;
+  }
+}
+
+template <bool MASS, bool HIST>
+__device__ __forceinline__ void whole_pass(int pri, Shared& sh, const float* xs, Segment seg, float m, float scale, const Weigher& w) {
+  if (pri == PRI_LOGP) whole_pass<MASS, HIST, PRI_LOGP>(sh, xs, seg, m, scale, w);
+  else if (pri == PRI_MARGIN) whole_pass<MASS, HIST, PRI_MARGIN>(sh, xs, seg, m, scale, w);
+  else whole_pass<MASS, HIST, PRI_ENTROPY>(sh, xs, seg, m, scale, w);
+}
+
 template <class T>
-__global__ void __launch_bounds__(THREADS) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
   float* xs = reinterpret_cast<float*>(smem_raw + ((sizeof(Shared) + 15) / 16) * 16);
@@ -257,6 +424,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleParams p) {
     }
   }
   xs += mis;
+  for (int i = tid; i < BINS; i += THREADS) sh.octaves_here[i] = 0;
+  for (int i = tid; i < TAB * COPIES; i += THREADS) sh.tab[i] = exp2((double)(i / COPIES) / TAB);
   mx = warp_max(mx);
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) { sh.fred[warp] = mx; sh.ired[warp] = bad; }
@@ -277,90 +446,78 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleParams p) {
     return;
   }
 
-  // ---- untempered sums
-  const Segment seg = split(0, n, WARPS, warp);
-  {
-    double z = 0, ent = 0;
-    float second = -INFINITY;
-    int at_max = 0, first_max = 0x7fffffff;
-    for (int i = seg.a + lane; i < seg.b; i += 32) {
-      const float x = xs[i], d = fmaxf(x - m, -1e4f), e = __expf(d);
-      z += e;
-      ent += (double)(e * d);
-      if (x == m) { ++at_max; first_max = min(first_max, first + i); }
-      else second = fmaxf(second, x);
-    }
-    z = warp_sum(z); ent = warp_sum(ent); second = warp_max(second);
-    at_max = __reduce_add_sync(0xffffffffu, at_max);
-    first_max = __reduce_min_sync(0xffffffffu, first_max);
-    if (tid == 0) { sh.at_max = 0; sh.first_max = 0x7fffffff; }
-    __syncthreads();
-    if (lane == 0) {
-      sh.dred[0][warp] = z; sh.dred[1][warp] = ent; sh.fred[warp] = second;
-      atomicAdd(&sh.at_max, at_max); atomicMin(&sh.first_max, first_max);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      double a = 0, b = 0;
-      float s = -INFINITY;
-      for (int i = 0; i < WARPS; ++i) { a += sh.dred[0][i]; b += sh.dred[1][i]; s = fmaxf(s, sh.fred[i]); }
-      sh.z = a; sh.ent = b; sh.second = s;
-    }
-  }
-
-  // ---- tempered: the kept set, its mass
-  const float t_f = p.t_row ? p.t_row[row] : 1.f;
-  const double t_raw = p.t_row ? (double)t_f : p.temperature;
+  // ---- this row's parameters
+  const double t_raw = p.t_row ? (double)p.t_row[row] : p.temperature;
   const bool greedy = !(t_raw > 0);
   const double temp = fmin(fmax(t_raw, 1e-6), 1e6);
-  Weigher w;
-  w.m = (double)m; w.inv_t = 1.0 / temp; w.scale = (double)(1ull << p.scale_bits);
-  Cut cut;
-  cut.k0 = cut.k1 = 0; cut.ties = 1; cut.before = 0; cut.here = 0; cut.mass = 0;
-  uint32_t k_min = 0;
-  bool chosen_cut = false;
-  u64 my_mass = 0;
   const double min_p = p.m_row ? (double)p.m_row[row] : p.min_p;
-  int round = 0;
-  auto kept = [&](float x, int i, int last_tie) {
-    const uint32_t k = order_key(x);
-    return (k > cut.k1 || (k >= cut.k0 && i <= last_tie)) && k >= k_min;
-  };
-  int last_tie = 0x7fffffff;
-  if (!greedy) {
-    if (min_p > 0) k_min = order_key(__double2float_ru((double)m + temp * log(fmin(min_p, 1.0))));
-    const double top_p = p.p_row ? (double)p.p_row[row] : p.top_p;
-    const int top_k = p.k_row ? p.k_row[row] : p.top_k;
-    u64 whole = 0;
-    if (top_k > 0 && top_k < p.V) {
-      cut = find_cut<false>(sh, xs, n, w, (u64)top_k, top_p < 1.0, round);
-      whole = cut.mass;
-      chosen_cut = true;
-    } else if (top_p < 1.0) {
-      u64 s = 0;
-      for (int i = seg.a + lane; i < seg.b; i += 32) s += w(xs[i]);
-      s = warp_sum(s);
-      if (lane == 0) sh.ured[warp] = s;
-      __syncthreads();
-      if (tid == 0) { u64 a = 0; for (int i = 0; i < WARPS; ++i) a += sh.ured[i]; sh.mass = a; }
+  const double top_p = p.p_row ? (double)p.p_row[row] : p.top_p;
+  const int top_k = p.k_row ? p.k_row[row] : p.top_k;
+  const bool by_count = !greedy && top_k > 0 && top_k < p.V, by_mass = !greedy && top_p < 1.0, by_ratio = !greedy && min_p > 0;
+  const double unit = 1.0 / (double)(1ull << p.scale_bits), log2e_t = 1.4426950408889634 / temp;
+  const float scale = (float)(PER_OCTAVE * log2e_t);
+  Weigher w;
+  w.c = TAB * log2e_t;
+  w.mc = -(double)m * w.c;
+  w.magic = 1.5 * (double)(1ull << (52 - p.scale_bits));
+  w.least = __double2float_ru((double)m - (p.scale_bits + 1.5) / log2e_t);
+  w.tab = sh.tab + (lane & (COPIES - 1));
+
+  // ---- the pass over every element
+  const Segment seg = split(0, n, WARPS, warp);
+  if (greedy) whole_pass<false, false>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_count) whole_pass<false, true>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_mass) whole_pass<true, true>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_ratio) whole_pass<false, false>(p.priority, sh, xs, seg, m, scale, w);
+  else whole_pass<true, false>(p.priority, sh, xs, seg, m, scale, w);
+
+  // ---- the kept set and its mass
+  Cut cut;
+  cut.lo = cut.hi = -INFINITY; cut.ties = 1; cut.before = 0; cut.here = 0; cut.mass = 0;
+  float least = -INFINITY;
+  int last_tie = 0x7fffffff, round = 0;
+  auto kept = [&](float x, int i) { return x >= least && (x > cut.hi || (x >= cut.lo && i <= last_tie)); };
+  if (greedy) {
+    int at = 0x7fffffff;
+    for (int i = seg.a + lane; i < seg.b; i += 32)
+      if (xs[i] == m) { at = first + i; break; }
+    at = __reduce_min_sync(0xffffffffu, at);
+    __syncthreads();
+    if (lane == 0) sh.ired[warp] = at;
+    __syncthreads();
+    if (tid == 0) {
+      for (int i = 1; i < WARPS; ++i) at = min(at, sh.ired[i]);
+      sh.first_max = at;
+    }
+  } else if (by_count || by_mass || by_ratio) {
+    if (by_ratio) least = __double2float_ru((double)m + temp * log(fmin(min_p, 1.0)));
+    if (by_count || by_mass) {
       cluster.sync();
-      for (int r = 0; r < ranks; ++r) whole += cluster.map_shared_rank(&sh, r)->mass;
-      cluster.sync();                                              // sh.mass is written once more below
+      u64 whole = 0;
+      for (int r = 0; r < ranks; ++r) whole += cluster.map_shared_rank(&sh, r)->whole;
+      for (int i = tid; i < BINS; i += THREADS) {
+        unsigned int c = 0;
+        for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(&sh, r)->octaves_here[i];
+        sh.octaves[i] = c;
+      }
+      __syncthreads();
+      if (by_count) {
+        cut = find_cut<false>(sh, xs, n, w, m, scale, unit, p.V, (u64)top_k, by_mass, round);
+        whole = cut.mass;
+      }
+      if (by_mass) {
+        const double goal = ceil(fmax(top_p, 0.0) * (double)whole);
+        cut = find_cut<true>(sh, xs, n, w, m, scale, unit, p.V, max((u64)1, min(whole, (u64)goal)), true, round);
+      }
     }
-    if (top_p < 1.0) {
-      const double goal = ceil(fmax(top_p, 0.0) * (double)whole);
-      const u64 target = max((u64)1, min(whole, (u64)goal));
-      cut = find_cut<true>(sh, xs, n, w, target, true, round);
-      chosen_cut = true;
-    }
-    if (chosen_cut && cut.before + cut.here > cut.ties) {          // this CTA holds ties that are not kept
+    if (cut.before + cut.here > cut.ties) {                        // this CTA holds ties that are not kept
       if (cut.before >= cut.ties) {
         last_tie = -1;
       } else {
-        // the (ties - before)-th element of [k0, k1] in this slice
+        // the (ties - before)-th element of [lo, hi] in this slice
         const u64 want = cut.ties - cut.before;
         int c = 0;
-        for (int i = seg.a + lane; i < seg.b; i += 32) { const uint32_t k = order_key(xs[i]); c += k >= cut.k0 && k <= cut.k1; }
+        for (int i = seg.a + lane; i < seg.b; i += 32) c += xs[i] >= cut.lo && xs[i] <= cut.hi;
         c = __reduce_add_sync(0xffffffffu, c);
         if (lane == 0) sh.ired[warp] = c;
         __syncthreads();
@@ -369,8 +526,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleParams p) {
         if (run < want && run + sh.ired[warp] >= want) {
           for (int i0 = seg.a; i0 < seg.b; i0 += 32) {
             const int i = i0 + lane;
-            const uint32_t k = i < seg.b ? order_key(xs[i]) : 0;
-            const unsigned int hit = __ballot_sync(0xffffffffu, i < seg.b && k >= cut.k0 && k <= cut.k1);
+            const unsigned int hit = __ballot_sync(0xffffffffu, i < seg.b && xs[i] >= cut.lo && xs[i] <= cut.hi);
             const int cnt = __popc(hit);
             if (run + cnt >= want) {
               if ((hit >> lane & 1) && run + __popc(hit & ((2u << lane) - 1)) == want) sh.idx_star = i;
@@ -385,17 +541,20 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleParams p) {
     }
     u64 s = 0;
     for (int i = seg.a + lane; i < seg.b; i += 32)
-      if (kept(xs[i], i, last_tie)) s += w(xs[i]);
+      if (kept(xs[i], i)) s += w(xs[i]);
     s = warp_sum(s);
+    __syncthreads();
     if (lane == 0) sh.ured[warp] = s;
     __syncthreads();
     if (tid == 0) { u64 a = 0; for (int i = 0; i < WARPS; ++i) a += sh.ured[i]; sh.mass = a; }
+  } else if (tid == 0) {
+    sh.mass = sh.whole;
   }
   cluster.sync();
 
   // ---- totals of the cluster, the draw
   double z = 0, ent = 0;
-  u64 total = 0, base = 0;
+  u64 total = 0, base = 0, my_mass = 0;
   float second = -INFINITY;
   int at_max = 0, first_max = 0x7fffffff;
   for (int r = 0; r < ranks; ++r) {
@@ -433,7 +592,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleParams p) {
       const Segment part = split(big.a, big.b, WARPS, warp);
       u64 s = 0;
       for (int i = part.a + lane; i < part.b; i += 32)
-        if (kept(xs[i], i, last_tie)) s += w(xs[i]);
+        if (kept(xs[i], i)) s += w(xs[i]);
       s = warp_sum(s);
       __syncthreads();
       if (lane == 0) sh.ured[warp] = s;
@@ -442,7 +601,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleParams p) {
       if (goal >= run && goal < run + s) {
         for (int i0 = part.a; i0 < part.b; i0 += 32) {
           const int i = i0 + lane;
-          const u64 wi = i < part.b && kept(xs[i], i, last_tie) ? w(xs[i]) : 0;
+          const u64 wi = i < part.b && kept(xs[i], i) ? w(xs[i]) : 0;
           const u64 inc = run + warp_scan(wi, lane);
           const unsigned int hit = __ballot_sync(0xffffffffu, inc > goal);
           if (hit) {
