@@ -85,6 +85,17 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+// the maximum, NaN if there is one
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
 __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {      // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -97,7 +108,6 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {      // inclusive
 struct Shared {
   // what this CTA tells the others; every exchange has fields of its own, so nothing is overwritten while a peer reads it
   float m;
-  int bad;
   double z, ent;
   float second;
   int at_max, first_max;
@@ -110,7 +120,7 @@ struct Shared {
   // this CTA alone
   float fred[WARPS];
   double dred[2][WARPS];
-  u64 ured[WARPS];
+  u64 ured[WARPS], above[WARPS];
   int ired[WARPS];
   u64 tot_mass[BINS];
   unsigned int tot_count[BINS];
@@ -125,29 +135,30 @@ struct Shared {
 
 // exp((x - m) / T) as a mass of 2^S units, rounded to nearest.  Table-driven (Tang's scheme, from the mathematics): with
 // z = 32 log2(e) (x - m) / T = n + r, |r| <= 1/2, it is 2^(n >> 5) 2^((n & 31) / 32) 2^(r / 32); the last factor by its Taylor series to
-// the fifth order (|r| ln2 / 32 <= 0.0109: truncated by 2.3e-15).  The table holds 16 copies of its 32 values, one per pair of
+// the fourth order (|r| ln2 / 32 <= 0.0109: truncated by 1.3e-12).  The table holds 16 copies of its 32 values, one per pair of
 // banks, so that the lookups of a half warp never collide.  Half the FP64 instructions of the library's exp, and no conversion back:
 // adding 1.5 2^(52 - S) leaves the rounded mass in the low bits.
 struct Weigher {
   double c, mc, magic;                      // z = x c + mc
   float least;                              // below it the mass rounds to 0
   const double* tab;                        // this thread's copy
-  __device__ __forceinline__ u64 operator()(float x) const {
+  __device__ __forceinline__ u64 operator()(float x) const { return raw(x) - (u64)__double_as_longlong(magic); }
+  // with the bits of `magic` still in it: for sums of many, from which they are taken once
+  __device__ __forceinline__ u64 raw(float x) const {
     constexpr double SHIFT = 6755399441055744.0;                   // 1.5 2^52: the sum's low word is the rounded integer
     constexpr double L = 0.02166084939249829;                      // ln2 / 32
     const double z = fma((double)x, c, mc);
     const double t = z + SHIFT;
     const int n = __double2loint(t);
     const double r = z - (t - SHIFT);
-    double q = L * L * L * L * L / 120;
-    q = fma(q, r, L * L * L * L / 24);
+    double q = L * L * L * L / 24;
     q = fma(q, r, L * L * L / 6);
     q = fma(q, r, L * L / 2);
     q = fma(q, r, L);
     q = fma(q, r, 1.0);
     const double v = q * tab[(n & (TAB - 1)) * COPIES];
     const double f = __hiloint2double(__double2hiint(v) + ((n >> 5) << 20), __double2loint(v)) + magic;
-    return x >= least ? (u64)(__double_as_longlong(f) - __double_as_longlong(magic)) : 0;
+    return (u64)__double_as_longlong(x >= least ? f : magic);
   }
 };
 
@@ -160,6 +171,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 struct Cut {
   float lo, hi;                             // values above hi are kept; of those in [lo, hi] the first `ties` by index
   u64 ties, mass;                           // mass: of everything kept
+  float first_hi;                           // the first round's upper end: each warp's mass above it is in Shared::above
   u64 before;                               // elements of [lo, hi] in CTAs with a lower rank
   u64 here;                                 // ... and in this one
 };
@@ -249,12 +261,13 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
 // elements of the range and, in the first round, those above it cost more than a comparison.
 template <bool MASS>
 __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, double unit, int V, u64 target,
-                        bool want_mass, int& round) {
+                        int& round) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Segment seg = split(0, n, WARPS, warp);
   first_range<MASS>(sh, m, scale, unit, V, target);
   uint32_t k0 = sh.range[0], k1 = sh.range[1];
+  const float first_hi = key_value(k1);
   u64 above_c = 0, above_m = 0;
   bool fresh = true;                                               // what lies above the range is not known yet
   for (;;) {
@@ -272,17 +285,18 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
       const float x = xs[i];
       if (x >= lo) {
         if (x > hi) {
-          if (fresh) { ++ac; if (MASS || want_mass) am += w(x); }
+          if (fresh) { ++ac; am += w(x); }
         } else {
           const uint32_t bin = (order_key(x) - k0) >> shift;
           atomicAdd(&sh.count[buf][bin], 1u);
-          if (MASS || want_mass) atomicAdd(&sh.hmass[buf][bin], w(x));
+          atomicAdd(&sh.hmass[buf][bin], w(x));
         }
       }
     }
     if (fresh) {
       ac = __reduce_add_sync(0xffffffffu, ac);
       am = warp_sum(am);
+      if (lane == 0) sh.above[warp] = am;
       if (lane == 0 && ac) { atomicAdd(&sh.above_count[buf], ac); atomicAdd(&sh.above_mass[buf], am); }
     }
     cluster.sync();
@@ -313,7 +327,7 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
     k0 = low;
     if (shift == 0 || cnt == 1) {
       Cut c;
-      c.lo = key_value(k0); c.hi = key_value(k1);
+      c.lo = key_value(k0); c.hi = key_value(k1); c.first_hi = first_hi;
       c.before = sh.below_count[bin]; c.here = sh.count[buf][bin];
       if (MASS) {
         const u64 each = mass / cnt;                              // equal values: equal masses
@@ -338,13 +352,14 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
   float z = 0, ent = 0, second = -INFINITY;
   int at_max = 0;
   u64 mass = 0;
+  int count = 0;
 #pragma unroll 4
   for (int i = seg.a + lane; i < seg.b; i += 32) {
     const float x = xs[i], d = x - m, e = __expf(d);
     z += e;
     if (PRI == PRI_ENTROPY) ent += e * fmaxf(d, -1e4f);
     if (PRI == PRI_MARGIN) { at_max += x == m; second = x < m ? fmaxf(second, x) : second; }
-    if (MASS) mass += w(x);
+    if (MASS) { mass += w.raw(x); ++count; }
     if (HIST) {
       const int b = octave_bin(x, m, scale);
       if (b < BINS - 1) atomicAdd(&sh.octaves_here[b], 1u);
@@ -358,7 +373,7 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
     at_max = __reduce_add_sync(0xffffffffu, at_max);
     if (lane == 0) { sh.fred[warp] = second; sh.ired[warp] = at_max; }
   }
-  if (MASS) { mass = warp_sum(mass); if (lane == 0) sh.ured[warp] = mass; }
+  if (MASS) { mass = warp_sum(mass - (u64)count * (u64)__double_as_longlong(w.magic)); if (lane == 0) sh.ured[warp] = mass; }
   __syncthreads();
   if (threadIdx.x == 0) {
     double a = 0, b = 0;
@@ -398,49 +413,66 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
   // ---- the slice into shared memory, its maximum
   const T* src = reinterpret_cast<const T*>(p.logits) + outer * p.s_outer + (row - outer * p.inner) * p.s_inner + first;
   const float* bias = p.bias ? p.bias + outer * p.V + first : nullptr;
-  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int VEC = 16 / (int)sizeof(T), UNROLL = sizeof(T) == 4 ? 4 : 2;
   const int mis = (int)((reinterpret_cast<uintptr_t>(src) / sizeof(T)) % VEC);      // keeps 16-byte pieces aligned on both sides
+  const int v0 = mis ? 1 : 0, v1 = (mis + n) / VEC;                                 // the whole pieces
+  const bool bias_vec = bias && ((reinterpret_cast<uintptr_t>(bias) / sizeof(float) + VEC - mis) & 3) == 0;
   float mx = -INFINITY;
-  int bad = 0;
-  for (int v = tid; v * VEC < mis + n; v += THREADS) {
-    const int i0 = v * VEC - mis;
-    T e[VEC];
-    if (i0 >= 0 && i0 + VEC <= n) {
-      *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(src + i0);
-    } else {
+  for (int v = v0 + tid; v < v1; v += THREADS * UNROLL) {
+    uint4 raw[UNROLL];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (i0 + j >= 0 && i0 + j < n) e[j] = src[i0 + j];
-    }
+    for (int k = 0; k < UNROLL; ++k)
+      if (v + k * THREADS < v1) raw[k] = __ldcs(reinterpret_cast<const uint4*>(src - mis) + v + k * THREADS);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int i = i0 + j;
-      if (i >= 0 && i < n) {
-        const float x = bias ? to_f32(e[j]) + bias[i] + 0.f : to_f32(e[j]) + 0.f;      // + 0: no negative zero
-        bad |= !(x < INFINITY);                                    // NaN or +inf
-        mx = fmaxf(mx, x);
-        xs[mis + i] = x;
+    for (int k = 0; k < UNROLL; ++k) {
+      const int at = (v + k * THREADS) * VEC;
+      if (v + k * THREADS < v1) {
+        const T* e = reinterpret_cast<const T*>(&raw[k]);
+        float x[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[j] = to_f32(e[j]);
+        if (bias_vec) {
+#pragma unroll
+          for (int j = 0; j < VEC; j += 4) {
+            const float4 t = __ldg(reinterpret_cast<const float4*>(bias + at - mis + j));
+            x[j] += t.x; x[j + 1] += t.y; x[j + 2] += t.z; x[j + 3] += t.w;
+          }
+        } else if (bias) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) x[j] += __ldg(bias + at - mis + j);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) { x[j] += 0.f; mx = max_nan(mx, x[j]); }       // + 0: no negative zero
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4*>(xs + at + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
       }
+    }
+  }
+  if (tid < 2 * VEC) {                                             // the ragged ends, an element each
+    const int head = v0 ? min(n, VEC - mis) : 0, tail = max(head, v1 * VEC - mis);
+    const int i = tid < VEC ? tid : tail + tid - VEC;
+    if (tid < VEC ? i < head : i < n) {
+      float x = to_f32(src[i]);
+      if (bias) x += bias[i];
+      x += 0.f;
+      mx = max_nan(mx, x);
+      xs[mis + i] = x;
     }
   }
   xs += mis;
   for (int i = tid; i < BINS; i += THREADS) sh.octaves_here[i] = 0;
   for (int i = tid; i < TAB * COPIES; i += THREADS) sh.tab[i] = exp2((double)(i / COPIES) / TAB);
-  mx = warp_max(mx);
-  bad = __any_sync(0xffffffffu, bad);
-  if (lane == 0) { sh.fred[warp] = mx; sh.ired[warp] = bad; }
+  mx = warp_max_nan(mx);
+  if (lane == 0) sh.fred[warp] = mx;
   __syncthreads();
   if (tid == 0) {
-    float m = -INFINITY;
-    int b = 0;
-    for (int i = 0; i < WARPS; ++i) { m = fmaxf(m, sh.fred[i]); b |= sh.ired[i]; }
-    sh.m = m; sh.bad = b;
+    for (int i = 1; i < WARPS; ++i) mx = max_nan(mx, sh.fred[i]);
+    sh.m = mx;
   }
   cluster.sync();
   float m = -INFINITY;
-  bad = 0;
-  for (int r = 0; r < ranks; ++r) { const Shared* q = cluster.map_shared_rank(&sh, r); m = fmaxf(m, q->m); bad |= q->bad; }
-  if (bad || m == -INFINITY) {                                     // the same in every CTA of the cluster
+  for (int r = 0; r < ranks; ++r) m = max_nan(m, cluster.map_shared_rank(&sh, r)->m);
+  if (!(m > -INFINITY && m < INFINITY)) {                          // NaN, +inf or nothing above -inf: the same in every CTA of the cluster
     if (me == 0 && tid == 0) { p.tokens[row] = -1; p.logp[row] = NAN; if (p.priority != PRI_LOGP) p.prio[row] = NAN; }
     cluster.sync();
     return;
@@ -473,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
 
   // ---- the kept set and its mass
   Cut cut;
-  cut.lo = cut.hi = -INFINITY; cut.ties = 1; cut.before = 0; cut.here = 0; cut.mass = 0;
+  cut.lo = cut.hi = cut.first_hi = -INFINITY; cut.ties = 1; cut.before = 0; cut.here = 0; cut.mass = 0;
   float least = -INFINITY;
   int last_tie = 0x7fffffff, round = 0;
   auto kept = [&](float x, int i) { return x >= least && (x > cut.hi || (x >= cut.lo && i <= last_tie)); };
@@ -502,12 +534,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
       }
       __syncthreads();
       if (by_count) {
-        cut = find_cut<false>(sh, xs, n, w, m, scale, unit, p.V, (u64)top_k, by_mass, round);
+        cut = find_cut<false>(sh, xs, n, w, m, scale, unit, p.V, (u64)top_k, round);
         whole = cut.mass;
       }
       if (by_mass) {
         const double goal = ceil(fmax(top_p, 0.0) * (double)whole);
-        cut = find_cut<true>(sh, xs, n, w, m, scale, unit, p.V, max((u64)1, min(whole, (u64)goal)), true, round);
+        cut = find_cut<true>(sh, xs, n, w, m, scale, unit, p.V, max((u64)1, min(whole, (u64)goal)), round);
       }
     }
     if (cut.before + cut.here > cut.ties) {                        // this CTA holds ties that are not kept
@@ -539,10 +571,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
         last_tie = sh.idx_star;
       }
     }
+    // what lies above the search's first range is summed already, unless min_p cuts into it
+    const bool summed = (by_count || by_mass) && least <= cut.first_hi;
+    const float up_to = summed ? cut.first_hi : INFINITY;
     u64 s = 0;
     for (int i = seg.a + lane; i < seg.b; i += 32)
-      if (kept(xs[i], i)) s += w(xs[i]);
-    s = warp_sum(s);
+      if (xs[i] <= up_to && kept(xs[i], i)) s += w(xs[i]);
+    s = warp_sum(s) + (summed ? sh.above[warp] : 0);
     __syncthreads();
     if (lane == 0) sh.ured[warp] = s;
     __syncthreads();
