@@ -32,9 +32,10 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 384;
 constexpr int WARPS = THREADS / 32;
-constexpr int BINS = 256;
+constexpr int OCTAVES = 256;                 // bins of the octave counts
+constexpr int BINS = 128;                    // of a round of the search
 constexpr int TAB = 32, COPIES = 16;
 constexpr int SLICE_MAX = 49152;            // elements of a slice at most (192 KB)
 constexpr int SLICE_GOOD = 16384;           // a slice up to which three CTAs fit an SM
@@ -85,6 +86,11 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // the maximum, NaN if there is one
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -105,6 +111,17 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {      // inclusive
   return v;
 }
 
+// 2^(j / 32)
+__constant__ double ROOTS[TAB] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+
 struct Shared {
   // what this CTA tells the others; every exchange has fields of its own, so nothing is overwritten while a peer reads it
   float m;
@@ -112,7 +129,7 @@ struct Shared {
   float second;
   int at_max, first_max;
   u64 whole, mass;                          // of the slice; of what is kept of it
-  unsigned int octaves_here[BINS];
+  unsigned int octaves_here[OCTAVES];
   unsigned int count[2][BINS];              // histograms of the threshold search, alternating between rounds
   u64 hmass[2][BINS];
   unsigned int above_count[2];
@@ -125,12 +142,17 @@ struct Shared {
   u64 tot_mass[BINS];
   unsigned int tot_count[BINS];
   unsigned int below_count[BINS];           // of the CTAs with a lower rank
-  unsigned int octaves[BINS];               // of all CTAs
+  unsigned int octaves[OCTAVES];              // of all CTAs
   uint32_t range[2];
   u64 tot_above_count, tot_above_mass;
   int pick_bin, idx_star;
   u64 pick_above_count, pick_above_mass;
   double tab[TAB * COPIES];
+  // this row's parameters, and at the end its answer but for the token
+  double temp, min_p, top_p, log2e_t, cut;
+  float scale, logz, pr;
+  int top_k, greedy;
+  u64 goal, base;
 };
 
 // exp((x - m) / T) as a mass of 2^S units, rounded to nearest.  Table-driven (Tang's scheme, from the mathematics): with
@@ -140,16 +162,16 @@ struct Shared {
 // adding 1.5 2^(52 - S) leaves the rounded mass in the low bits.
 struct Weigher {
   double c, mc, magic;                      // z = x c + mc
-  float least;                              // below it the mass rounds to 0
+  float least;                              // its mass rounds to 0, as that of everything below
   const double* tab;                        // this thread's copy
   __device__ __forceinline__ u64 operator()(float x) const { return raw(x) - (u64)__double_as_longlong(magic); }
   // with the bits of `magic` still in it: for sums of many, from which they are taken once
   __device__ __forceinline__ u64 raw(float x) const {
     constexpr double SHIFT = 6755399441055744.0;                   // 1.5 2^52: the sum's low word is the rounded integer
     constexpr double L = 0.02166084939249829;                      // ln2 / 32
-    const double z = fma((double)x, c, mc);
+    const double z = fma((double)fmaxf(x, least), c, mc);
     const double t = z + SHIFT;
-    const int n = __double2loint(t);
+    const int n = max(__double2loint(t), -1000 * TAB);
     const double r = z - (t - SHIFT);
     double q = L * L * L * L / 24;
     q = fma(q, r, L * L * L / 6);
@@ -157,8 +179,7 @@ struct Weigher {
     q = fma(q, r, L);
     q = fma(q, r, 1.0);
     const double v = q * tab[(n & (TAB - 1)) * COPIES];
-    const double f = __hiloint2double(__double2hiint(v) + ((n >> 5) << 20), __double2loint(v)) + magic;
-    return (u64)__double_as_longlong(x >= least ? f : magic);
+    return (u64)__double_as_longlong(__hiloint2double(__double2hiint(v) + (n & ~(TAB - 1)) * (1 << 15), __double2loint(v)) + magic);
   }
 };
 
@@ -187,7 +208,7 @@ __device__ __forceinline__ Segment split(int a, int b, int parts, int i) {      
 // not counted.  The rounding is monotone in x, so bins are ranges of the order, and an element's mass is known within 9 %.
 constexpr float PER_OCTAVE = 8.f;
 __device__ __forceinline__ int octave_bin(float x, float m, float scale) {
-  return __float_as_int(fminf((m - x) * scale, (float)(BINS - 1)) + 8388608.f) - 0x4b000000;
+  return __float_as_int(fminf((m - x) * scale, (float)(OCTAVES - 1)) + 8388608.f) - 0x4b000000;
 }
 
 // Sums the counts of all CTAs (thread i: bin i), and the running totals of the elements above.
@@ -220,7 +241,7 @@ template <bool MASS>
 __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, double unit, int V, u64 target) {
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
-    constexpr int EACH = BINS / 32;
+    constexpr int EACH = OCTAVES / 32;
     double lo = 0, hi = 0;
     for (int j = 0; j < EACH; ++j) {
       const int b = lane * EACH + j;
@@ -236,20 +257,20 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
     }
     slo -= lo; shi -= hi;
     const double goal = MASS ? (double)target * unit : (double)target, slack = MASS ? (double)V * unit : 0.0;
-    int first = BINS - 1, last = BINS - 1;
+    int first = OCTAVES - 1, last = OCTAVES - 1;
     for (int j = 0; j < EACH; ++j) {
       const int b = lane * EACH + j;
       const double c = (double)sh.octaves[b];
       slo += MASS ? c * exp2f(-(b + 0.5f) / PER_OCTAVE) : c;
       shi += MASS ? c * exp2f(-fmaxf(b - 0.5f, 0.f) / PER_OCTAVE) : c;
-      if (first == BINS - 1 && (MASS ? shi * 1.0001 + slack : shi) >= goal) first = b;
-      if (last == BINS - 1 && (MASS ? slo * 0.9999 - slack : slo) >= goal) last = b;
+      if (first == OCTAVES - 1 && (MASS ? shi * 1.0001 + slack : shi) >= goal) first = b;
+      if (last == OCTAVES - 1 && (MASS ? slo * 0.9999 - slack : slo) >= goal) last = b;
     }
     first = __reduce_min_sync(0xffffffffu, first);
     last = __reduce_min_sync(0xffffffffu, last);
     if (lane == 0) {
       const double near = fmax(first - 0.5, 0.0) / scale, far = (last + 0.5) / scale, eps = fabs((double)m) * 1e-6;
-      sh.range[0] = last == BINS - 1 ? 0u : order_key(__double2float_rd((double)m - far * (1 + 1e-5) - eps) + 0.f);
+      sh.range[0] = last == OCTAVES - 1 ? 0u : order_key(__double2float_rd((double)m - far * (1 + 1e-5) - eps) + 0.f);
       sh.range[1] = first == 0 ? 0xffffffffu : order_key(__double2float_ru((double)m - near * (1 - 1e-5) + eps) + 0.f);
     }
   }
@@ -260,12 +281,11 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
 // `target`: 256-way search over the order keys from the range above; a pass over the slice and a cluster barrier per round.  Only
 // elements of the range and, in the first round, those above it cost more than a comparison.
 template <bool MASS>
-__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, double unit, int V, u64 target,
-                        int& round) {
+__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, int bits, int V, u64 target, int& round) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Segment seg = split(0, n, WARPS, warp);
-  first_range<MASS>(sh, m, scale, unit, V, target);
+  first_range<MASS>(sh, m, scale, 1.0 / (double)(1ull << bits), V, target);
   uint32_t k0 = sh.range[0], k1 = sh.range[1];
   const float first_hi = key_value(k1);
   u64 above_c = 0, above_m = 0;
@@ -352,22 +372,27 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
   float z = 0, ent = 0, second = -INFINITY;
   int at_max = 0;
   u64 mass = 0;
-  int count = 0;
-#pragma unroll 4
-  for (int i = seg.a + lane; i < seg.b; i += 32) {
-    const float x = xs[i], d = x - m, e = __expf(d);
+  auto one = [&](float x) {
+    const float y = (x - m) * 1.44269504f, e = ex2(y);
     z += e;
-    if (PRI == PRI_ENTROPY) ent += e * fmaxf(d, -1e4f);
+    if (PRI == PRI_ENTROPY) ent = fmaf(e, fmaxf(y, -1e4f), ent);
     if (PRI == PRI_MARGIN) { at_max += x == m; second = x < m ? fmaxf(second, x) : second; }
-    if (MASS) { mass += w.raw(x); ++count; }
+    if (MASS) mass += w.raw(x);
     if (HIST) {
       const int b = octave_bin(x, m, scale);
-      if (b < BINS - 1) atomicAdd(&sh.octaves_here[b], 1u);
+      if (b < OCTAVES - 1) atomicAdd(&sh.octaves_here[b], 1u);
     }
+  };
+  int i = seg.a + lane;
+  for (; i + 96 < seg.b; i += 128) {
+    const float x0 = xs[i], x1 = xs[i + 32], x2 = xs[i + 64], x3 = xs[i + 96];
+    one(x0); one(x1); one(x2); one(x3);
   }
+  for (; i < seg.b; i += 32) one(xs[i]);
+  const int count = max(0, (seg.b - seg.a - lane + 31) >> 5);
   const double zs = warp_sum((double)z);
   if (lane == 0) sh.dred[0][warp] = zs;
-  if (PRI == PRI_ENTROPY) { const double v = warp_sum((double)ent); if (lane == 0) sh.dred[1][warp] = v; }
+  if (PRI == PRI_ENTROPY) { const double v = warp_sum((double)ent) * 0.6931471805599453; if (lane == 0) sh.dred[1][warp] = v; }
   if (PRI == PRI_MARGIN) {
     second = warp_max(second);
     at_max = __reduce_add_sync(0xffffffffu, at_max);
@@ -397,16 +422,22 @@ __device__ __forceinline__ void whole_pass(int pri, Shared& sh, const float* xs,
   else whole_pass<MASS, HIST, PRI_ENTROPY>(sh, xs, seg, m, scale, w);
 }
 
+__device__ __forceinline__ unsigned int cluster_id() {
+  unsigned int r;
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+  return r;
+}
+
 template <class T>
-__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
   float* xs = reinterpret_cast<float*>(smem_raw + ((sizeof(Shared) + 15) / 16) * 16);
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
-  const long long row = blockIdx.x / ranks;
+  const unsigned int row = cluster_id();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const long long outer = row / p.inner;
+  const long long outer = row / (unsigned int)p.inner;
   const int first = me * p.slice;
   const int n = max(0, min(p.slice, p.V - first));
 
@@ -417,6 +448,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
   const int mis = (int)((reinterpret_cast<uintptr_t>(src) / sizeof(T)) % VEC);      // keeps 16-byte pieces aligned on both sides
   const int v0 = mis ? 1 : 0, v1 = (mis + n) / VEC;                                 // the whole pieces
   const bool bias_vec = bias && ((reinterpret_cast<uintptr_t>(bias) / sizeof(float) + VEC - mis) & 3) == 0;
+  if (tid == 0) {
+    const double t = p.t_row ? (double)p.t_row[row] : p.temperature;
+    sh.greedy = !(t > 0);
+    sh.temp = fmin(fmax(t, 1e-6), 1e6);
+    sh.min_p = p.m_row ? (double)p.m_row[row] : p.min_p;
+    sh.top_p = p.p_row ? (double)p.p_row[row] : p.top_p;
+    sh.top_k = p.k_row ? p.k_row[row] : p.top_k;
+    sh.log2e_t = 1.4426950408889634 / sh.temp;
+    sh.cut = (p.scale_bits + 1.5) / sh.log2e_t;
+    sh.scale = (float)(PER_OCTAVE * sh.log2e_t);
+  }
   float mx = -INFINITY;
   for (int v = v0 + tid; v < v1; v += THREADS * UNROLL) {
     uint4 raw[UNROLL];
@@ -460,8 +502,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
     }
   }
   xs += mis;
-  for (int i = tid; i < BINS; i += THREADS) sh.octaves_here[i] = 0;
-  for (int i = tid; i < TAB * COPIES; i += THREADS) sh.tab[i] = exp2((double)(i / COPIES) / TAB);
+  for (int i = tid; i < OCTAVES; i += THREADS) sh.octaves_here[i] = 0;
+  for (int i = tid; i < TAB * COPIES; i += THREADS) sh.tab[i] = ROOTS[i / COPIES];
   mx = warp_max_nan(mx);
   if (lane == 0) sh.fred[warp] = mx;
   __syncthreads();
@@ -470,8 +512,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
     sh.m = mx;
   }
   cluster.sync();
-  float m = -INFINITY;
-  for (int r = 0; r < ranks; ++r) m = max_nan(m, cluster.map_shared_rank(&sh, r)->m);
+  const float m = warp_max_nan(lane < ranks ? cluster.map_shared_rank(&sh, lane)->m : -INFINITY);
   if (!(m > -INFINITY && m < INFINITY)) {                          // NaN, +inf or nothing above -inf: the same in every CTA of the cluster
     if (me == 0 && tid == 0) { p.tokens[row] = -1; p.logp[row] = NAN; if (p.priority != PRI_LOGP) p.prio[row] = NAN; }
     cluster.sync();
@@ -479,20 +520,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
   }
 
   // ---- this row's parameters
-  const double t_raw = p.t_row ? (double)p.t_row[row] : p.temperature;
-  const bool greedy = !(t_raw > 0);
-  const double temp = fmin(fmax(t_raw, 1e-6), 1e6);
-  const double min_p = p.m_row ? (double)p.m_row[row] : p.min_p;
-  const double top_p = p.p_row ? (double)p.p_row[row] : p.top_p;
-  const int top_k = p.k_row ? p.k_row[row] : p.top_k;
+  const bool greedy = sh.greedy;
+  const double min_p = sh.min_p, top_p = sh.top_p;
+  const int top_k = sh.top_k;
   const bool by_count = !greedy && top_k > 0 && top_k < p.V, by_mass = !greedy && top_p < 1.0, by_ratio = !greedy && min_p > 0;
-  const double unit = 1.0 / (double)(1ull << p.scale_bits), log2e_t = 1.4426950408889634 / temp;
-  const float scale = (float)(PER_OCTAVE * log2e_t);
+  const float scale = sh.scale;
   Weigher w;
-  w.c = TAB * log2e_t;
+  w.c = TAB * sh.log2e_t;
   w.mc = -(double)m * w.c;
-  w.magic = 1.5 * (double)(1ull << (52 - p.scale_bits));
-  w.least = __double2float_ru((double)m - (p.scale_bits + 1.5) / log2e_t);
+  w.magic = __hiloint2double(0x3ff80000 + ((52 - p.scale_bits) << 20), 0);        // 1.5 2^(52 - S)
+  w.least = __double2float_rd((double)m - sh.cut);
   w.tab = sh.tab + (lane & (COPIES - 1));
 
   // ---- the pass over every element
@@ -522,24 +559,24 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
       sh.first_max = at;
     }
   } else if (by_count || by_mass || by_ratio) {
-    if (by_ratio) least = __double2float_ru((double)m + temp * log(fmin(min_p, 1.0)));
+    if (by_ratio) least = __double2float_ru((double)m + sh.temp * log(fmin(min_p, 1.0)));
     if (by_count || by_mass) {
       cluster.sync();
       u64 whole = 0;
       for (int r = 0; r < ranks; ++r) whole += cluster.map_shared_rank(&sh, r)->whole;
-      for (int i = tid; i < BINS; i += THREADS) {
+      for (int i = tid; i < OCTAVES; i += THREADS) {
         unsigned int c = 0;
         for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(&sh, r)->octaves_here[i];
         sh.octaves[i] = c;
       }
       __syncthreads();
       if (by_count) {
-        cut = find_cut<false>(sh, xs, n, w, m, scale, unit, p.V, (u64)top_k, round);
+        cut = find_cut<false>(sh, xs, n, w, m, scale, p.scale_bits, p.V, (u64)top_k, round);
         whole = cut.mass;
       }
       if (by_mass) {
         const double goal = ceil(fmax(top_p, 0.0) * (double)whole);
-        cut = find_cut<true>(sh, xs, n, w, m, scale, unit, p.V, max((u64)1, min(whole, (u64)goal)), round);
+        cut = find_cut<true>(sh, xs, n, w, m, scale, p.scale_bits, p.V, max((u64)1, min(whole, (u64)goal)), round);
       }
     }
     if (cut.before + cut.here > cut.ties) {                        // this CTA holds ties that are not kept
@@ -588,38 +625,45 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
   cluster.sync();
 
   // ---- totals of the cluster, the draw
-  double z = 0, ent = 0;
-  u64 total = 0, base = 0, my_mass = 0;
-  float second = -INFINITY;
-  int at_max = 0, first_max = 0x7fffffff;
-  for (int r = 0; r < ranks; ++r) {
-    const Shared* q = cluster.map_shared_rank(&sh, r);
-    z += q->z; ent += q->ent;
-    second = fmaxf(second, q->second);
-    at_max += q->at_max; first_max = min(first_max, q->first_max);
-    if (!greedy) {
-      if (r == me) { base = total; my_mass = q->mass; }
-      total += q->mass;
+  if (warp == 0) {
+    const Shared* q = cluster.map_shared_rank(&sh, lane < ranks ? lane : 0);
+    const bool in = lane < ranks;
+    const double z = warp_sum(in ? q->z : 0.0);
+    const u64 part = in && !greedy ? q->mass : 0, upto = warp_scan(part, lane);
+    const u64 total = __shfl_sync(0xffffffffu, upto, 31), base = __shfl_sync(0xffffffffu, upto - part, me);
+    const float logz = logf((float)z);
+    float pr = 0.f;
+    if (p.priority == PRI_MARGIN) {
+      const float second = warp_max(in ? q->second : -INFINITY);
+      const int at_max = __reduce_add_sync(0xffffffffu, in ? q->at_max : 0);
+      pr = at_max > 1 ? 0.f : (float)((1.0 - (double)__expf(second - m)) / z);
+    } else if (p.priority == PRI_ENTROPY) {
+      const double ent = warp_sum(in ? q->ent : 0.0);
+      pr = (float)(ent / z - (double)logz);
+    }
+    if (greedy) {
+      const int at = __reduce_min_sync(0xffffffffu, in ? q->first_max : 0x7fffffff);
+      if (me == 0 && lane == 0) {
+        p.tokens[row] = at;
+        p.logp[row] = -logz;
+        if (p.priority != PRI_LOGP) p.prio[row] = pr;
+      }
+    } else if (lane == 0) {
+      const double u = (double)p.u[row];
+      const u64 goal = u > 0 ? (u64)(fmin(u, 1.0) * (double)total) : 0;
+      sh.goal = min(goal, total - 1);
+      sh.base = base; sh.logz = logz; sh.pr = pr;
     }
   }
-  const float logz = logf((float)z);
-  auto answer = [&](long long tok, float x) {
-    const float lp = (x - m) - logz;
-    p.tokens[row] = tok;
-    p.logp[row] = lp;
-    if (p.priority == PRI_LOGP) return;
-    float pr;
-    if (p.priority == PRI_MARGIN) pr = at_max > 1 ? 0.f : (float)((1.0 - (double)__expf(second - m)) / z);
-    else pr = (float)(ent / z - (double)logz);
-    p.prio[row] = pr;
-  };
-  if (greedy) {
-    if (me == 0 && tid == 0) answer(first_max, m);
-  } else {
-    const double u = (double)p.u[row];
-    u64 goal = u > 0 ? (u64)(fmin(u, 1.0) * (double)total) : 0;
-    if (goal >= total) goal = total - 1;
-    if (goal >= base && goal < base + my_mass) {                   // the draw falls into this slice
+  __syncthreads();
+  if (!greedy) {
+    const u64 goal = sh.goal, base = sh.base;
+    auto answer = [&](int tok, float x) {
+      p.tokens[row] = tok;
+      p.logp[row] = (x - m) - sh.logz;
+      if (p.priority != PRI_LOGP) p.prio[row] = sh.pr;
+    };
+    if (goal >= base && goal < base + sh.mass) {                   // the draw falls into this slice
       u64 run = base;
       int own = 0;
       while (own < WARPS - 1 && run + sh.ured[own] <= goal) run += sh.ured[own++];
@@ -654,7 +698,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleParams p
 template <class T>
 int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t s) {
   const size_t smem = ((sizeof(Shared) + 15) / 16) * 16 + ((size_t)p.slice + 16) * sizeof(float);
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  constexpr size_t most = ((sizeof(Shared) + 15) / 16) * 16 + ((size_t)SLICE_MAX + 16) * sizeof(float);
+  static_assert(most <= 227 * 1024, "a slice has to fit the shared memory of an SM");
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
   if (e != cudaSuccess) return 1000 + (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned int)(rows * ranks));
