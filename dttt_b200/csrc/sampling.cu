@@ -26,6 +26,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace cg = cooperative_groups;
 
 namespace {
@@ -695,12 +697,24 @@ __global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p
   cluster.sync();                                                  // nobody leaves while a peer may still read its memory
 }
 
+// Raises a kernel's shared memory limit once per device (`ready`: a bit per device).
+template <class K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<u64>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (ready.load() >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) ready.fetch_or(1ull << dev);
+  return e;
+}
+
 template <class T>
 int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t s) {
   const size_t smem = ((sizeof(Shared) + 15) / 16) * 16 + ((size_t)p.slice + 16) * sizeof(float);
   constexpr size_t most = ((sizeof(Shared) + 15) / 16) * 16 + ((size_t)SLICE_MAX + 16) * sizeof(float);
   static_assert(most <= 227 * 1024, "a slice has to fit the shared memory of an SM");
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  static std::atomic<u64> ready{0};
+  cudaError_t e = allow_shared(sample_kernel<T>, (int)most, ready);
   if (e != cudaSuccess) return 1000 + (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned int)(rows * ranks));
@@ -845,7 +859,8 @@ extern "C" int dttt_unmask(const long long* ids, const void* known, const float*
   if (B <= 0 || C <= 0) return 0;
   if (C > UM_SLOTS_MAX) return -2;
   const size_t smem = (size_t)C * sizeof(uint32_t);
-  cudaError_t e = cudaFuncSetAttribute(unmask_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, UM_SLOTS_MAX * (int)sizeof(uint32_t));
+  static std::atomic<u64> ready{0};
+  cudaError_t e = allow_shared(unmask_kernel, UM_SLOTS_MAX * (int)sizeof(uint32_t), ready);
   if (e != cudaSuccess) return 1000 + (int)e;
   unmask_kernel<<<B, UM_THREADS, smem, stream>>>(ids, (const uint8_t*)known, held, tokens, logp, priority, quota, (const uint8_t*)allowed,
                                                  sure, use_sure, ids_out, (uint8_t*)known_out, held_out, (uint8_t*)where_out, C);

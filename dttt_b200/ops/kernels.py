@@ -796,33 +796,52 @@ SAMPLE_VOCAB_MAX = 8 * 49152           # a row's f32 slices in the shared memory
 UNMASK_SLOTS_MAX = 32768               # a row's order keys in the shared memory of one CTA
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
+
+
+def _launch(what, fn, device, *args):
+    """``fn(*args, stream)`` with the device of the tensors current and its current stream: the launch path of calls so short that
+    the host sets their pace (pointers go as integers, no stream object, no device switch where there is nothing to switch)."""
+    global LAUNCHES
+    if _current() == device.index:
+        rc = fn(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device.index))
+    if rc:
+        raise _lib.KernelError(f"{what} launch failed rc={rc}")
+    LAUNCHES += 1
+
+
 def sample(x, u, bias, temperature, top_k, top_p, min_p, priority):
     """``x [outer, inner, V]`` (contiguous along V, any strides of the rows), ``u [outer, inner]``, ``bias [outer, V]`` or None; a
     parameter is a number or a contiguous tensor ``[outer, inner]`` (f32; int32 for ``top_k``).  ``(tokens, logp, priority)``
     ``[outer, inner]``; ``priority`` 0 logp (the same tensor) | 1 margin | 2 entropy."""
     outer, inner, V = x.shape
-    tokens = torch.empty(outer, inner, dtype=torch.int64, device=x.device)
-    logp = torch.empty(outer, inner, dtype=torch.float32, device=x.device)
-    prio = torch.empty_like(logp) if priority else None
-    if tokens.numel():
-        num = lambda p, off: (off, p) if torch.is_tensor(p) else (p, None)
-        (t, t_row), (k, k_row), (p, p_row), (m, m_row) = num(temperature, 1.0), num(top_k, 0), num(top_p, 1.0), num(min_p, 0.0)
-        with torch.cuda.device(x.device):
-            _check(_lib.lib().dttt_sample(_p(x), _LOGIT_TYPES[x.dtype], outer * inner, inner, x.stride(0), x.stride(1), V, _p(u), _p(bias),
-                                          float(t), _p(t_row), int(k), _p(k_row), float(p), _p(p_row), float(m), _p(m_row), priority,
-                                          _p(tokens), _p(logp), _p(prio), _stream()), "sample")
-    return tokens, logp, logp if prio is None else prio
+    dev = x.device
+    tokens = torch.empty((outer, inner), dtype=torch.int64, device=dev)
+    out = torch.empty((2 if priority else 1, outer, inner), dtype=torch.float32, device=dev)
+    logp = out[0]
+    prio = out[1] if priority else logp
+    if outer and inner:
+        num = lambda p, off: (off, p.data_ptr()) if isinstance(p, torch.Tensor) else (p, None)
+        _launch("sample", _lib.lib().dttt_sample, dev, x.data_ptr(), _LOGIT_TYPES[x.dtype], outer * inner, inner, x.stride(0), x.stride(1), V,
+                u.data_ptr(), None if bias is None else bias.data_ptr(), *num(temperature, 1.0), *num(top_k, 0), *num(top_p, 1.0),
+                *num(min_p, 0.0), priority, tokens.data_ptr(), logp.data_ptr(), prio.data_ptr())
+    return tokens, logp, prio
 
 
 def unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure):
     """Contiguous ``[B, C]`` tensors (``quota [B]``); ``(ids, known, held, where)`` after the commit."""
     B, C = ids.shape
-    ids_out, known_out, held_out, where = torch.empty_like(ids), torch.empty_like(known), torch.empty_like(held), torch.empty_like(known)
-    if ids.numel():
-        with torch.cuda.device(ids.device):
-            _check(_lib.lib().dttt_unmask(_p(ids), _p(known), _p(held), _p(tokens), _p(logp), _p(priority), _p(quota), _p(allowed),
-                                          0.0 if sure is None else float(sure), 0 if sure is None else 1, _p(ids_out), _p(known_out),
-                                          _p(held_out), _p(where), B, C, _stream()), "unmask")
+    ids_out, held_out = torch.empty_like(ids), torch.empty_like(held)
+    known_out, where = torch.empty((2, B, C), dtype=torch.bool, device=ids.device).unbind(0)
+    if B and C:
+        _launch("unmask", _lib.lib().dttt_unmask, ids.device, ids.data_ptr(), known.data_ptr(), held.data_ptr(), tokens.data_ptr(),
+                logp.data_ptr(), priority.data_ptr(), quota.data_ptr(), None if allowed is None else allowed.data_ptr(),
+                0.0 if sure is None else sure, 0 if sure is None else 1, ids_out.data_ptr(), known_out.data_ptr(), held_out.data_ptr(),
+                where.data_ptr(), B, C)
     return ids_out, known_out, held_out, where
 
 
@@ -838,14 +857,14 @@ def newton_schulz(g, steps, keep):
     holds every iteration's polynomial matrix with ``keep``, else scratch."""
     global LAUNCHES
     B, rows, cols = g.shape
-    d = min(rows, cols)
-    with torch.cuda.device(g.device):
-        y = torch.empty(B, rows, cols, dtype=torch.bfloat16, device=g.device)
-        norms = torch.empty(B, dtype=torch.float64, device=g.device)
-        polys = torch.empty(steps if keep else 1, B, d, -(-d // 8) * 8, dtype=torch.float16, device=g.device)
-        scratch = torch.empty(int(_lib.lib().dttt_newton_schulz_scratch(B, rows, cols)), dtype=torch.uint8, device=g.device)
-        _check(_lib.lib().dttt_newton_schulz(_p(g), int(g.dtype == torch.float32), B, rows, cols, steps, _p(scratch), _p(polys), int(keep),
-                                             _p(norms), _p(y), _p(_lib.status_tensor(g.device)), _stream()), "newton_schulz")
+    d, dev = min(rows, cols), g.device
+    y = torch.empty((B, rows, cols), dtype=torch.bfloat16, device=dev)
+    norms = torch.empty(B, dtype=torch.float64, device=dev)
+    polys = torch.empty((steps if keep else 1, B, d, -(-d // 8) * 8), dtype=torch.float16, device=dev)
+    l = _lib.lib()
+    scratch = torch.empty(l.dttt_newton_schulz_scratch(B, rows, cols), dtype=torch.uint8, device=dev)
+    _launch("newton_schulz", l.dttt_newton_schulz, dev, g.data_ptr(), int(g.dtype == torch.float32), B, rows, cols, steps,
+            scratch.data_ptr(), polys.data_ptr(), int(keep), norms.data_ptr(), y.data_ptr(), _lib.status_tensor(dev).data_ptr())
     LAUNCHES += 1 + 3 * steps
     return y, norms, polys
 
@@ -854,12 +873,12 @@ def newton_schulz_apply(r, norms, polys, out_dtype):
     """The linear map of a kept forward applied to ``r [B, rows, cols]`` (f32 or bf16, contiguous)."""
     global LAUNCHES
     B, rows, cols = r.shape
-    steps = polys.shape[0]
-    with torch.cuda.device(r.device):
-        out = torch.empty(B, rows, cols, dtype=out_dtype, device=r.device)
-        scratch = torch.empty(int(_lib.lib().dttt_newton_schulz_scratch(B, rows, cols)), dtype=torch.uint8, device=r.device)
-        _check(_lib.lib().dttt_newton_schulz_apply(_p(r), int(r.dtype == torch.float32), B, rows, cols, steps, _p(scratch), _p(polys),
-                                                   _p(norms), _p(out), int(out_dtype == torch.float32), _p(_lib.status_tensor(r.device)),
-                                                   _stream()), "newton_schulz_apply")
+    steps, dev = polys.shape[0], r.device
+    out = torch.empty((B, rows, cols), dtype=out_dtype, device=dev)
+    l = _lib.lib()
+    scratch = torch.empty(l.dttt_newton_schulz_scratch(B, rows, cols), dtype=torch.uint8, device=dev)
+    _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), int(r.dtype == torch.float32), B, rows, cols, steps,
+            scratch.data_ptr(), polys.data_ptr(), norms.data_ptr(), out.data_ptr(), int(out_dtype == torch.float32),
+            _lib.status_tensor(dev).data_ptr())
     LAUNCHES += 1 + steps
     return out

@@ -27,7 +27,7 @@ class _Apply(torch.autograd.Function):
     @staticmethod
     def forward(ctx, r, norms, polys, dtype):
         ctx.kept, ctx.dtype = (norms, polys), r.dtype
-        if not r.is_cuda:
+        if isinstance(polys, list):
             return ref.newton_schulz_apply(r, norms, polys).to(dtype)
         from . import kernels
         out_dtype = torch.float32 if dtype == torch.float32 else torch.bfloat16
@@ -51,12 +51,10 @@ class _NewtonSchulz(torch.autograd.Function):
 
 
 def _run(g: torch.Tensor, steps: int, keep: bool):
-    if not g.is_cuda:
+    from . import kernels
+    if not g.is_cuda or "newton_schulz" in kernels._DISABLED:
         y, norms, polys = ref.newton_schulz(g, steps)
         return y.to(torch.bfloat16), norms, polys
-    from . import kernels
-    if not kernels.available("newton_schulz"):
-        raise RuntimeError("newton_schulz: the kernels are not in the loaded library")
     y, norms, polys = kernels.newton_schulz(_flat(g), steps, keep)
     return y.view(g.shape), norms, polys
 

@@ -32,29 +32,25 @@ class Committed(NamedTuple):
     where: torch.Tensor           # bool: the slots this call committed
 
 
-def _need(cond: bool, msg: str) -> None:
-    if not cond:
-        raise ValueError(msg)
-
-
 def _param(name: str, value: Param, rows, dtype: torch.dtype, device, lo: float, hi: float, open_lo: bool = False):
     """A checked number, or a tensor expanded to one value per row."""
-    if torch.is_tensor(value) and (value.dim() > 0 or value.is_cuda):
-        _need(value.device == device, f"sample_tokens: {name} is on {value.device}, the logits on {device}")
+    if isinstance(value, torch.Tensor) and (value.dim() > 0 or value.is_cuda):
+        if value.device != device:
+            raise ValueError(f"sample_tokens: {name} is on {value.device}, the logits on {device}")
         whole = not (value.dtype.is_floating_point or value.dtype.is_complex or value.dtype == torch.bool)
-        _need(whole if dtype == torch.int32 else value.dtype.is_floating_point, f"sample_tokens: {name} of {value.dtype}")
+        if not (whole if dtype == torch.int32 else value.dtype.is_floating_point):
+            raise ValueError(f"sample_tokens: {name} of {value.dtype}")
         try:
-            value = value.clamp(-1, 2 ** 31 - 1) if value.dtype == torch.int64 else value
+            value = value.detach().clamp(-1, 2 ** 31 - 1) if value.dtype == torch.int64 else value.detach()
             return value.to(dtype).expand(rows).contiguous()
         except RuntimeError:
             raise ValueError(f"sample_tokens: {name} {tuple(value.shape)} does not broadcast to the rows {tuple(rows)}") from None
-    v = value.item() if torch.is_tensor(value) else value
-    _need((lo < v if open_lo else lo <= v) and v <= hi and math.isfinite(v),
-          f"sample_tokens: {name} = {v!r} is outside {'(' if open_lo else '['}{lo}, {hi}]")
+    v = value.item() if isinstance(value, torch.Tensor) else value
+    if not ((lo < v if open_lo else lo <= v) and v <= hi):
+        raise ValueError(f"sample_tokens: {name} = {v!r} is outside {'(' if open_lo else '['}{lo}, {hi}]")
     return int(v) if dtype == torch.int32 else float(v)
 
 
-@torch.no_grad()
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Param = 1.0, top_k: Param = 0, top_p: Param = 1.0,
                   min_p: Param = 0.0, bias: Optional[torch.Tensor] = None, priority: str = "logp") -> Drawn:
     """One token per row of ``logits [..., V]`` (f32, bf16 or f16; two or more dimensions), drawn with ``u [...]`` (f32 in [0, 1)).
@@ -71,36 +67,39 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Param =
     off; ``top_p >= 1``: off, ``<= 0``: the best token alone; ``min_p <= 0``: off, above 1: as 1; NaN: as off (``temperature``:
     greedy).  ``u`` outside [0, 1) is clamped, NaN taken as 0.  A row without a distribution (NaN or +inf in it, or every token
     at -inf) gives token -1 and NaN.  ``V`` up to 393216 on a CUDA device."""
-    _need(logits.dim() >= 2 and logits.shape[-1] > 0, f"sample_tokens: logits {tuple(logits.shape)}, at least [rows, V] are wanted")
-    _need(logits.dtype in (torch.float32, torch.bfloat16, torch.float16), f"sample_tokens: logits of {logits.dtype}")
-    _need(priority in PRIORITIES, f"sample_tokens: priority {priority!r} ({' | '.join(PRIORITIES)})")
-    rows, V, dev = logits.shape[:-1], logits.shape[-1], logits.device
-    _need(u.shape == rows and u.dtype == torch.float32 and u.device == dev,
-          f"sample_tokens: u {tuple(u.shape)} {u.dtype} on {u.device}, {tuple(rows)} float32 on {dev} is wanted")
-    if bias is not None:
-        _need(bias.shape == (rows[0], V) and bias.dtype == torch.float32 and bias.device == dev,
-              f"sample_tokens: bias {tuple(bias.shape)} {bias.dtype} on {bias.device}, {(rows[0], V)} float32 on {dev} is wanted")
+    rows, dev = logits.shape[:-1], logits.device
+    if not rows or logits.shape[-1] == 0:
+        raise ValueError(f"sample_tokens: logits {tuple(logits.shape)}, at least [rows, V] are wanted")
+    V = logits.shape[-1]
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"sample_tokens: logits of {logits.dtype}")
+    if priority not in PRIORITIES:
+        raise ValueError(f"sample_tokens: priority {priority!r} ({' | '.join(PRIORITIES)})")
+    if u.shape != rows or u.dtype != torch.float32 or u.device != dev:
+        raise ValueError(f"sample_tokens: u {tuple(u.shape)} {u.dtype} on {u.device}, {tuple(rows)} float32 on {dev} is wanted")
+    if bias is not None and (bias.shape != (rows[0], V) or bias.dtype != torch.float32 or bias.device != dev):
+        raise ValueError(f"sample_tokens: bias {tuple(bias.shape)} {bias.dtype} on {bias.device}, {(rows[0], V)} float32 on {dev} is wanted")
     t = _param("temperature", temperature, rows, torch.float32, dev, 0.0, 1e6)
     k = _param("top_k", top_k, rows, torch.int32, dev, 0, 2 ** 31 - 1)
     p = _param("top_p", top_p, rows, torch.float32, dev, 0.0, 1.0, open_lo=True)
     m = _param("min_p", min_p, rows, torch.float32, dev, 0.0, 1.0)
-    if not logits.is_cuda:
-        full = lambda v, dtype: v.to(dtype) if torch.is_tensor(v) else torch.full(rows, v, dtype=dtype)
-        return Drawn(*ref.sample_tokens(logits, u.nan_to_num(0.0), bias, full(t, torch.float64), full(k, torch.int64),
-                                        full(p, torch.float64).nan_to_num(1.0), full(m, torch.float64).nan_to_num(0.0), priority))
     from . import kernels
-    if not kernels.available("sampling"):
-        raise RuntimeError("sample_tokens: the sampling kernels are not in the loaded library")
-    _need(V <= kernels.SAMPLE_VOCAB_MAX, f"sample_tokens: V = {V} is above {kernels.SAMPLE_VOCAB_MAX}")
-    x = logits if logits.stride(-1) == 1 or V == 1 else logits.contiguous()
-    x = x.unsqueeze(1) if x.dim() == 2 else x.reshape(rows[0], math.prod(rows[1:]), V) if x.dim() > 3 else x
-    flat = lambda v: v.reshape(x.shape[:2]).contiguous() if torch.is_tensor(v) else v
-    out = kernels.sample(x, flat(u), None if bias is None else bias.contiguous(), flat(t), flat(k), flat(p), flat(m),
+    if not logits.is_cuda or "sampling" in kernels._DISABLED:
+        with torch.no_grad():
+            full = lambda v, dtype: v.to(dtype) if isinstance(v, torch.Tensor) else torch.full(rows, v, dtype=dtype, device=dev)
+            return Drawn(*ref.sample_tokens(logits, u.nan_to_num(0.0), bias, full(t, torch.float64), full(k, torch.int64),
+                                            full(p, torch.float64).nan_to_num(1.0), full(m, torch.float64).nan_to_num(0.0), priority))
+    if V > kernels.SAMPLE_VOCAB_MAX:
+        raise ValueError(f"sample_tokens: V = {V} is above {kernels.SAMPLE_VOCAB_MAX}")
+    x = logits if logits.stride(-1) == 1 or V == 1 else logits.detach().contiguous()
+    if len(rows) != 2:
+        x = x.unsqueeze(1) if len(rows) == 1 else x.reshape(rows[0], math.prod(rows[1:]), V)
+    flat = lambda v: v.reshape(x.shape[:2]) if isinstance(v, torch.Tensor) else v
+    out = kernels.sample(x, u.contiguous(), None if bias is None else bias.contiguous(), flat(t), flat(k), flat(p), flat(m),
                          PRIORITIES.index(priority))
-    return Drawn(*(o.view(rows) for o in out))
+    return Drawn(*out) if len(rows) == 2 else Drawn(*(o.view(rows) for o in out))
 
 
-@torch.no_grad()
 def unmask(ids: torch.Tensor, known: torch.Tensor, held: torch.Tensor, tokens: torch.Tensor, logp: torch.Tensor,
            priority: torch.Tensor, quota: torch.Tensor, *, allowed: Optional[torch.Tensor] = None,
            sure: Optional[float] = None) -> Committed:
@@ -109,20 +108,23 @@ def unmask(ids: torch.Tensor, known: torch.Tensor, held: torch.Tensor, tokens: t
     it.  ``ids``, ``known`` and ``held`` (the log-probability a slot was committed with) come back with ``tokens`` / True /
     ``logp`` at the committed slots.  Slots of equal priority rank by position, NaN ranks last; a slot that is not open ranks as
     one of priority ``-inf``.  ``C`` up to 32768 on a CUDA device."""
-    _need(ids.dim() == 2, f"unmask: ids {tuple(ids.shape)}, [B, C] is wanted")
+    shape, dev = ids.shape, ids.device
+    if len(shape) != 2:
+        raise ValueError(f"unmask: ids {tuple(shape)}, [B, C] is wanted")
     for name, t, dtype in (("ids", ids, torch.int64), ("known", known, torch.bool), ("held", held, torch.float32),
                            ("tokens", tokens, torch.int64), ("logp", logp, torch.float32), ("priority", priority, torch.float32),
                            ("allowed", allowed, torch.bool)):
-        _need(t is None or (t.shape == ids.shape and t.dtype == dtype and t.device == ids.device),
-              f"unmask: {name}: {tuple(ids.shape)} {dtype} on {ids.device} is wanted")
-    _need(quota.shape == ids.shape[:1] and quota.dtype == torch.int64 and quota.device == ids.device,
-          f"unmask: quota: {tuple(ids.shape[:1])} torch.int64 on {ids.device} is wanted")
-    _need(sure is None or not math.isnan(sure), "unmask: sure is NaN")
-    if not ids.is_cuda:
-        return Committed(*ref.unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure))
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != dev):
+            raise ValueError(f"unmask: {name} {tuple(t.shape)} {t.dtype} on {t.device}, {tuple(shape)} {dtype} on {dev} is wanted")
+    if quota.shape != shape[:1] or quota.dtype != torch.int64 or quota.device != dev:
+        raise ValueError(f"unmask: quota {tuple(quota.shape)} {quota.dtype} on {quota.device}, {tuple(shape[:1])} torch.int64 on {dev} is wanted")
+    if sure is not None and math.isnan(sure):
+        raise ValueError("unmask: sure is NaN")
     from . import kernels
-    if not kernels.available("sampling"):
-        raise RuntimeError("unmask: the sampling kernels are not in the loaded library")
-    _need(ids.shape[1] <= kernels.UNMASK_SLOTS_MAX, f"unmask: {ids.shape[1]} slots, above {kernels.UNMASK_SLOTS_MAX}")
-    c = lambda t: None if t is None else t.contiguous()
-    return Committed(*kernels.unmask(c(ids), c(known), c(held), c(tokens), c(logp), c(priority), c(quota), c(allowed), sure))
+    if not ids.is_cuda or "sampling" in kernels._DISABLED:
+        with torch.no_grad():
+            return Committed(*ref.unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure))
+    if shape[1] > kernels.UNMASK_SLOTS_MAX:
+        raise ValueError(f"unmask: {shape[1]} slots, above {kernels.UNMASK_SLOTS_MAX}")
+    return Committed(*kernels.unmask(ids.contiguous(), known.contiguous(), held.contiguous(), tokens.contiguous(), logp.contiguous(),
+                                     priority.contiguous(), quota.contiguous(), None if allowed is None else allowed.contiguous(), sure))
