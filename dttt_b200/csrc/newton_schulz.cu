@@ -14,7 +14,8 @@
 // is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12 for
 // those, 2^5 for the cotangent, which may grow 3.4445-fold per iteration.  Sums are f32 (tensor memory), the norms f64.
 //
-// Every product is C = alpha A B + beta D on CTA pairs: 256 x 256 tiles, tcgen05.mma.cta_group::2, plain per-CTA TMA loads.
+// Every product is C = alpha A B + beta D on CTA pairs: tiles of 256 rows and 256 or 128 columns, tcgen05.mma.cta_group::2, plain
+// per-CTA TMA loads.
 #include "host_check.h"
 #include "ptx_sm100.cuh"
 
@@ -27,15 +28,22 @@ namespace dttt {
 namespace ns {
 
 constexpr int BM = 128;        // rows of A per CTA (256 per pair)
-constexpr int BN = 256;        // output columns per pair; each CTA loads BN / 2 of them
 constexpr int BK = 64;
 constexpr int UMMA_K = 16;
-constexpr int STAGES = 6;
 constexpr int A_BYTES = BM * BK * 2;
-constexpr int B_BYTES = (BN / 2) * BK * 2;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int STAGING_BYTES = 4 * 4096;                        // epilogue: 32 rows x 128 bytes per warp
-constexpr int SMEM_TOTAL = STAGES * STAGE_BYTES + 1024 + STAGING_BYTES + 1024;
+constexpr int EPI_WARPS = 8;   // two per quarter of the accumulator's rows, half of the columns each
+constexpr int THREADS = (2 + EPI_WARPS) * 32;
+constexpr int STAGING_BYTES = EPI_WARPS * 4096;                // epilogue: 32 rows x 128 bytes per warp
+
+// BN: output columns per pair (256 or 128); each CTA loads BN / 2 of them.
+template <int BN>
+struct Tile {
+  static constexpr int B_BYTES = (BN / 2) * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN == 256 ? 6 : 8;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + STAGING_BYTES + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
+};
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float X_SCALE = 4096.f;           // of x, G and P
@@ -59,19 +67,24 @@ struct Params {
   int tiles_m, tiles_n;
 };
 
-__host__ __device__ inline int tiles_per_matrix(const Params& p) {
-  return p.symmetric ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+// A symmetric C takes the tiles that reach the diagonal or lie below it: with tiles `w` = 256 / BN to a square block, block row tm has
+// w (tm + 1) of them.
+__host__ __device__ inline int tiles_per_matrix(const Params& p, int w) {
+  return p.symmetric ? w * (p.tiles_m * (p.tiles_m + 1) / 2) : p.tiles_m * p.tiles_n;
 }
 
+template <int BN>
 __device__ __forceinline__ void tile_coords(int tile, const Params& p, int& b, int& tm, int& tn) {
-  const int per_batch = tiles_per_matrix(p);
+  constexpr int w = 256 / BN;
+  const int per_batch = tiles_per_matrix(p, w);
   b = tile / per_batch;
   const int t = tile - b * per_batch;
   if (p.symmetric) {
-    tm = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while (tm * (tm + 1) / 2 > t) --tm;                        // the root may round across a whole number
-    while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
-    tn = t - tm * (tm + 1) / 2;
+    const int q = t / w;                                       // counts square blocks row by row
+    tm = (int)((sqrtf(8.f * (float)q + 1.f) - 1.f) * 0.5f);
+    while (tm * (tm + 1) / 2 > q) --tm;                        // the root may round across a whole number
+    while ((tm + 1) * (tm + 2) / 2 <= q) ++tm;
+    tn = t - w * (tm * (tm + 1) / 2);
     return;
   }
   constexpr int GROUP = 8;                                     // bands of 8 pair rows, n fastest inside a band
@@ -168,8 +181,10 @@ __device__ __forceinline__ void store_transposed(__half* out, long long ld, int 
   }
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const Params p) {
+  constexpr int STAGES = Tile<BN>::STAGES, STAGE_BYTES = Tile<BN>::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);      // the leader's count both CTAs' bytes
@@ -182,13 +197,13 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-  const int num_tiles = p.batch * tiles_per_matrix(p);
+  const int num_tiles = p.batch * tiles_per_matrix(p, 256 / BN);
   const int kblocks = (p.K + BK - 1) / BK;
   constexpr uint32_t TMEM_COLS = 2 * BN;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 256); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 2 * EPI_WARPS * 32); }
     *abort_word = 0;
     fence_mbar_init();
     tma_prefetch_desc(&mapA);
@@ -210,7 +225,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
       bool ok = true;
       for (int tile = pair_id; tile < num_tiles && ok; tile += n_pairs) {
         int b, tm, tn;
-        tile_coords(tile, p, b, tm, tn);
+        tile_coords<BN>(tile, p, b, tm, tn);
         const int m0 = tm * 2 * BM + (int)rank * BM;
         const int n0 = tn * BN + (int)rank * (BN / 2);
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
@@ -270,14 +285,14 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, c0 = ((warp - 2) >> 2) * (BN / 2);      // tensor memory lanes belong to warps by their number mod 4
     uint32_t local_tile = 0;
     for (int tile = pair_id; tile < num_tiles; tile += n_pairs, ++local_tile) {
       int b, tm, tn;
-      tile_coords(tile, p, b, tm, tn);
+      tile_coords<BN>(tile, p, b, tm, tn);
       const int acc = local_tile & 1;
       const uint32_t acc_ph = (local_tile >> 1) & 1;
-      const int row0 = tm * 2 * BM + (int)rank * BM + quarter * 32, n0 = tn * BN;
+      const int row0 = tm * 2 * BM + (int)rank * BM + quarter * 32, n0 = tn * BN + c0;
       const int rows = p.M - row0;                             // of this warp's 32 (may be negative)
       float alpha = p.alpha, beta = p.beta;
       if (p.num || p.den) {
@@ -293,16 +308,16 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
       got = __shfl_sync(0xffffffffu, got, 0);
       if (!got) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + acc * BN + ((uint32_t)(quarter * 32) << 16);
-      uint8_t* stg = smem + STAGES * STAGE_BYTES + 1024 + quarter * 4096;
+      const uint32_t taddr = tmem_base + acc * BN + c0 + ((uint32_t)(quarter * 32) << 16);
+      uint8_t* stg = smem + STAGES * STAGE_BYTES + 1024 + (warp - 2) * 4096;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 64) {
+      for (int c = 0; c < BN / 2; c += 64) {
         uint32_t r[64];
         tmem_ld_32x32(taddr + c, reinterpret_cast<uint32_t(&)[32]>(r[0]));
         tmem_ld_32x32(taddr + c + 32, reinterpret_cast<uint32_t(&)[32]>(r[32]));
         if (d0) {
           stage_in(stg, lane, dnext);
-          if (c + 64 < BN) load_rows(d0 + c + 64, p.ldd, rows, (int)p.ldd - n0 - c - 64, lane, dnext);
+          if (c + 64 < BN / 2) load_rows(d0 + c + 64, p.ldd, rows, (int)p.ldd - n0 - c - 64, lane, dnext);
           __syncwarp();
         }
         tmem_ld_wait();
@@ -329,7 +344,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
           uint16_t* out = reinterpret_cast<uint16_t*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c;
           if ((p.ldc & 7) == 0) flush_lines(stg, lane, out, p.ldc, rows, (int)p.ldc - n0 - c);
           else flush_ragged(stg, lane, out, p.ldc, rows, p.N - n0 - c);
-          if (p.symmetric && tm != tn)
+          if (p.symmetric && tn < tm * (256 / BN))
             store_transposed(reinterpret_cast<__half*>(p.C) + (long long)b * p.c_batch + (long long)(n0 + c) * p.ldc + row0, p.ldc, p.N - n0 - c,
                              (int)p.ldc - row0, lane, r);
           __syncwarp();
@@ -420,13 +435,13 @@ struct Mat {
   long long ld;
 };
 
-// `mn`: the operand's rows run along the contraction (its M or N index is contiguous); the box is then 64 x BK, else BK x 128.
-static int make_map(CUtensorMap* map, const Mat& m, int batch, bool mn) {
+// `mn`: the operand's rows run along the contraction (its M or N index is contiguous); the box is then 64 x BK, else BK x box_rows.
+static int make_map(CUtensorMap* map, const Mat& m, int batch, bool mn, int box_rows) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return 101;
   cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)batch};
   cuuint64_t strides[2] = {(cuuint64_t)m.ld * 2, (cuuint64_t)m.ld * m.rows * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)(mn ? BK : 128), 1};
+  cuuint32_t box[3] = {64, (cuuint32_t)(mn ? BK : box_rows), 1};
   cuuint32_t estr[3] = {1, 1, 1};
   if (int c = check_map(m.ptr, 3, dims, strides, 2)) return c;
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(m.ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -444,7 +459,8 @@ static int prepare_device(int* n_sm) {
   if (bound_dev != dev) { cudaSetDevice(dev); cudaFree(0); bound_dev = dev; }      // the encoder needs a current context
   std::lock_guard<std::mutex> lock(mu);
   if (!(attr_mask >> dev & 1ull)) {
-    if (cudaFuncSetAttribute(ns_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL) != cudaSuccess) return 302;
+    if (cudaFuncSetAttribute(ns_product_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess) return 302;
     cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
     attr_mask |= 1ull << dev;
   }
@@ -462,9 +478,6 @@ struct Out {
 // C [M, N] = alpha op(A) op(B) + beta D over the batch (symmetric: C and D are, and only f16)
 static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, const Mat& B, bool b_mn, float alpha, float beta, const Mat* D,
                    const Out& o, bool symmetric, int* status, int n_sm, cudaStream_t stream) {
-  CUtensorMap mapA, mapB;
-  if (int r = make_map(&mapA, A, batch, a_mn)) return r;
-  if (int r = make_map(&mapB, B, batch, b_mn)) return r;
   Params p;
   memset(&p, 0, sizeof(p));
   p.M = M; p.N = N; p.K = K; p.batch = batch; p.a_mn_major = a_mn; p.b_mn_major = b_mn; p.alpha = alpha; p.beta = beta;
@@ -472,11 +485,25 @@ static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, cons
   p.C = o.C; p.out = o.kind; p.ldc = o.ld; p.c_batch = o.ld * M; p.num = o.num; p.den = o.den; p.status = status;
   p.symmetric = symmetric;
   p.tiles_m = (M + 2 * BM - 1) / (2 * BM);
-  p.tiles_n = (N + BN - 1) / BN;
-  const long long tiles = (long long)batch * tiles_per_matrix(p);
-  if (tiles > 0x3fffffff) return 303;
-  const int pairs = (int)(tiles < n_sm / 2 ? tiles : n_sm / 2);
-  ns_product_kernel<<<2 * pairs, 192, SMEM_TOTAL, stream>>>(mapA, mapB, p);
+  // Tiles of 256 or of 128 columns: whichever needs less time for its rounds over the pairs of SMs.  A narrow tile's k-block takes
+  // 0.62 of a wide one's (it moves 3/4 of the bytes for half the products), its share outside the main loop about half.
+  const int pairs = n_sm / 2, kb = (K + BK - 1) / BK;
+  long long tiles[2];
+  double cost[2];
+  for (int i = 0; i < 2; ++i) {
+    p.tiles_n = (N + (256 >> i) - 1) / (256 >> i);
+    tiles[i] = (long long)batch * tiles_per_matrix(p, 1 << i);
+    cost[i] = (double)((tiles[i] + pairs - 1) / pairs) * (kb * (i ? 0.62 : 1.0)) + (i ? 15 : 30);
+  }
+  const int narrow = cost[1] < cost[0];
+  p.tiles_n = (N + (256 >> narrow) - 1) / (256 >> narrow);
+  if (tiles[narrow] > 0x3fffffff) return 303;
+  CUtensorMap mapA, mapB;
+  if (int r = make_map(&mapA, A, batch, a_mn, BM)) return r;
+  if (int r = make_map(&mapB, B, batch, b_mn, narrow ? 64 : 128)) return r;
+  const int grid = 2 * (int)(tiles[narrow] < pairs ? tiles[narrow] : pairs);
+  if (narrow) ns_product_kernel<128><<<grid, THREADS, Tile<128>::SMEM, stream>>>(mapA, mapB, p);
+  else ns_product_kernel<256><<<grid, THREADS, Tile<256>::SMEM, stream>>>(mapA, mapB, p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
