@@ -56,7 +56,9 @@ struct Params {
   int a_mn_major, b_mn_major;
   float alpha, beta;
   const __half* D;             // or null; same shape as C
-  long long ldd, d_batch;
+  const __half* D2;            // TWO: a second one, and `diag` on the diagonal
+  long long ldd, d_batch;      // of both
+  float beta2, diag;
   void* C;
   int out;
   long long ldc, c_batch;
@@ -181,7 +183,7 @@ __device__ __forceinline__ void store_transposed(__half* out, long long ld, int 
   }
 }
 
-template <int BN>
+template <int BN, bool TWO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const Params p) {
   constexpr int STAGES = Tile<BN>::STAGES, STAGE_BYTES = Tile<BN>::STAGE_BYTES;
@@ -334,6 +336,26 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
           }
         }
         __syncwarp();
+        if (TWO) {
+          uint4 v[8];
+          load_rows(p.D2 + (d0 - p.D) + c, p.ldd, rows, (int)p.ldd - n0 - c, lane, v);
+          stage_in(stg, lane, v);
+          __syncwarp();
+          const int on = row0 + lane - n0 - c;                 // the column on the diagonal
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint4 dv = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16));
+            const __half2* dh = reinterpret_cast<const __half2*>(&dv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 df = __half22float2(dh[e >> 1]);
+              float& x = reinterpret_cast<float&>(r[8 * q + e]);
+              x = fmaf(p.beta2, e & 1 ? df.y : df.x, x);
+              if (8 * q + e == on) x += p.diag;
+            }
+          }
+          __syncwarp();
+        }
         if (p.out == OUT_F32) {
           store_f32(reinterpret_cast<float*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c, p.ldc, rows, p.N - n0 - c, lane, r);
           __syncwarp();                                        // the next load is one of the whole warp
@@ -365,10 +387,14 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
 }
 
 // ------------------------------------------------------------------ norms and the f16 copy
-constexpr int NORM_BLOCKS = 128;            // partial sums per matrix
+// Two passes over the matrix, 16 bytes a load; the second finds what the first left in L2 (the launcher takes matrices in groups
+// that fit).  Squares in 64 bits: no scale of the input overflows or vanishes, and the order of the sum is fixed.
+constexpr int NORM_BLOCKS = 512;            // partial sums per matrix at most
+constexpr int CAST_THREADS = 256;
 
-template <class T> __device__ __forceinline__ float load_f32(const T* p) { return (float)*p; }
-template <> __device__ __forceinline__ float load_f32<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+template <class T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 __device__ __forceinline__ double block_sum(double v) {
   __shared__ double part[32];
@@ -381,35 +407,72 @@ __device__ __forceinline__ double block_sum(double v) {
   return s;
 }
 
-// partial[b][j]: the squares of one of NORM_BLOCKS interleaved pieces of matrix b, in 64 bits
+// partial[b][j]: the squares of one of gridDim.x interleaved pieces of matrix b
 template <class T>
-__global__ void __launch_bounds__(256) ns_squares_kernel(const T* __restrict__ g, long long n, double* __restrict__ partial) {
+__global__ void __launch_bounds__(CAST_THREADS) ns_squares_kernel(const T* __restrict__ g, long long n, double* __restrict__ partial) {
+  constexpr int VEC = 16 / (int)sizeof(T), UNROLL = 4;
   const T* x = g + (long long)blockIdx.y * n;
-  double s = 0;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    const double v = (double)load_f32(x + i);
-    s += v * v;
+  const long long tid = (long long)blockIdx.x * CAST_THREADS + threadIdx.x, step = (long long)gridDim.x * CAST_THREADS;
+  const long long nv = (reinterpret_cast<uintptr_t>(x) & 15) == 0 ? n / VEC : 0;
+  double s[UNROLL] = {0, 0, 0, 0};
+  for (long long v = tid; v < nv; v += step * UNROLL) {
+    uint4 raw[UNROLL];
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) raw[k] = v + k * step < nv ? __ldg(reinterpret_cast<const uint4*>(x) + v + k * step) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) { const double e = (double)to_f32(reinterpret_cast<const T*>(&raw[k])[j]); s[k] = fma(e, e, s[k]); }
   }
-  s = block_sum(s);
-  if (threadIdx.x == 0) partial[(long long)blockIdx.y * NORM_BLOCKS + blockIdx.x] = s;
+  for (long long i = nv * VEC + tid; i < n; i += step) { const double e = (double)to_f32(x[i]); s[0] = fma(e, e, s[0]); }
+  const double sum = block_sum((s[0] + s[1]) + (s[2] + s[3]));
+  if (threadIdx.x == 0) partial[(long long)blockIdx.y * NORM_BLOCKS + blockIdx.x] = sum;
 }
 
 // x [rows, ld] = f16(scale g / |g|), norm[b] = |g|
 template <class T>
-__global__ void __launch_bounds__(256) ns_cast_kernel(const T* __restrict__ g, int rows, int cols, const double* __restrict__ partial,
-                                                     float scale, __half* __restrict__ x, int ld, double* __restrict__ norm) {
+__global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restrict__ g, int rows, int cols, const double* __restrict__ partial,
+                                                              int parts, float scale, __half* __restrict__ x, int ld, double* __restrict__ norm) {
   const int b = blockIdx.y;
-  const double v = (int)threadIdx.x < NORM_BLOCKS ? partial[(long long)b * NORM_BLOCKS + threadIdx.x] : 0.0;
+  double v = 0;
+  for (int i = threadIdx.x; i < parts; i += CAST_THREADS) v += partial[(long long)b * NORM_BLOCKS + i];
   const double whole = sqrt(block_sum(v));
   if (blockIdx.x == 0 && threadIdx.x == 0) norm[b] = whole;
+  // the factor as a product of two floats, so that no finite norm takes it out of their range: 2^e times something near `scale`
   const double f = whole == 0.0 ? 0.0 : (double)scale / whole;
+  int e = 0;
+  const double mant = frexp(f, &e);
+  const float f0 = (float)ldexp(mant, e / 2), f1 = (float)ldexp(1.0, e - e / 2);
   const T* src = g + (long long)b * rows * cols;
   __half* dst = x + (long long)b * rows * ld;
-  const long long n = (long long)rows * cols;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    const long long r = i / cols;
-    dst[r * ld + (i - r * cols)] = __float2half_rn((float)((double)load_f32(src + i) * f));
+  const long long n = (long long)rows * cols, step = (long long)gridDim.x * CAST_THREADS;
+  if (ld == cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {      // no padding: eight elements at a time
+    constexpr int LOADS = 8 * (int)sizeof(T) / 16, UNROLL = sizeof(T) == 4 ? 2 : 4;
+    const long long nv = n / 8;
+    for (long long i = (long long)blockIdx.x * CAST_THREADS + threadIdx.x; i < nv; i += step * UNROLL) {
+      uint4 raw[UNROLL][LOADS];
+#pragma unroll
+      for (int k = 0; k < UNROLL; ++k)
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l)
+          if (i + k * step < nv) raw[k][l] = __ldcs(reinterpret_cast<const uint4*>(src) + (i + k * step) * LOADS + l);
+#pragma unroll
+      for (int k = 0; k < UNROLL; ++k) {
+        if (i + k * step < nv) {
+          const T* t = reinterpret_cast<const T*>(&raw[k][0]);
+          uint4 o;
+          __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(to_f32(t[2 * j]) * f0 * f1, to_f32(t[2 * j + 1]) * f0 * f1);
+          reinterpret_cast<uint4*>(dst)[i + k * step] = o;
+        }
+      }
+    }
+    return;
   }
+  for (int r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int c = threadIdx.x; c < cols; c += CAST_THREADS)
+      dst[(long long)r * ld + c] = __float2half_rn(to_f32(src[(long long)r * cols + c]) * f0 * f1);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -459,8 +522,10 @@ static int prepare_device(int* n_sm) {
   if (bound_dev != dev) { cudaSetDevice(dev); cudaFree(0); bound_dev = dev; }      // the encoder needs a current context
   std::lock_guard<std::mutex> lock(mu);
   if (!(attr_mask >> dev & 1ull)) {
-    if (cudaFuncSetAttribute(ns_product_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess) return 302;
+    if (cudaFuncSetAttribute(ns_product_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<256, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess) return 302;
     cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
     attr_mask |= 1ull << dev;
   }
@@ -475,13 +540,15 @@ struct Out {
   const double *num, *den;
 };
 
-// C [M, N] = alpha op(A) op(B) + beta D over the batch (symmetric: C and D are, and only f16)
+// C [M, N] = alpha op(A) op(B) + beta D (+ beta2 D2 + diag I, with the layout of D) over the batch (symmetric: C and D are, and only f16)
 static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, const Mat& B, bool b_mn, float alpha, float beta, const Mat* D,
-                   const Out& o, bool symmetric, int* status, int n_sm, cudaStream_t stream) {
+                   const Out& o, bool symmetric, int* status, int n_sm, cudaStream_t stream, const Mat* D2 = nullptr, float beta2 = 0.f,
+                   float diag = 0.f) {
   Params p;
   memset(&p, 0, sizeof(p));
   p.M = M; p.N = N; p.K = K; p.batch = batch; p.a_mn_major = a_mn; p.b_mn_major = b_mn; p.alpha = alpha; p.beta = beta;
   if (D) { p.D = (const __half*)D->ptr; p.ldd = D->ld; p.d_batch = D->ld * D->rows; }
+  if (D2) { p.D2 = (const __half*)D2->ptr; p.beta2 = beta2; p.diag = diag; }
   p.C = o.C; p.out = o.kind; p.ldc = o.ld; p.c_batch = o.ld * M; p.num = o.num; p.den = o.den; p.status = status;
   p.symmetric = symmetric;
   p.tiles_m = (M + 2 * BM - 1) / (2 * BM);
@@ -502,8 +569,9 @@ static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, cons
   if (int r = make_map(&mapA, A, batch, a_mn, BM)) return r;
   if (int r = make_map(&mapB, B, batch, b_mn, narrow ? 64 : 128)) return r;
   const int grid = 2 * (int)(tiles[narrow] < pairs ? tiles[narrow] : pairs);
-  if (narrow) ns_product_kernel<128><<<grid, THREADS, Tile<128>::SMEM, stream>>>(mapA, mapB, p);
-  else ns_product_kernel<256><<<grid, THREADS, Tile<256>::SMEM, stream>>>(mapA, mapB, p);
+  const int smem = narrow ? Tile<128>::SMEM : Tile<256>::SMEM;
+  if (D2) (narrow ? ns_product_kernel<128, true> : ns_product_kernel<256, true>)<<<grid, THREADS, smem, stream>>>(mapA, mapB, p);
+  else (narrow ? ns_product_kernel<128, false> : ns_product_kernel<256, false>)<<<grid, THREADS, smem, stream>>>(mapA, mapB, p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
@@ -515,88 +583,168 @@ static int apply(int batch, int rows, int cols, const Mat& r, const Mat& P, floa
   return product(batch, rows, cols, cols, r, false, P, false, alpha, beta, &r, o, false, status, n_sm, stream);
 }
 
-static int cast(const void* g, int f32, int batch, int rows, int cols, double* partial, float scale, void* x, int ld, double* norm,
+template <class T>
+static int cast(const T* g, int batch, int rows, int cols, double* partial, float scale, __half* x, int ld, double* norm, int n_sm,
                 cudaStream_t stream) {
-  const long long n = (long long)rows * cols;
-  const dim3 gs(NORM_BLOCKS, batch);
-  const long long want = (n + 1023) / 1024;
-  const dim3 gc((unsigned int)(want < 592 ? want : 592), batch);
-  if (f32) {
-    ns_squares_kernel<float><<<gs, 256, 0, stream>>>((const float*)g, n, partial);
-    ns_cast_kernel<float><<<gc, 256, 0, stream>>>((const float*)g, rows, cols, partial, scale, (__half*)x, ld, norm);
-  } else {
-    ns_squares_kernel<__nv_bfloat16><<<gs, 256, 0, stream>>>((const __nv_bfloat16*)g, n, partial);
-    ns_cast_kernel<__nv_bfloat16><<<gc, 256, 0, stream>>>((const __nv_bfloat16*)g, rows, cols, partial, scale, (__half*)x, ld, norm);
+  const long long n = (long long)rows * cols, bytes = n * (long long)sizeof(T);
+  auto blocks = [](long long work, long long each, int most) { const long long w = (work + each - 1) / each; return (int)(w < most ? w : most); };
+  const int parts = blocks(n, 8192, NORM_BLOCKS);
+  const int casts = ld == cols ? blocks(n, 4096, 8 * n_sm) : blocks(rows, 1, 8 * n_sm);
+  // groups of about 48 MB: the second pass reads them from L2 (126 MB) while the f16 copies are written
+  const int group = (int)(bytes > (48ll << 20) ? 1 : (48ll << 20) / bytes);
+  for (int b = 0; b < batch; b += group) {
+    const int k = batch - b < group ? batch - b : group;
+    double* part = partial + (long long)b * NORM_BLOCKS;
+    ns_squares_kernel<T><<<dim3(parts, k), CAST_THREADS, 0, stream>>>(g + b * n, n, part);
+    ns_cast_kernel<T><<<dim3(casts, k), CAST_THREADS, 0, stream>>>(g + b * n, rows, cols, part, parts, scale, x + (long long)b * rows * ld, ld,
+                                                                  norm + b);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
+static int cast(const void* g, int f32, int batch, int rows, int cols, double* partial, float scale, void* x, int ld, double* norm, int n_sm,
+                cudaStream_t stream) {
+  if (f32) return cast<float>((const float*)g, batch, rows, cols, partial, scale, (__half*)x, ld, norm, n_sm, stream);
+  return cast<__nv_bfloat16>((const __nv_bfloat16*)g, batch, rows, cols, partial, scale, (__half*)x, ld, norm, n_sm, stream);
+}
+
 }  // namespace ns
 }  // namespace dttt
 
-// Bytes of the scratch area for `batch` matrices [rows, cols] (256-byte aligned base): two f16 copies, one d x d f16 matrix, the
-// partial sums and one norm (the cotangent's) per matrix.
-extern "C" long long dttt_newton_schulz_scratch(int batch, int rows, int cols) {
-  const long long ld = (cols + 7) / 8 * 8, d = rows < cols ? rows : cols, ldd = (d + 7) / 8 * 8;
-  auto up = [](long long v) { return (v + 255) / 256 * 256; };
-  return 2 * up(batch * rows * ld * 2) + up(batch * d * ldd * 2) + up(batch * dttt::ns::NORM_BLOCKS * 8ll) + up(batch * 8ll);
+namespace dttt {
+namespace ns {
+
+// How the iterations are grouped.  Two of them in one,
+//   x'' = (a I + P')(a I + P) x = (a^2 - s) x + N x,   N = P' P + a (P + P') + s I,
+// need G' of the second from G alone: with H = a G + P G, G' = a H + P H.  That replaces one product with x on each side of the
+// group (d^2 L and 2 d^2 L of the longer side L) by three d x d ones, which pays from L = 1.5 d on where the products are large
+// enough to be bound by the tensor cores.  `s` shifts N by its value at the singular value of a matrix with equal ones, so that
+// what rounds is the spread and not the bulk of it; unshifted, or with three iterations in one, the result is twice as far off.
+// The first two and the last two are grouped: 1.4e-3 (before the rounding of the result) as for single steps, in the middle and
+// for later pairs the cancellation costs more.
+struct Group {
+  int steps;
+  float alpha, shift;          // x' = alpha x + M x
+};
+
+static int make_plan(int rows, int cols, int steps, Group* g) {
+  const double d = rows < cols ? rows : cols, len = rows < cols ? cols : rows;
+  const bool pairs = d >= 512 && len >= 1.5 * d;
+  auto q = [](double l) { return (double)NS_A + NS_B * l + NS_C * l * l; };
+  double l = 1.0 / d;
+  int n = 0;
+  for (int k = 0; k < steps; ++n) {
+    const bool two = pairs && ((k == 0 && steps >= 2) || (k == steps - 2 && k >= 3));
+    const double next = l * q(l) * q(l);
+    if (two) {
+      g[n] = {2, (float)(q(l) * q(next)), (float)((double)NS_A * NS_A - q(l) * q(next))};
+      l = next * q(next) * q(next);
+      k += 2;
+    } else {
+      g[n] = {1, NS_A, 0.f};
+      l = next;
+      k += 1;
+    }
+  }
+  return n;
 }
 
-// g [batch, rows, cols] (f32 or bf16, contiguous) -> y bf16.  polys: f16 [steps or 1, batch, d, ceil8(d)]; with keep every step's
-// P_k stays there for the backward, else one slot is used again and again.  norms: f64 [batch].
-extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, int cols, int steps, void* scratch, void* polys, int keep,
+struct Scratch {
+  void *x[2], *gram, *h, *p;
+  double *partial, *norm;
+  long long bytes;
+  int ld, d, ldd;
+  Scratch(void* base, int batch, int rows, int cols) {
+    auto up = [](long long v) { return (v + 255) / 256 * 256; };
+    ld = (cols + 7) / 8 * 8; d = rows < cols ? rows : cols; ldd = (d + 7) / 8 * 8;
+    const long long xb = up((long long)batch * rows * ld * 2), gb = up((long long)batch * d * ldd * 2);
+    uint8_t* s = (uint8_t*)base;
+    auto take = [&](long long n) { uint8_t* r = s; s += n; return r; };
+    x[0] = take(xb); x[1] = take(xb);
+    gram = take(gb); h = take(gb); p = take(gb);
+    partial = (double*)take(up((long long)batch * NORM_BLOCKS * 8));
+    norm = (double*)take(up((long long)batch * 8));
+    bytes = s - (uint8_t*)base;
+  }
+};
+
+constexpr int MAX_STEPS = 32;
+
+}  // namespace ns
+}  // namespace dttt
+
+// Bytes of the scratch area for `batch` matrices [rows, cols] (256-byte aligned base).
+extern "C" long long dttt_newton_schulz_scratch(int batch, int rows, int cols) { return dttt::ns::Scratch(nullptr, batch, rows, cols).bytes; }
+
+// Groups of iterations, each with one d x d matrix of the linear map.
+extern "C" int dttt_newton_schulz_groups(int rows, int cols, int steps) {
+  dttt::ns::Group g[dttt::ns::MAX_STEPS];
+  return steps <= 0 || steps > dttt::ns::MAX_STEPS ? 0 : dttt::ns::make_plan(rows, cols, steps, g);
+}
+
+// g [batch, rows, cols] (f32 or bf16, contiguous) -> y bf16.  maps: f16 [groups or 1, batch, d, ceil8(d)]; with keep every group's
+// matrix stays there for the backward, else one slot is used again and again.  norms: f64 [batch].
+extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, int cols, int steps, void* scratch, void* maps, int keep,
                                   double* norms, void* y, int* status, cudaStream_t stream) {
   using namespace dttt::ns;
-  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || batch > 65535) return -2;
+  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
   int n_sm;
   if (int r = prepare_device(&n_sm)) return r;
-  const int ld = (cols + 7) / 8 * 8, d = rows < cols ? rows : cols, ldd = (d + 7) / 8 * 8;
-  auto up = [](long long v) { return (v + 255) / 256 * 256; };
-  uint8_t* s = (uint8_t*)scratch;
-  const long long xb = up((long long)batch * rows * ld * 2);
-  void* xs[2] = {s, s + xb};
-  void* gram = s + 2 * xb;
-  double* partial = (double*)((uint8_t*)gram + up((long long)batch * d * ldd * 2));
-  if (int r = cast(g, f32, batch, rows, cols, partial, X_SCALE, xs[0], ld, norms, stream)) return r;
+  const Scratch s(scratch, batch, rows, cols);
+  const int d = s.d, ldd = s.ldd;
+  if (int r = cast(g, f32, batch, rows, cols, s.partial, X_SCALE, s.x[0], s.ld, norms, n_sm, stream)) return r;
   const bool wide = rows <= cols;
-  for (int k = 0; k < steps; ++k) {
-    const Mat X = {xs[k & 1], rows, cols, ld}, G = {gram, d, d, ldd};
-    const Mat P = {(uint8_t*)polys + (keep ? (long long)k * batch * d * ldd * 2 : 0), d, d, ldd};
-    const Out og = {gram, OUT_F16, ldd, nullptr, nullptr}, op = {const_cast<void*>(P.ptr), OUT_F16, ldd, nullptr, nullptr};
+  Group plan[MAX_STEPS];
+  const int groups = make_plan(rows, cols, steps, plan);
+  const Mat G = {s.gram, d, d, ldd}, H = {s.h, d, d, ldd}, P1 = {s.p, d, d, ldd};
+  auto square = [&](const Mat& A, const Mat& B, float alpha, float beta, const Mat& D, const Mat& C, const Mat* D2 = nullptr, float beta2 = 0.f,
+                    float diag = 0.f) {
+    const Out o = {const_cast<void*>(C.ptr), OUT_F16, ldd, nullptr, nullptr};
+    return product(batch, d, d, d, A, false, B, false, alpha / X_SCALE, beta, &D, o, true, status, n_sm, stream, D2, beta2, diag);
+  };
+  for (int k = 0; k < groups; ++k) {
+    const Mat X = {s.x[k & 1], rows, cols, s.ld};
+    const Mat M = {(uint8_t*)maps + (keep ? (long long)k * batch * d * ldd * 2 : 0), d, d, ldd};
+    const Out og = {s.gram, OUT_F16, ldd, nullptr, nullptr};
     if (int r = product(batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, true, status, n_sm, stream)) return r;
-    if (int r = product(batch, d, d, d, G, false, G, false, NS_C / X_SCALE, NS_B, &G, op, true, status, n_sm, stream)) return r;
-    const bool last = k == steps - 1;
+    if (plan[k].steps == 1) {
+      if (int r = square(G, G, NS_C, NS_B, G, M)) return r;                                  // P = b G + c G G
+    } else {
+      if (int r = square(G, G, NS_C, NS_B, G, P1)) return r;
+      if (int r = square(P1, G, 1.f, NS_A, G, H)) return r;                                  // H = a G + P G
+      if (int r = square(P1, H, 1.f, NS_A, H, G)) return r;                                  // G' = a H + P H
+      if (int r = square(G, G, NS_C, NS_B, G, H)) return r;                                  // P'
+      if (int r = square(H, P1, 1.f, NS_A, P1, M, &H, NS_A, plan[k].shift * X_SCALE)) return r;      // N = P' P + a P + a P' + s I
+    }
+    const bool last = k == groups - 1;
     const float f = last ? 1.f / X_SCALE : 1.f;
-    const Out ox = {last ? y : xs[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : ld, nullptr, nullptr};
-    if (int r = apply(batch, rows, cols, X, P, f / X_SCALE, f * NS_A, ox, status, n_sm, stream)) return r;
+    const Out ox = {last ? y : s.x[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : s.ld, nullptr, nullptr};
+    if (int r = apply(batch, rows, cols, X, M, f / X_SCALE, f * plan[k].alpha, ox, status, n_sm, stream)) return r;
   }
   return 0;
 }
 
-// r [batch, rows, cols] (f32 or bf16) -> out (f32 or bf16) = prod_k (a I + P_k) r / norms, the P_k of a forward with keep.
-extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, int rows, int cols, int steps, void* scratch, const void* polys,
+// r [batch, rows, cols] (f32 or bf16) -> out (f32 or bf16) = prod_k (alpha_k I + M_k) r / norms, the maps of a forward with keep.
+extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, int rows, int cols, int steps, void* scratch, const void* maps,
                                         const double* norms, void* out, int out_f32, int* status, cudaStream_t stream) {
   using namespace dttt::ns;
-  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || batch > 65535) return -2;
+  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
   int n_sm;
   if (int r = prepare_device(&n_sm)) return r;
-  const int ld = (cols + 7) / 8 * 8, d = rows < cols ? rows : cols, ldd = (d + 7) / 8 * 8;
-  auto up = [](long long v) { return (v + 255) / 256 * 256; };
-  uint8_t* s = (uint8_t*)scratch;
-  const long long xb = up((long long)batch * rows * ld * 2);
-  void* xs[2] = {s, s + xb};
-  double* partial = (double*)(s + 2 * xb + up((long long)batch * d * ldd * 2));
-  double* own = (double*)((uint8_t*)partial + up((long long)batch * NORM_BLOCKS * 8));
-  if (int r = cast(r_in, f32, batch, rows, cols, partial, R_SCALE, xs[0], ld, own, stream)) return r;
-  for (int i = 0; i < steps; ++i) {
-    const Mat X = {xs[i & 1], rows, cols, ld};
-    const Mat P = {(const uint8_t*)polys + (long long)(steps - 1 - i) * batch * d * ldd * 2, d, d, ldd};
-    const bool last = i == steps - 1;
+  const Scratch s(scratch, batch, rows, cols);
+  if (int r = cast(r_in, f32, batch, rows, cols, s.partial, R_SCALE, s.x[0], s.ld, s.norm, n_sm, stream)) return r;
+  Group plan[MAX_STEPS];
+  const int groups = make_plan(rows, cols, steps, plan);
+  for (int i = 0; i < groups; ++i) {
+    const int k = groups - 1 - i;
+    const Mat X = {s.x[i & 1], rows, cols, s.ld};
+    const Mat M = {(const uint8_t*)maps + (long long)k * batch * s.d * s.ldd * 2, s.d, s.d, s.ldd};
+    const bool last = k == 0;
     const float f = last ? 1.f / R_SCALE : 1.f;
-    const Out o = {last ? out : xs[(i + 1) & 1], last ? (out_f32 ? OUT_F32 : OUT_BF16) : OUT_F16, last ? cols : ld, last ? own : nullptr,
+    const Out o = {last ? out : s.x[(i + 1) & 1], last ? (out_f32 ? OUT_F32 : OUT_BF16) : OUT_F16, last ? cols : s.ld, last ? s.norm : nullptr,
                    last ? norms : nullptr};
-    if (int r = apply(batch, rows, cols, X, P, f / X_SCALE, f * NS_A, o, status, n_sm, stream)) return r;
+    if (int r = apply(batch, rows, cols, X, M, f / X_SCALE, f * plan[k].alpha, o, status, n_sm, stream)) return r;
   }
   return 0;
 }

@@ -847,21 +847,22 @@ def unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure):
 
 # =============================================================================== Newton-Schulz family
 _lib.register("dttt_newton_schulz_scratch", _ll, [_i, _i, _i])
+_lib.register("dttt_newton_schulz_groups", _i, [_i, _i, _i])
 _lib.register("dttt_newton_schulz", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp])
 _lib.register("dttt_newton_schulz_apply", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp])
 _SYMBOL.update(newton_schulz="dttt_newton_schulz")
 
 
 def newton_schulz(g, steps, keep):
-    """``g [B, rows, cols]`` (f32 or bf16, contiguous) -> ``(y bf16, norms [B] f64, polys)``; ``polys`` (f16 ``[steps, B, d, ceil8(d)]``)
-    holds every iteration's polynomial matrix with ``keep``, else scratch."""
+    """``g [B, rows, cols]`` (f32 or bf16, contiguous) -> ``(y bf16, norms [B] f64, maps)``; ``maps`` (f16 ``[groups, B, d, ceil8(d)]``)
+    holds the matrix of every group of iterations with ``keep``, else it is scratch."""
     global LAUNCHES
     B, rows, cols = g.shape
     d, dev = min(rows, cols), g.device
     y = torch.empty((B, rows, cols), dtype=torch.bfloat16, device=dev)
     norms = torch.empty(B, dtype=torch.float64, device=dev)
-    polys = torch.empty((steps if keep else 1, B, d, -(-d // 8) * 8), dtype=torch.float16, device=dev)
     l = _lib.lib()
+    polys = torch.empty((l.dttt_newton_schulz_groups(rows, cols, steps) if keep else 1, B, d, -(-d // 8) * 8), dtype=torch.float16, device=dev)
     scratch = torch.empty(l.dttt_newton_schulz_scratch(B, rows, cols), dtype=torch.uint8, device=dev)
     _launch("newton_schulz", l.dttt_newton_schulz, dev, g.data_ptr(), int(g.dtype == torch.float32), B, rows, cols, steps,
             scratch.data_ptr(), polys.data_ptr(), int(keep), norms.data_ptr(), y.data_ptr(), _lib.status_tensor(dev).data_ptr())
@@ -869,16 +870,16 @@ def newton_schulz(g, steps, keep):
     return y, norms, polys
 
 
-def newton_schulz_apply(r, norms, polys, out_dtype):
+def newton_schulz_apply(r, norms, polys, steps, out_dtype):
     """The linear map of a kept forward applied to ``r [B, rows, cols]`` (f32 or bf16, contiguous)."""
     global LAUNCHES
     B, rows, cols = r.shape
-    steps, dev = polys.shape[0], r.device
+    dev = r.device
     out = torch.empty((B, rows, cols), dtype=out_dtype, device=dev)
     l = _lib.lib()
     scratch = torch.empty(l.dttt_newton_schulz_scratch(B, rows, cols), dtype=torch.uint8, device=dev)
     _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), int(r.dtype == torch.float32), B, rows, cols, steps,
             scratch.data_ptr(), polys.data_ptr(), norms.data_ptr(), out.data_ptr(), int(out_dtype == torch.float32),
             _lib.status_tensor(dev).data_ptr())
-    LAUNCHES += 1 + steps
+    LAUNCHES += 1 + polys.shape[0]
     return out

@@ -25,23 +25,24 @@ class _Apply(torch.autograd.Function):
     """``r -> M r / |g|`` with what a forward kept of ``g``; linear and self-adjoint."""
 
     @staticmethod
-    def forward(ctx, r, norms, polys, dtype):
-        ctx.kept, ctx.dtype = (norms, polys), r.dtype
+    def forward(ctx, r, norms, polys, steps, dtype):
+        ctx.kept, ctx.dtype = (norms, polys, steps), r.dtype
         if isinstance(polys, list):
             return ref.newton_schulz_apply(r, norms, polys).to(dtype)
         from . import kernels
         out_dtype = torch.float32 if dtype == torch.float32 else torch.bfloat16
-        return kernels.newton_schulz_apply(_flat(r), norms, polys, out_dtype).view(r.shape).to(dtype)
+        return kernels.newton_schulz_apply(_flat(r), norms, polys, steps, out_dtype).view(r.shape).to(dtype)
 
     @staticmethod
     def backward(ctx, c):
-        return _Apply.apply(c, *ctx.kept, ctx.dtype), None, None, None
+        return _Apply.apply(c, *ctx.kept, ctx.dtype), None, None, None, None
 
 
 class _NewtonSchulz(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, steps):
-        y, *ctx.kept = _run(g, steps, True)
+        y, norms, polys = _run(g, steps, True)
+        ctx.kept = norms, polys, steps
         ctx.dtype = g.dtype
         return y
 
