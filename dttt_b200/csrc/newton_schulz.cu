@@ -576,11 +576,11 @@ static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, cons
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
-// r (f16, scale S) -> a r + P r: into f16 or, at the end, into the caller's tensor
-static int apply(int batch, int rows, int cols, const Mat& r, const Mat& P, float alpha, float beta, const Out& o, int* status, int n_sm,
-                 cudaStream_t stream) {
-  if (rows <= cols) return product(batch, rows, cols, rows, P, false, r, true, alpha, beta, &r, o, false, status, n_sm, stream);
-  return product(batch, rows, cols, cols, r, false, P, false, alpha, beta, &r, o, false, status, n_sm, stream);
+// r (f16) -> beta r + alpha M r (r M^T of a tall one), or with the transpose of M: into f16 or, at the end, into the caller's tensor
+static int apply(int batch, int rows, int cols, const Mat& r, const Mat& M, bool transposed, float alpha, float beta, const Out& o, int* status,
+                 int n_sm, cudaStream_t stream) {
+  if (rows <= cols) return product(batch, rows, cols, rows, M, transposed, r, true, alpha, beta, &r, o, false, status, n_sm, stream);
+  return product(batch, rows, cols, cols, r, false, M, transposed, alpha, beta, &r, o, false, status, n_sm, stream);
 }
 
 template <class T>
@@ -617,12 +617,13 @@ namespace ns {
 
 // How the iterations are grouped.  Two of them in one,
 //   x'' = (a I + P')(a I + P) x = (a^2 - s) x + N x,   N = P' P + a (P + P') + s I,
-// need G' of the second from G alone: with H = a G + P G, G' = a H + P H.  That replaces one product with x on each side of the
-// group (d^2 L and 2 d^2 L of the longer side L) by three d x d ones, which pays from L = 1.5 d on where the products are large
-// enough to be bound by the tensor cores.  `s` shifts N by its value at the singular value of a matrix with equal ones, so that
-// what rounds is the spread and not the bulk of it; unshifted, or with three iterations in one, the result is twice as far off.
-// The first two and the last two are grouped: 1.4e-3 (before the rounding of the result) as for single steps, in the middle and
-// for later pairs the cancellation costs more.
+// need G' of the second from G alone: with H = (a I + P) G = a G + P G, G' = a H + H P.  That replaces one product with x on each side
+// of the group (d^2 L and 2 d^2 L of the longer side L) by three d x d ones, which pays from about L = 2 d on where the products are
+// large enough to be bound by the tensor cores: 4 x 2048 x 8192, five steps, 2.36 -> 1.77 ms.  `s` shifts N by its value at the singular
+// value of a matrix with equal ones, so that what rounds is the spread and not the bulk of it.  P, P' and G commute only up to
+// their roundings: G' is formed as H P, which is symmetric even so (P H, or N mirrored across its diagonal, is not, and the
+// difference is amplified: 5.2e-3 and 2.5e-3 off instead of 2.2e-3).  The first two and, from five on, the last two are grouped; a
+// pair in the middle, or three in one, loses to the cancellation in N what single steps keep.
 struct Group {
   int steps;
   float alpha, shift;          // x' = alpha x + M x
@@ -630,7 +631,7 @@ struct Group {
 
 static int make_plan(int rows, int cols, int steps, Group* g) {
   const double d = rows < cols ? rows : cols, len = rows < cols ? cols : rows;
-  const bool pairs = d >= 512 && len >= 1.5 * d;
+  const bool pairs = d >= 512 && len >= 2 * d;
   auto q = [](double l) { return (double)NS_A + NS_B * l + NS_C * l * l; };
   double l = 1.0 / d;
   int n = 0;
@@ -701,7 +702,7 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   auto square = [&](const Mat& A, const Mat& B, float alpha, float beta, const Mat& D, const Mat& C, const Mat* D2 = nullptr, float beta2 = 0.f,
                     float diag = 0.f) {
     const Out o = {const_cast<void*>(C.ptr), OUT_F16, ldd, nullptr, nullptr};
-    return product(batch, d, d, d, A, false, B, false, alpha / X_SCALE, beta, &D, o, true, status, n_sm, stream, D2, beta2, diag);
+    return product(batch, d, d, d, A, false, B, false, alpha / X_SCALE, beta, &D, o, D2 == nullptr, status, n_sm, stream, D2, beta2, diag);
   };
   for (int k = 0; k < groups; ++k) {
     const Mat X = {s.x[k & 1], rows, cols, s.ld};
@@ -713,14 +714,14 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
     } else {
       if (int r = square(G, G, NS_C, NS_B, G, P1)) return r;
       if (int r = square(P1, G, 1.f, NS_A, G, H)) return r;                                  // H = a G + P G
-      if (int r = square(P1, H, 1.f, NS_A, H, G)) return r;                                  // G' = a H + P H
+      if (int r = square(H, P1, 1.f, NS_A, H, G)) return r;                                  // G' = a H + H P
       if (int r = square(G, G, NS_C, NS_B, G, H)) return r;                                  // P'
       if (int r = square(H, P1, 1.f, NS_A, P1, M, &H, NS_A, plan[k].shift * X_SCALE)) return r;      // N = P' P + a P + a P' + s I
     }
     const bool last = k == groups - 1;
     const float f = last ? 1.f / X_SCALE : 1.f;
     const Out ox = {last ? y : s.x[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : s.ld, nullptr, nullptr};
-    if (int r = apply(batch, rows, cols, X, M, f / X_SCALE, f * plan[k].alpha, ox, status, n_sm, stream)) return r;
+    if (int r = apply(batch, rows, cols, X, M, false, f / X_SCALE, f * plan[k].alpha, ox, status, n_sm, stream)) return r;
   }
   return 0;
 }
@@ -744,7 +745,7 @@ extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, in
     const float f = last ? 1.f / R_SCALE : 1.f;
     const Out o = {last ? out : s.x[(i + 1) & 1], last ? (out_f32 ? OUT_F32 : OUT_BF16) : OUT_F16, last ? cols : s.ld, last ? s.norm : nullptr,
                    last ? norms : nullptr};
-    if (int r = apply(batch, rows, cols, X, M, f / X_SCALE, f * plan[k].alpha, o, status, n_sm, stream)) return r;
+    if (int r = apply(batch, rows, cols, X, M, true, f / X_SCALE, f * plan[k].alpha, o, status, n_sm, stream)) return r;
   }
   return 0;
 }
