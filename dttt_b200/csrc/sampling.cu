@@ -34,13 +34,15 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 384;
-constexpr int WARPS = THREADS / 32;
+constexpr int MAX_WARPS = 12;
 constexpr int OCTAVES = 256;                 // bins of the octave counts
 constexpr int BINS = 128;                    // of a round of the search
 constexpr int TAB = 32, COPIES = 16;
+constexpr int LIST = 32;
 constexpr int SLICE_MAX = 49152;            // elements of a slice at most (192 KB)
 constexpr int SLICE_GOOD = 16384;           // a slice up to which three CTAs fit an SM
+
+constexpr int SLICE_SMALL = 4096;
 
 enum { PRI_LOGP = 0, PRI_MARGIN = 1, PRI_ENTROPY = 2 };
 
@@ -137,13 +139,14 @@ struct Shared {
   unsigned int above_count[2];
   u64 above_mass[2];
   // this CTA alone
-  float fred[WARPS];
-  double dred[2][WARPS];
-  u64 ured[WARPS], above[WARPS];
-  int ired[WARPS];
+  float fred[MAX_WARPS];
+  double dred[2][MAX_WARPS];
+  u64 ured[MAX_WARPS], above[MAX_WARPS];
+  int ired[MAX_WARPS];
+  unsigned short list[MAX_WARPS][LIST];     // indices of a warp's elements in the search's first range; as many as there are, if they fit
+  int listed[MAX_WARPS];
   u64 tot_mass[BINS];
   unsigned int tot_count[BINS];
-  unsigned int below_count[BINS];           // of the CTAs with a lower rank
   unsigned int octaves[OCTAVES];              // of all CTAs
   uint32_t range[2];
   u64 tot_above_count, tot_above_mass;
@@ -214,21 +217,21 @@ __device__ __forceinline__ int octave_bin(float x, float m, float scale) {
 }
 
 // Sums the counts of all CTAs (thread i: bin i), and the running totals of the elements above.
-__device__ __forceinline__ void gather_counts(Shared& sh, int buf, bool mass) {
+template <int WARPS>
+__device__ __forceinline__ void gather_counts(Shared& sh, int buf) {
   cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
-  for (int i = threadIdx.x; i < BINS; i += THREADS) {
-    unsigned int c = 0, below = 0;
+  const int ranks = (int)cluster.num_blocks();
+  for (int i = threadIdx.x; i < BINS; i += WARPS * 32) {
+    unsigned int c = 0;
     u64 m = 0;
     for (int r = 0; r < ranks; ++r) {
       const Shared* p = cluster.map_shared_rank(&sh, r);
-      if (r == me) below = c;
       c += p->count[buf][i];
-      if (mass) m += p->hmass[buf][i];
+      m += p->hmass[buf][i];
     }
-    sh.tot_count[i] = c; sh.tot_mass[i] = m; sh.below_count[i] = below;
+    sh.tot_count[i] = c; sh.tot_mass[i] = m;
   }
-  if (threadIdx.x == THREADS - 1) {
+  if (threadIdx.x == WARPS * 32 - 1) {
     u64 c = 0, m = 0;
     for (int r = 0; r < ranks; ++r) { const Shared* p = cluster.map_shared_rank(&sh, r); c += p->above_count[buf]; m += p->above_mass[buf]; }
     sh.tot_above_count = c; sh.tot_above_mass = m;
@@ -282,7 +285,19 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
 // The shortest prefix of the row (value descending, index ascending) whose count (MASS false) or mass (MASS true) reaches
 // `target`: 256-way search over the order keys from the range above; a pass over the slice and a cluster barrier per round.  Only
 // elements of the range and, in the first round, those above it cost more than a comparison.
-template <bool MASS>
+// f(x, index, whether there is one) over a warp's elements of the search's first range, or over all of its elements where their
+// list overflowed; all lanes together.
+template <class F>
+__device__ __forceinline__ void for_range(const Shared& sh, const float* xs, Segment seg, int warp, int lane, F f) {
+  const int listed = sh.listed[warp];
+  if (listed <= LIST) {
+    for (int j = lane; j - lane < listed; j += 32) { const int i = j < listed ? sh.list[warp][j] : 0; f(xs[i], i, j < listed); }
+  } else {
+    for (int i = seg.a + lane; i - lane < seg.b; i += 32) f(i < seg.b ? xs[i] : -INFINITY, i, i < seg.b);
+  }
+}
+
+template <int WARPS, bool MASS>
 __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, int bits, int V, u64 target, int& round) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -298,31 +313,62 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
     int shift = 0;
     while ((k1 - k0) >> shift >= BINS) ++shift;
     const float lo = key_value(k0), hi = key_value(k1);
-    for (int i = tid; i < BINS; i += THREADS) { sh.count[buf][i] = 0; sh.hmass[buf][i] = 0; }
+    for (int i = tid; i < BINS; i += WARPS * 32) { sh.count[buf][i] = 0; sh.hmass[buf][i] = 0; }
     if (tid == 0) { sh.above_count[buf] = 0; sh.above_mass[buf] = 0; }
     __syncthreads();
-    unsigned int ac = 0;
-    u64 am = 0;
-    for (int i = seg.a + lane; i < seg.b; i += 32) {
-      const float x = xs[i];
-      if (x >= lo) {
-        if (x > hi) {
-          if (fresh) { ++ac; am += w(x); }
-        } else {
+    // `any`: the lanes that have one.  With many of them equal values meet in one addition: 16-bit logits and flat rows would put
+    // thousands of elements on one counter.
+    auto count = [&](float x, u64 wx, unsigned int any) {
+      if (any >> lane & 1) {
+        int k = 1;
+        bool adds = true;
+        if (__popc(any) >= 8) {
+          const unsigned int peers = __match_any_sync(any, __float_as_uint(x));
+          k = __popc(peers);
+          adds = lane == __ffs(peers) - 1;
+        }
+        if (adds) {
           const uint32_t bin = (order_key(x) - k0) >> shift;
-          atomicAdd(&sh.count[buf][bin], 1u);
-          atomicAdd(&sh.hmass[buf][bin], w(x));
+          atomicAdd(&sh.count[buf][bin], (unsigned int)k);
+          atomicAdd(&sh.hmass[buf][bin], (u64)k * wx);
         }
       }
-    }
+      __syncwarp();
+    };
     if (fresh) {
+      unsigned int ac = 0;
+      u64 am = 0;
+      int listed = 0;
+      for (int i0 = seg.a; i0 < seg.b; i0 += 32) {
+        const int i = i0 + lane;
+        const float x = i < seg.b ? xs[i] : NAN;
+        const unsigned int cand = __ballot_sync(0xffffffffu, x >= lo);
+        if (!cand) continue;
+        const u64 wx = w(x);
+        const unsigned int over = __ballot_sync(0xffffffffu, x > hi), any = cand & ~over;
+        if (over >> lane & 1) { ++ac; am += wx; }
+        if (any) {
+          const int at = listed + __popc(any & ((1u << lane) - 1));
+          if ((any >> lane & 1) && at < LIST) sh.list[warp][at] = (unsigned short)i;
+          listed += __popc(any);
+          count(x, wx, any);
+        }
+      }
       ac = __reduce_add_sync(0xffffffffu, ac);
       am = warp_sum(am);
-      if (lane == 0) sh.above[warp] = am;
-      if (lane == 0 && ac) { atomicAdd(&sh.above_count[buf], ac); atomicAdd(&sh.above_mass[buf], am); }
+      if (lane == 0) {
+        sh.above[warp] = am;
+        sh.listed[warp] = listed;
+        if (ac) { atomicAdd(&sh.above_count[buf], ac); atomicAdd(&sh.above_mass[buf], am); }
+      }
+    } else {
+      for_range(sh, xs, seg, warp, lane, [&](float x, int, bool in) {
+        const unsigned int any = __ballot_sync(0xffffffffu, in && x >= lo && x <= hi);
+        if (any) count(x, w(x), any);
+      });
     }
     cluster.sync();
-    gather_counts(sh, buf, true);
+    gather_counts<WARPS>(sh, buf);
     if (fresh) { above_c = sh.tot_above_count; above_m = sh.tot_above_mass; fresh = false; }
     if (warp == 0) {
       // lane 0 holds the highest bins: running totals from the top
@@ -350,7 +396,8 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
     if (shift == 0 || cnt == 1) {
       Cut c;
       c.lo = key_value(k0); c.hi = key_value(k1); c.first_hi = first_hi;
-      c.before = sh.below_count[bin]; c.here = sh.count[buf][bin];
+      c.before = __reduce_add_sync(0xffffffffu, lane < (int)cluster.block_rank() ? cluster.map_shared_rank(&sh, lane)->count[buf][bin] : 0u);
+      c.here = sh.count[buf][bin];
       if (MASS) {
         const u64 each = mass / cnt;                              // equal values: equal masses
         c.ties = (target - above_m + each - 1) / each;
@@ -368,7 +415,7 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
 
 // One pass over the slice for everything that needs every element: the untempered sum of exponentials, what the priority needs,
 // the tempered masses (per warp, MASS) and the octave counts (HIST).
-template <bool MASS, bool HIST, int PRI>
+template <int WARPS, bool MASS, bool HIST, int PRI>
 __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment seg, float m, float scale, const Weigher& w) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float z = 0, ent = 0, second = -INFINITY;
@@ -402,26 +449,26 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
   }
   if (MASS) { mass = warp_sum(mass - (u64)count * (u64)__double_as_longlong(w.magic)); if (lane == 0) sh.ured[warp] = mass; }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double a = 0, b = 0;
-    float s = -INFINITY;
-    int k = 0;
-    u64 ms = 0;
-    for (int i = 0; i < WARPS; ++i) {
-      a += sh.dred[0][i];
-      if (PRI == PRI_ENTROPY) b += sh.dred[1][i];
-      if (PRI == PRI_MARGIN) { s = fmaxf(s, sh.fred[i]); k += sh.ired[i]; }
-      if (MASS) ms += sh.ured[i];
-    }
-    sh.z = a; sh.ent = b; sh.second = s; sh.at_max = k; sh.whole = ms;
+  if (warp == 0) {                                                 // a value per warp, added up over the lanes
+    const bool in = lane < WARPS;
+    const double zt = warp_sum(in ? sh.dred[0][lane] : 0.0);
+    if (lane == 0) sh.z = zt;
+    if (MASS) { const u64 t = warp_sum(in ? sh.ured[lane] : 0ull); if (lane == 0) sh.whole = sh.mass = t; }
+  } else if (warp == 1 && PRI == PRI_ENTROPY) {
+    const double t = warp_sum(lane < WARPS ? sh.dred[1][lane] : 0.0);
+    if (lane == 0) sh.ent = t;
+  } else if (warp == 1 && PRI == PRI_MARGIN) {
+    const float t = warp_max(lane < WARPS ? sh.fred[lane] : -INFINITY);
+    const int k = __reduce_add_sync(0xffffffffu, lane < WARPS ? sh.ired[lane] : 0);
+    if (lane == 0) { sh.second = t; sh.at_max = k; }
   }
 }
 
-template <bool MASS, bool HIST>
+template <int WARPS, bool MASS, bool HIST>
 __device__ __forceinline__ void whole_pass(int pri, Shared& sh, const float* xs, Segment seg, float m, float scale, const Weigher& w) {
-  if (pri == PRI_LOGP) whole_pass<MASS, HIST, PRI_LOGP>(sh, xs, seg, m, scale, w);
-  else if (pri == PRI_MARGIN) whole_pass<MASS, HIST, PRI_MARGIN>(sh, xs, seg, m, scale, w);
-  else whole_pass<MASS, HIST, PRI_ENTROPY>(sh, xs, seg, m, scale, w);
+  if (pri == PRI_LOGP) whole_pass<WARPS, MASS, HIST, PRI_LOGP>(sh, xs, seg, m, scale, w);
+  else if (pri == PRI_MARGIN) whole_pass<WARPS, MASS, HIST, PRI_MARGIN>(sh, xs, seg, m, scale, w);
+  else whole_pass<WARPS, MASS, HIST, PRI_ENTROPY>(sh, xs, seg, m, scale, w);
 }
 
 __device__ __forceinline__ unsigned int cluster_id() {
@@ -430,8 +477,11 @@ __device__ __forceinline__ unsigned int cluster_id() {
   return r;
 }
 
-template <class T>
-__global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p) {
+static_assert(sizeof(Shared) <= 12600, "three CTAs with slices of 16032 elements (V = 128256) on an SM");
+
+template <class T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const SampleParams p) {
+  constexpr int THREADS = WARPS * 32;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
   float* xs = reinterpret_cast<float*>(smem_raw + ((sizeof(Shared) + 15) / 16) * 16);
@@ -504,15 +554,12 @@ __global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p
     }
   }
   xs += mis;
-  for (int i = tid; i < OCTAVES; i += THREADS) sh.octaves_here[i] = 0;
-  for (int i = tid; i < TAB * COPIES; i += THREADS) sh.tab[i] = ROOTS[i / COPIES];
+  for (int i = tid; i < OCTAVES; i += WARPS * 32) sh.octaves_here[i] = 0;
+  for (int i = tid; i < TAB * COPIES; i += WARPS * 32) sh.tab[i] = ROOTS[i / COPIES];
   mx = warp_max_nan(mx);
   if (lane == 0) sh.fred[warp] = mx;
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < WARPS; ++i) mx = max_nan(mx, sh.fred[i]);
-    sh.m = mx;
-  }
+  if (warp == 0) { mx = warp_max_nan(lane < WARPS ? sh.fred[lane] : -INFINITY); if (lane == 0) sh.m = mx; }
   cluster.sync();
   const float m = warp_max_nan(lane < ranks ? cluster.map_shared_rank(&sh, lane)->m : -INFINITY);
   if (!(m > -INFINITY && m < INFINITY)) {                          // NaN, +inf or nothing above -inf: the same in every CTA of the cluster
@@ -536,11 +583,11 @@ __global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p
 
   // ---- the pass over every element
   const Segment seg = split(0, n, WARPS, warp);
-  if (greedy) whole_pass<false, false>(p.priority, sh, xs, seg, m, scale, w);
-  else if (by_count) whole_pass<false, true>(p.priority, sh, xs, seg, m, scale, w);
-  else if (by_mass) whole_pass<true, true>(p.priority, sh, xs, seg, m, scale, w);
-  else if (by_ratio) whole_pass<false, false>(p.priority, sh, xs, seg, m, scale, w);
-  else whole_pass<true, false>(p.priority, sh, xs, seg, m, scale, w);
+  if (greedy) whole_pass<WARPS, false, false>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_count) whole_pass<WARPS, false, true>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_mass) whole_pass<WARPS, true, true>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_ratio) whole_pass<WARPS, false, false>(p.priority, sh, xs, seg, m, scale, w);
+  else whole_pass<WARPS, true, false>(p.priority, sh, xs, seg, m, scale, w);
 
   // ---- the kept set and its mass
   Cut cut;
@@ -556,29 +603,26 @@ __global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p
     __syncthreads();
     if (lane == 0) sh.ired[warp] = at;
     __syncthreads();
-    if (tid == 0) {
-      for (int i = 1; i < WARPS; ++i) at = min(at, sh.ired[i]);
-      sh.first_max = at;
-    }
+    if (warp == 0) { at = __reduce_min_sync(0xffffffffu, lane < WARPS ? sh.ired[lane] : 0x7fffffff); if (lane == 0) sh.first_max = at; }
   } else if (by_count || by_mass || by_ratio) {
     if (by_ratio) least = __double2float_ru((double)m + sh.temp * log(fmin(min_p, 1.0)));
     if (by_count || by_mass) {
       cluster.sync();
       u64 whole = 0;
       for (int r = 0; r < ranks; ++r) whole += cluster.map_shared_rank(&sh, r)->whole;
-      for (int i = tid; i < OCTAVES; i += THREADS) {
+      for (int i = tid; i < OCTAVES; i += WARPS * 32) {
         unsigned int c = 0;
         for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(&sh, r)->octaves_here[i];
         sh.octaves[i] = c;
       }
       __syncthreads();
       if (by_count) {
-        cut = find_cut<false>(sh, xs, n, w, m, scale, p.scale_bits, p.V, (u64)top_k, round);
+        cut = find_cut<WARPS, false>(sh, xs, n, w, m, scale, p.scale_bits, p.V, (u64)top_k, round);
         whole = cut.mass;
       }
       if (by_mass) {
         const double goal = ceil(fmax(top_p, 0.0) * (double)whole);
-        cut = find_cut<true>(sh, xs, n, w, m, scale, p.scale_bits, p.V, max((u64)1, min(whole, (u64)goal)), round);
+        cut = find_cut<WARPS, true>(sh, xs, n, w, m, scale, p.scale_bits, p.V, max((u64)1, min(whole, (u64)goal)), round);
       }
     }
     if (cut.before + cut.here > cut.ties) {                        // this CTA holds ties that are not kept
@@ -612,17 +656,19 @@ __global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p
     }
     // what lies above the search's first range is summed already, unless min_p cuts into it
     const bool summed = (by_count || by_mass) && least <= cut.first_hi;
-    const float up_to = summed ? cut.first_hi : INFINITY;
     u64 s = 0;
-    for (int i = seg.a + lane; i < seg.b; i += 32)
-      if (xs[i] <= up_to && kept(xs[i], i)) s += w(xs[i]);
-    s = warp_sum(s) + (summed ? sh.above[warp] : 0);
+    if (summed) {
+      for_range(sh, xs, seg, warp, lane, [&](float x, int i, bool in) { if (in && x <= cut.first_hi && kept(x, i)) s += w(x); });
+      s = warp_sum(s) + sh.above[warp];
+    } else {
+      for (int i = seg.a + lane; i < seg.b; i += 32)
+        if (kept(xs[i], i)) s += w(xs[i]);
+      s = warp_sum(s);
+    }
     __syncthreads();
     if (lane == 0) sh.ured[warp] = s;
     __syncthreads();
-    if (tid == 0) { u64 a = 0; for (int i = 0; i < WARPS; ++i) a += sh.ured[i]; sh.mass = a; }
-  } else if (tid == 0) {
-    sh.mass = sh.whole;
+    if (warp == 0) { const u64 t = warp_sum(lane < WARPS ? sh.ured[lane] : 0ull); if (lane == 0) sh.mass = t; }
   }
   cluster.sync();
 
@@ -658,6 +704,7 @@ __global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p
     }
   }
   __syncthreads();
+  cluster.barrier_arrive();                                        // nothing of a peer's memory is read any more
   if (!greedy) {
     const u64 goal = sh.goal, base = sh.base;
     auto answer = [&](int tok, float x) {
@@ -694,7 +741,8 @@ __global__ void __launch_bounds__(THREADS, 3) sample_kernel(const SampleParams p
       }
     }
   }
-  cluster.sync();                                                  // nobody leaves while a peer may still read its memory
+  __syncwarp();
+  cluster.barrier_wait();                                          // nobody leaves while a peer may still read its memory
 }
 
 // Raises a kernel's shared memory limit once per device (`ready`: a bit per device).
@@ -708,17 +756,17 @@ cudaError_t allow_shared(K kernel, int bytes, std::atomic<u64>& ready) {
   return e;
 }
 
-template <class T>
+template <class T, int WARPS>
 int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t s) {
   const size_t smem = ((sizeof(Shared) + 15) / 16) * 16 + ((size_t)p.slice + 16) * sizeof(float);
   constexpr size_t most = ((sizeof(Shared) + 15) / 16) * 16 + ((size_t)SLICE_MAX + 16) * sizeof(float);
   static_assert(most <= 227 * 1024, "a slice has to fit the shared memory of an SM");
   static std::atomic<u64> ready{0};
-  cudaError_t e = allow_shared(sample_kernel<T>, (int)most, ready);
+  cudaError_t e = allow_shared(sample_kernel<T, WARPS>, (int)most, ready);
   if (e != cudaSuccess) return 1000 + (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned int)(rows * ranks));
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(WARPS * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -727,7 +775,7 @@ int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+  e = cudaLaunchKernelEx(&cfg, sample_kernel<T, WARPS>, p);
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
@@ -845,10 +893,12 @@ extern "C" int dttt_sample(const void* logits, int dtype, long long rows, int in
   p.u = u; p.bias = bias; p.t_row = t_row; p.k_row = k_row; p.p_row = p_row; p.m_row = m_row;
   p.temperature = temperature; p.top_p = top_p; p.min_p = min_p; p.top_k = top_k;
   p.tokens = tokens; p.logp = logp; p.prio = prio;
+  // small slices by four warps, so that what a row costs apart from its elements is paid by fewer of them
+  const bool small = p.slice <= SLICE_SMALL;
   switch (dtype) {
-    case 0: return launch_sample<float>(p, rows, ranks, stream);
-    case 1: return launch_sample<__nv_bfloat16>(p, rows, ranks, stream);
-    case 2: return launch_sample<__half>(p, rows, ranks, stream);
+    case 0: return small ? launch_sample<float, 4>(p, rows, ranks, stream) : launch_sample<float, 12>(p, rows, ranks, stream);
+    case 1: return small ? launch_sample<__nv_bfloat16, 4>(p, rows, ranks, stream) : launch_sample<__nv_bfloat16, 12>(p, rows, ranks, stream);
+    case 2: return small ? launch_sample<__half, 4>(p, rows, ranks, stream) : launch_sample<__half, 12>(p, rows, ranks, stream);
   }
   return -2;
 }
