@@ -34,11 +34,11 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int MAX_WARPS = 12;
+constexpr int MAX_WARPS = 16;
 constexpr int OCTAVES = 256;                 // bins of the octave counts
 constexpr int BINS = 128;                    // of a round of the search
 constexpr int TAB = 32, COPIES = 16;
-constexpr int LIST = 32;
+constexpr int LIST = 256;                    // entries of all warps
 constexpr int SLICE_MAX = 49152;            // elements of a slice at most (192 KB)
 constexpr int SLICE_GOOD = 16384;           // a slice up to which three CTAs fit an SM
 
@@ -85,6 +85,11 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -127,12 +132,11 @@ __constant__ double ROOTS[TAB] = {
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 
 struct Shared {
-  // what this CTA tells the others; every exchange has fields of its own, so nothing is overwritten while a peer reads it
+  // what the other CTAs read; nothing of it is overwritten before a cluster barrier that follows their reads
   float m;
-  double z, ent;
-  float second;
-  int at_max, first_max;
-  u64 whole, mass;                          // of the slice; of what is kept of it
+  float z[MAX_WARPS], ent[MAX_WARPS];       // a value per warp (`ent`: of either priority)
+  int at_max[MAX_WARPS], first_max[MAX_WARPS];
+  u64 mass[MAX_WARPS];                      // of every element, or of the kept ones
   unsigned int octaves_here[OCTAVES];
   unsigned int count[2][BINS];              // histograms of the threshold search, alternating between rounds
   u64 hmass[2][BINS];
@@ -140,14 +144,12 @@ struct Shared {
   u64 above_mass[2];
   // this CTA alone
   float fred[MAX_WARPS];
-  double dred[2][MAX_WARPS];
-  u64 ured[MAX_WARPS], above[MAX_WARPS];
-  int ired[MAX_WARPS];
-  unsigned short list[MAX_WARPS][LIST];     // indices of a warp's elements in the search's first range; as many as there are, if they fit
-  int listed[MAX_WARPS];
+  u64 above[MAX_WARPS], sub[MAX_WARPS];
+  int ties[MAX_WARPS], listed[MAX_WARPS];
+  unsigned short list[LIST];                // indices of each warp's elements in the search's first range, if they fit its share
   u64 tot_mass[BINS];
   unsigned int tot_count[BINS];
-  unsigned int octaves[OCTAVES];              // of all CTAs
+  unsigned int octaves[OCTAVES];            // of all CTAs
   uint32_t range[2];
   u64 tot_above_count, tot_above_mass;
   int pick_bin, idx_star;
@@ -155,9 +157,9 @@ struct Shared {
   double tab[TAB * COPIES];
   // this row's parameters, and at the end its answer but for the token
   double temp, min_p, top_p, log2e_t, cut;
-  float scale, logz, pr;
+  float scale, u, logz, pr;
   int top_k, greedy;
-  u64 goal, base;
+  u64 whole, goal, base, mine;
 };
 
 // exp((x - m) / T) as a mass of 2^S units, rounded to nearest.  Table-driven (Tang's scheme, from the mathematics): with
@@ -216,27 +218,32 @@ __device__ __forceinline__ int octave_bin(float x, float m, float scale) {
   return __float_as_int(fminf((m - x) * scale, (float)(OCTAVES - 1)) + 8388608.f) - 0x4b000000;
 }
 
-// Sums the counts of all CTAs (thread i: bin i), and the running totals of the elements above.
-template <int WARPS>
-__device__ __forceinline__ void gather_counts(Shared& sh, int buf) {
+constexpr int MAX_RANKS = 8;
+// The sum over the cluster's CTAs of what `get` takes from one's shared memory; all loads in flight at once.
+template <class V, class F>
+__device__ __forceinline__ V over_ranks(Shared& sh, F get) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks();
-  for (int i = threadIdx.x; i < BINS; i += WARPS * 32) {
-    unsigned int c = 0;
-    u64 m = 0;
-    for (int r = 0; r < ranks; ++r) {
-      const Shared* p = cluster.map_shared_rank(&sh, r);
-      c += p->count[buf][i];
-      m += p->hmass[buf][i];
-    }
-    sh.tot_count[i] = c; sh.tot_mass[i] = m;
+  V v[MAX_RANKS], sum = 0;
+#pragma unroll
+  for (int r = 0; r < MAX_RANKS; ++r) v[r] = r < ranks ? get(*cluster.map_shared_rank(&sh, r)) : V(0);
+#pragma unroll
+  for (int r = 0; r < MAX_RANKS; ++r) sum += v[r];
+  return sum;
+}
+
+// The per-warp values of all CTAs, in order of the slices, over the lanes of a warp: `per` of them to a lane (a CTA's warps are a
+// whole number of lanes).
+template <int WARPS, class V, class F>
+__device__ __forceinline__ V warp_values(Shared& sh, int lane, V none, F get) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int all = (int)cluster.num_blocks() * WARPS, per = max(1, all / 32);
+  V v = none;
+  for (int j = 0; j < per; ++j) {
+    const int e = lane * per + j;
+    if (e < all) v = get(v, *cluster.map_shared_rank(&sh, e / WARPS), e % WARPS);
   }
-  if (threadIdx.x == WARPS * 32 - 1) {
-    u64 c = 0, m = 0;
-    for (int r = 0; r < ranks; ++r) { const Shared* p = cluster.map_shared_rank(&sh, r); c += p->above_count[buf]; m += p->above_mass[buf]; }
-    sh.tot_above_count = c; sh.tot_above_mass = m;
-  }
-  __syncthreads();
+  return v;
 }
 
 // From the octave counts, the range of values that has to hold the last element of the prefix whose count or mass reaches
@@ -247,56 +254,61 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
     constexpr int EACH = OCTAVES / 32;
-    double lo = 0, hi = 0;
+    constexpr float STEP = 0.917004043f;                           // 2^(-1/8); its powers here are off by less than 1e-6
+    const float w_lo = exp2f(-(lane * EACH + 0.5f) / PER_OCTAVE), w_hi = exp2f(-(lane * EACH - 0.5f) / PER_OCTAVE);
+    float lo[EACH], hi[EACH], wl = w_lo, wh = w_hi;
+    float slo = 0, shi = 0;
+#pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      const int b = lane * EACH + j;
-      const double c = (double)sh.octaves[b];
-      lo += MASS ? c * exp2f(-(b + 0.5f) / PER_OCTAVE) : c;
-      hi += MASS ? c * exp2f(-fmaxf(b - 0.5f, 0.f) / PER_OCTAVE) : c;
+      const float c = (float)sh.octaves[lane * EACH + j];
+      slo += MASS ? c * wl : c;
+      shi += MASS ? c * fminf(wh, 1.f) : c;
+      lo[j] = slo; hi[j] = shi;
+      wl *= STEP; wh *= STEP;
     }
-    double slo = lo, shi = hi;
+    float blo = slo, bhi = shi;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double a = __shfl_up_sync(0xffffffffu, slo, o), b = __shfl_up_sync(0xffffffffu, shi, o);
-      if (lane >= o) { slo += a; shi += b; }
+      const float a = __shfl_up_sync(0xffffffffu, blo, o), b = __shfl_up_sync(0xffffffffu, bhi, o);
+      if (lane >= o) { blo += a; bhi += b; }
     }
-    slo -= lo; shi -= hi;
-    const double goal = MASS ? (double)target * unit : (double)target, slack = MASS ? (double)V * unit : 0.0;
+    blo -= slo; bhi -= shi;
+    // counts are whole numbers below 2^24: their float sums are exact
+    const float goal = MASS ? (float)((double)target * unit) : (float)target, slack = MASS ? (float)((double)V * unit) : 0.f;
     int first = OCTAVES - 1, last = OCTAVES - 1;
-    for (int j = 0; j < EACH; ++j) {
-      const int b = lane * EACH + j;
-      const double c = (double)sh.octaves[b];
-      slo += MASS ? c * exp2f(-(b + 0.5f) / PER_OCTAVE) : c;
-      shi += MASS ? c * exp2f(-fmaxf(b - 0.5f, 0.f) / PER_OCTAVE) : c;
-      if (first == OCTAVES - 1 && (MASS ? shi * 1.0001 + slack : shi) >= goal) first = b;
-      if (last == OCTAVES - 1 && (MASS ? slo * 0.9999 - slack : slo) >= goal) last = b;
+#pragma unroll
+    for (int j = EACH - 1; j >= 0; --j) {
+      if ((MASS ? (bhi + hi[j]) * 1.0001f + slack : bhi + hi[j]) >= goal) first = min(first, lane * EACH + j);
+      if ((MASS ? (blo + lo[j]) * 0.9999f - slack : blo + lo[j]) >= goal) last = min(last, lane * EACH + j);
     }
     first = __reduce_min_sync(0xffffffffu, first);
     last = __reduce_min_sync(0xffffffffu, last);
-    if (lane == 0) {
-      const double near = fmax(first - 0.5, 0.0) / scale, far = (last + 0.5) / scale, eps = fabs((double)m) * 1e-6;
-      sh.range[0] = last == OCTAVES - 1 ? 0u : order_key(__double2float_rd((double)m - far * (1 + 1e-5) - eps) + 0.f);
-      sh.range[1] = first == 0 ? 0xffffffffu : order_key(__double2float_ru((double)m - near * (1 - 1e-5) + eps) + 0.f);
+    if (lane < 2) {
+      const float edge = lane ? fmaxf(first - 0.5f, 0.f) * (1.f - 1e-5f) : (last + 0.5f) * (1.f + 1e-5f);
+      const double at = (double)m - (double)edge / (double)scale, eps = fabs((double)m) * 1e-6;
+      sh.range[lane] = lane ? (first == 0 ? 0xffffffffu : order_key(__double2float_ru(at + eps) + 0.f))
+                            : (last == OCTAVES - 1 ? 0u : order_key(__double2float_rd(at - eps) + 0.f));
     }
   }
   __syncthreads();
 }
 
-// The shortest prefix of the row (value descending, index ascending) whose count (MASS false) or mass (MASS true) reaches
-// `target`: 256-way search over the order keys from the range above; a pass over the slice and a cluster barrier per round.  Only
-// elements of the range and, in the first round, those above it cost more than a comparison.
 // f(x, index, whether there is one) over a warp's elements of the search's first range, or over all of its elements where their
 // list overflowed; all lanes together.
-template <class F>
+template <int WARPS, class F>
 __device__ __forceinline__ void for_range(const Shared& sh, const float* xs, Segment seg, int warp, int lane, F f) {
   const int listed = sh.listed[warp];
-  if (listed <= LIST) {
-    for (int j = lane; j - lane < listed; j += 32) { const int i = j < listed ? sh.list[warp][j] : 0; f(xs[i], i, j < listed); }
+  constexpr int ROOM = LIST / WARPS;
+  if (listed <= ROOM) {
+    for (int j = lane; j - lane < listed; j += 32) { const int i = j < listed ? sh.list[warp * ROOM + j] : 0; f(xs[i], i, j < listed); }
   } else {
     for (int i = seg.a + lane; i - lane < seg.b; i += 32) f(i < seg.b ? xs[i] : -INFINITY, i, i < seg.b);
   }
 }
 
+// The shortest prefix of the row (value descending, index ascending) whose count (MASS false) or mass (MASS true) reaches
+// `target`: 128-way search over the order keys from the range above; a pass over the slice and a cluster barrier per round.  Only
+// elements of the range and, in the first round, those above it cost more than a comparison.
 template <int WARPS, bool MASS>
 __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, int bits, int V, u64 target, int& round) {
   cg::cluster_group cluster = cg::this_cluster();
@@ -313,9 +325,6 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
     int shift = 0;
     while ((k1 - k0) >> shift >= BINS) ++shift;
     const float lo = key_value(k0), hi = key_value(k1);
-    for (int i = tid; i < BINS; i += WARPS * 32) { sh.count[buf][i] = 0; sh.hmass[buf][i] = 0; }
-    if (tid == 0) { sh.above_count[buf] = 0; sh.above_mass[buf] = 0; }
-    __syncthreads();
     // `any`: the lanes that have one.  With many of them equal values meet in one addition: 16-bit logits and flat rows would put
     // thousands of elements on one counter.
     auto count = [&](float x, u64 wx, unsigned int any) {
@@ -339,19 +348,29 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
       unsigned int ac = 0;
       u64 am = 0;
       int listed = 0;
-      for (int i0 = seg.a; i0 < seg.b; i0 += 32) {
-        const int i = i0 + lane;
-        const float x = i < seg.b ? xs[i] : NAN;
-        const unsigned int cand = __ballot_sync(0xffffffffu, x >= lo);
-        if (!cand) continue;
-        const u64 wx = w(x);
-        const unsigned int over = __ballot_sync(0xffffffffu, x > hi), any = cand & ~over;
-        if (over >> lane & 1) { ++ac; am += wx; }
-        if (any) {
-          const int at = listed + __popc(any & ((1u << lane) - 1));
-          if ((any >> lane & 1) && at < LIST) sh.list[warp][at] = (unsigned short)i;
-          listed += __popc(any);
-          count(x, wx, any);
+      for (int i0 = seg.a; i0 < seg.b; i0 += 128) {
+        float xk[4];
+        bool some = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          xk[k] = i0 + k * 32 + lane < seg.b ? xs[i0 + k * 32 + lane] : NAN;
+          some |= xk[k] >= lo;
+        }
+        if (!__any_sync(0xffffffffu, some)) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x = xk[k];
+          const unsigned int cand = __ballot_sync(0xffffffffu, x >= lo);
+          if (!cand) continue;
+          const u64 wx = w(x);
+          const unsigned int over = __ballot_sync(0xffffffffu, x > hi), any = cand & ~over;
+          if (over >> lane & 1) { ++ac; am += wx; }
+          if (any) {
+            const int at = listed + __popc(any & ((1u << lane) - 1));
+            if ((any >> lane & 1) && at < LIST / WARPS) sh.list[warp * (LIST / WARPS) + at] = (unsigned short)(i0 + k * 32 + lane);
+            listed += __popc(any);
+            count(x, wx, any);
+          }
         }
       }
       ac = __reduce_add_sync(0xffffffffu, ac);
@@ -362,33 +381,48 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
         if (ac) { atomicAdd(&sh.above_count[buf], ac); atomicAdd(&sh.above_mass[buf], am); }
       }
     } else {
-      for_range(sh, xs, seg, warp, lane, [&](float x, int, bool in) {
+      for_range<WARPS>(sh, xs, seg, warp, lane, [&](float x, int, bool in) {
         const unsigned int any = __ballot_sync(0xffffffffu, in && x >= lo && x <= hi);
         if (any) count(x, w(x), any);
       });
     }
     cluster.sync();
-    gather_counts<WARPS>(sh, buf);
+    for (int i = tid; i < BINS; i += WARPS * 32) {
+      sh.tot_count[i] = over_ranks<unsigned int>(sh, [&](const Shared& q) { return q.count[buf][i]; });
+      sh.tot_mass[i] = over_ranks<u64>(sh, [&](const Shared& q) { return q.hmass[buf][i]; });
+      sh.count[buf ^ 1][i] = 0; sh.hmass[buf ^ 1][i] = 0;             // the next round's; the last round's readers are past the barrier
+    }
+    if (warp == WARPS - 1) {
+      if (lane == 0) sh.tot_above_count = over_ranks<unsigned int>(sh, [&](const Shared& q) { return q.above_count[buf]; });
+      if (lane == 1) sh.tot_above_mass = over_ranks<u64>(sh, [&](const Shared& q) { return q.above_mass[buf]; });
+      if (lane == 2) { sh.above_count[buf ^ 1] = 0; sh.above_mass[buf ^ 1] = 0; }
+    }
+    __syncthreads();
     if (fresh) { above_c = sh.tot_above_count; above_m = sh.tot_above_mass; fresh = false; }
     if (warp == 0) {
       // lane 0 holds the highest bins: running totals from the top
-      u64 c = 0, ms = 0;
-      for (int j = 0; j < BINS / 32; ++j) { const int b = BINS - 1 - (lane * (BINS / 32) + j); c += sh.tot_count[b]; ms += sh.tot_mass[b]; }
-      u64 pc = above_c + warp_scan(c, lane) - c, pm = above_m + warp_scan(ms, lane) - ms;      // before this lane's bins
+      constexpr int EACH = BINS / 32;
+      u64 part[EACH], sum = 0;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) { const int b = BINS - 1 - (lane * EACH + j); part[j] = MASS ? sh.tot_mass[b] : sh.tot_count[b]; sum += part[j]; }
+      u64 run = (MASS ? above_m : above_c) + warp_scan(sum, lane) - sum, at = 0;      // before this lane's bins
       int found = -1;
-      u64 fc = 0, fm = 0;
-      for (int j = 0; j < BINS / 32; ++j) {
-        const int b = BINS - 1 - (lane * (BINS / 32) + j);
-        const u64 reach = MASS ? pm + sh.tot_mass[b] : pc + sh.tot_count[b];
-        if (found < 0 && reach >= target) { found = b; fc = pc; fm = pm; }
-        pc += sh.tot_count[b]; pm += sh.tot_mass[b];
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        if (found < 0 && run + part[j] >= target) { found = BINS - 1 - (lane * EACH + j); at = run; }
+        run += part[j];
       }
       const unsigned int any = __ballot_sync(0xffffffffu, found >= 0);
-      if (lane == (any ? __ffs(any) - 1 : 0)) { sh.pick_bin = max(found, 0); sh.pick_above_count = fc; sh.pick_above_mass = fm; }
+      const int from = any ? __ffs(any) - 1 : 0, bin = max(__shfl_sync(0xffffffffu, found, from), 0);
+      u64 over = 0;                                                  // the other measure of the bins above
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) { const int b = BINS - 1 - (lane * EACH + j); if (!MASS && b > bin) over += sh.tot_mass[b]; }
+      if (!MASS) over = warp_sum(over);
+      if (lane == from) { sh.pick_bin = bin; sh.pick_above_count = at; sh.pick_above_mass = MASS ? at : above_m + over; }
     }
     __syncthreads();
     const uint32_t bin = (uint32_t)sh.pick_bin;
-    above_c = sh.pick_above_count; above_m = sh.pick_above_mass;
+    above_c = MASS ? 0 : sh.pick_above_count; above_m = sh.pick_above_mass;
     const u64 cnt = sh.tot_count[bin], mass = sh.tot_mass[bin];
     const uint32_t low = k0 + (bin << shift);
     k1 = min(low + ((1u << shift) - 1u), k1);
@@ -439,29 +473,15 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
   }
   for (; i < seg.b; i += 32) one(xs[i]);
   const int count = max(0, (seg.b - seg.a - lane + 31) >> 5);
-  const double zs = warp_sum((double)z);
-  if (lane == 0) sh.dred[0][warp] = zs;
-  if (PRI == PRI_ENTROPY) { const double v = warp_sum((double)ent) * 0.6931471805599453; if (lane == 0) sh.dred[1][warp] = v; }
+  z = warp_sum(z);
+  if (lane == 0) sh.z[warp] = z;
+  if (PRI == PRI_ENTROPY) { ent = warp_sum(ent); if (lane == 0) sh.ent[warp] = ent; }
   if (PRI == PRI_MARGIN) {
     second = warp_max(second);
     at_max = __reduce_add_sync(0xffffffffu, at_max);
-    if (lane == 0) { sh.fred[warp] = second; sh.ired[warp] = at_max; }
+    if (lane == 0) { sh.ent[warp] = second; sh.at_max[warp] = at_max; }
   }
-  if (MASS) { mass = warp_sum(mass - (u64)count * (u64)__double_as_longlong(w.magic)); if (lane == 0) sh.ured[warp] = mass; }
-  __syncthreads();
-  if (warp == 0) {                                                 // a value per warp, added up over the lanes
-    const bool in = lane < WARPS;
-    const double zt = warp_sum(in ? sh.dred[0][lane] : 0.0);
-    if (lane == 0) sh.z = zt;
-    if (MASS) { const u64 t = warp_sum(in ? sh.ured[lane] : 0ull); if (lane == 0) sh.whole = sh.mass = t; }
-  } else if (warp == 1 && PRI == PRI_ENTROPY) {
-    const double t = warp_sum(lane < WARPS ? sh.dred[1][lane] : 0.0);
-    if (lane == 0) sh.ent = t;
-  } else if (warp == 1 && PRI == PRI_MARGIN) {
-    const float t = warp_max(lane < WARPS ? sh.fred[lane] : -INFINITY);
-    const int k = __reduce_add_sync(0xffffffffu, lane < WARPS ? sh.ired[lane] : 0);
-    if (lane == 0) { sh.second = t; sh.at_max = k; }
-  }
+  if (MASS) { mass = warp_sum(mass - (u64)count * (u64)__double_as_longlong(w.magic)); if (lane == 0) sh.mass[warp] = mass; }
 }
 
 template <int WARPS, bool MASS, bool HIST>
@@ -480,7 +500,7 @@ __device__ __forceinline__ unsigned int cluster_id() {
 static_assert(sizeof(Shared) <= 12600, "three CTAs with slices of 16032 elements (V = 128256) on an SM");
 
 template <class T, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 1) sample_kernel(const SampleParams p) {
   constexpr int THREADS = WARPS * 32;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
@@ -510,6 +530,8 @@ __global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const Sa
     sh.log2e_t = 1.4426950408889634 / sh.temp;
     sh.cut = (p.scale_bits + 1.5) / sh.log2e_t;
     sh.scale = (float)(PER_OCTAVE * sh.log2e_t);
+    sh.u = p.u[row];
+    for (int b = 0; b < 2; ++b) { sh.above_count[b] = 0; sh.above_mass[b] = 0; }
   }
   float mx = -INFINITY;
   for (int v = v0 + tid; v < v1; v += THREADS * UNROLL) {
@@ -555,6 +577,7 @@ __global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const Sa
   }
   xs += mis;
   for (int i = tid; i < OCTAVES; i += WARPS * 32) sh.octaves_here[i] = 0;
+  for (int i = tid; i < BINS; i += WARPS * 32) { sh.count[0][i] = 0; sh.hmass[0][i] = 0; }
   for (int i = tid; i < TAB * COPIES; i += WARPS * 32) sh.tab[i] = ROOTS[i / COPIES];
   mx = warp_max_nan(mx);
   if (lane == 0) sh.fred[warp] = mx;
@@ -600,22 +623,19 @@ __global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const Sa
     for (int i = seg.a + lane; i < seg.b; i += 32)
       if (xs[i] == m) { at = first + i; break; }
     at = __reduce_min_sync(0xffffffffu, at);
-    __syncthreads();
-    if (lane == 0) sh.ired[warp] = at;
-    __syncthreads();
-    if (warp == 0) { at = __reduce_min_sync(0xffffffffu, lane < WARPS ? sh.ired[lane] : 0x7fffffff); if (lane == 0) sh.first_max = at; }
+    if (lane == 0) sh.first_max[warp] = at;
   } else if (by_count || by_mass || by_ratio) {
     if (by_ratio) least = __double2float_ru((double)m + sh.temp * log(fmin(min_p, 1.0)));
     if (by_count || by_mass) {
       cluster.sync();
-      u64 whole = 0;
-      for (int r = 0; r < ranks; ++r) whole += cluster.map_shared_rank(&sh, r)->whole;
-      for (int i = tid; i < OCTAVES; i += WARPS * 32) {
-        unsigned int c = 0;
-        for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(&sh, r)->octaves_here[i];
-        sh.octaves[i] = c;
+      for (int i = tid; i < OCTAVES; i += WARPS * 32)
+        sh.octaves[i] = over_ranks<unsigned int>(sh, [&](const Shared& q) { return q.octaves_here[i]; });
+      if (warp == WARPS - 1 && !by_count) {
+        const u64 t = warp_sum(warp_values<WARPS>(sh, lane, (u64)0, [](u64 v, const Shared& q, int k) { return v + q.mass[k]; }));
+        if (lane == 0) sh.whole = t;
       }
       __syncthreads();
+      u64 whole = sh.whole;
       if (by_count) {
         cut = find_cut<WARPS, false>(sh, xs, n, w, m, scale, p.scale_bits, p.V, (u64)top_k, round);
         whole = cut.mass;
@@ -634,11 +654,11 @@ __global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const Sa
         int c = 0;
         for (int i = seg.a + lane; i < seg.b; i += 32) c += xs[i] >= cut.lo && xs[i] <= cut.hi;
         c = __reduce_add_sync(0xffffffffu, c);
-        if (lane == 0) sh.ired[warp] = c;
+        if (lane == 0) sh.ties[warp] = c;
         __syncthreads();
         u64 run = 0;
-        for (int i = 0; i < warp; ++i) run += sh.ired[i];
-        if (run < want && run + sh.ired[warp] >= want) {
+        for (int i = 0; i < warp; ++i) run += sh.ties[i];
+        if (run < want && run + sh.ties[warp] >= want) {
           for (int i0 = seg.a; i0 < seg.b; i0 += 32) {
             const int i = i0 + lane;
             const unsigned int hit = __ballot_sync(0xffffffffu, i < seg.b && xs[i] >= cut.lo && xs[i] <= cut.hi);
@@ -658,49 +678,53 @@ __global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const Sa
     const bool summed = (by_count || by_mass) && least <= cut.first_hi;
     u64 s = 0;
     if (summed) {
-      for_range(sh, xs, seg, warp, lane, [&](float x, int i, bool in) { if (in && x <= cut.first_hi && kept(x, i)) s += w(x); });
+      for_range<WARPS>(sh, xs, seg, warp, lane, [&](float x, int i, bool in) { if (in && x <= cut.first_hi && kept(x, i)) s += w(x); });
       s = warp_sum(s) + sh.above[warp];
     } else {
       for (int i = seg.a + lane; i < seg.b; i += 32)
         if (kept(xs[i], i)) s += w(xs[i]);
       s = warp_sum(s);
     }
-    __syncthreads();
-    if (lane == 0) sh.ured[warp] = s;
-    __syncthreads();
-    if (warp == 0) { const u64 t = warp_sum(lane < WARPS ? sh.ured[lane] : 0ull); if (lane == 0) sh.mass = t; }
+    if (lane == 0) sh.mass[warp] = s;
   }
   cluster.sync();
 
   // ---- totals of the cluster, the draw
   if (warp == 0) {
-    const Shared* q = cluster.map_shared_rank(&sh, lane < ranks ? lane : 0);
-    const bool in = lane < ranks;
-    const double z = warp_sum(in ? q->z : 0.0);
-    const u64 part = in && !greedy ? q->mass : 0, upto = warp_scan(part, lane);
-    const u64 total = __shfl_sync(0xffffffffu, upto, 31), base = __shfl_sync(0xffffffffu, upto - part, me);
+    if (greedy) {
+      const int at = __reduce_min_sync(0xffffffffu, warp_values<WARPS>(sh, lane, 0x7fffffff, [](int v, const Shared& q, int k) { return min(v, q.first_max[k]); }));
+      if (me == 0 && lane == 0) p.tokens[row] = at;
+    } else {
+      const u64 part = warp_values<WARPS>(sh, lane, (u64)0, [](u64 v, const Shared& q, int k) { return v + q.mass[k]; });
+      const u64 upto = warp_scan(part, lane), total = __shfl_sync(0xffffffffu, upto, 31);
+      const int each = WARPS / max(1, ranks * WARPS / 32);           // lanes to a CTA
+      const u64 base = __shfl_sync(0xffffffffu, upto - part, me * each);
+      const u64 end = __shfl_sync(0xffffffffu, upto, (me + 1) * each - 1);
+      if (lane == 0) {
+        const double u = (double)sh.u;
+        const u64 goal = u > 0 ? (u64)(fmin(u, 1.0) * (double)total) : 0;
+        sh.goal = min(goal, total - 1);
+        sh.base = base; sh.mine = end - base;
+      }
+    }
+  } else if (warp == 1) {
+    const double z = warp_sum(warp_values<WARPS>(sh, lane, 0.0, [](double v, const Shared& q, int k) { return v + (double)q.z[k]; }));
     const float logz = logf((float)z);
     float pr = 0.f;
     if (p.priority == PRI_MARGIN) {
-      const float second = warp_max(in ? q->second : -INFINITY);
-      const int at_max = __reduce_add_sync(0xffffffffu, in ? q->at_max : 0);
+      const float second = warp_max(warp_values<WARPS>(sh, lane, -INFINITY, [](float v, const Shared& q, int k) { return fmaxf(v, q.ent[k]); }));
+      const int at_max = __reduce_add_sync(0xffffffffu, warp_values<WARPS>(sh, lane, 0, [](int v, const Shared& q, int k) { return v + q.at_max[k]; }));
       pr = at_max > 1 ? 0.f : (float)((1.0 - (double)__expf(second - m)) / z);
     } else if (p.priority == PRI_ENTROPY) {
-      const double ent = warp_sum(in ? q->ent : 0.0);
-      pr = (float)(ent / z - (double)logz);
+      const double ent = warp_sum(warp_values<WARPS>(sh, lane, 0.0, [](double v, const Shared& q, int k) { return v + (double)q.ent[k]; }));
+      pr = (float)(ent * 0.6931471805599453 / z - (double)logz);
     }
-    if (greedy) {
-      const int at = __reduce_min_sync(0xffffffffu, in ? q->first_max : 0x7fffffff);
-      if (me == 0 && lane == 0) {
-        p.tokens[row] = at;
+    if (lane == 0) {
+      sh.logz = logz; sh.pr = pr;
+      if (greedy && me == 0) {
         p.logp[row] = -logz;
         if (p.priority != PRI_LOGP) p.prio[row] = pr;
       }
-    } else if (lane == 0) {
-      const double u = (double)p.u[row];
-      const u64 goal = u > 0 ? (u64)(fmin(u, 1.0) * (double)total) : 0;
-      sh.goal = min(goal, total - 1);
-      sh.base = base; sh.logz = logz; sh.pr = pr;
     }
   }
   __syncthreads();
@@ -712,20 +736,19 @@ __global__ void __launch_bounds__(WARPS * 32, 36 / WARPS) sample_kernel(const Sa
       p.logp[row] = (x - m) - sh.logz;
       if (p.priority != PRI_LOGP) p.prio[row] = sh.pr;
     };
-    if (goal >= base && goal < base + sh.mass) {                   // the draw falls into this slice
+    if (goal >= base && goal < base + sh.mine) {                   // the draw falls into this slice
       u64 run = base;
       int own = 0;
-      while (own < WARPS - 1 && run + sh.ured[own] <= goal) run += sh.ured[own++];
+      while (own < WARPS - 1 && run + sh.mass[own] <= goal) run += sh.mass[own++];
       const Segment big = split(0, n, WARPS, own);
       const Segment part = split(big.a, big.b, WARPS, warp);
       u64 s = 0;
       for (int i = part.a + lane; i < part.b; i += 32)
         if (kept(xs[i], i)) s += w(xs[i]);
       s = warp_sum(s);
+      if (lane == 0) sh.sub[warp] = s;
       __syncthreads();
-      if (lane == 0) sh.ured[warp] = s;
-      __syncthreads();
-      for (int i = 0; i < warp; ++i) run += sh.ured[i];
+      for (int i = 0; i < warp; ++i) run += sh.sub[i];
       if (goal >= run && goal < run + s) {
         for (int i0 = part.a; i0 < part.b; i0 += 32) {
           const int i = i0 + lane;
@@ -777,6 +800,15 @@ int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, sample_kernel<T, WARPS>, p);
   return e == cudaSuccess ? 0 : 1000 + (int)e;
+}
+
+// Small slices take four warps, so that fewer of them pay what a row costs apart from its elements; where the rows leave SMs free
+// sixteen share the slice, else eight (three CTAs to an SM).
+template <class T>
+int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t s) {
+  if (p.slice <= SLICE_SMALL) return launch_sample<T, 4>(p, rows, ranks, s);
+  if (rows * ranks <= 148) return launch_sample<T, 16>(p, rows, ranks, s);
+  return launch_sample<T, 8>(p, rows, ranks, s);
 }
 
 // ------------------------------------------------------------------------------------------------------ unmask
@@ -893,12 +925,10 @@ extern "C" int dttt_sample(const void* logits, int dtype, long long rows, int in
   p.u = u; p.bias = bias; p.t_row = t_row; p.k_row = k_row; p.p_row = p_row; p.m_row = m_row;
   p.temperature = temperature; p.top_p = top_p; p.min_p = min_p; p.top_k = top_k;
   p.tokens = tokens; p.logp = logp; p.prio = prio;
-  // small slices by four warps, so that what a row costs apart from its elements is paid by fewer of them
-  const bool small = p.slice <= SLICE_SMALL;
   switch (dtype) {
-    case 0: return small ? launch_sample<float, 4>(p, rows, ranks, stream) : launch_sample<float, 12>(p, rows, ranks, stream);
-    case 1: return small ? launch_sample<__nv_bfloat16, 4>(p, rows, ranks, stream) : launch_sample<__nv_bfloat16, 12>(p, rows, ranks, stream);
-    case 2: return small ? launch_sample<__half, 4>(p, rows, ranks, stream) : launch_sample<__half, 12>(p, rows, ranks, stream);
+    case 0: return launch_sample<float>(p, rows, ranks, stream);
+    case 1: return launch_sample<__nv_bfloat16>(p, rows, ranks, stream);
+    case 2: return launch_sample<__half>(p, rows, ranks, stream);
   }
   return -2;
 }
