@@ -768,6 +768,271 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
   cluster.barrier_wait();                                          // nobody leaves while a peer may still read its memory
 }
 
+// ------------------------------------------------------------------------------------------------ the untruncated draw
+// Without top-k, top-p and min-p nothing has to wait for the row's maximum: a warp reads a chunk of 1024 elements into registers,
+// takes the chunk's own maximum, and leaves the chunk's sums relative to it (the masses as integers, as above).  A second launch, a
+// warp per row, brings them to the row's maximum in 64 bits, finds the chunk that holds the draw and reads it once more.  Chunks
+// start at 16-byte boundaries, so the first may be short.
+constexpr int CHUNK = 1024, CHUNK_BITS = 50;      // 1024 2^50 <= 2^62
+constexpr long long STREAM_LEAST = 2ll << 20;     // elements from which two launches beat one with its cluster barriers
+
+struct __align__(16) Chunk {
+  float m, z, e;               // maximum (NaN or +inf if there is one), sum of exp(x - m), the priority's own value
+  int at_max;                  // elements at the maximum (margin)
+  u64 mass;
+  int first, pad;              // index of the first element at the maximum
+};
+
+template <class T>
+struct RowView {
+  const T* src;
+  const float* bias;
+  int mis, chunks;
+  __device__ __forceinline__ RowView(const SampleParams& p, unsigned int row) {
+    const unsigned int outer = row / (unsigned int)p.inner;
+    src = reinterpret_cast<const T*>(p.logits) + outer * p.s_outer + (row - outer * (unsigned int)p.inner) * p.s_inner;
+    bias = p.bias ? p.bias + (long long)outer * p.V : nullptr;
+    constexpr int VEC = 16 / (int)sizeof(T);
+    mis = (int)((reinterpret_cast<uintptr_t>(src) / sizeof(T)) % VEC);
+    chunks = (mis + p.V + CHUNK - 1) / CHUNK;
+  }
+  // the lane's elements of chunk c: pieces of 16 bytes, 32 lanes side by side; -inf where the row has none.  Element k of them has index
+  // c CHUNK - mis + ((k / VEC) 32 + lane) VEC + k % VEC.
+  __device__ __forceinline__ void load(int V, int c, int lane, float (&x)[32]) const {
+    constexpr int VEC = 16 / (int)sizeof(T), PIECES = 32 / VEC;
+    const int at0 = c * CHUNK - mis + lane * VEC;
+    uint4 raw[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int at = at0 + j * 32 * VEC;
+      if (at >= 0 && at + VEC <= V) {
+        raw[j] = __ldcs(reinterpret_cast<const uint4*>(src + at));
+      } else {
+        T e[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) e[k] = at + k >= 0 && at + k < V ? src[at + k] : T(-INFINITY);
+        raw[j] = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[j * VEC + k] = to_f32(reinterpret_cast<const T*>(&raw[j])[k]) + 0.f;
+    if (bias) {
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const int i = at0 + j * 32 * VEC + k;
+          if (i >= 0 && i < V) x[j * VEC + k] = x[j * VEC + k] + __ldg(bias + i) + 0.f;
+        }
+    }
+  }
+};
+
+__device__ __forceinline__ double row_temperature(const SampleParams& p, unsigned int row) {
+  const double t = p.t_row ? (double)p.t_row[row] : p.temperature;
+  return t > 0 ? fmin(fmax(t, 1e-6), 1e6) : 0.0;                   // 0: greedy
+}
+
+// the masses of one chunk, relative to its maximum
+__device__ __forceinline__ Weigher chunk_weigher(double temp, float m, const double* tab) {
+  const double log2e_t = 1.4426950408889634 / temp;
+  Weigher w;
+  w.c = TAB * log2e_t;
+  w.mc = -(double)m * w.c;
+  w.magic = __hiloint2double(0x3ff80000 + ((52 - CHUNK_BITS) << 20), 0);
+  w.least = __double2float_rd((double)m - (CHUNK_BITS + 1.5) / log2e_t);
+  w.tab = tab;
+  return w;
+}
+
+constexpr int STREAM_THREADS = 256;
+
+template <class T, int PRI>
+__global__ void __launch_bounds__(STREAM_THREADS, 3) chunk_kernel(const SampleParams p, unsigned int rows, unsigned int most, Chunk* __restrict__ out) {
+  __shared__ double tab[TAB * COPIES];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < TAB * COPIES; i += STREAM_THREADS) tab[i] = ROOTS[i / COPIES];
+  __syncthreads();
+  const unsigned int all = rows * most, step = gridDim.x * (STREAM_THREADS / 32);      // below 2^31 (the launcher)
+  for (unsigned int t = blockIdx.x * (STREAM_THREADS / 32) + warp; t < all; t += step) {
+    const unsigned int row = t / most;
+    const int c = (int)(t - row * most);
+    const RowView<T> view(p, row);
+    if (c >= view.chunks) continue;
+    const double temp = row_temperature(p, row);
+    float x[32];
+    view.load(p.V, c, lane, x);
+    float m = x[0];
+#pragma unroll
+    for (int k = 1; k < 32; ++k) m = max_nan(m, x[k]);
+    m = warp_max_nan(m);
+    Chunk r = {m, 0.f, PRI == PRI_MARGIN ? -INFINITY : 0.f, 0, 0, 0x7fffffff, 0};
+    if (m > -INFINITY && m < INFINITY) {
+      float z = 0, e = r.e;
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const float y = (x[k] - m) * 1.44269504f, v = ex2(y);
+        z += v;
+        if (PRI == PRI_ENTROPY) e = fmaf(v, fmaxf(y, -1e4f), e);
+        if (PRI == PRI_MARGIN) { n += x[k] == m; e = x[k] < m ? fmaxf(e, x[k]) : e; }
+      }
+      r.z = warp_sum(z);
+      if (PRI == PRI_ENTROPY) r.e = warp_sum(e);
+      if (PRI == PRI_MARGIN) { r.e = warp_max(e); r.at_max = __reduce_add_sync(0xffffffffu, n); }
+      if (temp > 0) {
+        const Weigher w = chunk_weigher(temp, m, tab + (lane & (COPIES - 1)));
+        u64 mass = 0;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) mass += w.raw(x[k]);
+        r.mass = warp_sum(mass - 32 * (u64)__double_as_longlong(w.magic));
+      } else {
+        constexpr int VEC = 16 / (int)sizeof(T);
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int k = 31; k >= 0; --k)
+          if (x[k] == m) at = c * CHUNK - view.mis + ((k / VEC) * 32 + lane) * VEC + k % VEC;
+        r.first = __reduce_min_sync(0xffffffffu, at);
+      }
+    }
+    if (lane == 0) out[t] = r;
+  }
+}
+
+// A warp per row.
+template <class T>
+__global__ void __launch_bounds__(32) chunk_draw_kernel(const SampleParams p, int most, const Chunk* __restrict__ in) {
+  __shared__ double tab[TAB * COPIES];
+  const int lane = threadIdx.x;
+  const unsigned int row = blockIdx.x;
+  const RowView<T> view(p, row);
+  const Chunk* r = in + (long long)row * most;
+  const double temp = row_temperature(p, row), u = (double)p.u[row];
+  for (int i = lane; i < TAB * COPIES; i += 32) tab[i] = ROOTS[i / COPIES];
+  __syncwarp();
+  const int per = (view.chunks + 31) / 32, c0 = min(view.chunks, lane * per), c1 = min(view.chunks, c0 + per);      // in order over the lanes
+  float m = -INFINITY;
+  for (int c = c0; c < c1; ++c) m = max_nan(m, r[c].m);
+  m = warp_max_nan(m);
+  if (!(m > -INFINITY && m < INFINITY)) {
+    if (lane == 0) { p.tokens[row] = -1; p.logp[row] = NAN; if (p.priority != PRI_LOGP) p.prio[row] = NAN; }
+    return;
+  }
+  // everything relative to the row's maximum, in 64 bits
+  double z = 0, ent = 0, mass = 0;
+  float second = -INFINITY;
+  int at_max = 0, first = 0x7fffffff;
+  for (int c = c0; c < c1; ++c) {
+    const Chunk q = r[c];
+    if (q.m == -INFINITY) continue;
+    const double d = (double)q.m - (double)m, f = exp(d);
+    z += (double)q.z * f;
+    if (p.priority == PRI_ENTROPY) ent += ((double)q.e * 0.6931471805599453 + (double)q.z * d) * f;      // sum e^(x - m) (x - m)
+    if (p.priority == PRI_MARGIN) {
+      second = fmaxf(second, q.m == m ? q.e : q.m);
+      if (q.m == m) at_max += q.at_max;
+    }
+    if (temp > 0) mass += (double)q.mass * exp(d / temp);
+    else if (q.m == m) first = min(first, q.first);
+  }
+  z = warp_sum(z);
+  const float logz = logf((float)z);
+  float pr = 0.f;
+  if (p.priority == PRI_MARGIN) {
+    second = warp_max(second);
+    at_max = __reduce_add_sync(0xffffffffu, at_max);
+    pr = at_max > 1 ? 0.f : (float)((1.0 - (double)__expf(second - m)) / z);
+  } else if (p.priority == PRI_ENTROPY) {
+    pr = (float)(warp_sum(ent) / z - (double)logz);
+  }
+  auto answer = [&](int tok, float x) {
+    p.tokens[row] = tok;
+    p.logp[row] = (x - m) - logz;
+    if (p.priority != PRI_LOGP) p.prio[row] = pr;
+  };
+  if (!(temp > 0)) {
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) answer(first, m);
+    return;
+  }
+  double upto = mass;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  const double total = __shfl_sync(0xffffffffu, upto, 31), goal = u > 0 ? fmin(u, 1.0) * total : 0.0;
+  // the first lane, and its first chunk, whose running mass exceeds the goal; rounding at the very end: the last chunk with a mass
+  const unsigned int past = __ballot_sync(0xffffffffu, upto > goal), some = __ballot_sync(0xffffffffu, mass > 0);
+  const int own = past & some ? __ffs(past & some) - 1 : 31 - __clz(some);
+  int chunk = -1;
+  double rest = 0;
+  if (lane == own) {
+    double run = upto - mass;
+    for (int c = c0; c < c1; ++c) {
+      const Chunk q = r[c];
+      if (q.m == -INFINITY || q.mass == 0) continue;
+      const double f = exp(((double)q.m - (double)m) / temp), v = (double)q.mass * f;
+      if (!(v > 0)) continue;
+      chunk = c;
+      rest = (goal - run) / f;
+      if (run + v > goal) break;
+      run += v;
+    }
+  }
+  chunk = __shfl_sync(0xffffffffu, chunk, own);
+  rest = __shfl_sync(0xffffffffu, rest, own);
+  const u64 held = r[chunk].mass;
+  const u64 want = min(rest > 0 ? (u64)rest : 0, held - 1);
+  const float mc = r[chunk].m;
+  const Weigher w = chunk_weigher(temp, mc, tab + (lane & (COPIES - 1)));
+  float x[32];
+  view.load(p.V, chunk, lane, x);
+  constexpr int VEC = 16 / (int)sizeof(T), PIECES = 32 / VEC;
+  u64 run = 0;
+  for (int j = 0; j < PIECES; ++j) {
+    u64 s = 0;
+#pragma unroll
+    for (int jj = 0; jj < PIECES; ++jj)
+      if (jj == j)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s += w(x[jj * VEC + k]);
+    const u64 inc = run + warp_scan(s, lane);
+    const unsigned int hit = __ballot_sync(0xffffffffu, inc > want);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) {
+        u64 before = inc - s;
+        bool done = false;
+#pragma unroll
+        for (int jj = 0; jj < PIECES; ++jj)
+          if (jj == j)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+              before += w(x[jj * VEC + k]);
+              if (!done && before > want) { done = true; answer(chunk * CHUNK - view.mis + (j * 32 + lane) * VEC + k, x[jj * VEC + k]); }
+            }
+      }
+      break;
+    }
+    run = __shfl_sync(0xffffffffu, inc, 31);
+  }
+}
+
+template <class T>
+int launch_stream(const SampleParams& p, long long rows, Chunk* scratch, cudaStream_t s) {
+  const int most = (p.V + 7 + CHUNK - 1) / CHUNK;
+  const long long warps = rows * most, blocks = (warps + STREAM_THREADS / 32 - 1) / (STREAM_THREADS / 32);
+  const int grid = (int)(blocks < 148 * 3 ? blocks : 148 * 3);
+  if (p.priority == PRI_LOGP) chunk_kernel<T, PRI_LOGP><<<grid, STREAM_THREADS, 0, s>>>(p, (unsigned int)rows, most, scratch);
+  else if (p.priority == PRI_MARGIN) chunk_kernel<T, PRI_MARGIN><<<grid, STREAM_THREADS, 0, s>>>(p, (unsigned int)rows, most, scratch);
+  else chunk_kernel<T, PRI_ENTROPY><<<grid, STREAM_THREADS, 0, s>>>(p, (unsigned int)rows, most, scratch);
+  chunk_draw_kernel<T><<<(unsigned int)rows, 32, 0, s>>>(p, most, scratch);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 1000 + (int)e;
+}
+
 // Raises a kernel's shared memory limit once per device (`ready`: a bit per device).
 template <class K>
 cudaError_t allow_shared(K kernel, int bytes, std::atomic<u64>& ready) {
@@ -907,12 +1172,19 @@ extern "C" int dttt_sample_ranks(int V) {
   return V <= 8 * SLICE_MAX ? 8 : 0;
 }
 
+// Bytes of scratch that dttt_sample wants for `rows` rows whose draw no parameter truncates (0: none).
+extern "C" long long dttt_sample_scratch(long long rows, int V) {
+  const long long most = (V + 7ll + CHUNK - 1) / CHUNK;
+  return rows * V >= STREAM_LEAST && rows * most <= 0x7fffffffll ? rows * most * (long long)sizeof(Chunk) : 0;
+}
+
 // logits: rows [outer, inner] of V elements (dtype 0 f32, 1 bf16, 2 f16), element strides s_outer / s_inner, contiguous along V.
-// *_row: per-row parameter arrays or null (then the scalar).  Outputs contiguous [rows].
+// *_row: per-row parameter arrays or null (then the scalar).  Outputs contiguous [rows].  `scratch` (16-byte aligned): of
+// dttt_sample_scratch, only for rows that no parameter truncates; null takes the kernel on clusters.
 extern "C" int dttt_sample(const void* logits, int dtype, long long rows, int inner, long long s_outer, long long s_inner, int V,
                            const float* u, const float* bias, double temperature, const float* t_row, int top_k, const int* k_row,
                            double top_p, const float* p_row, double min_p, const float* m_row, int priority, long long* tokens,
-                           float* logp, float* prio, cudaStream_t stream) {
+                           float* logp, float* prio, void* scratch, cudaStream_t stream) {
   if (rows <= 0) return 0;
   const int ranks = dttt_sample_ranks(V);
   if (ranks == 0 || inner <= 0 || rows * ranks > 0x7fffffffll) return -2;
@@ -925,6 +1197,14 @@ extern "C" int dttt_sample(const void* logits, int dtype, long long rows, int in
   p.u = u; p.bias = bias; p.t_row = t_row; p.k_row = k_row; p.p_row = p_row; p.m_row = m_row;
   p.temperature = temperature; p.top_p = top_p; p.min_p = min_p; p.top_k = top_k;
   p.tokens = tokens; p.logp = logp; p.prio = prio;
+  if (scratch) {
+    switch (dtype) {
+      case 0: return launch_stream<float>(p, rows, (Chunk*)scratch, stream);
+      case 1: return launch_stream<__nv_bfloat16>(p, rows, (Chunk*)scratch, stream);
+      case 2: return launch_stream<__half>(p, rows, (Chunk*)scratch, stream);
+    }
+    return -2;
+  }
   switch (dtype) {
     case 0: return launch_sample<float>(p, rows, ranks, stream);
     case 1: return launch_sample<__nv_bfloat16>(p, rows, ranks, stream);

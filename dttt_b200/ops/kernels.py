@@ -788,7 +788,8 @@ def gdn_chunk_bwd(k, v, beta, log_alpha, S0, gS):
 # =============================================================================== decoding family
 _d = _ct.c_double
 _lib.register("dttt_sample_ranks", _i, [_i])
-_lib.register("dttt_sample", _i, [_vp, _i, _ll, _i, _ll, _ll, _i, _vp, _vp, _d, _vp, _i, _vp, _d, _vp, _d, _vp, _i, _vp, _vp, _vp, _vp])
+_lib.register("dttt_sample_scratch", _ll, [_ll, _i])
+_lib.register("dttt_sample", _i, [_vp, _i, _ll, _i, _ll, _ll, _i, _vp, _vp, _d, _vp, _i, _vp, _d, _vp, _d, _vp, _i, _vp, _vp, _vp, _vp, _vp])
 _lib.register("dttt_unmask", _i, [_vp] * 8 + [_f, _i] + [_vp] * 4 + [_i, _i, _vp])
 _SYMBOL.update(sampling="dttt_sample")
 _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -826,9 +827,17 @@ def sample(x, u, bias, temperature, top_k, top_p, min_p, priority):
     prio = out[1] if priority else logp
     if outer and inner:
         num = lambda p, off: (off, p.data_ptr()) if isinstance(p, torch.Tensor) else (p, None)
-        _launch("sample", _lib.lib().dttt_sample, dev, x.data_ptr(), _LOGIT_TYPES[x.dtype], outer * inner, inner, x.stride(0), x.stride(1), V,
+        l, scratch = _lib.lib(), None
+        if type(top_p) is float and top_p == 1.0 and type(min_p) is float and min_p == 0.0 and type(top_k) is int and not 0 < top_k < V:
+            size = l.dttt_sample_scratch(outer * inner, V)               # nothing is truncated: two passes over chunks from some size on
+            scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        _launch("sample", l.dttt_sample, dev, x.data_ptr(), _LOGIT_TYPES[x.dtype], outer * inner, inner, x.stride(0), x.stride(1), V,
                 u.data_ptr(), None if bias is None else bias.data_ptr(), *num(temperature, 1.0), *num(top_k, 0), *num(top_p, 1.0),
-                *num(min_p, 0.0), priority, tokens.data_ptr(), logp.data_ptr(), prio.data_ptr())
+                *num(min_p, 0.0), priority, tokens.data_ptr(), logp.data_ptr(), prio.data_ptr(),
+                None if scratch is None else scratch.data_ptr())
+        if scratch is not None:
+            global LAUNCHES
+            LAUNCHES += 1
     return tokens, logp, prio
 
 

@@ -66,7 +66,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Param =
     not read by the host and are taken as ``temperature <= 0``: greedy, else clamped to [1e-6, 1e6]; ``top_k <= 0`` or ``>= V``:
     off; ``top_p >= 1``: off, ``<= 0``: the best token alone; ``min_p <= 0``: off, above 1: as 1; NaN: as off (``temperature``:
     greedy).  ``u`` outside [0, 1) is clamped, NaN taken as 0.  A row without a distribution (NaN or +inf in it, or every token
-    at -inf) gives token -1 and NaN.  ``V`` up to 393216 on a CUDA device."""
+    at -inf) gives token -1 and NaN.  On a CUDA device ``V`` goes up to 393216."""
     rows, dev = logits.shape[:-1], logits.device
     if not rows or logits.shape[-1] == 0:
         raise ValueError(f"sample_tokens: logits {tuple(logits.shape)}, at least [rows, V] are wanted")

@@ -121,13 +121,33 @@ def test_every_draw_number_of_one_row():
     assert (out.tokens.diff() >= 0).all()
 
 
+@pytest.mark.parametrize("V", [1000, 2049, 32001, 128256, 390001])
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.0), dict(temperature=0.6), dict(temperature=1e-6), dict(temperature=1e6)])
+def test_untruncated_draws_over_chunks(V, kw):
+    """Enough elements for the two passes over chunks: every type, priority, ragged row starts, bias, rows without a distribution."""
+    rows = -(-(2 << 20) // V) + 3
+    for dtype, priority in ((torch.float32, "entropy"), (torch.bfloat16, "margin"), (torch.float16, "logp")):
+        for kind in ("zipf", "ties", "few"):
+            x, u = logits((1, rows + 1), V + 3, dtype, seed=V, kind=kind)
+            x, u = x[:, 1:, 3:], u[:, 1:].clone()
+            x[0, 0] = float("-inf")
+            x[0, 1, V // 2] = float("nan")
+            x[0, 2, V - 1] = float("inf")
+            u[0, 3], u[0, 4], u[0, 5] = 0.0, 1.0, 1 - 2 ** -24
+            bias = torch.where(torch.rand(1, V, device="cuda") < 0.2, -2.0, 0.0)
+            out = check(x, u, priority, bias=bias if kind == "zipf" else None, **kw)
+            assert (out.tokens[0, :3] == -1).all() and (out.tokens[0, 3:] >= 0).all()
+    t = torch.rand(1, rows, device="cuda") - 0.3                            # greedy rows among drawn ones
+    check(*logits((1, rows), V, seed=1), temperature=t)
+
+
 def test_above_the_three_cta_slices_and_refusal():
     from dttt_b200.ops.sampling import sample_tokens
     for V in (131073, 393216):
         for kw in (dict(top_p=0.9), dict(top_k=50), dict()):
             check(*logits((1, 2), V), **kw)
     with pytest.raises(ValueError, match="393216"):
-        sample_tokens(torch.zeros(1, 393217, device="cuda"), torch.zeros(1, device="cuda"))
+        sample_tokens(torch.zeros(1, 393217, device="cuda"), torch.zeros(1, device="cuda"), top_k=5)
     with pytest.raises(ValueError, match="u "):
         sample_tokens(torch.zeros(1, 10, device="cuda"), torch.zeros(1))
 
