@@ -37,7 +37,7 @@ typedef unsigned long long u64;
 constexpr int MAX_WARPS = 16;
 constexpr int OCTAVES = 256;                 // bins of the octave counts
 constexpr int BINS = 128;                    // of a round of the search
-constexpr int TAB = 32, COPIES = 16;
+constexpr int TAB = 64, COPIES = 8;
 constexpr int LIST = 256;                    // entries of all warps
 constexpr int SLICE_MAX = 49152;            // elements of a slice at most (192 KB)
 constexpr int SLICE_GOOD = 16384;           // a slice up to which three CTAs fit an SM
@@ -120,16 +120,19 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {      // inclusive
   return v;
 }
 
-// 2^(j / 32)
+// 2^(j / 64)
 __constant__ double ROOTS[TAB] = {
-    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
-    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
-    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
-    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
-    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
-    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
-    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
-    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284, 1.0442737824274138, 1.0556451783605572,
+    1.0671404006768237, 1.0787607977571199, 1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812, 1.189207115002721, 1.202156731452703,
+    1.215247359980469, 1.22848053610687, 1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303, 1.3542555469368927, 1.3690024229745905,
+    1.383909881963832, 1.3989796725383112, 1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384, 1.5422108254079407, 1.559004400237837,
+    1.5759808451078865, 1.593142151342267, 1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062, 1.7562521603732995, 1.7753764925265212,
+    1.7947090750031072, 1.8142521755003989, 1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
 
 struct Shared {
   // what the other CTAs read; nothing of it is overwritten before a cluster barrier that follows their reads
@@ -163,30 +166,42 @@ struct Shared {
 };
 
 // exp((x - m) / T) as a mass of 2^S units, rounded to nearest.  Table-driven (Tang's scheme, from the mathematics): with
-// z = 32 log2(e) (x - m) / T = n + r, |r| <= 1/2, it is 2^(n >> 5) 2^((n & 31) / 32) 2^(r / 32); the last factor by its Taylor series to
-// the fourth order (|r| ln2 / 32 <= 0.0109: truncated by 1.3e-12).  The table holds 16 copies of its 32 values, one per pair of
-// banks, so that the lookups of a half warp never collide.  Half the FP64 instructions of the library's exp, and no conversion back:
-// adding 1.5 2^(52 - S) leaves the rounded mass in the low bits.
+// z = 64 log2(e) (x - m) / T = n + r, |r| <= 1/2, it is 2^(n >> 6) 2^((n & 63) / 64) 2^(r / 64); the last factor by its Taylor series to
+// the third order (|r| ln2 / 64 <= 0.0054: truncated by 3.6e-11, which is the same for equal values, smooth in r and shifts a
+// border of the draw by about 1e-11 of the whole).  The table holds copies of its values in banks of their own, so that a half
+// warp's lookups collide two by two at most.  Half the FP64 instructions of the library's exp, and no conversion back: adding
+// 1.5 2^(52 - S) leaves the rounded mass in the low bits.
+// `coarse`: T is so small that the floats next to m are 400 octaves away: whatever is below m has no mass.
 struct Weigher {
   double c, mc, magic;                      // z = x c + mc
-  float least;                              // its mass rounds to 0, as that of everything below
+  float m, least;                           // the mass of `least` rounds to 0, as that of everything below
+  bool coarse;
   const double* tab;                        // this thread's copy
-  __device__ __forceinline__ u64 operator()(float x) const { return raw(x) - (u64)__double_as_longlong(magic); }
-  // with the bits of `magic` still in it: for sums of many, from which they are taken once
-  __device__ __forceinline__ u64 raw(float x) const {
+  __device__ __forceinline__ Weigher(double log2e_t, float m_, double cut, int bits, const double* tab_) : m(m_), tab(tab_) {
+    c = TAB * log2e_t;
+    mc = -(double)m * c;
+    magic = __hiloint2double(0x3ff80000 + ((52 - bits) << 20), 0);         // 1.5 2^(52 - S)
+    least = __double2float_rd((double)m - cut);
+    coarse = !(((double)m - (double)least) * c < 400.0 * TAB);
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (coarse) return x < m ? 0 : (u64)(__double_as_longlong(magic + 1.0) - __double_as_longlong(magic));
+    return fine(x) - (u64)__double_as_longlong(magic);
+  }
+  // not coarse; with the bits of `magic` still in it: for sums of many, from which they are taken once
+  __device__ __forceinline__ u64 fine(float x) const {
     constexpr double SHIFT = 6755399441055744.0;                   // 1.5 2^52: the sum's low word is the rounded integer
-    constexpr double L = 0.02166084939249829;                      // ln2 / 32
+    constexpr double L = 0.010830424696249145;                     // ln2 / 64
     const double z = fma((double)fmaxf(x, least), c, mc);
     const double t = z + SHIFT;
-    const int n = max(__double2loint(t), -1000 * TAB);
+    const int n = __double2loint(t);
     const double r = z - (t - SHIFT);
-    double q = L * L * L * L / 24;
-    q = fma(q, r, L * L * L / 6);
+    double q = L * L * L / 6;
     q = fma(q, r, L * L / 2);
     q = fma(q, r, L);
     q = fma(q, r, 1.0);
     const double v = q * tab[(n & (TAB - 1)) * COPIES];
-    return (u64)__double_as_longlong(__hiloint2double(__double2hiint(v) + (n & ~(TAB - 1)) * (1 << 15), __double2loint(v)) + magic);
+    return (u64)__double_as_longlong(__hiloint2double(__double2hiint(v) + (n & ~(TAB - 1)) * (1 << 14), __double2loint(v)) + magic);
   }
 };
 
@@ -460,7 +475,7 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
     z += e;
     if (PRI == PRI_ENTROPY) ent = fmaf(e, fmaxf(y, -1e4f), ent);
     if (PRI == PRI_MARGIN) { at_max += x == m; second = x < m ? fmaxf(second, x) : second; }
-    if (MASS) mass += w.raw(x);
+    if (MASS) mass += w.fine(x);
     if (HIST) {
       const int b = octave_bin(x, m, scale);
       if (b < OCTAVES - 1) atomicAdd(&sh.octaves_here[b], 1u);
@@ -481,7 +496,15 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
     at_max = __reduce_add_sync(0xffffffffu, at_max);
     if (lane == 0) { sh.ent[warp] = second; sh.at_max[warp] = at_max; }
   }
-  if (MASS) { mass = warp_sum(mass - (u64)count * (u64)__double_as_longlong(w.magic)); if (lane == 0) sh.mass[warp] = mass; }
+  if (MASS) {
+    mass -= (u64)count * (u64)__double_as_longlong(w.magic);
+    if (w.coarse) {                                                // the same for the whole row
+      mass = 0;
+      for (int k = seg.a + lane; k < seg.b; k += 32) mass += w(xs[k]);
+    }
+    mass = warp_sum(mass);
+    if (lane == 0) sh.mass[warp] = mass;
+  }
 }
 
 template <int WARPS, bool MASS, bool HIST>
@@ -597,12 +620,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
   const int top_k = sh.top_k;
   const bool by_count = !greedy && top_k > 0 && top_k < p.V, by_mass = !greedy && top_p < 1.0, by_ratio = !greedy && min_p > 0;
   const float scale = sh.scale;
-  Weigher w;
-  w.c = TAB * sh.log2e_t;
-  w.mc = -(double)m * w.c;
-  w.magic = __hiloint2double(0x3ff80000 + ((52 - p.scale_bits) << 20), 0);        // 1.5 2^(52 - S)
-  w.least = __double2float_rd((double)m - sh.cut);
-  w.tab = sh.tab + (lane & (COPIES - 1));
+  const Weigher w(sh.log2e_t, m, sh.cut, p.scale_bits, sh.tab + (lane & (COPIES - 1)));
 
   // ---- the pass over every element
   const Segment seg = split(0, n, WARPS, warp);
@@ -817,14 +835,14 @@ struct RowView {
 #pragma unroll
     for (int j = 0; j < PIECES; ++j)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[j * VEC + k] = to_f32(reinterpret_cast<const T*>(&raw[j])[k]) + 0.f;
+      for (int k = 0; k < VEC; ++k) x[j * VEC + k] = to_f32(reinterpret_cast<const T*>(&raw[j])[k]);
     if (bias) {
 #pragma unroll
       for (int j = 0; j < PIECES; ++j)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           const int i = at0 + j * 32 * VEC + k;
-          if (i >= 0 && i < V) x[j * VEC + k] = x[j * VEC + k] + __ldg(bias + i) + 0.f;
+          if (i >= 0 && i < V) x[j * VEC + k] += __ldg(bias + i);
         }
     }
   }
@@ -838,13 +856,7 @@ __device__ __forceinline__ double row_temperature(const SampleParams& p, unsigne
 // the masses of one chunk, relative to its maximum
 __device__ __forceinline__ Weigher chunk_weigher(double temp, float m, const double* tab) {
   const double log2e_t = 1.4426950408889634 / temp;
-  Weigher w;
-  w.c = TAB * log2e_t;
-  w.mc = -(double)m * w.c;
-  w.magic = __hiloint2double(0x3ff80000 + ((52 - CHUNK_BITS) << 20), 0);
-  w.least = __double2float_rd((double)m - (CHUNK_BITS + 1.5) / log2e_t);
-  w.tab = tab;
-  return w;
+  return Weigher(log2e_t, m, (CHUNK_BITS + 1.5) / log2e_t, CHUNK_BITS, tab);
 }
 
 constexpr int STREAM_THREADS = 256;
@@ -872,22 +884,34 @@ __global__ void __launch_bounds__(STREAM_THREADS, 3) chunk_kernel(const SamplePa
     if (m > -INFINITY && m < INFINITY) {
       float z = 0, e = r.e;
       int n = 0;
+      if (PRI == PRI_ENTROPY || temp != 1.0) {                     // at T = 1 the masses are these exponentials
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float y = (x[k] - m) * 1.44269504f, v = ex2(y);
-        z += v;
-        if (PRI == PRI_ENTROPY) e = fmaf(v, fmaxf(y, -1e4f), e);
-        if (PRI == PRI_MARGIN) { n += x[k] == m; e = x[k] < m ? fmaxf(e, x[k]) : e; }
+        for (int k = 0; k < 32; ++k) {
+          const float y = (x[k] - m) * 1.44269504f, v = ex2(y);
+          z += v;
+          if (PRI == PRI_ENTROPY) e = fmaf(v, fmaxf(y, -1e4f), e);
+        }
+        r.z = warp_sum(z);
       }
-      r.z = warp_sum(z);
+      if (PRI == PRI_MARGIN) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) { n += x[k] == m; e = x[k] < m ? fmaxf(e, x[k]) : e; }
+      }
       if (PRI == PRI_ENTROPY) r.e = warp_sum(e);
       if (PRI == PRI_MARGIN) { r.e = warp_max(e); r.at_max = __reduce_add_sync(0xffffffffu, n); }
       if (temp > 0) {
         const Weigher w = chunk_weigher(temp, m, tab + (lane & (COPIES - 1)));
         u64 mass = 0;
+        if (w.coarse) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) mass += w.raw(x[k]);
-        r.mass = warp_sum(mass - 32 * (u64)__double_as_longlong(w.magic));
+          for (int k = 0; k < 32; ++k) mass += w(x[k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) mass += w.fine(x[k]);
+          mass -= 32 * (u64)__double_as_longlong(w.magic);
+        }
+        r.mass = warp_sum(mass);
+        if (PRI != PRI_ENTROPY && temp == 1.0) r.z = (float)((double)r.mass * (1.0 / (double)(1ull << CHUNK_BITS)));
       } else {
         constexpr int VEC = 16 / (int)sizeof(T);
         int at = 0x7fffffff;
