@@ -12,6 +12,8 @@ decoding cannot drift apart.  State per sequence: the clean K/V window of every 
 Sampler options (``DecodeOpts``): confidence or random commit order, Gumbel sampling, probability threshold
 (parallel decoding), presence penalty, a re-masking corrector loop, sub-block (semi-autoregressive) filling,
 and the priority measure (log-probability, top-2 margin or negative entropy) - reference ``generate.py:196-355``.
+``sampler = "inverse"``, and any of ``top_k`` / ``top_p`` / ``min_p``, draws by the inverse distribution function from one
+uniform number per slot (``ops.sampling.sample_tokens``: one or two kernel launches instead of a Gumbel number per token).
 With the outer shift slot ``i`` predicts token ``i+1`` and the first token of a block comes from the previous
 block's tail logit.
 """
@@ -30,6 +32,7 @@ from .engine import Engine
 from .models.blocks import Net
 from .ops import attention as A
 from .ops import functional as Fn
+from .ops import sampling
 from .schema import ModelConfig, TrainConfig
 from .ttt import inner as IN
 from .ttt import objective as OBJ
@@ -152,6 +155,14 @@ class DecodeOpts:
     remask_k: int = 16
     subblock: int = 0
     priority: str = "logp"            # logp | margin | entropy
+    top_k: int = 0                    # > 0: draw among that many likeliest tokens
+    top_p: float = 1.0                # < 1: draw among the likeliest tokens that hold this share of the probability
+    min_p: float = 0.0                # > 0: draw among tokens at least this likely, relative to the likeliest
+    sampler: str = "gumbel"           # gumbel | inverse (one uniform number per slot); truncated draws are always inverse
+
+    @property
+    def inverse(self) -> bool:
+        return self.sampler == "inverse" or self.top_k > 0 or self.top_p < 1 or self.min_p > 0
 
 
 # ---- confidence unmasking of one block (reference generate.py:227-355: LLaDA-style, with the options of ``DecodeOpts``)
@@ -209,6 +220,8 @@ class BlockUnmasker:
         x = self.masked_input(visible)
         logits = block_forward(self.net, x, self.pos, self.state, pos_q=self.pos_q, own_kv=own_kv)[0]
         logits[..., self.mask_id] = float("-inf")
+        if o.inverse:
+            return self.draw(logits, x, key)
         if self.outer_shift:                                        # slot i is predicted at slot i - 1; slot 0 by the previous block's tail
             lead = self.prev_tail.clone() if self.prev_tail is not None else torch.zeros(self.B, self.V, device=self.dev)
             lead[..., self.mask_id] = float("-inf")
@@ -225,18 +238,34 @@ class BlockUnmasker:
         chosen = logp.gather(-1, tokens[..., None])[..., 0]
         return tokens, chosen, _PRIORITY[o.priority](logp, chosen)
 
-    def pick(self, priority: torch.Tensor, key: torch.Tensor, quota: torch.Tensor, allowed=None) -> torch.Tensor:
-        """The ``quota [B]`` open (and allowed) slots of highest priority; with ``order = random`` the priority is a draw."""
-        if self.opts.order == "random":
-            priority = rng.uniform(rng.fold_in(key, 1).to("cpu"), (self.B, self.C)).to(self.dev)
-        shut = self.known if allowed is None else (self.known | ~allowed)
-        priority = torch.where(shut, torch.full_like(priority, float("-inf")), priority)
-        return (_rank_of(priority) < quota[:, None]) & ~shut
+    def draw(self, logits: torch.Tensor, x: torch.Tensor, key: torch.Tensor):
+        """Proposals from one uniform number per slot; under the outer shift slot 0 is drawn from the previous block's tail and
+        the others in place, from the rows before them."""
+        o = self.opts
+        u = rng.uniform(key.to("cpu"), (self.B, self.C)).to(self.dev)
+        bias = None
+        if o.presence_penalty > 0:
+            seen = torch.zeros(self.B, self.V, device=self.dev).scatter_(1, x, 1.0)
+            seen[:, self.mask_id] = 0
+            bias = seen * -o.presence_penalty
+        kw = dict(temperature=max(float(self.temperature), 0.0), top_k=o.top_k, top_p=o.top_p, min_p=o.min_p, bias=bias, priority=o.priority)
+        if not self.outer_shift:
+            return sampling.sample_tokens(logits, u, **kw)
+        lead = self.prev_tail.clone() if self.prev_tail is not None else torch.zeros(self.B, self.V, device=self.dev)
+        lead[..., self.mask_id] = float("-inf")
+        parts = zip(sampling.sample_tokens(lead[:, None], u[:, :1], **kw), sampling.sample_tokens(logits[:, :-1], u[:, 1:], **kw))
+        return tuple(torch.cat(p, 1) for p in parts)
 
-    def commit(self, where: torch.Tensor, tokens: torch.Tensor, logp: torch.Tensor) -> None:
-        self.ids = torch.where(where, tokens, self.ids)
-        self.committed_logp = torch.where(where, logp, self.committed_logp)
-        self.known = self.known | where
+    def order(self, priority: torch.Tensor, key: torch.Tensor) -> torch.Tensor:
+        """What the slots are ranked by: with ``order = random`` a draw."""
+        if self.opts.order == "random":
+            return rng.uniform(rng.fold_in(key, 1).to("cpu"), (self.B, self.C)).to(self.dev)
+        return priority
+
+    def commit(self, tokens, logp, priority: torch.Tensor, quota: torch.Tensor, allowed=None, sure=None) -> None:
+        """Fill the ``quota [B]`` open (and allowed) slots of highest priority, and those whose proposal reaches ``sure``."""
+        self.ids, self.known, self.committed_logp, _ = sampling.unmask(self.ids.long(), self.known, self.committed_logp, tokens, logp, priority,
+                                                                       quota, allowed=allowed, sure=sure)
 
     # ---- schedules
     def sweep(self, n_steps: int, allowed=None, own_kv=None) -> None:
@@ -246,7 +275,7 @@ class BlockUnmasker:
             tokens, logp, priority = self.propose(self.known, key, own_kv)
             open_ = ~self.known if allowed is None else (~self.known & allowed)
             quota = torch.ceil(open_.sum(-1).float() / (n_steps - i)).long()
-            self.commit(self.pick(priority, key, quota, allowed), tokens, logp)
+            self.commit(tokens, logp, self.order(priority, key), quota, allowed)
 
     def until_confident(self, threshold: float) -> None:
         """Each round commits every slot whose proposal reaches ``threshold`` probability, and at least the best one."""
@@ -255,8 +284,7 @@ class BlockUnmasker:
         while (~self.known).any() and rounds < self.C:
             key = self.keys.take()
             tokens, logp, priority = self.propose(self.known, key)
-            sure = (logp >= float(np.log(threshold))) & ~self.known
-            self.commit(sure | self.pick(priority, key, one), tokens, logp)
+            self.commit(tokens, logp, self.order(priority, key), one, sure=float(np.log(threshold)))
             rounds += 1
 
     def revise(self, rounds: int, k: int) -> None:
@@ -276,6 +304,8 @@ def _check_decode_opts(opts: DecodeOpts, C: int, read_block: int, outer_shift: b
         raise ValueError(f"DecodeOpts order {opts.order!r} / priority {opts.priority!r}")
     if opts.subblock < 0 or (opts.subblock and (C % opts.subblock or opts.threshold > 0)):
         raise ValueError(f"DecodeOpts.subblock {opts.subblock}: a divisor of the block size {C}, without threshold")
+    if opts.sampler not in ("gumbel", "inverse") or opts.top_k < 0 or not 0 < opts.top_p <= 1 or not 0 <= opts.min_p <= 1:
+        raise ValueError(f"DecodeOpts sampler {opts.sampler!r}, top_k {opts.top_k}, top_p {opts.top_p}, min_p {opts.min_p}")
     if read_block and (opts.threshold > 0 or opts.remask_loop > 0 or opts.subblock not in (0, read_block) or not outer_shift):
         raise ValueError(f"read_block {read_block}: its groups are decoded in order, with the outer shift")
 
@@ -417,6 +447,8 @@ def main(argv=None) -> None:
     ap.add_argument("--presence_penalty", type=float, default=0.0); ap.add_argument("--remask_loop", type=int, default=0)
     ap.add_argument("--remask_k", type=int, default=16); ap.add_argument("--subblock", type=int, default=0)
     ap.add_argument("--priority", default="logp")
+    ap.add_argument("--top_k", type=int, default=0); ap.add_argument("--top_p", type=float, default=1.0)
+    ap.add_argument("--min_p", type=float, default=0.0); ap.add_argument("--sampler", default="gumbel", choices=["gumbel", "inverse"])
     ap.add_argument("--unigram_path", default="bucket/data/tokens/unigram_llama3.i64")
     ap.add_argument("--seed", type=int, default=0)
     a = ap.parse_args(argv)
@@ -438,7 +470,8 @@ def main(argv=None) -> None:
                    inner_lr=a.inner_lr, inner_clip=a.inner_clip, inner_mask_ratio=a.inner_mask_ratio, inner_views=a.inner_views,
                    inner_mask_span=a.inner_mask_span, inner_update_rule=a.inner_update, inner_mask_mode=a.inner_mask_mode,
                    inner_target_frac=a.inner_target_frac, inner_task=a.inner_task, outer_shift=a.outer_shift, wc=wc, unigram=uni,
-                   opts=DecodeOpts(a.order, False, a.threshold, a.presence_penalty, a.remask_loop, a.remask_k, a.subblock, a.priority))
+                   opts=DecodeOpts(a.order, False, a.threshold, a.presence_penalty, a.remask_loop, a.remask_k, a.subblock, a.priority,
+                                   a.top_k, a.top_p, a.min_p, a.sampler))
     new = out[len(prompt):].tolist()
     print(tok.decode(new) if tok is not None else ",".join(map(str, new)))
 

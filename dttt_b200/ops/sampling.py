@@ -107,7 +107,7 @@ def unmask(ids: torch.Tensor, known: torch.Tensor, held: torch.Tensor, tokens: t
     (not ``known``, and ``allowed`` where given), and with ``sure`` also every slot that is not known and whose ``logp`` reaches
     it.  ``ids``, ``known`` and ``held`` (the log-probability a slot was committed with) come back with ``tokens`` / True /
     ``logp`` at the committed slots.  Slots of equal priority rank by position, NaN ranks last; a slot that is not open ranks as
-    one of priority ``-inf``.  ``C`` up to 32768 on a CUDA device."""
+    one of priority ``-inf``.  One launch for ``C`` up to 32768 on a CUDA device, the statement of ``ops.reference`` beyond."""
     shape, dev = ids.shape, ids.device
     if len(shape) != 2:
         raise ValueError(f"unmask: ids {tuple(shape)}, [B, C] is wanted")
@@ -121,10 +121,8 @@ def unmask(ids: torch.Tensor, known: torch.Tensor, held: torch.Tensor, tokens: t
     if sure is not None and math.isnan(sure):
         raise ValueError("unmask: sure is NaN")
     from . import kernels
-    if not ids.is_cuda or "sampling" in kernels._DISABLED:
+    if not ids.is_cuda or "sampling" in kernels._DISABLED or shape[1] > kernels.UNMASK_SLOTS_MAX:
         with torch.no_grad():
             return Committed(*ref.unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure))
-    if shape[1] > kernels.UNMASK_SLOTS_MAX:
-        raise ValueError(f"unmask: {shape[1]} slots, above {kernels.UNMASK_SLOTS_MAX}")
     return Committed(*kernels.unmask(ids.contiguous(), known.contiguous(), held.contiguous(), tokens.contiguous(), logp.contiguous(),
                                      priority.contiguous(), quota.contiguous(), None if allowed is None else allowed.contiguous(), sure))

@@ -1,0 +1,54 @@
+"""Decoding with truncated and inverse draws and the five-step write: determinism, agreement of the options, refusals."""
+import pytest
+import torch
+
+from util import make_engine, tiny_model
+from dttt_b200 import generate as G
+from dttt_b200.ckpt import store as CK
+from dttt_b200.utils import rng
+
+PROMPT = torch.randint(0, 120, (11,), generator=torch.Generator().manual_seed(3))
+
+
+def run(net, opts, seed=5, **kw):
+    return G.generate(net, PROMPT, 14, rng.key(seed), steps=4, fused_ce_block=0, opts=opts, **kw)
+
+
+@pytest.mark.parametrize("opts", [G.DecodeOpts(top_k=5), G.DecodeOpts(top_p=0.8), G.DecodeOpts(min_p=0.1), G.DecodeOpts(sampler="inverse"),
+                                  G.DecodeOpts(top_k=20, top_p=0.9, min_p=0.02, priority="margin", presence_penalty=0.5),
+                                  G.DecodeOpts(top_p=0.7, priority="entropy", remask_loop=1, remask_k=3),
+                                  G.DecodeOpts(top_p=0.9, threshold=0.05), G.DecodeOpts(top_p=0.9, order="random")])
+@pytest.mark.parametrize("kw", [dict(), dict(outer_shift=True, inner_task="causal", inner_update_rule="muon5")])
+def test_draws_are_deterministic_and_keep_the_prompt(opts, kw):
+    net = make_engine().net(train=False)
+    a, b, c = run(net, opts, temperature=1.0, **kw), run(net, opts, temperature=1.0, **kw), run(net, opts, seed=6, temperature=1.0, **kw)
+    assert a.shape == (25,) and torch.equal(a, b) and torch.equal(a[:11], PROMPT) and not torch.equal(a, c)
+    assert (a != 127).all() and (a >= 0).all()
+
+
+def test_the_best_token_alone_is_the_greedy_choice():
+    net = make_engine().net(train=False)
+    for kw in (dict(), dict(outer_shift=True, inner_task="causal")):
+        greedy = run(net, G.DecodeOpts(), temperature=0.0, **kw)
+        assert torch.equal(greedy, run(net, G.DecodeOpts(sampler="inverse"), temperature=0.0, **kw))
+        assert torch.equal(greedy, run(net, G.DecodeOpts(top_k=1), temperature=1.0, **kw))
+        assert torch.equal(greedy, run(net, G.DecodeOpts(top_p=1e-6), temperature=0.7, **kw))
+
+
+def test_read_block_and_cli(tmp_path, capsys):
+    eng = make_engine(mc=tiny_model(read_block=4))
+    out = G.generate(eng.net(train=False), PROMPT[:5], 12, rng.key(1), steps=4, temperature=1.0, fused_ce_block=0, outer_shift=True,
+                     inner_task="causal", opts=G.DecodeOpts(top_p=0.9))
+    assert out.shape == (17,)
+    d = CK.save(str(tmp_path / "ck"), 0, make_engine(), "h")
+    G.main(["--ckpt", d, "--prompt_ids", "5,6,7,8", "--max_new_tokens", "6", "--steps", "2", "--inner_task", "causal", "--temperature", "0.8",
+            "--top_k", "30", "--top_p", "0.9", "--min_p", "0.01", "--sampler", "inverse", "--inner_update", "muon5"])
+    printed = capsys.readouterr().out.strip().split(",")
+    assert len(printed) == 6 and all(0 <= int(x) < 128 for x in printed)
+
+
+@pytest.mark.parametrize("opts", [G.DecodeOpts(sampler="beam"), G.DecodeOpts(top_k=-1), G.DecodeOpts(top_p=0.0), G.DecodeOpts(top_p=1.5),
+                                  G.DecodeOpts(min_p=-0.1), G.DecodeOpts(min_p=1.1)])
+def test_refusals(opts):
+    with pytest.raises(ValueError, match="DecodeOpts"):
+        run(make_engine().net(train=False), opts)
