@@ -1101,7 +1101,59 @@ int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t
 }
 
 // ------------------------------------------------------------------------------------------------------ unmask
-// One block per row.  The quota-th slot in rank order is found by a radix search over the order keys in shared memory.
+// One block per row.  Rows of up to 1024 slots: a thread per slot, everything it needs loaded at once, and the key of the quota-th slot
+// in rank order built bit by bit from counts over the block (32 barriers, about 1.5 us; latency is all there is to it).  Longer
+// rows: a radix search over the order keys in shared memory.
+constexpr int UM_ROW = 1024;
+
+__global__ void __launch_bounds__(UM_ROW) unmask_row_kernel(const long long* __restrict__ ids, const uint8_t* __restrict__ known,
+                                                           const float* __restrict__ held, const long long* __restrict__ tokens,
+                                                           const float* __restrict__ logp, const float* __restrict__ priority,
+                                                           const long long* __restrict__ quota, const uint8_t* __restrict__ allowed,
+                                                           float sure, int use_sure, long long* __restrict__ ids_out,
+                                                           uint8_t* __restrict__ known_out, float* __restrict__ held_out,
+                                                           uint8_t* __restrict__ where_out, int C) {
+  __shared__ int warp_count[UM_ROW / 32];
+  const int i = threadIdx.x, warp = i >> 5, lane = i & 31;
+  const long long at = (long long)blockIdx.x * C + i;
+  const bool in = i < C;
+  const long long q = quota[blockIdx.x];
+  bool is_known = true, ok = false;
+  float pri = 0.f, lp = 0.f, was = 0.f;
+  long long id = 0, token = 0;
+  if (in) {
+    is_known = known[at]; ok = allowed ? allowed[at] : true;
+    pri = priority[at]; lp = logp[at]; was = held[at]; id = ids[at]; token = tokens[at];
+  }
+  const bool shut = is_known || !ok;
+  const float v = shut ? -INFINITY : pri + 0.f;
+  const uint32_t key = !in || v != v ? 0u : order_key(v);         // 0: NaN, and threads without a slot, which come after the slots
+  bool take = q >= C;
+  if (q > 0 && q < C) {
+    const int want = (int)q;
+    uint32_t least = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = least | 1u << bit;
+      if (__syncthreads_count(key >= cand) >= want) least = cand;
+    }
+    const int ties = want - __syncthreads_count(key > least);
+    const unsigned int eq = __ballot_sync(0xffffffffu, in && key == least);
+    if (lane == 0) warp_count[warp] = __popc(eq);
+    __syncthreads();
+    int run = __popc(eq & ((1u << lane) - 1));
+    for (int k = 0; k < warp; ++k) run += warp_count[k];
+    take = key > least || (key == least && run < ties);
+  }
+  if (in) {
+    take = (take && !shut) || (use_sure && lp >= sure && !is_known);
+    ids_out[at] = take ? token : id;
+    known_out[at] = is_known || take;
+    held_out[at] = take ? lp : was;
+    where_out[at] = take;
+  }
+}
+
 constexpr int UM_THREADS = 256;
 constexpr int UM_SLOTS_MAX = 32768;
 
@@ -1242,6 +1294,12 @@ extern "C" int dttt_unmask(const long long* ids, const void* known, const float*
                            long long* ids_out, void* known_out, float* held_out, void* where_out, int B, int C, cudaStream_t stream) {
   if (B <= 0 || C <= 0) return 0;
   if (C > UM_SLOTS_MAX) return -2;
+  if (C <= UM_ROW) {
+    unmask_row_kernel<<<B, (C + 31) / 32 * 32, 0, stream>>>(ids, (const uint8_t*)known, held, tokens, logp, priority, quota, (const uint8_t*)allowed,
+                                                            sure, use_sure, ids_out, (uint8_t*)known_out, held_out, (uint8_t*)where_out, C);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : 1000 + (int)e;
+  }
   const size_t smem = (size_t)C * sizeof(uint32_t);
   static std::atomic<u64> ready{0};
   cudaError_t e = allow_shared(unmask_kernel, UM_SLOTS_MAX * (int)sizeof(uint32_t), ready);
