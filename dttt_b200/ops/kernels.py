@@ -816,36 +816,34 @@ def _launch(what, fn, device, *args):
 
 
 def sample(x, u, bias, temperature, top_k, top_p, min_p, priority):
-    """``x [outer, inner, V]`` (contiguous along V, any strides of the rows), ``u [outer, inner]``, ``bias [outer, V]`` or None; a
-    parameter is a number or a contiguous tensor ``[outer, inner]`` (f32; int32 for ``top_k``).  ``(tokens, logp, priority)``
-    ``[outer, inner]``; ``priority`` 0 logp (the same tensor) | 1 margin | 2 entropy."""
+    """``x [outer, inner, V]`` (contiguous along V, any strides of the rows), ``u`` its rows' numbers (contiguous), ``bias [outer, V]``
+    or None; a parameter is a number or a contiguous tensor of a value per row (f32; int32 for ``top_k``).  ``(tokens, logp,
+    priority)`` in the shape of ``u``; ``priority`` 0 logp (the same tensor) | 1 margin | 2 entropy."""
+    global LAUNCHES
     outer, inner, V = x.shape
-    dev = x.device
-    tokens = torch.empty((outer, inner), dtype=torch.int64, device=dev)
-    out = torch.empty((2 if priority else 1, outer, inner), dtype=torch.float32, device=dev)
-    logp = out[0]
-    prio = out[1] if priority else logp
+    tokens, logp = torch.empty_like(u, dtype=torch.int64), torch.empty_like(u)
+    prio = torch.empty_like(u) if priority else logp
     if outer and inner:
-        num = lambda p, off: (off, p.data_ptr()) if isinstance(p, torch.Tensor) else (p, None)
-        l, scratch = _lib.lib(), None
-        if type(top_p) is float and top_p == 1.0 and type(min_p) is float and min_p == 0.0 and type(top_k) is int and not 0 < top_k < V:
+        l, scratch, dev, T = _lib.lib(), None, x.device, torch.Tensor
+        t, t_row = (1.0, temperature.data_ptr()) if isinstance(temperature, T) else (temperature, None)
+        k, k_row = (0, top_k.data_ptr()) if isinstance(top_k, T) else (top_k, None)
+        p, p_row = (1.0, top_p.data_ptr()) if isinstance(top_p, T) else (top_p, None)
+        m, m_row = (0.0, min_p.data_ptr()) if isinstance(min_p, T) else (min_p, None)
+        if p == 1.0 and m == 0.0 and not 0 < k < V and k_row is None and p_row is None and m_row is None:
             size = l.dttt_sample_scratch(outer * inner, V)               # nothing is truncated: two passes over chunks from some size on
-            scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+            if size:
+                scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+                LAUNCHES += 1
         _launch("sample", l.dttt_sample, dev, x.data_ptr(), _LOGIT_TYPES[x.dtype], outer * inner, inner, x.stride(0), x.stride(1), V,
-                u.data_ptr(), None if bias is None else bias.data_ptr(), *num(temperature, 1.0), *num(top_k, 0), *num(top_p, 1.0),
-                *num(min_p, 0.0), priority, tokens.data_ptr(), logp.data_ptr(), prio.data_ptr(),
-                None if scratch is None else scratch.data_ptr())
-        if scratch is not None:
-            global LAUNCHES
-            LAUNCHES += 1
+                u.data_ptr(), None if bias is None else bias.data_ptr(), t, t_row, k, k_row, p, p_row, m, m_row, priority,
+                tokens.data_ptr(), logp.data_ptr(), prio.data_ptr(), None if scratch is None else scratch.data_ptr())
     return tokens, logp, prio
 
 
 def unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure):
     """Contiguous ``[B, C]`` tensors (``quota [B]``); ``(ids, known, held, where)`` after the commit."""
     B, C = ids.shape
-    ids_out, held_out = torch.empty_like(ids), torch.empty_like(held)
-    known_out, where = torch.empty((2, B, C), dtype=torch.bool, device=ids.device).unbind(0)
+    ids_out, held_out, known_out, where = torch.empty_like(ids), torch.empty_like(held), torch.empty_like(known), torch.empty_like(known)
     if B and C:
         _launch("unmask", _lib.lib().dttt_unmask, ids.device, ids.data_ptr(), known.data_ptr(), held.data_ptr(), tokens.data_ptr(),
                 logp.data_ptr(), priority.data_ptr(), quota.data_ptr(), None if allowed is None else allowed.data_ptr(),

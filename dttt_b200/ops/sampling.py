@@ -79,10 +79,15 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Param =
         raise ValueError(f"sample_tokens: u {tuple(u.shape)} {u.dtype} on {u.device}, {tuple(rows)} float32 on {dev} is wanted")
     if bias is not None and (bias.shape != (rows[0], V) or bias.dtype != torch.float32 or bias.device != dev):
         raise ValueError(f"sample_tokens: bias {tuple(bias.shape)} {bias.dtype} on {bias.device}, {(rows[0], V)} float32 on {dev} is wanted")
-    t = _param("temperature", temperature, rows, torch.float32, dev, 0.0, 1e6)
-    k = _param("top_k", top_k, rows, torch.int32, dev, 0, 2 ** 31 - 1)
-    p = _param("top_p", top_p, rows, torch.float32, dev, 0.0, 1.0, open_lo=True)
-    m = _param("min_p", min_p, rows, torch.float32, dev, 0.0, 1.0)
+    t, k, p, m = temperature, top_k, top_p, min_p
+    if not (type(t) is float and 0.0 <= t <= 1e6):
+        t = _param("temperature", t, rows, torch.float32, dev, 0.0, 1e6)
+    if not (type(k) is int and 0 <= k < 2 ** 31):
+        k = _param("top_k", k, rows, torch.int32, dev, 0, 2 ** 31 - 1)
+    if not (type(p) is float and 0.0 < p <= 1.0):
+        p = _param("top_p", p, rows, torch.float32, dev, 0.0, 1.0, open_lo=True)
+    if not (type(m) is float and 0.0 <= m <= 1.0):
+        m = _param("min_p", m, rows, torch.float32, dev, 0.0, 1.0)
     from . import kernels
     if not logits.is_cuda or "sampling" in kernels._DISABLED:
         with torch.no_grad():
@@ -94,10 +99,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Param =
     x = logits if logits.stride(-1) == 1 or V == 1 else logits.detach().contiguous()
     if len(rows) != 2:
         x = x.unsqueeze(1) if len(rows) == 1 else x.reshape(rows[0], math.prod(rows[1:]), V)
-    flat = lambda v: v.reshape(x.shape[:2]) if isinstance(v, torch.Tensor) else v
-    out = kernels.sample(x, u.contiguous(), None if bias is None else bias.contiguous(), flat(t), flat(k), flat(p), flat(m),
-                         PRIORITIES.index(priority))
-    return Drawn(*out) if len(rows) == 2 else Drawn(*(o.view(rows) for o in out))
+    return Drawn(*kernels.sample(x, u.detach().contiguous() if u.requires_grad else u.contiguous(),
+                                 None if bias is None else bias.contiguous(), t, k, p, m, PRIORITIES.index(priority)))
 
 
 def unmask(ids: torch.Tensor, known: torch.Tensor, held: torch.Tensor, tokens: torch.Tensor, logp: torch.Tensor,
