@@ -475,6 +475,226 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
       dst[(long long)r * ld + c] = __float2half_rn(to_f32(src[(long long)r * cols + c]) * f0 * f1);
 }
 
+// ------------------------------------------------------------------ small matrices: everything in one CTA
+// d <= 128 and L <= 512: one CTA per matrix holds x [128, L] (transposed when rows > cols), G and P in shared memory and runs all
+// iterations in one launch; what such sizes cost otherwise is launches.  x lies as blocks of 128 rows x 64 columns with 128-byte
+// swizzle, which is the K-major operand of G = x x^T and, read with its columns as N, the MN-major one of P x.  Rows and columns
+// beyond the matrix are zero and stay so.  Also the derivative (`apply`): the kept P of every iteration is read back.
+constexpr int SMALL_D = 128, SMALL_L = 512, SMALL_THREADS = 256;
+constexpr int BLOCK_BYTES = SMALL_D * 128;                     // 128 rows x 64 f16
+
+struct SmallParams {
+  const void* in;
+  int rows, cols, steps, apply, keep, out, ldd;
+  float scale;                 // of the f16 copy
+  __half* maps;                // [steps or 1, batch, d, ldd]
+  long long map_stride;
+  double* norms;               // written by the forward, read by the derivative
+  void* y;
+  int* status;
+};
+
+__device__ __forceinline__ int small_offset(int row, int col) {      // bytes; of the 16-byte piece that starts at col
+  return (col >> 6) * BLOCK_BYTES + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) * 16);
+}
+__device__ __forceinline__ void store_small(uint8_t* at, int row, int col, const float (&v)[32]) {      // 32 columns from a multiple of 32
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint4 o;
+    __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
+    *reinterpret_cast<uint4*>(at + small_offset(row, col + 8 * q)) = o;
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const bool wide = p.rows <= p.cols;
+  const int d = wide ? p.rows : p.cols, L = wide ? p.cols : p.rows, Lp = (L + 63) / 64 * 64;
+  uint8_t* sg = sx + (Lp / 64) * BLOCK_BYTES;
+  uint8_t* sp = sg + 2 * BLOCK_BYTES;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sp + 2 * BLOCK_BYTES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
+  volatile int* abort_word = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+  const uint32_t tmem_cols = Lp > 256 ? 512 : Lp > 128 ? 256 : 128;
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    *abort_word = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  // the norm, then the scaled f16 copy
+  const T* g = reinterpret_cast<const T*>(p.in) + (long long)b * p.rows * p.cols;
+  double s = 0;
+  for (int i = tid; i < p.rows * p.cols; i += SMALL_THREADS) { const double e = (double)to_f32(g[i]); s = fma(e, e, s); }
+  const double whole = sqrt(block_sum(s));
+  if (!p.apply && tid == 0) p.norms[b] = whole;
+  const double f = whole == 0.0 ? 0.0 : (double)p.scale / whole;
+  const int pieces = Lp / 8;
+  for (int i = tid; i < SMALL_D * pieces; i += SMALL_THREADS) {
+    const int row = wide ? i / pieces : i % SMALL_D, col = (wide ? i % pieces : i / SMALL_D) * 8;
+    uint4 o;
+    __half* h = reinterpret_cast<__half*>(&o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = row < d && col + e < L;
+      h[e] = in ? __float2half_rn((float)((double)to_f32(g[wide ? row * p.cols + col + e : (col + e) * p.cols + row]) * f)) : __half(0.f);
+    }
+    *reinterpret_cast<uint4*>(sx + small_offset(row, col)) = o;
+  }
+  float last = 1.f / p.scale;                                  // brings the last product to the result's scale
+  if (p.apply) { const double n = p.norms[b]; last = n == 0.0 ? 0.f : (float)(whole / n / (double)p.scale); }
+  tc_fence_before();
+  fence_async_proxy();                                         // the tensor core reads what these threads wrote
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+  const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+  uint32_t phase = 0;
+  bool ok = true;
+  // one product: issued by thread 0, waited for by all
+  auto wait = [&]() {
+    ok = mbar_wait_bounded(bar, phase, abort_word, p.status, ERR_WAIT_TMEM_FULL);
+    phase ^= 1;
+    ok = __syncthreads_and(ok);
+    tc_fence_after();
+    return ok;
+  };
+  auto hand_over = [&]() {                                     // accumulators read, operands written: the next product may start
+    tc_fence_before();
+    fence_async_proxy();
+    __syncthreads();
+    tc_fence_after();
+  };
+  for (int k = 0; k < p.steps && ok; ++k) {
+    const int at = p.apply ? p.steps - 1 - k : p.keep ? k : 0;
+    __half* map = p.maps ? p.maps + at * p.map_stride + (long long)b * d * p.ldd : nullptr;
+    if (!p.apply) {
+      if (tid == 0) {
+        const uint32_t a = smem_u32(sx), idesc = make_idesc_f16(128, 128, 0, 0);
+        for (int i = 0; i < Lp / 16; ++i) {
+          const uint64_t desc = make_smem_desc(a + (i >> 2) * BLOCK_BYTES + (i & 3) * 32, 16, 1024);
+          umma_f16(tmem, desc, desc, idesc, i > 0);
+        }
+        umma_commit(bar);
+      }
+      if (!wait()) break;
+      float gr[2][32];                                         // this thread's 64 entries of G
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32(lanes + half * 64 + c * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) gr[c][j] = __uint_as_float(r[j]) * (1.f / X_SCALE);
+        store_small(sg, row, half * 64 + c * 32, gr[c]);
+      }
+      hand_over();
+      if (tid == 0) {
+        const uint32_t a = smem_u32(sg), idesc = make_idesc_f16(128, 128, 0, 0);
+        for (int i = 0; i < 8; ++i) {
+          const uint64_t desc = make_smem_desc(a + (i >> 2) * BLOCK_BYTES + (i & 3) * 32, 16, 1024);
+          umma_f16(tmem, desc, desc, idesc, i > 0);
+        }
+        umma_commit(bar);
+      }
+      if (!wait()) break;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col = half * 64 + c * 32;
+        uint32_t r[32];
+        tmem_ld_32x32(lanes + col, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) gr[c][j] = fmaf(NS_B, gr[c][j], NS_C / X_SCALE * __uint_as_float(r[j]));
+        store_small(sp, row, col, gr[c]);
+        if (p.keep && row < d)
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col + j < d) map[(long long)row * p.ldd + col + j] = __float2half_rn(gr[c][j]);
+      }
+    } else {
+      for (int i = tid; i < SMALL_D * (SMALL_D / 8); i += SMALL_THREADS) {
+        const int r = i / (SMALL_D / 8), col = i % (SMALL_D / 8) * 8;
+        uint4 o = make_uint4(0, 0, 0, 0);
+        __half* h = reinterpret_cast<__half*>(&o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (r < d && col + e < d) h[e] = map[(long long)r * p.ldd + col + e];
+        *reinterpret_cast<uint4*>(sp + small_offset(r, col)) = o;
+      }
+    }
+    hand_over();
+    if (tid == 0) {
+      const uint32_t a = smem_u32(sp), x = smem_u32(sx);
+      for (int n0 = 0; n0 < Lp; n0 += 256) {
+        const int n = min(256, Lp - n0);
+        const uint32_t idesc = make_idesc_f16(128, n, 0, 1);
+        for (int i = 0; i < 8; ++i)
+          umma_f16(tmem + n0, make_smem_desc(a + (i >> 2) * BLOCK_BYTES + (i & 3) * 32, 16, 1024),
+                   make_smem_desc(x + (n0 >> 6) * BLOCK_BYTES + i * (UMMA_K * 128), BLOCK_BYTES, 1024), idesc, i > 0);
+      }
+      umma_commit(bar);
+    }
+    if (!wait()) break;
+    const bool end = k == p.steps - 1;
+    const float fin = end ? last : 1.f;
+    for (int col = half * 32; col < Lp; col += 64) {
+      uint32_t r[32];
+      tmem_ld_32x32(lanes + col, r);
+      tmem_ld_wait();
+      float v[32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint4 o = *reinterpret_cast<const uint4*>(sx + small_offset(row, col + 8 * q));
+        const __half* h = reinterpret_cast<const __half*>(&o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * q + e] = fin * fmaf(NS_A, __half2float(h[e]), __uint_as_float(r[8 * q + e]) * (1.f / X_SCALE));
+      }
+      if (!end) {
+        store_small(sx, row, col, v);
+      } else if (row < d) {
+        const long long base = (long long)b * p.rows * p.cols;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (col + j < L) {
+            const long long o = base + (wide ? (long long)row * p.cols + col + j : (long long)(col + j) * p.cols + row);
+            if (p.out == OUT_F32) reinterpret_cast<float*>(p.y)[o] = v[j];
+            else reinterpret_cast<__nv_bfloat16*>(p.y)[o] = __float2bfloat16(v[j]);
+          }
+      }
+    }
+    hand_over();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+static bool is_small(int rows, int cols) {
+  const int d = rows < cols ? rows : cols, L = rows < cols ? cols : rows;
+  return d <= SMALL_D && L <= SMALL_L;
+}
+
+static int launch_small(const SmallParams& p, int f32, int batch, cudaStream_t stream) {
+  const int L = p.rows < p.cols ? p.cols : p.rows, smem = ((L + 63) / 64 + 4) * BLOCK_BYTES + 2048;
+  if (f32) ns_small_kernel<float><<<batch, SMALL_THREADS, smem, stream>>>(p);
+  else ns_small_kernel<__nv_bfloat16><<<batch, SMALL_THREADS, smem, stream>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 1000 + (int)e;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -525,7 +745,9 @@ static int prepare_device(int* n_sm) {
     if (cudaFuncSetAttribute(ns_product_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
         cudaFuncSetAttribute(ns_product_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
         cudaFuncSetAttribute(ns_product_kernel<256, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess) return 302;
+        cudaFuncSetAttribute(ns_product_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 4) * BLOCK_BYTES + 2048) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_small_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 4) * BLOCK_BYTES + 2048) != cudaSuccess) return 302;
     cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
     attr_mask |= 1ull << dev;
   }
@@ -676,7 +898,9 @@ constexpr int MAX_STEPS = 32;
 }  // namespace dttt
 
 // Bytes of the scratch area for `batch` matrices [rows, cols] (256-byte aligned base).
-extern "C" long long dttt_newton_schulz_scratch(int batch, int rows, int cols) { return dttt::ns::Scratch(nullptr, batch, rows, cols).bytes; }
+extern "C" long long dttt_newton_schulz_scratch(int batch, int rows, int cols) {
+  return dttt::ns::is_small(rows, cols) ? 0 : dttt::ns::Scratch(nullptr, batch, rows, cols).bytes;
+}
 
 // Groups of iterations, each with one d x d matrix of the linear map.
 extern "C" int dttt_newton_schulz_groups(int rows, int cols, int steps) {
@@ -692,6 +916,11 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
   int n_sm;
   if (int r = prepare_device(&n_sm)) return r;
+  if (is_small(rows, cols)) {
+    const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
+    const SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, X_SCALE, (__half*)maps, (long long)batch * small * ld, norms, y, status};
+    return launch_small(p, f32, batch, stream);
+  }
   const Scratch s(scratch, batch, rows, cols);
   const int d = s.d, ldd = s.ldd;
   if (int r = cast(g, f32, batch, rows, cols, s.partial, X_SCALE, s.x[0], s.ld, norms, n_sm, stream)) return r;
@@ -733,6 +962,12 @@ extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, in
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
   int n_sm;
   if (int r = prepare_device(&n_sm)) return r;
+  if (is_small(rows, cols)) {
+    const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
+    const SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, R_SCALE, (__half*)const_cast<void*>(maps),
+                           (long long)batch * small * ld, const_cast<double*>(norms), out, status};
+    return launch_small(p, f32, batch, stream);
+  }
   const Scratch s(scratch, batch, rows, cols);
   if (int r = cast(r_in, f32, batch, rows, cols, s.partial, R_SCALE, s.x[0], s.ld, s.norm, n_sm, stream)) return r;
   Group plan[MAX_STEPS];

@@ -869,11 +869,16 @@ def newton_schulz(g, steps, keep):
     y = torch.empty((B, rows, cols), dtype=torch.bfloat16, device=dev)
     norms = torch.empty(B, dtype=torch.float64, device=dev)
     l = _lib.lib()
-    polys = torch.empty((l.dttt_newton_schulz_groups(rows, cols, steps) if keep else 1, B, d, -(-d // 8) * 8), dtype=torch.float16, device=dev)
-    scratch = torch.empty(l.dttt_newton_schulz_scratch(B, rows, cols), dtype=torch.uint8, device=dev)
+    size = l.dttt_newton_schulz_scratch(B, rows, cols)                   # 0: small matrices, one launch that needs none
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    polys = None
+    if keep or size:
+        polys = torch.empty((l.dttt_newton_schulz_groups(rows, cols, steps) if keep else 1, B, d, -(-d // 8) * 8), dtype=torch.float16, device=dev)
     _launch("newton_schulz", l.dttt_newton_schulz, dev, g.data_ptr(), int(g.dtype == torch.float32), B, rows, cols, steps,
-            scratch.data_ptr(), polys.data_ptr(), int(keep), norms.data_ptr(), y.data_ptr(), _lib.status_tensor(dev).data_ptr())
-    LAUNCHES += 1 + 3 * steps
+            scratch.data_ptr() if size else None, None if polys is None else polys.data_ptr(), int(keep), norms.data_ptr(), y.data_ptr(),
+            _lib.status_tensor(dev).data_ptr())
+    if size:
+        LAUNCHES += 1 + 3 * steps
     return y, norms, polys
 
 
@@ -884,9 +889,11 @@ def newton_schulz_apply(r, norms, polys, steps, out_dtype):
     dev = r.device
     out = torch.empty((B, rows, cols), dtype=out_dtype, device=dev)
     l = _lib.lib()
-    scratch = torch.empty(l.dttt_newton_schulz_scratch(B, rows, cols), dtype=torch.uint8, device=dev)
+    size = l.dttt_newton_schulz_scratch(B, rows, cols)
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), int(r.dtype == torch.float32), B, rows, cols, steps,
-            scratch.data_ptr(), polys.data_ptr(), norms.data_ptr(), out.data_ptr(), int(out_dtype == torch.float32),
+            scratch.data_ptr() if size else None, polys.data_ptr(), norms.data_ptr(), out.data_ptr(), int(out_dtype == torch.float32),
             _lib.status_tensor(dev).data_ptr())
-    LAUNCHES += 1 + polys.shape[0]
+    if size:
+        LAUNCHES += 1 + polys.shape[0]
     return out
