@@ -531,23 +531,67 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
     tmem_relinquish();
   }
   // the norm, then the scaled f16 copy
-  const T* g = reinterpret_cast<const T*>(p.in) + (long long)b * p.rows * p.cols;
+  const T* __restrict__ g = reinterpret_cast<const T*>(p.in) + (long long)b * p.rows * p.cols;
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const bool aligned = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  const int n = p.rows * p.cols, nv = aligned ? n / VEC : 0;
   double s = 0;
-  for (int i = tid; i < p.rows * p.cols; i += SMALL_THREADS) { const double e = (double)to_f32(g[i]); s = fma(e, e, s); }
+  for (int i = tid; i < nv; i += 8 * SMALL_THREADS) {
+    uint4 raw[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      raw[k] = i + k * SMALL_THREADS < nv ? __ldg(reinterpret_cast<const uint4*>(g) + i + k * SMALL_THREADS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) { const double e = (double)to_f32(reinterpret_cast<const T*>(&raw[k])[j]); s = fma(e, e, s); }
+  }
+  for (int i = nv * VEC + tid; i < n; i += 8 * SMALL_THREADS) {
+    float e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = i + k * SMALL_THREADS < n ? to_f32(g[i + k * SMALL_THREADS]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s = fma((double)e[k], (double)e[k], s);
+  }
   const double whole = sqrt(block_sum(s));
   if (!p.apply && tid == 0) p.norms[b] = whole;
   const double f = whole == 0.0 ? 0.0 : (double)p.scale / whole;
-  const int pieces = Lp / 8;
-  for (int i = tid; i < SMALL_D * pieces; i += SMALL_THREADS) {
-    const int row = wide ? i / pieces : i % SMALL_D, col = (wide ? i % pieces : i / SMALL_D) * 8;
-    uint4 o;
-    __half* h = reinterpret_cast<__half*>(&o);
+  int ex = 0;
+  const double mant = frexp(f, &ex);
+  const float f0 = (float)ldexp(mant, ex / 2), f1 = (float)ldexp(1.0, ex - ex / 2);      // two factors: no finite norm leaves their range
+  // pieces of 8 columns of x, neighbouring threads on neighbouring memory; four of them in flight
+  const int pieces = Lp / 8, all = SMALL_D * pieces;
+  const bool vec = wide && aligned && p.cols % 8 == 0;
+  for (int i0 = tid; i0 < all; i0 += 4 * SMALL_THREADS) {
+    float x[4][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool in = row < d && col + e < L;
-      h[e] = in ? __float2half_rn((float)((double)to_f32(g[wide ? row * p.cols + col + e : (col + e) * p.cols + row]) * f)) : __half(0.f);
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * SMALL_THREADS;
+      const int row = wide ? i / pieces : i % SMALL_D, col = (wide ? i % pieces : i / SMALL_D) * 8;
+      const bool rows_in = i < all && row < d;
+      if (vec) {
+        uint4 raw[8 / VEC];
+#pragma unroll
+        for (int l = 0; l < 8 / VEC; ++l)
+          raw[l] = rows_in && col < L ? __ldg(reinterpret_cast<const uint4*>(g + row * p.cols + col) + l) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[k][e] = to_f32(reinterpret_cast<const T*>(raw)[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[k][e] = rows_in && col + e < L ? to_f32(g[wide ? row * p.cols + col + e : (col + e) * p.cols + row]) : 0.f;
+      }
     }
-    *reinterpret_cast<uint4*>(sx + small_offset(row, col)) = o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * SMALL_THREADS;
+      const int row = wide ? i / pieces : i % SMALL_D, col = (wide ? i % pieces : i / SMALL_D) * 8;
+      uint4 o;
+      __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(x[k][2 * e] * f0 * f1, x[k][2 * e + 1] * f0 * f1);
+      if (i < all) *reinterpret_cast<uint4*>(sx + small_offset(row, col)) = o;
+    }
   }
   float last = 1.f / p.scale;                                  // brings the last product to the result's scale
   if (p.apply) { const double n = p.norms[b]; last = n == 0.0 ? 0.f : (float)(whole / n / (double)p.scale); }
@@ -661,8 +705,18 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
       }
       if (!end) {
         store_small(sx, row, col, v);
+      } else if (row < d && wide && p.out == OUT_BF16 && p.cols % 8 == 0) {
+        uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.y) + (long long)b * n + row * p.cols + col);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint4 w;
+          __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[8 * q + 2 * e], v[8 * q + 2 * e + 1]);
+          if (col + 8 * q < L) o[q] = w;
+        }
       } else if (row < d) {
-        const long long base = (long long)b * p.rows * p.cols;
+        const long long base = (long long)b * n;
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (col + j < L) {
