@@ -108,7 +108,7 @@ __device__ __forceinline__ void load_rows(const __half* d, long long ld, int row
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int rr = i * 4 + (lane >> 3);
-    v[i] = d && rr < rows && piece * 8 < cols ? __ldg(reinterpret_cast<const uint4*>(d + rr * ld + piece * 8)) : make_uint4(0, 0, 0, 0);
+    v[i] = d && rr < rows && piece * 8 < cols ? __ldcg(reinterpret_cast<const uint4*>(d + rr * ld + piece * 8)) : make_uint4(0, 0, 0, 0);
   }
 }
 __device__ __forceinline__ void stage_in(uint8_t* stg, int lane, const uint4 (&v)[8]) {
@@ -220,6 +220,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // launched while the product before it still runs (programmatic dependence): up to here nothing touched global memory
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -773,7 +776,7 @@ struct Mat {
 };
 
 // `mn`: the operand's rows run along the contraction (its M or N index is contiguous); the box is then 64 x BK, else BK x box_rows.
-static int make_map(CUtensorMap* map, const Mat& m, int batch, bool mn, int box_rows) {
+static int encode_map(CUtensorMap* map, const Mat& m, int batch, bool mn, int box_rows) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return 101;
   cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)batch};
@@ -785,6 +788,22 @@ static int make_map(CUtensorMap* map, const Mat& m, int batch, bool mn, int box_
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : 200 + (int)r;
 }
+
+// One call's tensor maps: its products use the same few buffers again and again, and encoding a map takes the host a microsecond.
+struct Maps {
+  struct Entry { Mat m; bool mn; int box_rows; CUtensorMap map; } e[24];
+  int n = 0;
+  int get(const CUtensorMap** out, const Mat& m, int batch, bool mn, int box_rows) {
+    for (int i = 0; i < n; ++i)
+      if (e[i].m.ptr == m.ptr && e[i].m.rows == m.rows && e[i].m.cols == m.cols && e[i].m.ld == m.ld && e[i].mn == mn &&
+          (mn || e[i].box_rows == box_rows)) { *out = &e[i].map; return 0; }
+    const int at = n < 24 ? n++ : 23;                        // more than there is room for (kept maps of many steps): the last is replaced
+    if (int r = encode_map(&e[at].map, m, batch, mn, box_rows)) return r;
+    e[at].m = m; e[at].mn = mn; e[at].box_rows = box_rows;
+    *out = &e[at].map;
+    return 0;
+  }
+};
 
 static int prepare_device(int* n_sm) {
   static std::mutex mu;
@@ -817,7 +836,7 @@ struct Out {
 };
 
 // C [M, N] = alpha op(A) op(B) + beta D (+ beta2 D2 + diag I, with the layout of D) over the batch (symmetric: C and D are, and only f16)
-static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, const Mat& B, bool b_mn, float alpha, float beta, const Mat* D,
+static int product(Maps& maps, int batch, int M, int N, int K, const Mat& A, bool a_mn, const Mat& B, bool b_mn, float alpha, float beta, const Mat* D,
                    const Out& o, bool symmetric, int* status, int n_sm, cudaStream_t stream, const Mat* D2 = nullptr, float beta2 = 0.f,
                    float diag = 0.f) {
   Params p;
@@ -841,22 +860,31 @@ static int product(int batch, int M, int N, int K, const Mat& A, bool a_mn, cons
   const int narrow = cost[1] < cost[0];
   p.tiles_n = (N + (256 >> narrow) - 1) / (256 >> narrow);
   if (tiles[narrow] > 0x3fffffff) return 303;
-  CUtensorMap mapA, mapB;
-  if (int r = make_map(&mapA, A, batch, a_mn, BM)) return r;
-  if (int r = make_map(&mapB, B, batch, b_mn, narrow ? 64 : 128)) return r;
-  const int grid = 2 * (int)(tiles[narrow] < pairs ? tiles[narrow] : pairs);
-  const int smem = narrow ? Tile<128>::SMEM : Tile<256>::SMEM;
-  if (D2) (narrow ? ns_product_kernel<128, true> : ns_product_kernel<256, true>)<<<grid, THREADS, smem, stream>>>(mapA, mapB, p);
-  else (narrow ? ns_product_kernel<128, false> : ns_product_kernel<256, false>)<<<grid, THREADS, smem, stream>>>(mapA, mapB, p);
-  const cudaError_t e = cudaGetLastError();
+  const CUtensorMap *mapA, *mapB;
+  CUtensorMap copyA;                                           // a later lookup may replace an entry
+  if (int r = maps.get(&mapA, A, batch, a_mn, BM)) return r;
+  copyA = *mapA;
+  if (int r = maps.get(&mapB, B, batch, b_mn, narrow ? 64 : 128)) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (int)(tiles[narrow] < pairs ? tiles[narrow] : pairs));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = narrow ? Tile<128>::SMEM : Tile<256>::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // the prologue overlaps the product before
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, D2 ? (narrow ? ns_product_kernel<128, true> : ns_product_kernel<256, true>)
+                                                    : (narrow ? ns_product_kernel<128, false> : ns_product_kernel<256, false>), copyA, *mapB, p);
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
 // r (f16) -> beta r + alpha M r (r M^T of a tall one), or with the transpose of M: into f16 or, at the end, into the caller's tensor
-static int apply(int batch, int rows, int cols, const Mat& r, const Mat& M, bool transposed, float alpha, float beta, const Out& o, int* status,
+static int apply(Maps& maps, int batch, int rows, int cols, const Mat& r, const Mat& M, bool transposed, float alpha, float beta, const Out& o, int* status,
                  int n_sm, cudaStream_t stream) {
-  if (rows <= cols) return product(batch, rows, cols, rows, M, transposed, r, true, alpha, beta, &r, o, false, status, n_sm, stream);
-  return product(batch, rows, cols, cols, r, false, M, transposed, alpha, beta, &r, o, false, status, n_sm, stream);
+  if (rows <= cols) return product(maps, batch, rows, cols, rows, M, transposed, r, true, alpha, beta, &r, o, false, status, n_sm, stream);
+  return product(maps, batch, rows, cols, cols, r, false, M, transposed, alpha, beta, &r, o, false, status, n_sm, stream);
 }
 
 template <class T>
@@ -962,9 +990,9 @@ extern "C" int dttt_newton_schulz_groups(int rows, int cols, int steps) {
   return steps <= 0 || steps > dttt::ns::MAX_STEPS ? 0 : dttt::ns::make_plan(rows, cols, steps, g);
 }
 
-// g [batch, rows, cols] (f32 or bf16, contiguous) -> y bf16.  maps: f16 [groups or 1, batch, d, ceil8(d)]; with keep every group's
+// g [batch, rows, cols] (f32 or bf16, contiguous) -> y bf16.  kept: f16 [groups or 1, batch, d, ceil8(d)]; with keep every group's
 // matrix stays there for the backward, else one slot is used again and again.  norms: f64 [batch].
-extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, int cols, int steps, void* scratch, void* maps, int keep,
+extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, int cols, int steps, void* scratch, void* kept, int keep,
                                   double* norms, void* y, int* status, cudaStream_t stream) {
   using namespace dttt::ns;
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
@@ -972,26 +1000,27 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   if (int r = prepare_device(&n_sm)) return r;
   if (is_small(rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    const SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, X_SCALE, (__half*)maps, (long long)batch * small * ld, norms, y, status};
+    const SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, X_SCALE, (__half*)kept, (long long)batch * small * ld, norms, y, status};
     return launch_small(p, f32, batch, stream);
   }
   const Scratch s(scratch, batch, rows, cols);
   const int d = s.d, ldd = s.ldd;
   if (int r = cast(g, f32, batch, rows, cols, s.partial, X_SCALE, s.x[0], s.ld, norms, n_sm, stream)) return r;
   const bool wide = rows <= cols;
+  Maps maps;
   Group plan[MAX_STEPS];
   const int groups = make_plan(rows, cols, steps, plan);
   const Mat G = {s.gram, d, d, ldd}, H = {s.h, d, d, ldd}, P1 = {s.p, d, d, ldd};
   auto square = [&](const Mat& A, const Mat& B, float alpha, float beta, const Mat& D, const Mat& C, const Mat* D2 = nullptr, float beta2 = 0.f,
                     float diag = 0.f) {
     const Out o = {const_cast<void*>(C.ptr), OUT_F16, ldd, nullptr, nullptr};
-    return product(batch, d, d, d, A, false, B, false, alpha / X_SCALE, beta, &D, o, D2 == nullptr, status, n_sm, stream, D2, beta2, diag);
+    return product(maps, batch, d, d, d, A, false, B, false, alpha / X_SCALE, beta, &D, o, D2 == nullptr, status, n_sm, stream, D2, beta2, diag);
   };
   for (int k = 0; k < groups; ++k) {
     const Mat X = {s.x[k & 1], rows, cols, s.ld};
-    const Mat M = {(uint8_t*)maps + (keep ? (long long)k * batch * d * ldd * 2 : 0), d, d, ldd};
+    const Mat M = {(uint8_t*)kept + (keep ? (long long)k * batch * d * ldd * 2 : 0), d, d, ldd};
     const Out og = {s.gram, OUT_F16, ldd, nullptr, nullptr};
-    if (int r = product(batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, true, status, n_sm, stream)) return r;
+    if (int r = product(maps, batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, true, status, n_sm, stream)) return r;
     if (plan[k].steps == 1) {
       if (int r = square(G, G, NS_C, NS_B, G, M)) return r;                                  // P = b G + c G G
     } else {
@@ -1004,13 +1033,13 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
     const bool last = k == groups - 1;
     const float f = last ? 1.f / X_SCALE : 1.f;
     const Out ox = {last ? y : s.x[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : s.ld, nullptr, nullptr};
-    if (int r = apply(batch, rows, cols, X, M, false, f / X_SCALE, f * plan[k].alpha, ox, status, n_sm, stream)) return r;
+    if (int r = apply(maps, batch, rows, cols, X, M, false, f / X_SCALE, f * plan[k].alpha, ox, status, n_sm, stream)) return r;
   }
   return 0;
 }
 
 // r [batch, rows, cols] (f32 or bf16) -> out (f32 or bf16) = prod_k (alpha_k I + M_k) r / norms, the maps of a forward with keep.
-extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, int rows, int cols, int steps, void* scratch, const void* maps,
+extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, int rows, int cols, int steps, void* scratch, const void* kept,
                                         const double* norms, void* out, int out_f32, int* status, cudaStream_t stream) {
   using namespace dttt::ns;
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
@@ -1018,23 +1047,24 @@ extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, in
   if (int r = prepare_device(&n_sm)) return r;
   if (is_small(rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    const SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, R_SCALE, (__half*)const_cast<void*>(maps),
+    const SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, R_SCALE, (__half*)const_cast<void*>(kept),
                            (long long)batch * small * ld, const_cast<double*>(norms), out, status};
     return launch_small(p, f32, batch, stream);
   }
   const Scratch s(scratch, batch, rows, cols);
   if (int r = cast(r_in, f32, batch, rows, cols, s.partial, R_SCALE, s.x[0], s.ld, s.norm, n_sm, stream)) return r;
+  Maps maps;
   Group plan[MAX_STEPS];
   const int groups = make_plan(rows, cols, steps, plan);
   for (int i = 0; i < groups; ++i) {
     const int k = groups - 1 - i;
     const Mat X = {s.x[i & 1], rows, cols, s.ld};
-    const Mat M = {(const uint8_t*)maps + (long long)k * batch * s.d * s.ldd * 2, s.d, s.d, s.ldd};
+    const Mat M = {(const uint8_t*)kept + (long long)k * batch * s.d * s.ldd * 2, s.d, s.d, s.ldd};
     const bool last = k == 0;
     const float f = last ? 1.f / R_SCALE : 1.f;
     const Out o = {last ? out : s.x[(i + 1) & 1], last ? (out_f32 ? OUT_F32 : OUT_BF16) : OUT_F16, last ? cols : s.ld, last ? s.norm : nullptr,
                    last ? norms : nullptr};
-    if (int r = apply(batch, rows, cols, X, M, true, f / X_SCALE, f * plan[k].alpha, o, status, n_sm, stream)) return r;
+    if (int r = apply(maps, batch, rows, cols, X, M, true, f / X_SCALE, f * plan[k].alpha, o, status, n_sm, stream)) return r;
   }
   return 0;
 }
