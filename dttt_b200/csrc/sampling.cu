@@ -38,6 +38,7 @@ constexpr int MAX_WARPS = 16;
 constexpr int OCTAVES = 256;                 // bins of the octave counts
 constexpr int BINS = 128;                    // of a round of the search
 constexpr int TAB = 64, COPIES = 8;
+constexpr int FEW = 256;                    // candidates up to which one CTA finishes a row
 constexpr int LIST = 256;                    // entries of all warps
 constexpr int SLICE_MAX = 49152;            // elements of a slice at most (192 KB)
 constexpr int SLICE_GOOD = 16384;           // a slice up to which three CTAs fit an SM
@@ -141,8 +142,9 @@ struct Shared {
   int at_max[MAX_WARPS], first_max[MAX_WARPS];
   u64 mass[MAX_WARPS];                      // of every element, or of the kept ones
   unsigned int octaves_here[OCTAVES];
-  unsigned int count[2][BINS];              // histograms of the threshold search, alternating between rounds
-  u64 hmass[2][BINS];
+  int pushed;                               // entries of the candidate list, which in CTA 0 takes the place of the histograms
+  alignas(16) u64 hmass[2][BINS];           // histograms of the threshold search, alternating between rounds
+  unsigned int count[2][BINS];
   unsigned int above_count[2];
   u64 above_mass[2];
   // this CTA alone
@@ -154,6 +156,7 @@ struct Shared {
   unsigned int tot_count[BINS];
   unsigned int octaves[OCTAVES];            // of all CTAs
   uint32_t range[2];
+  int last_bin, candidates;                 // the octaves down to last_bin hold the prefix; so many elements
   u64 tot_above_count, tot_above_mass;
   int pick_bin, idx_star;
   u64 pick_above_count, pick_above_mass;
@@ -273,8 +276,11 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
     const float w_lo = exp2f(-(lane * EACH + 0.5f) / PER_OCTAVE), w_hi = exp2f(-(lane * EACH - 0.5f) / PER_OCTAVE);
     float lo[EACH], hi[EACH], wl = w_lo, wh = w_hi;
     float slo = 0, shi = 0;
+    unsigned int n[EACH], sn = 0;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
+      sn += sh.octaves[lane * EACH + j];
+      n[j] = sn;
       const float c = (float)sh.octaves[lane * EACH + j];
       slo += MASS ? c * wl : c;
       shi += MASS ? c * fminf(wh, 1.f) : c;
@@ -282,12 +288,14 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
       wl *= STEP; wh *= STEP;
     }
     float blo = slo, bhi = shi;
+    unsigned int bn = sn;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const float a = __shfl_up_sync(0xffffffffu, blo, o), b = __shfl_up_sync(0xffffffffu, bhi, o);
-      if (lane >= o) { blo += a; bhi += b; }
+      const unsigned int c = __shfl_up_sync(0xffffffffu, bn, o);
+      if (lane >= o) { blo += a; bhi += b; bn += c; }
     }
-    blo -= slo; bhi -= shi;
+    blo -= slo; bhi -= shi; bn -= sn;
     // counts are whole numbers below 2^24: their float sums are exact
     const float goal = MASS ? (float)((double)target * unit) : (float)target, slack = MASS ? (float)((double)V * unit) : 0.f;
     int first = OCTAVES - 1, last = OCTAVES - 1;
@@ -298,6 +306,9 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
     }
     first = __reduce_min_sync(0xffffffffu, first);
     last = __reduce_min_sync(0xffffffffu, last);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j)
+      if (lane * EACH + j == last) { sh.last_bin = last; sh.candidates = last == OCTAVES - 1 ? 0x7fffffff : (int)(bn + n[j]); }
     if (lane < 2) {
       const float edge = lane ? fmaxf(first - 0.5f, 0.f) * (1.f - 1e-5f) : (last + 0.5f) * (1.f + 1e-5f);
       const double at = (double)m - (double)edge / (double)scale, eps = fabs((double)m) * 1e-6;
@@ -325,11 +336,12 @@ __device__ __forceinline__ void for_range(const Shared& sh, const float* xs, Seg
 // `target`: 128-way search over the order keys from the range above; a pass over the slice and a cluster barrier per round.  Only
 // elements of the range and, in the first round, those above it cost more than a comparison.
 template <int WARPS, bool MASS>
-__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, int bits, int V, u64 target, int& round) {
+__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, int bits, int V, u64 target, bool ranged,
+                        int& round) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Segment seg = split(0, n, WARPS, warp);
-  first_range<MASS>(sh, m, scale, 1.0 / (double)(1ull << bits), V, target);
+  if (!ranged) first_range<MASS>(sh, m, scale, 1.0 / (double)(1ull << bits), V, target);
   uint32_t k0 = sh.range[0], k1 = sh.range[1];
   const float first_hi = key_value(k1);
   u64 above_c = 0, above_m = 0;
@@ -520,6 +532,131 @@ __device__ __forceinline__ unsigned int cluster_id() {
   return r;
 }
 
+// By one warp: log of the untempered sum, and the priority where it is not the log-probability.
+template <int WARPS>
+__device__ __forceinline__ float2 untempered(const SampleParams& p, Shared& sh, int lane, float m) {
+  const double z = warp_sum(warp_values<WARPS>(sh, lane, 0.0, [](double v, const Shared& q, int k) { return v + (double)q.z[k]; }));
+  const float logz = logf((float)z);
+  float pr = 0.f;
+  if (p.priority == PRI_MARGIN) {
+    const float second = warp_max(warp_values<WARPS>(sh, lane, -INFINITY, [](float v, const Shared& q, int k) { return fmaxf(v, q.ent[k]); }));
+    const int at_max = __reduce_add_sync(0xffffffffu, warp_values<WARPS>(sh, lane, 0, [](int v, const Shared& q, int k) { return v + q.at_max[k]; }));
+    pr = at_max > 1 ? 0.f : (float)((1.0 - (double)__expf(second - m)) / z);
+  } else if (p.priority == PRI_ENTROPY) {
+    const double ent = warp_sum(warp_values<WARPS>(sh, lane, 0.0, [](double v, const Shared& q, int k) { return v + (double)q.ent[k]; }));
+    pr = (float)(ent * 0.6931471805599453 / z - (double)logz);
+  }
+  return make_float2(logz, pr);
+}
+
+// The row's end where no more than FEW elements lie in the octaves that hold the kept ones: all CTAs push theirs into the list of CTA
+// 0 and leave; it ranks them against one another (by value, then index), which gives every cut at once, and draws.  The pushes come
+// in any order and nothing depends on it.
+struct Candidate { float x; int i; };
+static_assert(sizeof(Shared::hmass) + sizeof(Shared::count) >= FEW * sizeof(Candidate), "the candidate list takes the histograms' place");
+template <int WARPS>
+__device__ __noinline__ void few_candidates(const SampleParams& p, Shared& sh, const float* xs, Segment seg, int first, unsigned int row, float m,
+                                            float scale, const Weigher& w, int top_k, double top_p, u64 whole, float least) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = (int)cluster.block_rank();
+  Shared* home = cluster.map_shared_rank(&sh, 0);
+  Candidate* list = reinterpret_cast<Candidate*>(&home->hmass[0][0]);
+  const int last = sh.last_bin, n = sh.candidates;
+  for (int i0 = seg.a; i0 < seg.b; i0 += 128) {
+    float x[4];
+    unsigned int in = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * 32 + lane;
+      x[k] = i < seg.b ? xs[i] : -INFINITY;
+      if (octave_bin(x[k], m, scale) <= last) in |= 1u << k;
+    }
+    if (!__any_sync(0xffffffffu, in)) continue;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned int any = __ballot_sync(0xffffffffu, in >> k & 1);
+      if (!any) continue;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&home->pushed, __popc(any));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(any & ((1u << lane) - 1));
+      if ((in >> k & 1) && at < FEW) list[at] = {x[k], first + i0 + k * 32 + lane};
+    }
+  }
+  if (me == 0 && warp == 1) {                                      // the others' sums, before they leave
+    const float2 t = untempered<WARPS>(p, sh, lane, m);
+    if (lane == 0) { sh.logz = t.x; sh.pr = t.y; }
+  }
+  cluster.sync();
+  if (me != 0) return;
+  // a candidate per thread (or two): its place in the order and the mass before it
+  constexpr int THREADS = WARPS * 32, EACH = (FEW + THREADS - 1) / THREADS;
+  u64* mass = reinterpret_cast<u64*>(sh.tab);                      // in the place of the table, which is read for the last time here
+  static_assert(sizeof(Shared::tab) >= FEW * sizeof(u64), "room for the masses");
+  u64 before[EACH], upto[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) before[e] = tid + e * THREADS < n ? w(list[tid + e * THREADS].x) : 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (tid + e * THREADS < n) mass[tid + e * THREADS] = before[e];
+  __syncthreads();
+  int rank[EACH];
+  u64 topped = 0;                                                  // the mass of the first top_k
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int j = tid + e * THREADS;
+    before[e] = 0; rank[e] = 0;
+    if (j < n) {
+      const Candidate c = list[j];
+#pragma unroll 4
+      for (int o = 0; o < n; ++o) {
+        const Candidate q = list[o];
+        const bool ahead = q.x > c.x || (q.x == c.x && q.i < c.i);
+        rank[e] += ahead;
+        before[e] += ahead ? mass[o] : 0;
+      }
+      if (rank[e] < top_k) topped += mass[j];
+    }
+  }
+  topped = warp_sum(topped);
+  if (lane == 0) sh.sub[warp] = topped;
+  __syncthreads();
+  if (top_k < p.V) { whole = 0; for (int k = 0; k < WARPS; ++k) whole += sh.sub[k]; }
+  const u64 goal = max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole)));
+  __syncthreads();
+  u64 kept = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int j = tid + e * THREADS;
+    if (j < n) {
+      if (!(rank[e] < top_k && (top_p >= 1.0 || before[e] < goal) && list[j].x >= least)) mass[j] = 0;
+      kept += mass[j];
+    }
+  }
+  kept = warp_sum(kept);
+  if (lane == 0) sh.sub[warp] = kept;
+  __syncthreads();
+  u64 total = 0;
+  for (int k = 0; k < WARPS; ++k) total += sh.sub[k];
+  const double u = (double)sh.u;
+  const u64 want = min(u > 0 ? (u64)(fmin(u, 1.0) * (double)total) : 0, total - 1);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int j = tid + e * THREADS;
+    if (j < n && mass[j]) {
+      const Candidate c = list[j];
+      upto[e] = 0;                                                 // in order of the indices
+#pragma unroll 4
+      for (int o = 0; o < n; ++o) upto[e] += list[o].i <= c.i ? mass[o] : 0;
+      if (upto[e] > want && upto[e] - mass[j] <= want) {
+        p.tokens[row] = c.i;
+        p.logp[row] = (c.x - m) - sh.logz;
+        if (p.priority != PRI_LOGP) p.prio[row] = sh.pr;
+      }
+    }
+  }
+}
+
 static_assert(sizeof(Shared) <= 12600, "three CTAs with slices of 16032 elements (V = 128256) on an SM");
 
 template <class T, int WARPS>
@@ -555,6 +692,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
     sh.scale = (float)(PER_OCTAVE * sh.log2e_t);
     sh.u = p.u[row];
     for (int b = 0; b < 2; ++b) { sh.above_count[b] = 0; sh.above_mass[b] = 0; }
+    sh.pushed = 0;
   }
   float mx = -INFINITY;
   for (int v = v0 + tid; v < v1; v += THREADS * UNROLL) {
@@ -654,13 +792,21 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
       }
       __syncthreads();
       u64 whole = sh.whole;
+      const double unit = 1.0 / (double)(1ull << p.scale_bits);
+      const u64 goal = max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole)));      // of a cut by mass alone
+      if (by_count) first_range<false>(sh, m, scale, unit, p.V, (u64)top_k);
+      else first_range<true>(sh, m, scale, unit, p.V, goal);
+      if (sh.candidates <= FEW) {
+        few_candidates<WARPS>(p, sh, xs, seg, first, row, m, scale, w, by_count ? top_k : p.V, by_mass ? top_p : 2.0, whole, least);
+        return;
+      }
       if (by_count) {
-        cut = find_cut<WARPS, false>(sh, xs, n, w, m, scale, p.scale_bits, p.V, (u64)top_k, round);
+        cut = find_cut<WARPS, false>(sh, xs, n, w, m, scale, p.scale_bits, p.V, (u64)top_k, true, round);
         whole = cut.mass;
       }
       if (by_mass) {
-        const double goal = ceil(fmax(top_p, 0.0) * (double)whole);
-        cut = find_cut<WARPS, true>(sh, xs, n, w, m, scale, p.scale_bits, p.V, max((u64)1, min(whole, (u64)goal)), round);
+        const u64 target = by_count ? max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole))) : goal;
+        cut = find_cut<WARPS, true>(sh, xs, n, w, m, scale, p.scale_bits, p.V, target, !by_count, round);
       }
     }
     if (cut.before + cut.here > cut.ties) {                        // this CTA holds ties that are not kept
@@ -726,17 +872,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
       }
     }
   } else if (warp == 1) {
-    const double z = warp_sum(warp_values<WARPS>(sh, lane, 0.0, [](double v, const Shared& q, int k) { return v + (double)q.z[k]; }));
-    const float logz = logf((float)z);
-    float pr = 0.f;
-    if (p.priority == PRI_MARGIN) {
-      const float second = warp_max(warp_values<WARPS>(sh, lane, -INFINITY, [](float v, const Shared& q, int k) { return fmaxf(v, q.ent[k]); }));
-      const int at_max = __reduce_add_sync(0xffffffffu, warp_values<WARPS>(sh, lane, 0, [](int v, const Shared& q, int k) { return v + q.at_max[k]; }));
-      pr = at_max > 1 ? 0.f : (float)((1.0 - (double)__expf(second - m)) / z);
-    } else if (p.priority == PRI_ENTROPY) {
-      const double ent = warp_sum(warp_values<WARPS>(sh, lane, 0.0, [](double v, const Shared& q, int k) { return v + (double)q.ent[k]; }));
-      pr = (float)(ent * 0.6931471805599453 / z - (double)logz);
-    }
+    const float2 t = untempered<WARPS>(p, sh, lane, m);
+    const float logz = t.x, pr = t.y;
     if (lane == 0) {
       sh.logz = logz; sh.pr = pr;
       if (greedy && me == 0) {
