@@ -866,7 +866,7 @@ def newton_schulz(g, steps, keep):
     global LAUNCHES
     B, rows, cols = g.shape
     d, dev = min(rows, cols), g.device
-    y = torch.empty((B, rows, cols), dtype=torch.bfloat16, device=dev)
+    y = torch.empty_like(g, dtype=torch.bfloat16)
     norms = torch.empty(B, dtype=torch.float64, device=dev)
     l = _lib.lib()
     size = l.dttt_newton_schulz_scratch(B, rows, cols)                   # 0: small matrices, one launch that needs none
@@ -887,7 +887,7 @@ def newton_schulz_apply(r, norms, polys, steps, out_dtype):
     global LAUNCHES
     B, rows, cols = r.shape
     dev = r.device
-    out = torch.empty((B, rows, cols), dtype=out_dtype, device=dev)
+    out = torch.empty_like(r, dtype=out_dtype)
     l = _lib.lib()
     size = l.dttt_newton_schulz_scratch(B, rows, cols)
     scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None

@@ -18,20 +18,25 @@ from . import reference as ref
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
     t = t if t.dtype in (torch.float32, torch.bfloat16) else t.float()
-    return t.reshape(-1, *t.shape[-2:]).contiguous()
+    t = t if t.dim() == 3 else t.reshape(-1, *t.shape[-2:])
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _linear(r: torch.Tensor, norms, maps, steps: int, dtype: torch.dtype) -> torch.Tensor:
+    """``M r / |g|`` with what a forward kept of ``g``."""
+    if isinstance(maps, list):
+        return ref.newton_schulz_apply(r, norms, maps).to(dtype)
+    from . import kernels
+    return kernels.newton_schulz_apply(_flat(r), norms, maps, steps, dtype).view(r.shape)
 
 
 class _Apply(torch.autograd.Function):
-    """``r -> M r / |g|`` with what a forward kept of ``g``; linear and self-adjoint."""
+    """``_linear`` as a differentiable operation: linear and self-adjoint."""
 
     @staticmethod
-    def forward(ctx, r, norms, polys, steps, dtype):
-        ctx.kept, ctx.dtype = (norms, polys, steps), r.dtype
-        if isinstance(polys, list):
-            return ref.newton_schulz_apply(r, norms, polys).to(dtype)
-        from . import kernels
-        out_dtype = torch.float32 if dtype == torch.float32 else torch.bfloat16
-        return kernels.newton_schulz_apply(_flat(r), norms, polys, steps, out_dtype).view(r.shape).to(dtype)
+    def forward(ctx, r, norms, maps, steps, dtype):
+        ctx.kept, ctx.dtype = (norms, maps, steps), r.dtype
+        return _linear(r, norms, maps, steps, dtype)
 
     @staticmethod
     def backward(ctx, c):
@@ -41,14 +46,13 @@ class _Apply(torch.autograd.Function):
 class _NewtonSchulz(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, steps):
-        y, norms, polys = _run(g, steps, True)
-        ctx.kept = norms, polys, steps
-        ctx.dtype = g.dtype
+        y, norms, maps = _run(g, steps, True)
+        ctx.kept, ctx.dtype = (norms, maps, steps), g.dtype
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        return _Apply.apply(gy, *ctx.kept, ctx.dtype), None
+        return (_Apply.apply if torch.is_grad_enabled() else _linear)(gy, *ctx.kept, ctx.dtype), None
 
 
 def _run(g: torch.Tensor, steps: int, keep: bool):
@@ -56,8 +60,8 @@ def _run(g: torch.Tensor, steps: int, keep: bool):
     if not g.is_cuda or "newton_schulz" in kernels._DISABLED:
         y, norms, polys = ref.newton_schulz(g, steps)
         return y.to(torch.bfloat16), norms, polys
-    y, norms, polys = kernels.newton_schulz(_flat(g), steps, keep)
-    return y.view(g.shape), norms, polys
+    y, norms, maps = kernels.newton_schulz(_flat(g), steps, keep)
+    return y.view(g.shape), norms, maps
 
 
 def newton_schulz(g: torch.Tensor, steps: int = 5) -> torch.Tensor:
