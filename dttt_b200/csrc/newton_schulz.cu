@@ -621,9 +621,21 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
     __syncthreads();
     tc_fence_after();
   };
+  // the kept P, [d, ldd], as rows of 16-byte pieces; the derivative takes them from the last to the first, each read a step ahead
+  constexpr int KEPT = SMALL_D * SMALL_D / 8 / SMALL_THREADS;
+  const int kept_pieces = p.ldd / 8;
+  auto map_of = [&](int k) { return p.maps + k * p.map_stride + (long long)b * d * p.ldd; };
+  uint4 next[KEPT];
+  auto fetch = [&](int k) {
+    const __half* map = map_of(p.steps - 1 - k);
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+      const int at = tid + i * SMALL_THREADS, r = at / (SMALL_D / 8), q = at % (SMALL_D / 8);
+      next[i] = r < d && q < kept_pieces ? reinterpret_cast<const uint4*>(map + r * p.ldd)[q] : make_uint4(0, 0, 0, 0);
+    }
+  };
+  if (p.apply) fetch(0);
   for (int k = 0; k < p.steps && ok; ++k) {
-    const int at = p.apply ? p.steps - 1 - k : p.keep ? k : 0;
-    __half* map = p.maps ? p.maps + at * p.map_stride + (long long)b * d * p.ldd : nullptr;
     if (!p.apply) {
       if (tid == 0) {
         const uint32_t a = smem_u32(sx), idesc = make_idesc_f16(128, 128, 0, 0);
@@ -663,21 +675,14 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
 #pragma unroll
         for (int j = 0; j < 32; ++j) gr[c][j] = fmaf(NS_B, gr[c][j], NS_C / X_SCALE * __uint_as_float(r[j]));
         store_small(sp, row, col, gr[c]);
-        if (p.keep && row < d)
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col + j < d) map[(long long)row * p.ldd + col + j] = __float2half_rn(gr[c][j]);
       }
     } else {
-      for (int i = tid; i < SMALL_D * (SMALL_D / 8); i += SMALL_THREADS) {
-        const int r = i / (SMALL_D / 8), col = i % (SMALL_D / 8) * 8;
-        uint4 o = make_uint4(0, 0, 0, 0);
-        __half* h = reinterpret_cast<__half*>(&o);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (r < d && col + e < d) h[e] = map[(long long)r * p.ldd + col + e];
-        *reinterpret_cast<uint4*>(sp + small_offset(r, col)) = o;
+      for (int i = 0; i < KEPT; ++i) {
+        const int at = tid + i * SMALL_THREADS;
+        *reinterpret_cast<uint4*>(sp + small_offset(at / (SMALL_D / 8), at % (SMALL_D / 8) * 8)) = next[i];
       }
+      if (k + 1 < p.steps) fetch(k + 1);
     }
     hand_over();
     if (tid == 0) {
@@ -691,6 +696,11 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
       }
       umma_commit(bar);
     }
+    if (!p.apply && p.keep)                                    // while the product runs; the padding of P is zero
+      for (int i = tid; i < d * kept_pieces; i += SMALL_THREADS) {
+        const int r = i / kept_pieces, q = i % kept_pieces;
+        reinterpret_cast<uint4*>(map_of(k) + r * p.ldd)[q] = *reinterpret_cast<const uint4*>(sp + small_offset(r, q * 8));
+      }
     if (!wait()) break;
     const bool end = k == p.steps - 1;
     const float fin = end ? last : 1.f;
