@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
 // iterations in one launch; what such sizes cost otherwise is launches.  x lies as blocks of 128 rows x 64 columns with 128-byte
 // swizzle, which is the K-major operand of G = x x^T and, read with its columns as N, the MN-major one of P x.  Rows and columns
 // beyond the matrix are zero and stay so.  Also the derivative (`apply`): the kept P of every iteration is read back.
-constexpr int SMALL_D = 128, SMALL_L = 512, SMALL_THREADS = 256;
+constexpr int SMALL_D = 128, SMALL_L = 512, SMALL_THREADS = 512;
 constexpr int BLOCK_BYTES = SMALL_D * 128;                     // 128 rows x 64 f16
 
 struct SmallParams {
@@ -563,15 +563,18 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   const double mant = frexp(f, &ex);
   const float f0 = (float)ldexp(mant, ex / 2), f1 = (float)ldexp(1.0, ex - ex / 2);      // two factors: no finite norm leaves their range
   // pieces of 8 columns of x, neighbouring threads on neighbouring memory; four of them in flight
-  const int pieces = Lp / 8, all = SMALL_D * pieces;
+  const int pieces = Lp / 8, all = d * pieces;
+  for (int i = all + tid; i < SMALL_D * pieces; i += SMALL_THREADS)      // rows beyond the matrix
+    *reinterpret_cast<uint4*>(sx + small_offset(i / pieces, i % pieces * 8)) = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < 4 * BLOCK_BYTES / 16; i += SMALL_THREADS) reinterpret_cast<uint4*>(sg)[i] = make_uint4(0, 0, 0, 0);      // of G and P
   const bool vec = wide && aligned && p.cols % 8 == 0;
   for (int i0 = tid; i0 < all; i0 += 4 * SMALL_THREADS) {
     float x[4][8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + k * SMALL_THREADS;
-      const int row = wide ? i / pieces : i % SMALL_D, col = (wide ? i % pieces : i / SMALL_D) * 8;
-      const bool rows_in = i < all && row < d;
+      const int row = wide ? i / pieces : i % d, col = (wide ? i % pieces : i / d) * 8;
+      const bool rows_in = i < all;
       if (vec) {
         uint4 raw[8 / VEC];
 #pragma unroll
@@ -588,7 +591,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + k * SMALL_THREADS;
-      const int row = wide ? i / pieces : i % SMALL_D, col = (wide ? i % pieces : i / SMALL_D) * 8;
+      const int row = wide ? i / pieces : i % d, col = (wide ? i % pieces : i / d) * 8;
       uint4 o;
       __half2* h = reinterpret_cast<__half2*>(&o);
 #pragma unroll
@@ -603,7 +606,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+  const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
+  const bool rows_here = quarter * 32 < d;                      // the others stay zero
   const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
   uint32_t phase = 0;
   bool ok = true;
@@ -646,15 +650,14 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         umma_commit(bar);
       }
       if (!wait()) break;
-      float gr[2][32];                                         // this thread's 64 entries of G
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      float gr[32];                                            // this thread's entries of G
+      if (rows_here) {
         uint32_t r[32];
-        tmem_ld_32x32(lanes + half * 64 + c * 32, r);
+        tmem_ld_32x32(lanes + part * 32, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) gr[c][j] = __uint_as_float(r[j]) * (1.f / X_SCALE);
-        store_small(sg, row, half * 64 + c * 32, gr[c]);
+        for (int j = 0; j < 32; ++j) gr[j] = __uint_as_float(r[j]) * (1.f / X_SCALE);
+        store_small(sg, row, part * 32, gr);
       }
       hand_over();
       if (tid == 0) {
@@ -666,15 +669,13 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         umma_commit(bar);
       }
       if (!wait()) break;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int col = half * 64 + c * 32;
+      if (rows_here) {
         uint32_t r[32];
-        tmem_ld_32x32(lanes + col, r);
+        tmem_ld_32x32(lanes + part * 32, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) gr[c][j] = fmaf(NS_B, gr[c][j], NS_C / X_SCALE * __uint_as_float(r[j]));
-        store_small(sp, row, col, gr[c]);
+        for (int j = 0; j < 32; ++j) gr[j] = fmaf(NS_B, gr[j], NS_C / X_SCALE * __uint_as_float(r[j]));
+        store_small(sp, row, part * 32, gr);
       }
     } else {
 #pragma unroll
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
     if (!wait()) break;
     const bool end = k == p.steps - 1;
     const float fin = end ? last : 1.f;
-    for (int col = half * 32; col < Lp; col += 64) {
+    for (int col = rows_here ? part * 32 : Lp; col < Lp; col += 128) {
       uint32_t r[32];
       tmem_ld_32x32(lanes + col, r);
       tmem_ld_wait();
