@@ -184,7 +184,7 @@ struct Weigher {
     c = TAB * log2e_t;
     mc = -(double)m * c;
     magic = __hiloint2double(0x3ff80000 + ((52 - bits) << 20), 0);         // 1.5 2^(52 - S)
-    least = __double2float_rd((double)m - cut);
+    least = fminf(__double2float_rd((double)m - cut), nextafterf(m, -INFINITY));      // below m, even where m - cut is m
     coarse = !(((double)m - (double)least) * c < 400.0 * TAB);
   }
   __device__ __forceinline__ u64 operator()(float x) const {

@@ -104,6 +104,19 @@ def test_rows_without_a_distribution_and_edge_draws():
             assert out.tokens[0, 0] == out.tokens[1, 1] == out.tokens[2, 2] == -1 and out.priority[0, 0].isnan()
 
 
+@pytest.mark.parametrize("V", [70, 5000, 50001])
+@pytest.mark.parametrize("top", [-3e38, -1e30, 1e30, 3e38, 1e12])
+def test_values_whose_neighbours_are_octaves_away(V, top):
+    """At 1e30 the next smaller float is far more than any temperature away: all of the mass is at the maximum."""
+    x, u = logits((4, 8), V)
+    x = x.abs().neg() * 1e25
+    x[:] += top
+    x[0], x[1, :, ::3] = top, top
+    for kw in PARAMS:
+        check(x, u, **kw)
+    check(x.repeat(5, 9, 1), u.repeat(5, 9))                               # enough rows for the two-launch form at the largest V
+
+
 def test_parameters_per_row():
     x, u = logits((6, 8), 30000, seed=3)
     gen = torch.Generator(device="cuda").manual_seed(1)
