@@ -142,6 +142,8 @@ struct Shared {
   int at_max[MAX_WARPS], first_max[MAX_WARPS];
   u64 mass[MAX_WARPS];                      // of every element, or of the kept ones
   unsigned int octaves_here[OCTAVES];
+  u64 all_mass;                             // of every element, where the search adds it up
+  float zt[MAX_WARPS];                      // tempered sums in 32 bits, of every element
   int pushed;                               // entries of the candidate list, which in CTA 0 takes the place of the histograms
   alignas(16) u64 hmass[2][BINS];           // histograms of the threshold search, alternating between rounds
   unsigned int count[2][BINS];
@@ -152,9 +154,14 @@ struct Shared {
   u64 above[MAX_WARPS], sub[MAX_WARPS];
   int ties[MAX_WARPS], listed[MAX_WARPS];
   unsigned short list[LIST];                // indices of each warp's elements in the search's first range, if they fit its share
-  u64 tot_mass[BINS];
-  unsigned int tot_count[BINS];
-  unsigned int octaves[OCTAVES];            // of all CTAs
+  union {
+    struct {
+      u64 tot_mass[BINS];
+      unsigned int tot_count[BINS];
+      unsigned int octaves[OCTAVES];        // of all CTAs
+    };
+    u64 few_mass[FEW];                      // of the candidates, where CTA 0 finishes the row
+  };
   uint32_t range[2];
   int last_bin, candidates;                 // the octaves down to last_bin hold the prefix; so many elements
   u64 tot_above_count, tot_above_mass;
@@ -163,6 +170,7 @@ struct Shared {
   double tab[TAB * COPIES];
   // this row's parameters, and at the end its answer but for the token
   double temp, min_p, top_p, log2e_t, cut;
+  double rough;                             // 32-bit sum of the tempered masses, in units of the maximum's
   float scale, u, logz, pr;
   int top_k, greedy;
   u64 whole, goal, base, mine;
@@ -188,7 +196,7 @@ struct Weigher {
     coarse = !(((double)m - (double)least) * c < 400.0 * TAB);
   }
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (coarse) return x < m ? 0 : (u64)(__double_as_longlong(magic + 1.0) - __double_as_longlong(magic));
+    if (coarse) return x >= m ? (u64)(__double_as_longlong(magic + 1.0) - __double_as_longlong(magic)) : 0;
     return fine(x) - (u64)__double_as_longlong(magic);
   }
   // not coarse; with the bits of `magic` still in it: for sums of many, from which they are taken once
@@ -265,10 +273,11 @@ __device__ __forceinline__ V warp_values(Shared& sh, int lane, V none, F get) {
 }
 
 // From the octave counts, the range of values that has to hold the last element of the prefix whose count or mass reaches
-// `target`.  Warp 0 computes it, from the top bin down, with every element's mass between those of its bin's borders (1e-4 is far
-// more than the rounding of the bins can shift them); the borders are widened by more than the rounding of m - x.
+// `goal` (a mass as a part of exp(0), known to 2e-4 of itself, give or take `slack`).  Warp 0 computes it, from the top bin down, with
+// every element's mass between those of its bin's borders (1e-4 is far more than the rounding of the bins can shift them); the
+// borders are widened by more than the rounding of m - x.
 template <bool MASS>
-__device__ __forceinline__ void first_range(Shared& sh, float m, float scale, double unit, int V, u64 target) {
+__device__ __forceinline__ void first_range(Shared& sh, float m, float scale, float goal, float slack) {
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
     constexpr int EACH = OCTAVES / 32;
@@ -297,12 +306,11 @@ __device__ __forceinline__ void first_range(Shared& sh, float m, float scale, do
     }
     blo -= slo; bhi -= shi; bn -= sn;
     // counts are whole numbers below 2^24: their float sums are exact
-    const float goal = MASS ? (float)((double)target * unit) : (float)target, slack = MASS ? (float)((double)V * unit) : 0.f;
     int first = OCTAVES - 1, last = OCTAVES - 1;
 #pragma unroll
     for (int j = EACH - 1; j >= 0; --j) {
-      if ((MASS ? (bhi + hi[j]) * 1.0001f + slack : bhi + hi[j]) >= goal) first = min(first, lane * EACH + j);
-      if ((MASS ? (blo + lo[j]) * 0.9999f - slack : blo + lo[j]) >= goal) last = min(last, lane * EACH + j);
+      if ((MASS ? (bhi + hi[j]) * 1.0003f + slack : bhi + hi[j]) >= goal) first = min(first, lane * EACH + j);
+      if ((MASS ? (blo + lo[j]) * 0.9997f - slack : blo + lo[j]) >= goal) last = min(last, lane * EACH + j);
     }
     first = __reduce_min_sync(0xffffffffu, first);
     last = __reduce_min_sync(0xffffffffu, last);
@@ -335,13 +343,14 @@ __device__ __forceinline__ void for_range(const Shared& sh, const float* xs, Seg
 // The shortest prefix of the row (value descending, index ascending) whose count (MASS false) or mass (MASS true) reaches
 // `target`: 128-way search over the order keys from the range above; a pass over the slice and a cluster barrier per round.  Only
 // elements of the range and, in the first round, those above it cost more than a comparison.
-template <int WARPS, bool MASS>
-__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, float m, float scale, int bits, int V, u64 target, bool ranged,
-                        int& round) {
+//
+// ALL: the target is a part, `target_of`, of the mass of all elements, which the first round adds up on its way: every element is
+// weighed once, and the range comes from a 32-bit sum.
+template <int WARPS, bool MASS, bool ALL, class F>
+__device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, u64 target, F target_of, int& round) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Segment seg = split(0, n, WARPS, warp);
-  if (!ranged) first_range<MASS>(sh, m, scale, 1.0 / (double)(1ull << bits), V, target);
   uint32_t k0 = sh.range[0], k1 = sh.range[1];
   const float first_hi = key_value(k1);
   u64 above_c = 0, above_m = 0;
@@ -373,7 +382,7 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
     };
     if (fresh) {
       unsigned int ac = 0;
-      u64 am = 0;
+      u64 am = 0, all = 0;
       int listed = 0;
       for (int i0 = seg.a; i0 < seg.b; i0 += 128) {
         float xk[4];
@@ -383,13 +392,18 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
           xk[k] = i0 + k * 32 + lane < seg.b ? xs[i0 + k * 32 + lane] : NAN;
           some |= xk[k] >= lo;
         }
-        if (!__any_sync(0xffffffffu, some)) continue;
+        if (!ALL && !__any_sync(0xffffffffu, some)) continue;
+        u64 wk[4];
+        if (ALL) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { wk[k] = w(xk[k]); all += wk[k]; }      // NaN, where there is none: 0
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float x = xk[k];
           const unsigned int cand = __ballot_sync(0xffffffffu, x >= lo);
           if (!cand) continue;
-          const u64 wx = w(x);
+          const u64 wx = ALL ? wk[k] : w(x);
           const unsigned int over = __ballot_sync(0xffffffffu, x > hi), any = cand & ~over;
           if (over >> lane & 1) { ++ac; am += wx; }
           if (any) {
@@ -402,7 +416,9 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
       }
       ac = __reduce_add_sync(0xffffffffu, ac);
       am = warp_sum(am);
+      if (ALL) all = warp_sum(all);
       if (lane == 0) {
+        if (ALL) atomicAdd(&sh.all_mass, all);
         sh.above[warp] = am;
         sh.listed[warp] = listed;
         if (ac) { atomicAdd(&sh.above_count[buf], ac); atomicAdd(&sh.above_mass[buf], am); }
@@ -423,8 +439,10 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
       if (lane == 0) sh.tot_above_count = over_ranks<unsigned int>(sh, [&](const Shared& q) { return q.above_count[buf]; });
       if (lane == 1) sh.tot_above_mass = over_ranks<u64>(sh, [&](const Shared& q) { return q.above_mass[buf]; });
       if (lane == 2) { sh.above_count[buf ^ 1] = 0; sh.above_mass[buf ^ 1] = 0; }
+      if (ALL && fresh && lane == 3) sh.whole = over_ranks<u64>(sh, [&](const Shared& q) { return q.all_mass; });
     }
     __syncthreads();
+    if (ALL && fresh) target = target_of(sh.whole);
     if (fresh) { above_c = sh.tot_above_count; above_m = sh.tot_above_mass; fresh = false; }
     if (warp == 0) {
       // lane 0 holds the highest bins: running totals from the top
@@ -475,18 +493,22 @@ __device__ Cut find_cut(Shared& sh, const float* xs, int n, const Weigher& w, fl
 }
 
 // One pass over the slice for everything that needs every element: the untempered sum of exponentials, what the priority needs,
-// the tempered masses (per warp, MASS) and the octave counts (HIST).
-template <int WARPS, bool MASS, bool HIST, int PRI>
+// the tempered masses (per warp, MASS) or their 32-bit sum (ROUGH) and the octave counts (HIST).
+// The 32-bit sum is off by less than 1e-5 of itself: three roundings of the argument shift a term by 3 2^-24 ln2 |y| of itself, 4e-6
+// at |y| = 32 octaves (below which all terms together make up less than V 2^-32), the exponential is off by 2^-22, and at most
+// 51 terms to an accumulator (a slice of 49152 elements, 256 threads) and the tree after it add (51 + 8) 2^-24 = 3.5e-6.
+template <int WARPS, bool MASS, bool HIST, bool ROUGH, int PRI>
 __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment seg, float m, float scale, const Weigher& w) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float z = 0, ent = 0, second = -INFINITY;
+  float z = 0, zt[4] = {0, 0, 0, 0}, ent = 0, second = -INFINITY;
   int at_max = 0;
   u64 mass = 0;
-  auto one = [&](float x) {
+  auto one = [&](float x, int k) {
     const float y = (x - m) * 1.44269504f, e = ex2(y);
     z += e;
     if (PRI == PRI_ENTROPY) ent = fmaf(e, fmaxf(y, -1e4f), ent);
     if (PRI == PRI_MARGIN) { at_max += x == m; second = x < m ? fmaxf(second, x) : second; }
+    if (ROUGH) zt[k] += ex2((x - m) * (scale * (1.f / PER_OCTAVE)));
     if (MASS) mass += w.fine(x);
     if (HIST) {
       const int b = octave_bin(x, m, scale);
@@ -496,12 +518,13 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
   int i = seg.a + lane;
   for (; i + 96 < seg.b; i += 128) {
     const float x0 = xs[i], x1 = xs[i + 32], x2 = xs[i + 64], x3 = xs[i + 96];
-    one(x0); one(x1); one(x2); one(x3);
+    one(x0, 0); one(x1, 1); one(x2, 2); one(x3, 3);
   }
-  for (; i < seg.b; i += 32) one(xs[i]);
+  for (; i < seg.b; i += 32) one(xs[i], 0);
   const int count = max(0, (seg.b - seg.a - lane + 31) >> 5);
   z = warp_sum(z);
   if (lane == 0) sh.z[warp] = z;
+  if (ROUGH) { const float t = warp_sum((zt[0] + zt[1]) + (zt[2] + zt[3])); if (lane == 0) sh.zt[warp] = t; }
   if (PRI == PRI_ENTROPY) { ent = warp_sum(ent); if (lane == 0) sh.ent[warp] = ent; }
   if (PRI == PRI_MARGIN) {
     second = warp_max(second);
@@ -519,11 +542,11 @@ __device__ __forceinline__ void whole_pass(Shared& sh, const float* xs, Segment 
   }
 }
 
-template <int WARPS, bool MASS, bool HIST>
+template <int WARPS, bool MASS, bool HIST, bool ROUGH>
 __device__ __forceinline__ void whole_pass(int pri, Shared& sh, const float* xs, Segment seg, float m, float scale, const Weigher& w) {
-  if (pri == PRI_LOGP) whole_pass<WARPS, MASS, HIST, PRI_LOGP>(sh, xs, seg, m, scale, w);
-  else if (pri == PRI_MARGIN) whole_pass<WARPS, MASS, HIST, PRI_MARGIN>(sh, xs, seg, m, scale, w);
-  else whole_pass<WARPS, MASS, HIST, PRI_ENTROPY>(sh, xs, seg, m, scale, w);
+  if (pri == PRI_LOGP) whole_pass<WARPS, MASS, HIST, ROUGH, PRI_LOGP>(sh, xs, seg, m, scale, w);
+  else if (pri == PRI_MARGIN) whole_pass<WARPS, MASS, HIST, ROUGH, PRI_MARGIN>(sh, xs, seg, m, scale, w);
+  else whole_pass<WARPS, MASS, HIST, ROUGH, PRI_ENTROPY>(sh, xs, seg, m, scale, w);
 }
 
 __device__ __forceinline__ unsigned int cluster_id() {
@@ -549,19 +572,74 @@ __device__ __forceinline__ float2 untempered(const SampleParams& p, Shared& sh, 
   return make_float2(logz, pr);
 }
 
+// A row of global memory as chunks of 1024 elements that start at 16-byte boundaries; the first may be short.
+constexpr int CHUNK = 1024;
+template <class T>
+struct RowView {
+  const T* src;
+  const float* bias;
+  int mis, chunks;
+  __device__ __forceinline__ RowView(const SampleParams& p, unsigned int row) {
+    const unsigned int outer = row / (unsigned int)p.inner;
+    src = reinterpret_cast<const T*>(p.logits) + outer * p.s_outer + (row - outer * (unsigned int)p.inner) * p.s_inner;
+    bias = p.bias ? p.bias + (long long)outer * p.V : nullptr;
+    constexpr int VEC = 16 / (int)sizeof(T);
+    mis = (int)((reinterpret_cast<uintptr_t>(src) / sizeof(T)) % VEC);
+    chunks = (mis + p.V + CHUNK - 1) / CHUNK;
+  }
+  // the lane's elements of chunk c: pieces of 16 bytes, 32 lanes side by side; -inf where the row has none.  Element k of them has index
+  // c CHUNK - mis + ((k / VEC) 32 + lane) VEC + k % VEC.
+  __device__ __forceinline__ void load(int V, int c, int lane, float (&x)[32]) const {
+    constexpr int VEC = 16 / (int)sizeof(T), PIECES = 32 / VEC;
+    const int at0 = c * CHUNK - mis + lane * VEC;
+    uint4 raw[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int at = at0 + j * 32 * VEC;
+      if (at >= 0 && at + VEC <= V) {
+        raw[j] = __ldcs(reinterpret_cast<const uint4*>(src + at));
+      } else {
+        T e[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) e[k] = at + k >= 0 && at + k < V ? src[at + k] : T(-INFINITY);
+        raw[j] = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[j * VEC + k] = to_f32(reinterpret_cast<const T*>(&raw[j])[k]);
+    if (bias) {
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const int i = at0 + j * 32 * VEC + k;
+          if (i >= 0 && i < V) x[j * VEC + k] += __ldg(bias + i);
+        }
+    }
+  }
+};
+
 // The row's end where no more than FEW elements lie in the octaves that hold the kept ones: all CTAs push theirs into the list of CTA
 // 0 and leave; it ranks them against one another (by value, then index), which gives every cut at once, and draws.  The pushes come
 // in any order and nothing depends on it.
 struct Candidate { float x; int i; };
 static_assert(sizeof(Shared::hmass) + sizeof(Shared::count) >= FEW * sizeof(Candidate), "the candidate list takes the histograms' place");
-template <int WARPS>
+//
+// The goal of top-p is a part of the mass of all elements, of which the caller has a 32-bit sum.  What the kept set is follows from
+// it, except where a border lies in the few 1e-5 that it leaves open: then CTA 0 reads the row once more and adds up the masses.
+constexpr double ROUGH_ERROR = 1e-5;
+template <class T, int WARPS>
 __device__ __noinline__ void few_candidates(const SampleParams& p, Shared& sh, const float* xs, Segment seg, int first, unsigned int row, float m,
-                                            float scale, const Weigher& w, int top_k, double top_p, u64 whole, float least) {
+                                            float scale, const Weigher& w_in, int top_k, double top_p, float least) {
+  const Weigher w = w_in;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = (int)cluster.block_rank();
   Shared* home = cluster.map_shared_rank(&sh, 0);
   Candidate* list = reinterpret_cast<Candidate*>(&home->hmass[0][0]);
   const int last = sh.last_bin, n = sh.candidates;
+  const bool all = top_k >= p.V;                                   // the goal is a part of every element's mass
   for (int i0 = seg.a; i0 < seg.b; i0 += 128) {
     float x[4];
     unsigned int in = 0;
@@ -590,15 +668,11 @@ __device__ __noinline__ void few_candidates(const SampleParams& p, Shared& sh, c
   if (me != 0) return;
   // a candidate per thread (or two): its place in the order and the mass before it
   constexpr int THREADS = WARPS * 32, EACH = (FEW + THREADS - 1) / THREADS;
-  u64* mass = reinterpret_cast<u64*>(sh.tab);                      // in the place of the table, which is read for the last time here
-  static_assert(sizeof(Shared::tab) >= FEW * sizeof(u64), "room for the masses");
+  u64* mass = sh.few_mass;
   u64 before[EACH], upto[EACH];
 #pragma unroll
-  for (int e = 0; e < EACH; ++e) before[e] = tid + e * THREADS < n ? w(list[tid + e * THREADS].x) : 0;
-  __syncthreads();
-#pragma unroll
   for (int e = 0; e < EACH; ++e)
-    if (tid + e * THREADS < n) mass[tid + e * THREADS] = before[e];
+    if (tid + e * THREADS < n) mass[tid + e * THREADS] = w(list[tid + e * THREADS].x);
   __syncthreads();
   int rank[EACH];
   u64 topped = 0;                                                  // the mass of the first top_k
@@ -621,9 +695,36 @@ __device__ __noinline__ void few_candidates(const SampleParams& p, Shared& sh, c
   topped = warp_sum(topped);
   if (lane == 0) sh.sub[warp] = topped;
   __syncthreads();
-  if (top_k < p.V) { whole = 0; for (int k = 0; k < WARPS; ++k) whole += sh.sub[k]; }
-  const u64 goal = max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole)));
-  __syncthreads();
+  auto target_of = [&](u64 whole) { return max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole))); };
+  u64 whole = 0, goal = 0;
+  if (!all) {
+    for (int k = 0; k < WARPS; ++k) whole += sh.sub[k];
+    goal = target_of(whole);
+    __syncthreads();
+  } else {
+    const double rough = sh.rough * (double)(1ull << p.scale_bits), off = rough * ROUGH_ERROR + p.V;
+    goal = target_of((u64)fmax(rough - off, 0.0));
+    const u64 goal_hi = target_of((u64)(rough + off));
+    bool open = false;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) open |= tid + e * THREADS < n && before[e] >= goal && before[e] < goal_hi;
+    if (__syncthreads_or(open)) {
+      const RowView<T> view(p, row);
+      for (int c = warp; c < view.chunks; c += WARPS) {
+        float x[32];
+        view.load(p.V, c, lane, x);
+#pragma unroll 8
+        for (int k = 0; k < 32; ++k) whole += w(x[k]);
+      }
+      whole = warp_sum(whole);
+      if (lane == 0) sh.sub[warp] = whole;
+      __syncthreads();
+      whole = 0;
+      for (int k = 0; k < WARPS; ++k) whole += sh.sub[k];
+      goal = target_of(whole);
+      __syncthreads();
+    }
+  }
   u64 kept = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
@@ -693,6 +794,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
     sh.u = p.u[row];
     for (int b = 0; b < 2; ++b) { sh.above_count[b] = 0; sh.above_mass[b] = 0; }
     sh.pushed = 0;
+    sh.all_mass = 0;
   }
   float mx = -INFINITY;
   for (int v = v0 + tid; v < v1; v += THREADS * UNROLL) {
@@ -762,11 +864,11 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
 
   // ---- the pass over every element
   const Segment seg = split(0, n, WARPS, warp);
-  if (greedy) whole_pass<WARPS, false, false>(p.priority, sh, xs, seg, m, scale, w);
-  else if (by_count) whole_pass<WARPS, false, true>(p.priority, sh, xs, seg, m, scale, w);
-  else if (by_mass) whole_pass<WARPS, true, true>(p.priority, sh, xs, seg, m, scale, w);
-  else if (by_ratio) whole_pass<WARPS, false, false>(p.priority, sh, xs, seg, m, scale, w);
-  else whole_pass<WARPS, true, false>(p.priority, sh, xs, seg, m, scale, w);
+  if (greedy) whole_pass<WARPS, false, false, false>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_count) whole_pass<WARPS, false, true, false>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_mass) whole_pass<WARPS, false, true, true>(p.priority, sh, xs, seg, m, scale, w);
+  else if (by_ratio) whole_pass<WARPS, false, false, false>(p.priority, sh, xs, seg, m, scale, w);
+  else whole_pass<WARPS, true, false, false>(p.priority, sh, xs, seg, m, scale, w);
 
   // ---- the kept set and its mass
   Cut cut;
@@ -787,26 +889,28 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
       for (int i = tid; i < OCTAVES; i += WARPS * 32)
         sh.octaves[i] = over_ranks<unsigned int>(sh, [&](const Shared& q) { return q.octaves_here[i]; });
       if (warp == WARPS - 1 && !by_count) {
-        const u64 t = warp_sum(warp_values<WARPS>(sh, lane, (u64)0, [](u64 v, const Shared& q, int k) { return v + q.mass[k]; }));
-        if (lane == 0) sh.whole = t;
+        const double t = warp_sum(warp_values<WARPS>(sh, lane, 0.0, [](double v, const Shared& q, int k) { return v + (double)q.zt[k]; }));
+        if (lane == 0) sh.rough = t;
       }
       __syncthreads();
-      u64 whole = sh.whole;
       const double unit = 1.0 / (double)(1ull << p.scale_bits);
-      const u64 goal = max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole)));      // of a cut by mass alone
-      if (by_count) first_range<false>(sh, m, scale, unit, p.V, (u64)top_k);
-      else first_range<true>(sh, m, scale, unit, p.V, goal);
+      const float slack = (float)((double)(p.V + 1) * unit);       // masses are rounded to units
+      if (by_count) first_range<false>(sh, m, scale, (float)top_k, 0.f);
+      else first_range<true>(sh, m, scale, (float)(fmin(fmax(top_p, 0.0), 1.0) * sh.rough), slack);
       if (sh.candidates <= FEW) {
-        few_candidates<WARPS>(p, sh, xs, seg, first, row, m, scale, w, by_count ? top_k : p.V, by_mass ? top_p : 2.0, whole, least);
+        few_candidates<T, WARPS>(p, sh, xs, seg, first, row, m, scale, w, by_count ? top_k : p.V, by_mass ? top_p : 2.0, least);
         return;
       }
+      auto target_of = [&](u64 whole) { return max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole))); };
       if (by_count) {
-        cut = find_cut<WARPS, false>(sh, xs, n, w, m, scale, p.scale_bits, p.V, (u64)top_k, true, round);
-        whole = cut.mass;
-      }
-      if (by_mass) {
-        const u64 target = by_count ? max((u64)1, min(whole, (u64)ceil(fmax(top_p, 0.0) * (double)whole))) : goal;
-        cut = find_cut<WARPS, true>(sh, xs, n, w, m, scale, p.scale_bits, p.V, target, !by_count, round);
+        cut = find_cut<WARPS, false, false>(sh, xs, n, w, (u64)top_k, target_of, round);
+        if (by_mass) {
+          const u64 target = target_of(cut.mass);
+          first_range<true>(sh, m, scale, (float)((double)target * unit), slack);
+          cut = find_cut<WARPS, true, false>(sh, xs, n, w, target, target_of, round);
+        }
+      } else {
+        cut = find_cut<WARPS, true, true>(sh, xs, n, w, 0, target_of, round);
       }
     }
     if (cut.before + cut.here > cut.ties) {                        // this CTA holds ties that are not kept
@@ -926,9 +1030,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
 // ------------------------------------------------------------------------------------------------ the untruncated draw
 // Without top-k, top-p and min-p nothing has to wait for the row's maximum: a warp reads a chunk of 1024 elements into registers,
 // takes the chunk's own maximum, and leaves the chunk's sums relative to it (the masses as integers, as above).  A second launch, a
-// warp per row, brings them to the row's maximum in 64 bits, finds the chunk that holds the draw and reads it once more.  Chunks
-// start at 16-byte boundaries, so the first may be short.
-constexpr int CHUNK = 1024, CHUNK_BITS = 50;      // 1024 2^50 <= 2^62
+// warp per row, brings them to the row's maximum in 64 bits, finds the chunk that holds the draw and reads it once more.
+constexpr int CHUNK_BITS = 50;                    // 1024 2^50 <= 2^62
 constexpr long long STREAM_LEAST = 2ll << 20;     // elements from which two launches beat one with its cluster barriers
 
 struct __align__(16) Chunk {
@@ -936,53 +1039,6 @@ struct __align__(16) Chunk {
   int at_max;                  // elements at the maximum (margin)
   u64 mass;
   int first, pad;              // index of the first element at the maximum
-};
-
-template <class T>
-struct RowView {
-  const T* src;
-  const float* bias;
-  int mis, chunks;
-  __device__ __forceinline__ RowView(const SampleParams& p, unsigned int row) {
-    const unsigned int outer = row / (unsigned int)p.inner;
-    src = reinterpret_cast<const T*>(p.logits) + outer * p.s_outer + (row - outer * (unsigned int)p.inner) * p.s_inner;
-    bias = p.bias ? p.bias + (long long)outer * p.V : nullptr;
-    constexpr int VEC = 16 / (int)sizeof(T);
-    mis = (int)((reinterpret_cast<uintptr_t>(src) / sizeof(T)) % VEC);
-    chunks = (mis + p.V + CHUNK - 1) / CHUNK;
-  }
-  // the lane's elements of chunk c: pieces of 16 bytes, 32 lanes side by side; -inf where the row has none.  Element k of them has index
-  // c CHUNK - mis + ((k / VEC) 32 + lane) VEC + k % VEC.
-  __device__ __forceinline__ void load(int V, int c, int lane, float (&x)[32]) const {
-    constexpr int VEC = 16 / (int)sizeof(T), PIECES = 32 / VEC;
-    const int at0 = c * CHUNK - mis + lane * VEC;
-    uint4 raw[PIECES];
-#pragma unroll
-    for (int j = 0; j < PIECES; ++j) {
-      const int at = at0 + j * 32 * VEC;
-      if (at >= 0 && at + VEC <= V) {
-        raw[j] = __ldcs(reinterpret_cast<const uint4*>(src + at));
-      } else {
-        T e[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) e[k] = at + k >= 0 && at + k < V ? src[at + k] : T(-INFINITY);
-        raw[j] = *reinterpret_cast<const uint4*>(e);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < PIECES; ++j)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[j * VEC + k] = to_f32(reinterpret_cast<const T*>(&raw[j])[k]);
-    if (bias) {
-#pragma unroll
-      for (int j = 0; j < PIECES; ++j)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const int i = at0 + j * 32 * VEC + k;
-          if (i >= 0 && i < V) x[j * VEC + k] += __ldg(bias + i);
-        }
-    }
-  }
 };
 
 __device__ __forceinline__ double row_temperature(const SampleParams& p, unsigned int row) {

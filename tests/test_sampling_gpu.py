@@ -7,6 +7,8 @@ Bound of the log-probability: ``x - m`` rounds once (2^-24 of at most 80: 4.8e-6
 probability-weighted error of the fast exponential, ``(2 + 1.2 E|d|) 2^-23`` with ``E|d| <= log V < 13`` (2.1e-6), the logarithm
 and the last subtraction round once each (2^-24 of at most 80 and 13: 5.6e-6): 1.3e-5 in all.  The margin and the entropy are
 weighted means with the same weights: 2.1e-6 of at most 1, and of at most 13 (2.8e-5 with the logarithm's share)."""
+import math
+
 import pytest
 import torch
 
@@ -115,6 +117,24 @@ def test_values_whose_neighbours_are_octaves_away(V, top):
     for kw in PARAMS:
         check(x, u, **kw)
     check(x.repeat(5, 9, 1), u.repeat(5, 9))                               # enough rows for the two-launch form at the largest V
+
+
+@pytest.mark.parametrize("V", [3000, 20000, 128256])
+@pytest.mark.parametrize("near", [100, 700])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_p_next_to_a_border(V, near, dtype):
+    """top_p so close to the part of the mass that a prefix has that 32-bit sums would not tell on which side it is: a billionth of it
+    is more than the 64-bit masses are off."""
+    x, u = logits((2, 8), V)
+    x = x.clamp(-1, 1) * 0.5
+    x[..., near:] -= 3 + math.log(V / near)                                # few candidates, or more than fit a list
+    x = x[..., torch.randperm(V, device="cuda")].to(dtype)
+    x[1] = x[0] = x[0, 0].clone()
+    w = torch.exp((x[0, 0].double() - x[0, 0].max().double()) / 0.7).sort(descending=True).values
+    part = w.cumsum(0) / w.sum()
+    for j in (0, 3, near // 3, near - 10):
+        for off in (-1e-5, -1e-9, 1e-9, 1e-5, 1e-3):
+            check(x, u, temperature=0.7, top_p=part[j].item() * (1 + off), bias=torch.zeros(2, V, device="cuda") if j == 3 else None)
 
 
 def test_parameters_per_row():
