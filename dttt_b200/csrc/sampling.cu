@@ -640,18 +640,23 @@ __device__ __noinline__ void few_candidates(const SampleParams& p, Shared& sh, c
   Candidate* list = reinterpret_cast<Candidate*>(&home->hmass[0][0]);
   const int last = sh.last_bin, n = sh.candidates;
   const bool all = top_k >= p.V;                                   // the goal is a part of every element's mass
-  for (int i0 = seg.a; i0 < seg.b; i0 += 128) {
-    float x[4];
-    unsigned int in = 0;
+  const float lo = key_value(sh.range[0]);                         // not above any element of the octaves
+  for (int i0 = seg.a; i0 < seg.b; i0 += 256) {
+    float x[8];
+    float most = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
       const int i = i0 + k * 32 + lane;
       x[k] = i < seg.b ? xs[i] : -INFINITY;
-      if (octave_bin(x[k], m, scale) <= last) in |= 1u << k;
+      most = fmaxf(most, x[k]);
     }
-    if (!__any_sync(0xffffffffu, in)) continue;
+    if (!__any_sync(0xffffffffu, most >= lo)) continue;
+    unsigned int in = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k)
+      if (octave_bin(x[k], m, scale) <= last) in |= 1u << k;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
       const unsigned int any = __ballot_sync(0xffffffffu, in >> k & 1);
       if (!any) continue;
       int at = 0;
