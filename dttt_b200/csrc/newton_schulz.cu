@@ -10,7 +10,7 @@
 //
 // Operands are f16, not bf16: the same tensor-core rate with three more bits.  Five iterations multiply small singular values by
 // up to 3.4 each, and what the roundings of x and P leave in those directions grows with them: 1.2e-2 of the result with bf16
-// operands, 1.5e-3 with f16 (Gaussian and gradient-like matrices; the bf16 result itself rounds by 1.7e-3).  Everything that
+// operands, about 1.1e-3 with f16 (Gaussian and gradient-like matrices; the bf16 result itself rounds by 1.7e-3).  Everything that
 // is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12 for
 // those, 2^5 for the cotangent, which may grow 3.4445-fold per iteration.  Sums are f32 (tensor memory), the norms f64.
 //
@@ -45,6 +45,7 @@ struct Tile {
   static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
 };
 
+constexpr int MAX_STEPS = 32;
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float X_SCALE = 4096.f;           // of x, G and P
 constexpr float R_SCALE = 32.f;             // of the cotangent
@@ -56,9 +57,9 @@ struct Params {
   int a_mn_major, b_mn_major;
   float alpha, beta;
   const __half* D;             // or null; same shape as C
-  const __half* D2;            // TWO: a second one, and `diag` on the diagonal
+  const __half* D2;            // TWO: a second one
   long long ldd, d_batch;      // of both
-  float beta2, diag;
+  float beta2, diag;           // `diag` is added on the diagonal
   void* C;
   int out;
   long long ldc, c_batch;
@@ -344,7 +345,6 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
           load_rows(p.D2 + (d0 - p.D) + c, p.ldd, rows, (int)p.ldd - n0 - c, lane, v);
           stage_in(stg, lane, v);
           __syncwarp();
-          const int on = row0 + lane - n0 - c;                 // the column on the diagonal
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const uint4 dv = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16));
@@ -354,10 +354,15 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
               const float2 df = __half22float2(dh[e >> 1]);
               float& x = reinterpret_cast<float&>(r[8 * q + e]);
               x = fmaf(p.beta2, e & 1 ? df.y : df.x, x);
-              if (8 * q + e == on) x += p.diag;
             }
           }
           __syncwarp();
+        }
+        const int on = row0 + lane - n0 - c;                   // the column on the diagonal
+        if (p.diag != 0.f && __any_sync(0xffffffffu, on >= 0 && on < 64)) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e == on) r[e] = __float_as_uint(__uint_as_float(r[e]) + p.diag);
         }
         if (p.out == OUT_F32) {
           store_f32(reinterpret_cast<float*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c, p.ldc, rows, p.N - n0 - c, lane, r);
@@ -495,6 +500,7 @@ struct SmallParams {
   double* norms;               // written by the forward, read by the derivative
   void* y;
   int* status;
+  float alpha[MAX_STEPS];      // x' = alpha x + M x with M = P + (a - alpha) I
 };
 
 __device__ __forceinline__ int small_offset(int row, int col) {      // bytes; of the 16-byte piece that starts at col
@@ -640,6 +646,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   };
   if (p.apply) fetch(0);
   for (int k = 0; k < p.steps && ok; ++k) {
+    const float alpha = p.alpha[p.apply ? p.steps - 1 - k : k];
     if (!p.apply) {
       if (tid == 0) {
         const uint32_t a = smem_u32(sx), idesc = make_idesc_f16(128, 128, 0, 0);
@@ -656,7 +663,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         tmem_ld_32x32(lanes + part * 32, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) gr[j] = __uint_as_float(r[j]) * (1.f / X_SCALE);
+        for (int j = 0; j < 32; ++j) gr[j] = __half2float(__float2half_rn(__uint_as_float(r[j]) * (1.f / X_SCALE)));      // one G for both terms
         store_small(sg, row, part * 32, gr);
       }
       hand_over();
@@ -674,7 +681,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         tmem_ld_32x32(lanes + part * 32, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) gr[j] = fmaf(NS_B, gr[j], NS_C / X_SCALE * __uint_as_float(r[j]));
+        for (int j = 0; j < 32; ++j)
+          gr[j] = fmaf(NS_B, gr[j], NS_C / X_SCALE * __uint_as_float(r[j])) + (row == part * 32 + j ? (NS_A - alpha) * X_SCALE : 0.f);
         store_small(sp, row, part * 32, gr);
       }
     } else {
@@ -715,7 +723,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         const uint4 o = *reinterpret_cast<const uint4*>(sx + small_offset(row, col + 8 * q));
         const __half* h = reinterpret_cast<const __half*>(&o);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * q + e] = fin * fmaf(NS_A, __half2float(h[e]), __uint_as_float(r[8 * q + e]) * (1.f / X_SCALE));
+        for (int e = 0; e < 8; ++e) v[8 * q + e] = fin * fmaf(alpha, __half2float(h[e]), __uint_as_float(r[8 * q + e]) * (1.f / X_SCALE));
       }
       if (!end) {
         store_small(sx, row, col, v);
@@ -846,7 +854,7 @@ struct Out {
   const double *num, *den;
 };
 
-// C [M, N] = alpha op(A) op(B) + beta D (+ beta2 D2 + diag I, with the layout of D) over the batch (symmetric: C and D are, and only f16)
+// C [M, N] = alpha op(A) op(B) + beta D (+ beta2 D2, with the layout of D) + diag I over the batch (symmetric: C and D are, and only f16)
 static int product(Maps& maps, int batch, int M, int N, int K, const Mat& A, bool a_mn, const Mat& B, bool b_mn, float alpha, float beta, const Mat* D,
                    const Out& o, bool symmetric, int* status, int n_sm, cudaStream_t stream, const Mat* D2 = nullptr, float beta2 = 0.f,
                    float diag = 0.f) {
@@ -854,7 +862,8 @@ static int product(Maps& maps, int batch, int M, int N, int K, const Mat& A, boo
   memset(&p, 0, sizeof(p));
   p.M = M; p.N = N; p.K = K; p.batch = batch; p.a_mn_major = a_mn; p.b_mn_major = b_mn; p.alpha = alpha; p.beta = beta;
   if (D) { p.D = (const __half*)D->ptr; p.ldd = D->ld; p.d_batch = D->ld * D->rows; }
-  if (D2) { p.D2 = (const __half*)D2->ptr; p.beta2 = beta2; p.diag = diag; }
+  if (D2) { p.D2 = (const __half*)D2->ptr; p.beta2 = beta2; }
+  p.diag = diag;
   p.C = o.C; p.out = o.kind; p.ldc = o.ld; p.c_batch = o.ld * M; p.num = o.num; p.den = o.den; p.status = status;
   p.symmetric = symmetric;
   p.tiles_m = (M + 2 * BM - 1) / (2 * BM);
@@ -934,8 +943,9 @@ namespace ns {
 //   x'' = (a I + P')(a I + P) x = (a^2 - s) x + N x,   N = P' P + a (P + P') + s I,
 // need G' of the second from G alone: with H = (a I + P) G = a G + P G, G' = a H + H P.  That replaces one product with x on each side
 // of the group (d^2 L and 2 d^2 L of the longer side L) by three d x d ones, which pays from about L = 2 d on where the products are
-// large enough to be bound by the tensor cores: 4 x 2048 x 8192, five steps, 2.36 -> 1.77 ms.  `s` shifts N by its value at the singular
-// value of a matrix with equal ones, so that what rounds is the spread and not the bulk of it.  P, P' and G commute only up to
+// large enough to be bound by the tensor cores: 4 x 2048 x 8192, five steps, 2.36 -> 1.77 ms.  `s` shifts N (of a single one, P) by its
+// value at the singular value of a matrix with equal ones, so that what rounds is the spread and not the bulk of it, 2.7 I next to
+// a result of 0.7: the error of y before its rounding to bf16 falls from 1.5e-3 to 1.1e-3 (101 x 346).  P, P' and G commute only up to
 // their roundings: G' is formed as H P, which is symmetric even so (P H, or N mirrored across its diagonal, is not, and the
 // difference is amplified: 5.2e-3 and 2.5e-3 off instead of 2.2e-3).  The first two and, from five on, the last two are grouped; a
 // pair in the middle, or three in one, loses to the cancellation in N what single steps keep.
@@ -958,7 +968,7 @@ static int make_plan(int rows, int cols, int steps, Group* g) {
       l = next * q(next) * q(next);
       k += 2;
     } else {
-      g[n] = {1, NS_A, 0.f};
+      g[n] = {1, (float)q(l), (float)(NS_A - q(l))};
       l = next;
       k += 1;
     }
@@ -985,8 +995,6 @@ struct Scratch {
   }
 };
 
-constexpr int MAX_STEPS = 32;
-
 }  // namespace ns
 }  // namespace dttt
 
@@ -1009,9 +1017,12 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
   int n_sm;
   if (int r = prepare_device(&n_sm)) return r;
+  Group plan[MAX_STEPS];
+  const int groups = make_plan(rows, cols, steps, plan);
   if (is_small(rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    const SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, X_SCALE, (__half*)kept, (long long)batch * small * ld, norms, y, status};
+    SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, X_SCALE, (__half*)kept, (long long)batch * small * ld, norms, y, status};
+    for (int k = 0; k < steps; ++k) p.alpha[k] = plan[k].alpha;
     return launch_small(p, f32, batch, stream);
   }
   const Scratch s(scratch, batch, rows, cols);
@@ -1019,8 +1030,6 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   if (int r = cast(g, f32, batch, rows, cols, s.partial, X_SCALE, s.x[0], s.ld, norms, n_sm, stream)) return r;
   const bool wide = rows <= cols;
   Maps maps;
-  Group plan[MAX_STEPS];
-  const int groups = make_plan(rows, cols, steps, plan);
   const Mat G = {s.gram, d, d, ldd}, H = {s.h, d, d, ldd}, P1 = {s.p, d, d, ldd};
   auto square = [&](const Mat& A, const Mat& B, float alpha, float beta, const Mat& D, const Mat& C, const Mat* D2 = nullptr, float beta2 = 0.f,
                     float diag = 0.f) {
@@ -1033,7 +1042,7 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
     const Out og = {s.gram, OUT_F16, ldd, nullptr, nullptr};
     if (int r = product(maps, batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, true, status, n_sm, stream)) return r;
     if (plan[k].steps == 1) {
-      if (int r = square(G, G, NS_C, NS_B, G, M)) return r;                                  // P = b G + c G G
+      if (int r = square(G, G, NS_C, NS_B, G, M, nullptr, 0.f, plan[k].shift * X_SCALE)) return r;      // P + s I = b G + c G G + s I
     } else {
       if (int r = square(G, G, NS_C, NS_B, G, P1)) return r;
       if (int r = square(P1, G, 1.f, NS_A, G, H)) return r;                                  // H = a G + P G
@@ -1056,17 +1065,18 @@ extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, in
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
   int n_sm;
   if (int r = prepare_device(&n_sm)) return r;
+  Group plan[MAX_STEPS];
+  const int groups = make_plan(rows, cols, steps, plan);
   if (is_small(rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    const SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, R_SCALE, (__half*)const_cast<void*>(kept),
+    SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, R_SCALE, (__half*)const_cast<void*>(kept),
                            (long long)batch * small * ld, const_cast<double*>(norms), out, status};
+    for (int k = 0; k < steps; ++k) p.alpha[k] = plan[k].alpha;
     return launch_small(p, f32, batch, stream);
   }
   const Scratch s(scratch, batch, rows, cols);
   if (int r = cast(r_in, f32, batch, rows, cols, s.partial, R_SCALE, s.x[0], s.ld, s.norm, n_sm, stream)) return r;
   Maps maps;
-  Group plan[MAX_STEPS];
-  const int groups = make_plan(rows, cols, steps, plan);
   for (int i = 0; i < groups; ++i) {
     const int k = groups - 1 - i;
     const Mat X = {s.x[i & 1], rows, cols, s.ld};
