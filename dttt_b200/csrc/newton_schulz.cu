@@ -14,8 +14,14 @@
 // is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12 for
 // those, 2^5 for the cotangent, which may grow 3.4445-fold per iteration.  Sums are f32 (tensor memory), the norms f64.
 //
-// Every product is C = alpha A B + beta D on CTA pairs: tiles of 256 rows and 256 or 128 columns, tcgen05.mma.cta_group::2, plain
-// per-CTA TMA loads.
+// Every product is C = alpha A B + beta D (+ s I) on CTA pairs: tiles of 256 rows and 256 or 128 columns, tcgen05.mma.cta_group::2,
+// plain per-CTA TMA loads, symmetric results formed for the tiles on and below the diagonal and stored twice.  What bounds it:
+//   * large matrices: the tensor cores.  4 x 2048 x 8192 f32, five steps: 1.83 ms for 2.23 TFLOP (symmetric halves counted once) =
+//     1220 TFLOP/s, tensor pipe 91 % busy in a product with x; 8192 x 2048 with its derivative 0.84 ms = 1075 TFLOP/s.
+//   * middle ones: the chain of products, each of which is one round of tiles whose first loads, store and mirrored store are
+//     not hidden: 3 x 509 x 1283, five steps 167 us and its derivative 53 us, 8 to 11 us a product; programmatic launches start a
+//     product's prologue under the one before (263 -> 230 us).  All of them in one cooperative launch gained nothing.
+//   * d <= 128 and L <= 512: one CTA and one launch (below), 21 us for 2 x 128 x 256 and two steps.
 #include "host_check.h"
 #include "ptx_sm100.cuh"
 
@@ -57,9 +63,9 @@ struct Params {
   int a_mn_major, b_mn_major;
   float alpha, beta;
   const __half* D;             // or null; same shape as C
-  const __half* D2;            // TWO: a second one
+  const __half* D2;            // MODE 1: a second one
   long long ldd, d_batch;      // of both
-  float beta2, diag;           // `diag` is added on the diagonal
+  float beta2, diag;           // MODE 1 and 2: `diag` is added on the diagonal
   void* C;
   int out;
   long long ldc, c_batch;
@@ -184,7 +190,7 @@ __device__ __forceinline__ void store_transposed(__half* out, long long ld, int 
   }
 }
 
-template <int BN, bool TWO>
+template <int BN, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const Params p) {
   constexpr int STAGES = Tile<BN>::STAGES, STAGE_BYTES = Tile<BN>::STAGE_BYTES;
@@ -340,7 +346,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
           }
         }
         __syncwarp();
-        if (TWO) {
+        if (MODE == 1) {
           uint4 v[8];
           load_rows(p.D2 + (d0 - p.D) + c, p.ldd, rows, (int)p.ldd - n0 - c, lane, v);
           stage_in(stg, lane, v);
@@ -358,11 +364,15 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
           }
           __syncwarp();
         }
-        const int on = row0 + lane - n0 - c;                   // the column on the diagonal
-        if (p.diag != 0.f && __any_sync(0xffffffffu, on >= 0 && on < 64)) {
+        if (MODE != 0) {                                       // rows start at multiples of 32, columns of 64
+          const int on = row0 - n0 - c;
+          if (on == 0) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e == on) r[e] = __float_as_uint(__uint_as_float(r[e]) + p.diag);
+            for (int e = 0; e < 32; ++e) if (e == lane) r[e] = __float_as_uint(__uint_as_float(r[e]) + p.diag);
+          } else if (on == 32) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) if (e == lane) r[32 + e] = __float_as_uint(__uint_as_float(r[32 + e]) + p.diag);
+          }
         }
         if (p.out == OUT_F32) {
           store_f32(reinterpret_cast<float*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c, p.ldc, rows, p.N - n0 - c, lane, r);
@@ -488,6 +498,11 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
 // iterations in one launch; what such sizes cost otherwise is launches.  x lies as blocks of 128 rows x 64 columns with 128-byte
 // swizzle, which is the K-major operand of G = x x^T and, read with its columns as N, the MN-major one of P x.  Rows and columns
 // beyond the matrix are zero and stay so.  Also the derivative (`apply`): the kept P of every iteration is read back.
+// Five steps with keep, here / as products of their own, in us (batch 1; batch 512):
+//   16 x 64  21 / 73 (68 / 413)   64 x 256  29 / 77 (115 / 563)   128 x 512  54 / 89 (243 / 889)   512 x 128  63 / 89 (321 / 704)
+// and of the derivative 128 x 256 25 / 35 (107 / 248), 128 x 512 41 / 35 (194 / 481), 512 x 128 49 / 35 (272 / 294): only alone do the
+// longest ones lose.  Longer matrices on a cluster of CTAs that add up parts of G lost to the products at every size but a batch
+// of 8 to 148 short rows (128 x 1024: 186 / 100, 148 of them 382 / 450).  Sixteen warps: with eight, 512 x 128 took 77.
 constexpr int SMALL_D = 128, SMALL_L = 512, SMALL_THREADS = 512;
 constexpr int BLOCK_BYTES = SMALL_D * 128;                     // 128 rows x 64 f16
 
@@ -834,10 +849,12 @@ static int prepare_device(int* n_sm) {
   if (bound_dev != dev) { cudaSetDevice(dev); cudaFree(0); bound_dev = dev; }      // the encoder needs a current context
   std::lock_guard<std::mutex> lock(mu);
   if (!(attr_mask >> dev & 1ull)) {
-    if (cudaFuncSetAttribute(ns_product_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<256, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
+    if (cudaFuncSetAttribute(ns_product_kernel<256, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<128, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<256, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<256, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_product_kernel<128, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
         cudaFuncSetAttribute(ns_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 4) * BLOCK_BYTES + 2048) != cudaSuccess ||
         cudaFuncSetAttribute(ns_small_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 4) * BLOCK_BYTES + 2048) != cudaSuccess) return 302;
     cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
@@ -895,8 +912,10 @@ static int product(Maps& maps, int batch, int M, int N, int K, const Mat& A, boo
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, D2 ? (narrow ? ns_product_kernel<128, true> : ns_product_kernel<256, true>)
-                                                    : (narrow ? ns_product_kernel<128, false> : ns_product_kernel<256, false>), copyA, *mapB, p);
+  const int mode = D2 ? 1 : diag != 0.f ? 2 : 0;               // a kernel of its own each: with all of it the epilogue spills
+  auto* const kernel = narrow ? (mode == 0 ? ns_product_kernel<128, 0> : mode == 1 ? ns_product_kernel<128, 1> : ns_product_kernel<128, 2>)
+                              : (mode == 0 ? ns_product_kernel<256, 0> : mode == 1 ? ns_product_kernel<256, 1> : ns_product_kernel<256, 2>);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, copyA, *mapB, p);
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
@@ -943,10 +962,11 @@ namespace ns {
 //   x'' = (a I + P')(a I + P) x = (a^2 - s) x + N x,   N = P' P + a (P + P') + s I,
 // need G' of the second from G alone: with H = (a I + P) G = a G + P G, G' = a H + H P.  That replaces one product with x on each side
 // of the group (d^2 L and 2 d^2 L of the longer side L) by three d x d ones, which pays from about L = 2 d on where the products are
-// large enough to be bound by the tensor cores: 4 x 2048 x 8192, five steps, 2.36 -> 1.77 ms.  `s` shifts N (of a single one, P) by its
-// value at the singular value of a matrix with equal ones, so that what rounds is the spread and not the bulk of it, 2.7 I next to
-// a result of 0.7: the error of y before its rounding to bf16 falls from 1.5e-3 to 1.1e-3 (101 x 346).  P, P' and G commute only up to
-// their roundings: G' is formed as H P, which is symmetric even so (P H, or N mirrored across its diagonal, is not, and the
+// large enough to be bound by the tensor cores: 4 x 2048 x 8192, five steps, 2.36 -> 1.77 ms.  `s` shifts N by its value at the singular
+// value of a matrix with equal ones, so that what rounds is the spread and not the bulk of it.  Single ones are shifted likewise:
+// unshifted, 2.7 I next to a result of 0.7 rounds (101 x 346, five steps: 1.5e-3 off before the rounding to bf16 instead of 1.1e-3).
+// With s = b^2 / 4c, P + s I would be the one product c (G + b / 2c I)^2: 170 instead of 173 us for 1000 x 1024, but 2.34e-3 off
+// instead of 2.06e-3.  P, P' and G commute only up to their roundings: G' is formed as H P, which is symmetric even so (P H, or N mirrored across its diagonal, is not, and the
 // difference is amplified: 5.2e-3 and 2.5e-3 off instead of 2.2e-3).  The first two and, from five on, the last two are grouped; a
 // pair in the middle, or three in one, loses to the cancellation in N what single steps keep.
 struct Group {
@@ -1042,7 +1062,7 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
     const Out og = {s.gram, OUT_F16, ldd, nullptr, nullptr};
     if (int r = product(maps, batch, d, d, wide ? cols : rows, X, !wide, X, !wide, 1.f / X_SCALE, 0.f, nullptr, og, true, status, n_sm, stream)) return r;
     if (plan[k].steps == 1) {
-      if (int r = square(G, G, NS_C, NS_B, G, M, nullptr, 0.f, plan[k].shift * X_SCALE)) return r;      // P + s I = b G + c G G + s I
+      if (int r = square(G, G, NS_C, NS_B, G, M, nullptr, 0.f, plan[k].shift * X_SCALE)) return r;      // M = b G + c G G + s I
     } else {
       if (int r = square(G, G, NS_C, NS_B, G, P1)) return r;
       if (int r = square(P1, G, 1.f, NS_A, G, H)) return r;                                  // H = a G + P G
