@@ -19,7 +19,18 @@
 //
 // A row is spread over a cluster of 1 .. 8 CTAs, each of which keeps its slice (f32, after the bias) in shared memory, so the
 // logits are read from global memory once whatever the number of passes; the CTAs exchange maxima, histograms and masses
-// through distributed shared memory.
+// through distributed shared memory.  A pass counts every element into octaves of its mass, 1/8 octave wide, which bounds where the
+// truncation can end; if no more than 256 elements lie in the octaves that are kept, one CTA finishes the row from a list of them
+// (top-p, 512 x 128256: 383 us without that, 212 with), else a 128-way search goes on among the elements of the last
+// octaves.  Without truncation nothing has to wait for the maximum, and many rows take two streaming launches instead.
+//
+// What bounds it, at V = 128256 (f32, 525 MB for 1024 rows, 81 us at the copy rate):
+//   one row, top-p: 16 us.  Latency: load 1.5 us, three exchanges over the cluster, ranking the list 3.4 us.
+//   1024 rows, top-p 0.9: 440 us = 1.2 TB/s.  A CTA takes 17 us, of which loading 4.5, its pass 4, looking for candidates 1.4 and the
+//     exchanges 6.5; three to an SM hide each other's waits only in part (issue slots 42 % busy).
+//   1024 rows, untruncated: 203 + 12 us = 2.5 TB/s, bound by issue: 39 instructions an element, of which the 64-bit exponential
+//     (FP64 pipe 36 % busy, issue slots 68 %) is most.
+//   252 rows bf16 with bias, top-k 50 and min-p: 114 us for 67 MB: 4.5 rounds of CTAs as above.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,7 +49,7 @@ constexpr int MAX_WARPS = 16;
 constexpr int OCTAVES = 256;                 // bins of the octave counts
 constexpr int BINS = 128;                    // of a round of the search
 constexpr int TAB = 64, COPIES = 8;
-constexpr int FEW = 256;                    // candidates up to which one CTA finishes a row
+constexpr int FEW = 256;                     // candidates up to which one CTA finishes a row
 constexpr int LIST = 256;                    // entries of all warps
 constexpr int SLICE_MAX = 49152;            // elements of a slice at most (192 KB)
 constexpr int SLICE_GOOD = 16384;           // a slice up to which three CTAs fit an SM
@@ -1037,7 +1048,9 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
 // takes the chunk's own maximum, and leaves the chunk's sums relative to it (the masses as integers, as above).  A second launch, a
 // warp per row, brings them to the row's maximum in 64 bits, finds the chunk that holds the draw and reads it once more.
 constexpr int CHUNK_BITS = 50;                    // 1024 2^50 <= 2^62
-constexpr long long STREAM_LEAST = 2ll << 20;     // elements from which two launches beat one with its cluster barriers
+// Elements from which a draw takes two launches.  One / two, us: 8 x 128256 12.4 / 18.5, 16 x 128256 18.5 / 18.6, 32 x 128256 20.6 / 22.7,
+// 64 x 128256 33.0 / 28.8, 1024 x 128256 348 / 185; 1024 x 2048 16.5 / 20.6, 4096 x 1000 41 / 43.
+constexpr long long STREAM_LEAST = 2ll << 20;
 
 struct __align__(16) Chunk {
   float m, z, e;               // maximum (NaN or +inf if there is one), sum of exp(x - m), the priority's own value
@@ -1289,19 +1302,24 @@ int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
-// Small slices take four warps, so that fewer of them pay what a row costs apart from its elements; where the rows leave SMs free
-// sixteen share the slice, else eight (three CTAs to an SM).
+// Warps to a CTA.  Sixteen while every CTA finds an SM of its own (clusters of eight: fourteen of them are resident at once),
+// else eight, three CTAs to an SM; small slices, of which there are more than that, take four, so that fewer warps pay what a
+// row costs apart from its elements.  Top-p, us with 16 / 8 / 4 warps:
+//   V = 128256: 14 rows 14.5 / 18.6, 16 rows 24.7 / 18.6, 64 rows 57 / 38      V = 4000: 148 rows 12.4 / 12.4 / 16.5, 296 rows
+//   22.6 / 14.5 / 16.7, 600 rows 47 / 26.8 / 23.0                               V = 1000: 600 rows 48 / 27 / 18.6
 template <class T>
 int launch_sample(const SampleParams& p, long long rows, int ranks, cudaStream_t s) {
-  if (p.slice <= SLICE_SMALL) return launch_sample<T, 4>(p, rows, ranks, s);
-  if (rows * ranks <= 148) return launch_sample<T, 16>(p, rows, ranks, s);
+  const long long ctas = rows * ranks;
+  if (ctas <= (ranks == 8 ? 112 : 148)) return launch_sample<T, 16>(p, rows, ranks, s);
+  if (p.slice <= SLICE_SMALL && ctas > 444) return launch_sample<T, 4>(p, rows, ranks, s);
   return launch_sample<T, 8>(p, rows, ranks, s);
 }
 
 // ------------------------------------------------------------------------------------------------------ unmask
 // One block per row.  Rows of up to 1024 slots: a thread per slot, everything it needs loaded at once, and the key of the quota-th slot
 // in rank order built bit by bit from counts over the block (32 barriers, about 1.5 us; latency is all there is to it).  Longer
-// rows: a radix search over the order keys in shared memory.
+// rows: a radix search over the order keys in shared memory.  Thread per slot / radix: 1 x 16 4.3 / 6.3 us, 1 x 1024 and 64 x 1024
+// 6.3 / 10.4, 256 x 1024 10.4 / 10.3.
 constexpr int UM_ROW = 1024;
 
 __global__ void __launch_bounds__(UM_ROW) unmask_row_kernel(const long long* __restrict__ ids, const uint8_t* __restrict__ known,
