@@ -860,6 +860,13 @@ _lib.register("dttt_newton_schulz_apply", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp
 _SYMBOL.update(newton_schulz="dttt_newton_schulz")
 
 
+def _status_word(dev):
+    """The device's status word; one made during a capture would hold nothing until the graph is replayed."""
+    if dev.index not in _lib._status and torch.cuda.is_current_stream_capturing():
+        raise _lib.KernelError("newton_schulz: the first call on a device cannot be captured into a graph; call it once before the capture")
+    return _lib.status_tensor(dev).data_ptr()
+
+
 def newton_schulz(g, steps, keep):
     """``g [B, rows, cols]`` (f32 or bf16, contiguous) -> ``(y bf16, norms [B] f64, maps)``; ``maps`` (f16 ``[groups, B, d, ceil8(d)]``)
     holds the matrix of every group of iterations with ``keep``, else it is scratch."""
@@ -876,7 +883,7 @@ def newton_schulz(g, steps, keep):
         polys = torch.empty((l.dttt_newton_schulz_groups(rows, cols, steps) if keep else 1, B, d, -(-d // 8) * 8), dtype=torch.float16, device=dev)
     _launch("newton_schulz", l.dttt_newton_schulz, dev, g.data_ptr(), int(g.dtype == torch.float32), B, rows, cols, steps,
             scratch.data_ptr() if size else None, None if polys is None else polys.data_ptr(), int(keep), norms.data_ptr(), y.data_ptr(),
-            _lib.status_tensor(dev).data_ptr())
+            _status_word(dev))
     if size:
         LAUNCHES += 1 + 3 * steps
     return y, norms, polys
@@ -893,7 +900,7 @@ def newton_schulz_apply(r, norms, polys, steps, out_dtype):
     scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), int(r.dtype == torch.float32), B, rows, cols, steps,
             scratch.data_ptr() if size else None, polys.data_ptr(), norms.data_ptr(), out.data_ptr(), int(out_dtype == torch.float32),
-            _lib.status_tensor(dev).data_ptr())
+            _status_word(dev))
     if size:
         LAUNCHES += 1 + polys.shape[0]
     return out

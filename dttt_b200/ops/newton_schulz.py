@@ -70,7 +70,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5) -> torch.Tensor:
     The norms are taken in 64 bits, so any finite scale of ``g`` will do; a zero matrix gives zeros (and a zero derivative), one
     that holds NaN or infinities gives NaN.  On a CUDA device operands round to f16: singular values below about 2^-11 of the
     largest come out with the noise of those roundings, and the derivative has the accuracy of bf16 whatever the type of ``g``.
-    At most 65535 matrices a call."""
+    At most 65535 matrices a call; the first call on a device cannot be captured into a graph."""
     if g.dim() < 2 or g.shape[-1] == 0 or g.shape[-2] == 0:
         raise ValueError(f"newton_schulz: g {tuple(g.shape)}, [..., rows, cols] with non-empty matrices is wanted")
     if g.dtype not in (torch.float32, torch.bfloat16):

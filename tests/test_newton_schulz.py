@@ -88,3 +88,11 @@ def test_the_write_rule_keeps_the_gradient_norm_and_trains():
     loss, grads, _ = loss_and_grads(eng, torch.randint(0, 120, (2, 32), generator=gen), loss_config(eng.tc))
     assert loss == loss and all(torch.isfinite(v).all() for v in grads.values())
     assert grads["fast_weight.gate.weight"].abs().sum() > 0
+
+
+def test_the_first_call_on_a_device_is_not_captured(monkeypatch):
+    from dttt_b200.ops import _lib, kernels
+    monkeypatch.setattr(_lib, "_status", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(_lib.KernelError, match="before the capture"):
+        kernels._status_word(torch.device("cuda", 0))

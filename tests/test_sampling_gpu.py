@@ -209,6 +209,30 @@ def test_repeats_streams_and_graphs():
     assert all(a.equal(b) for a, b in zip(held, sample_tokens(x2, u2, **kw)))
 
 
+@pytest.mark.parametrize("kw", [dict(temperature=0.8, top_p=0.9), dict(temperature=0.9), dict(top_k=700, min_p=1e-4), dict(temperature=1.3, top_p=0.99)])
+def test_two_graphs_at_once(kw):
+    """Each graph has its own workspaces; replayed side by side on two streams, on inputs that change between replays."""
+    from dttt_b200.ops.sampling import sample_tokens
+    sides, held = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for n in range(2):
+        x, u = logits((1, 70), 40001, seed=n)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = sample_tokens(x, u, **kw)
+        held.append((graph, x, u, out))
+    for turn in range(3):
+        for n, (graph, x, u, out) in enumerate(held):
+            x2, u2 = logits((1, 70), 40001, seed=10 * turn + n, kind=("zipf", "ties", "flat")[turn])
+            x.copy_(x2); u.copy_(u2)
+        torch.cuda.synchronize()
+        for side, (graph, *_) in zip(sides, held):
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, x, u, out in held:
+            assert all(a.equal(b) for a, b in zip(out, sample_tokens(x, u, **kw)))
+
+
 # ------------------------------------------------------------------------------------------------------------ commit
 def commit_args(B, C, seed=0, special=False):
     gen = torch.Generator(device="cuda").manual_seed(seed)
