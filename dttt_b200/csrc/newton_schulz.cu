@@ -10,7 +10,7 @@
 //
 // Operands are f16, not bf16: the same tensor-core rate with three more bits.  Five iterations multiply small singular values by
 // up to 3.4 each, and what the roundings of x and P leave in those directions grows with them: 1.2e-2 of the result with bf16
-// operands, about 1.1e-3 with f16 (Gaussian and gradient-like matrices; the bf16 result itself rounds by 1.7e-3).  Everything that
+// operands, 1.0e-3 to 1.5e-3 with f16 (Gaussian and gradient-like matrices; the bf16 result itself rounds by 1.7e-3).  Everything that
 // is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12 for
 // those, 2^5 for the cotangent, which may grow 3.4445-fold per iteration.  Sums are f32 (tensor memory), the norms f64.
 //
@@ -21,7 +21,7 @@
 //   * middle ones: the chain of products, each of which is one round of tiles whose first loads, store and mirrored store are
 //     not hidden: 3 x 509 x 1283, five steps 167 us and its derivative 53 us, 8 to 11 us a product; programmatic launches start a
 //     product's prologue under the one before (263 -> 230 us).  All of them in one cooperative launch gained nothing.
-//   * d <= 128 and L <= 512: one CTA and one launch (below), 21 us for 2 x 128 x 256 and two steps.
+//   * d <= 128 and L <= 4096: one CTA or cluster and one launch (below), 21 us for 2 x 128 x 256 and two steps.
 #include "host_check.h"
 #include "ptx_sm100.cuh"
 
@@ -493,22 +493,25 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
       dst[(long long)r * ld + c] = __float2half_rn(to_f32(src[(long long)r * cols + c]) * f0 * f1);
 }
 
-// ------------------------------------------------------------------ small matrices: everything in one CTA
-// d <= 128 and L <= 512: one CTA per matrix holds x [128, L] (transposed when rows > cols), G and P in shared memory and runs all
-// iterations in one launch; what such sizes cost otherwise is launches.  x lies as blocks of 128 rows x 64 columns with 128-byte
-// swizzle, which is the K-major operand of G = x x^T and, read with its columns as N, the MN-major one of P x.  Rows and columns
-// beyond the matrix are zero and stay so.  Also the derivative (`apply`): the kept P of every iteration is read back.
-// Five steps with keep, here / as products of their own, in us (batch 1; batch 512):
-//   16 x 64  21 / 73 (68 / 413)   64 x 256  29 / 77 (115 / 563)   128 x 512  54 / 89 (243 / 889)   512 x 128  63 / 89 (321 / 704)
-// and of the derivative 128 x 256 25 / 35 (107 / 248), 128 x 512 41 / 35 (194 / 481), 512 x 128 49 / 35 (272 / 294): only alone do the
-// longest ones lose.  Longer matrices on a cluster of CTAs that add up parts of G lost to the products at every size but a batch
-// of 8 to 148 short rows (128 x 1024: 186 / 100, 148 of them 382 / 450).  Sixteen warps: with eight, 512 x 128 took 77.
-constexpr int SMALL_D = 128, SMALL_L = 512, SMALL_THREADS = 512;
+// ------------------------------------------------------------------ few rows or columns: everything on chip
+// d <= 128 and L <= 4096: one CTA, or a cluster of up to eight with 512 columns each, holds x [128, L] (transposed when rows > cols), G
+// and P in shared memory and runs all iterations in one launch; what such sizes cost otherwise is launches.  x lies as blocks of 128
+// rows x 64 columns with 128-byte swizzle, which is the K-major operand of G = x x^T and, read with its columns as N, the MN-major
+// one of P x.  Rows and columns beyond the matrix are zero and stay so.  In a cluster each CTA adds up a share of the partial G of
+// all, rounds it and hands it round; P is then formed by everyone.  Also the derivative (`apply`): the kept P of every iteration is
+// read back.  A wait that runs out sets the status word and the kernel goes on to its end, so that no CTA waits for one that left.
+// Five steps with keep and their derivative, here / as products of their own, in us (one matrix; 300 of them):
+//   16 x 64      23 + 15 / 73 + 30 (62 + 37 / 245 + 75)        64 x 256   31 + 21 / 77 + 32 (90 + 60 / 330 + 126)
+//   128 x 512    53 + 39 / 89 + 35 (165 + 125 / 521 + 282)     512 x 128  64 + 49 / 89 + 35 (191 + 152 / 412 + 172)
+//   64 x 1024    62 + 33 / 96 + 35 (304 + 160 / 824 + 485)     128 x 4096 96 + 41 / 155 + 37 (1985 + 878 / 2600 + 1964)
+//   1024 x 64    70 + 42 / 95 + 33 (348 + 208 / 610 + 265)     4096 x 128 136 + 64 / 158 + 37 (2823 + 1339 / 1869 + 1212)
+// Bound by the latency of its three dependent products a step and, with many matrices, by loading x and by the epilogues.
+constexpr int SMALL_D = 128, SMALL_L = 512, SMALL_RANKS = 8, SMALL_THREADS = 512;
 constexpr int BLOCK_BYTES = SMALL_D * 128;                     // 128 rows x 64 f16
 
 struct SmallParams {
   const void* in;
-  int rows, cols, steps, apply, keep, out, ldd;
+  int rows, cols, steps, apply, keep, out, ldd, ranks, slice;      // `slice`: columns of x per CTA, a multiple of 64
   float scale;                 // of the f16 copy
   __half* maps;                // [steps or 1, batch, d, ldd]
   long long map_stride;
@@ -532,18 +535,37 @@ __device__ __forceinline__ void store_small(uint8_t* at, int row, int col, const
   }
 }
 
+// piece of four floats `q` of row `row` of a 128 x 128 f32 matrix, swizzled so that neighbouring rows fall into different banks
+__device__ __forceinline__ int part_offset(int row, int q) { return row * 512 + ((q ^ (row & 31)) * 16); }
+__device__ __forceinline__ float4 ld_cluster_f32x4(const void* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_u32(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ double ld_cluster_f64(const double* p, int rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_u32(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_cluster_b128(void* p, int rank, const uint4& v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_u32(p, rank)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 template <class T>
 __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sx = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const bool wide = p.rows <= p.cols;
-  const int d = wide ? p.rows : p.cols, L = wide ? p.cols : p.rows, Lp = (L + 63) / 64 * 64;
-  uint8_t* sg = sx + (Lp / 64) * BLOCK_BYTES;
-  uint8_t* sp = sg + 2 * BLOCK_BYTES;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(sp + 2 * BLOCK_BYTES);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 1);
+  const int me = p.ranks > 1 ? (int)cluster_ctarank() : 0, b = blockIdx.x / p.ranks;
+  const int d = wide ? p.rows : p.cols, c0 = me * p.slice, L = max(0, min(p.slice, (wide ? p.cols : p.rows) - c0));
+  const int Lp = max(64, (L + 63) / 64 * 64);                  // a CTA without columns keeps a block of zeros
+  uint8_t* sg = sx + (p.slice / 64) * BLOCK_BYTES;
+  uint8_t* sp = sg + 2 * BLOCK_BYTES;                          // P; in a cluster first this CTA's part of G, 128 x 128 f32
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sp + (p.ranks > 1 ? 4 : 2) * BLOCK_BYTES);
+  double* squares = reinterpret_cast<double*>(bar + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(squares + 1);
   volatile int* abort_word = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t tmem_cols = Lp > 256 ? 512 : Lp > 128 ? 256 : 128;
   if (tid == 0) {
     mbar_init(bar, 1);
@@ -560,7 +582,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   const bool aligned = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
   const int n = p.rows * p.cols, nv = aligned ? n / VEC : 0;
   double s = 0;
-  for (int i = tid; i < nv; i += 8 * SMALL_THREADS) {
+  for (int i = tid + me * 8 * SMALL_THREADS; i < nv; i += 8 * SMALL_THREADS * p.ranks) {
     uint4 raw[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -570,15 +592,22 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
 #pragma unroll
       for (int j = 0; j < VEC; ++j) { const double e = (double)to_f32(reinterpret_cast<const T*>(&raw[k])[j]); s = fma(e, e, s); }
   }
-  for (int i = nv * VEC + tid; i < n; i += 8 * SMALL_THREADS) {
+  for (int i = nv * VEC + tid + me * 8 * SMALL_THREADS; i < n; i += 8 * SMALL_THREADS * p.ranks) {
     float e[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) e[k] = i + k * SMALL_THREADS < n ? to_f32(g[i + k * SMALL_THREADS]) : 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) s = fma((double)e[k], (double)e[k], s);
   }
-  const double whole = sqrt(block_sum(s));
-  if (!p.apply && tid == 0) p.norms[b] = whole;
+  s = block_sum(s);
+  if (p.ranks > 1) {
+    if (tid == 0) *squares = s;
+    cluster_sync_all();
+    s = 0;
+    for (int r = 0; r < p.ranks; ++r) s += ld_cluster_f64(squares, r);      // the same order for all
+  }
+  const double whole = sqrt(s);
+  if (!p.apply && tid == 0 && me == 0) p.norms[b] = whole;
   const double f = whole == 0.0 ? 0.0 : (double)p.scale / whole;
   int ex = 0;
   const double mant = frexp(f, &ex);
@@ -600,13 +629,13 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         uint4 raw[8 / VEC];
 #pragma unroll
         for (int l = 0; l < 8 / VEC; ++l)
-          raw[l] = rows_in && col < L ? __ldg(reinterpret_cast<const uint4*>(g + row * p.cols + col) + l) : make_uint4(0, 0, 0, 0);
+          raw[l] = rows_in && col < L ? __ldg(reinterpret_cast<const uint4*>(g + row * p.cols + c0 + col) + l) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[k][e] = to_f32(reinterpret_cast<const T*>(raw)[e]);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          x[k][e] = rows_in && col + e < L ? to_f32(g[wide ? row * p.cols + col + e : (col + e) * p.cols + row]) : 0.f;
+          x[k][e] = rows_in && col + e < L ? to_f32(g[wide ? row * p.cols + c0 + col + e : (c0 + col + e) * p.cols + row]) : 0.f;
       }
     }
 #pragma unroll
@@ -631,14 +660,12 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   const bool rows_here = quarter * 32 < d;                      // the others stay zero
   const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
   uint32_t phase = 0;
-  bool ok = true;
   // one product: issued by thread 0, waited for by all
   auto wait = [&]() {
-    ok = mbar_wait_bounded(bar, phase, abort_word, p.status, ERR_WAIT_TMEM_FULL);
+    mbar_wait_bounded(bar, phase, abort_word, p.status, ERR_WAIT_TMEM_FULL);
     phase ^= 1;
-    ok = __syncthreads_and(ok);
+    __syncthreads();
     tc_fence_after();
-    return ok;
   };
   auto hand_over = [&]() {                                     // accumulators read, operands written: the next product may start
     tc_fence_before();
@@ -660,7 +687,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
     }
   };
   if (p.apply) fetch(0);
-  for (int k = 0; k < p.steps && ok; ++k) {
+  for (int k = 0; k < p.steps; ++k) {
     const float alpha = p.alpha[p.apply ? p.steps - 1 - k : k];
     if (!p.apply) {
       if (tid == 0) {
@@ -671,15 +698,59 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         }
         umma_commit(bar);
       }
-      if (!wait()) break;
+      wait();
       float gr[32];                                            // this thread's entries of G
       if (rows_here) {
         uint32_t r[32];
         tmem_ld_32x32(lanes + part * 32, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) gr[j] = __half2float(__float2half_rn(__uint_as_float(r[j]) * (1.f / X_SCALE)));      // one G for both terms
-        store_small(sg, row, part * 32, gr);
+        for (int j = 0; j < 32; ++j) {
+          const float v = __uint_as_float(r[j]) * (1.f / X_SCALE);
+          gr[j] = p.ranks == 1 ? __half2float(__float2half_rn(v)) : v;      // one G, rounded, for both terms
+        }
+        if (p.ranks == 1) {
+          store_small(sg, row, part * 32, gr);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(sp + part_offset(row, part * 8 + q)) = make_float4(gr[4 * q], gr[4 * q + 1], gr[4 * q + 2], gr[4 * q + 3]);
+        }
+      }
+      if (p.ranks > 1) {
+        tc_fence_before();
+        cluster_sync_all();
+        // this CTA's share of the rows: summed over the parts in order, to everyone's G
+        const int share = SMALL_D / p.ranks, live = (d + 31) / 32 * 32;
+        for (int i = tid; i < share * 16; i += SMALL_THREADS) {
+          const int r = me * share + i / 16, q = i % 16;
+          if (r >= live) continue;
+          float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+          for (int k0 = 0; k0 < p.ranks; k0 += 2) {            // two or more; four loads in flight
+            const float4 a0 = ld_cluster_f32x4(sp + part_offset(r, 2 * q), k0), a1 = ld_cluster_f32x4(sp + part_offset(r, 2 * q + 1), k0);
+            const float4 b0 = ld_cluster_f32x4(sp + part_offset(r, 2 * q), k0 + 1), b1 = ld_cluster_f32x4(sp + part_offset(r, 2 * q + 1), k0 + 1);
+            v[0] += a0.x + b0.x; v[1] += a0.y + b0.y; v[2] += a0.z + b0.z; v[3] += a0.w + b0.w;
+            v[4] += a1.x + b1.x; v[5] += a1.y + b1.y; v[6] += a1.z + b1.z; v[7] += a1.w + b1.w;
+          }
+          uint4 o;
+          __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+          for (int k2 = 0; k2 < p.ranks; ++k2) st_cluster_b128(sg + small_offset(r, q * 8), k2, o);
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");       // the tensor cores of all read what these threads wrote
+        cluster_sync_all();
+        tc_fence_after();
+        if (rows_here) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint4 o = *reinterpret_cast<const uint4*>(sg + small_offset(row, part * 32 + q * 8));
+            const __half* h = reinterpret_cast<const __half*>(&o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gr[8 * q + e] = __half2float(h[e]);
+          }
+        }
       }
       hand_over();
       if (tid == 0) {
@@ -690,7 +761,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         }
         umma_commit(bar);
       }
-      if (!wait()) break;
+      wait();
       if (rows_here) {
         uint32_t r[32];
         tmem_ld_32x32(lanes + part * 32, r);
@@ -721,11 +792,11 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
       umma_commit(bar);
     }
     if (!p.apply && p.keep)                                    // while the product runs; the padding of P is zero
-      for (int i = tid; i < d * kept_pieces; i += SMALL_THREADS) {
+      for (int i = tid + me * SMALL_THREADS; i < d * kept_pieces; i += SMALL_THREADS * p.ranks) {
         const int r = i / kept_pieces, q = i % kept_pieces;
         reinterpret_cast<uint4*>(map_of(k) + r * p.ldd)[q] = *reinterpret_cast<const uint4*>(sp + small_offset(r, q * 8));
       }
-    if (!wait()) break;
+    wait();
     const bool end = k == p.steps - 1;
     const float fin = end ? last : 1.f;
     for (int col = rows_here ? part * 32 : Lp; col < Lp; col += 128) {
@@ -743,7 +814,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
       if (!end) {
         store_small(sx, row, col, v);
       } else if (row < d && wide && p.out == OUT_BF16 && p.cols % 8 == 0) {
-        uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.y) + (long long)b * n + row * p.cols + col);
+        uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.y) + (long long)b * n + row * p.cols + c0 + col);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint4 w;
@@ -757,7 +828,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (col + j < L) {
-            const long long o = base + (wide ? (long long)row * p.cols + col + j : (long long)(col + j) * p.cols + row);
+            const long long o = base + (wide ? (long long)row * p.cols + c0 + col + j : (long long)(c0 + col + j) * p.cols + row);
             if (p.out == OUT_F32) reinterpret_cast<float*>(p.y)[o] = v[j];
             else reinterpret_cast<__nv_bfloat16*>(p.y)[o] = __float2bfloat16(v[j]);
           }
@@ -766,6 +837,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
     hand_over();
   }
   tc_fence_before();
+  if (p.ranks > 1) cluster_sync_all();                         // nobody leaves while a peer may still reach in
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
@@ -773,16 +845,32 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   }
 }
 
-static bool is_small(int rows, int cols) {
+// Matrices whose elements come one by one (tall ones, rows that do not start at 16 bytes) take a cluster only where that is made up
+// for: 84 x 915 191 us as against 146 of the products, 17 of them 195 / 196, 300 993 / 1624; tall ones above.
+static bool is_small(int batch, int rows, int cols) {
   const int d = rows < cols ? rows : cols, L = rows < cols ? cols : rows;
-  return d <= SMALL_D && L <= SMALL_L;
+  return d <= SMALL_D && L <= SMALL_L * SMALL_RANKS && (L <= SMALL_L || (rows < cols && (cols % 8 == 0 || batch >= 16)) || (cols < rows && d * L <= SMALL_D * SMALL_L));
 }
+static constexpr int small_smem(int slice, int ranks) { return (slice / 64 + (ranks > 1 ? 6 : 4)) * BLOCK_BYTES + 2048; }
+static_assert(small_smem(SMALL_L, SMALL_RANKS) + 256 <= 227 * 1024, "shared memory of an SM");
 
-static int launch_small(const SmallParams& p, int f32, int batch, cudaStream_t stream) {
-  const int L = p.rows < p.cols ? p.cols : p.rows, smem = ((L + 63) / 64 + 4) * BLOCK_BYTES + 2048;
-  if (f32) ns_small_kernel<float><<<batch, SMALL_THREADS, smem, stream>>>(p);
-  else ns_small_kernel<__nv_bfloat16><<<batch, SMALL_THREADS, smem, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
+static int launch_small(SmallParams p, int f32, int batch, cudaStream_t stream) {
+  const int L = p.rows < p.cols ? p.cols : p.rows;
+  p.ranks = 1;
+  while (p.ranks * SMALL_L < L) p.ranks *= 2;
+  p.slice = ((L + p.ranks - 1) / p.ranks + 63) / 64 * 64;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(batch * p.ranks);
+  cfg.blockDim = dim3(SMALL_THREADS);
+  cfg.dynamicSmemBytes = small_smem(p.slice, p.ranks);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = f32 ? cudaLaunchKernelEx(&cfg, ns_small_kernel<float>, p) : cudaLaunchKernelEx(&cfg, ns_small_kernel<__nv_bfloat16>, p);
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
@@ -855,8 +943,8 @@ static int prepare_device(int* n_sm) {
         cudaFuncSetAttribute(ns_product_kernel<128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
         cudaFuncSetAttribute(ns_product_kernel<256, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
         cudaFuncSetAttribute(ns_product_kernel<128, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 4) * BLOCK_BYTES + 2048) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_small_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (SMALL_L / 64 + 4) * BLOCK_BYTES + 2048) != cudaSuccess) return 302;
+        cudaFuncSetAttribute(ns_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_L, SMALL_RANKS)) != cudaSuccess ||
+        cudaFuncSetAttribute(ns_small_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_L, SMALL_RANKS)) != cudaSuccess) return 302;
     cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
     attr_mask |= 1ull << dev;
   }
@@ -1020,7 +1108,7 @@ struct Scratch {
 
 // Bytes of the scratch area for `batch` matrices [rows, cols] (256-byte aligned base).
 extern "C" long long dttt_newton_schulz_scratch(int batch, int rows, int cols) {
-  return dttt::ns::is_small(rows, cols) ? 0 : dttt::ns::Scratch(nullptr, batch, rows, cols).bytes;
+  return dttt::ns::is_small(batch, rows, cols) ? 0 : dttt::ns::Scratch(nullptr, batch, rows, cols).bytes;
 }
 
 // Groups of iterations, each with one d x d matrix of the linear map.
@@ -1039,9 +1127,9 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   if (int r = prepare_device(&n_sm)) return r;
   Group plan[MAX_STEPS];
   const int groups = make_plan(rows, cols, steps, plan);
-  if (is_small(rows, cols)) {
+  if (is_small(batch, rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, X_SCALE, (__half*)kept, (long long)batch * small * ld, norms, y, status};
+    SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, 1, 0, X_SCALE, (__half*)kept, (long long)batch * small * ld, norms, y, status};
     for (int k = 0; k < steps; ++k) p.alpha[k] = plan[k].alpha;
     return launch_small(p, f32, batch, stream);
   }
@@ -1087,9 +1175,9 @@ extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, in
   if (int r = prepare_device(&n_sm)) return r;
   Group plan[MAX_STEPS];
   const int groups = make_plan(rows, cols, steps, plan);
-  if (is_small(rows, cols)) {
+  if (is_small(batch, rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, R_SCALE, (__half*)const_cast<void*>(kept),
+    SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, 1, 0, R_SCALE, (__half*)const_cast<void*>(kept),
                            (long long)batch * small * ld, const_cast<double*>(norms), out, status};
     for (int k = 0; k < steps; ++k) p.alpha[k] = plan[k].alpha;
     return launch_small(p, f32, batch, stream);

@@ -42,7 +42,8 @@ def off(a, b):
 
 SHAPES = [(127, 511), (512, 128), (3, 129, 300), (2, 128, 513), (5, 40, 1), (8, 8), (64, 64), (1, 65, 127), (3, 128, 256), (2, 256, 128), (5, 100, 36), (257, 256), (256, 257), (2, 509, 1283), (1283, 509),
           (2, 2, 130, 700), (512, 2048), (1024, 1000), (12, 96, 96), (768, 64), (17, 4096),
-          (3, 128, 4096), (4090, 127), (2, 100, 2049), (5, 1100, 64), (129, 1032), (64, 4097)]
+          (3, 128, 4096), (4090, 127), (2, 100, 2049), (5, 1100, 64), (129, 1032), (64, 4097),
+          (16, 30, 2049), (20, 100, 701), (1024, 64), (128, 1088)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
