@@ -501,8 +501,8 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
 // all, rounds it and hands it round; P is then formed by everyone.  Also the derivative (`apply`): the kept P of every iteration is
 // read back.  A wait that runs out sets the status word and the kernel goes on to its end, so that no CTA waits for one that left.
 // Five steps with keep and their derivative, here / as products of their own, in us (one matrix; 300 of them):
-//   16 x 64      23 + 15 / 73 + 30 (62 + 37 / 245 + 75)        64 x 256   31 + 21 / 77 + 32 (90 + 60 / 330 + 126)
-//   128 x 512    53 + 39 / 89 + 35 (165 + 125 / 521 + 282)     512 x 128  64 + 49 / 89 + 35 (191 + 152 / 412 + 172)
+//   16 x 64      23 + 15 / 73 + 30                             64 x 256   31 + 21 / 77 + 32
+//   128 x 512    53 + 39 / 89 + 35                             512 x 128  64 + 49 / 89 + 35
 //   64 x 1024    62 + 33 / 96 + 35 (304 + 160 / 824 + 485)     128 x 4096 96 + 41 / 155 + 37 (1985 + 878 / 2600 + 1964)
 //   1024 x 64    70 + 42 / 95 + 33 (348 + 208 / 610 + 265)     4096 x 128 136 + 64 / 158 + 37 (2823 + 1339 / 1869 + 1212)
 // Bound by the latency of its three dependent products a step and, with many matrices, by loading x and by the epilogues.
