@@ -209,6 +209,7 @@ class BlockUnmasker:
         self.pos_q = pos + 1 if outer_shift else None
         self.blank = torch.full_like(ids, self.mask_id)
         self.committed_logp = torch.zeros(self.B, self.C, device=self.dev)
+        self.void = torch.zeros((), dtype=torch.bool, device=self.dev)      # a draw met logits without a distribution
         self.keys = _KeyChain(key)
 
     def masked_input(self, visible: torch.Tensor) -> torch.Tensor:
@@ -240,7 +241,8 @@ class BlockUnmasker:
 
     def draw(self, logits: torch.Tensor, x: torch.Tensor, key: torch.Tensor):
         """Proposals from one uniform number per slot; under the outer shift slot 0 is drawn from the previous block's tail and
-        the others in place, from the rows before them."""
+        the others in place, from the rows before them.  A row without a distribution has no token: the block is refused when it
+        is complete (``check``), and until then token 0 stands in, because what is proposed is committed, embedded and scattered by."""
         o = self.opts
         u = rng.uniform(key.to("cpu"), (self.B, self.C)).to(self.dev)
         bias = None
@@ -250,11 +252,18 @@ class BlockUnmasker:
             bias = seen * -o.presence_penalty
         kw = dict(temperature=max(float(self.temperature), 0.0), top_k=o.top_k, top_p=o.top_p, min_p=o.min_p, bias=bias, priority=o.priority)
         if not self.outer_shift:
-            return sampling.sample_tokens(logits, u, **kw)
-        lead = self.prev_tail.clone() if self.prev_tail is not None else torch.zeros(self.B, self.V, device=self.dev)
-        lead[..., self.mask_id] = float("-inf")
-        parts = zip(sampling.sample_tokens(lead[:, None], u[:, :1], **kw), sampling.sample_tokens(logits[:, :-1], u[:, 1:], **kw))
-        return tuple(torch.cat(p, 1) for p in parts)
+            tokens, logp, priority = sampling.sample_tokens(logits, u, **kw)
+        else:
+            lead = self.prev_tail.clone() if self.prev_tail is not None else torch.zeros(self.B, self.V, device=self.dev)
+            lead[..., self.mask_id] = float("-inf")
+            parts = zip(sampling.sample_tokens(lead[:, None], u[:, :1], **kw), sampling.sample_tokens(logits[:, :-1], u[:, 1:], **kw))
+            tokens, logp, priority = (torch.cat(p, 1) for p in parts)
+        self.void |= (tokens < 0).any()
+        return tokens.clamp_(min=0), logp, priority
+
+    def check(self) -> None:
+        if self.opts.inverse and bool(self.void):
+            raise FloatingPointError("decode_block: logits without a distribution (NaN or +inf in a row, or nothing above -inf)")
 
     def order(self, priority: torch.Tensor, key: torch.Tensor) -> torch.Tensor:
         """What the slots are ranked by: with ``order = random`` a draw."""
@@ -336,6 +345,7 @@ def decode_block(net: Net, ids, known, pos, state: DecodeState, key, steps: int,
     else:
         work.sweep(steps)
     work.revise(opts.remask_loop, opts.remask_k)
+    work.check()
     tail = block_tail(net, work.ids, pos, state) if outer_shift else torch.zeros(work.B, cfg.vocab_size, device=ids.device)
     return work.ids, tail
 

@@ -52,3 +52,31 @@ def test_a_training_step_with_the_five_step_write():
     torch.cuda.synchronize()
     _lib.check_status()
     assert m["finite"] == 1.0 and m["gnorm_fast_weight"] > 0
+
+
+def test_a_diverged_model_is_refused():
+    """Logits without a distribution: an error at the end of the block, and token ids inside the vocabulary until then."""
+    from dttt_b200 import generate as G
+    from dttt_b200.engine import Engine
+    from dttt_b200.ops import embed as E
+    from dttt_b200.schema import ModelConfig
+    from dttt_b200.utils import rng
+    mc = ModelConfig(vocab_size=4096, hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2,
+                     head_dim=64, suffix_len=2, chunk_size=128, window_chunks=2, qk_norm=True, mask_token_id=4095, pad_token_id=4094,
+                     eos_token_id=4094)
+    eng = Engine(mc, tiny_train(compute_dtype="bfloat16", fused_ce_block=2048, seq_len=512), device=torch.device("cuda", 0))
+    net, plain = eng.net(train=False), E.embedding
+    with torch.no_grad():
+        net.p("final_norm.weight").fill_(float("nan"))
+
+    def looked_up(table, ids, *a, **k):
+        assert ((ids >= 0) & (ids < 4096)).all()                            # on the host, before the lookup is launched
+        return plain(table, ids, *a, **k)
+
+    E.embedding = looked_up
+    try:
+        with pytest.raises(FloatingPointError, match="distribution"):
+            G.generate(net, torch.arange(20), 100, rng.key(1), steps=3, temperature=0.9, outer_shift=True, inner_task="causal",
+                       opts=G.DecodeOpts(top_p=0.9, presence_penalty=0.5))
+    finally:
+        E.embedding = plain

@@ -52,3 +52,20 @@ def test_read_block_and_cli(tmp_path, capsys):
 def test_refusals(opts):
     with pytest.raises(ValueError, match="DecodeOpts"):
         run(make_engine().net(train=False), opts)
+
+
+@pytest.mark.parametrize("opts", [G.DecodeOpts(top_p=0.9), G.DecodeOpts(top_k=5, presence_penalty=0.5), G.DecodeOpts(sampler="inverse", threshold=0.1),
+                                  G.DecodeOpts(min_p=0.1, remask_loop=1, remask_k=3)])
+@pytest.mark.parametrize("kw", [dict(), dict(outer_shift=True, inner_task="causal")])
+def test_logits_without_a_distribution_are_an_error_and_never_an_index(opts, kw, monkeypatch):
+    """A model that has diverged: every row of logits is NaN, so there is no token to commit; what the embedding is asked for stays
+    inside its table."""
+    from dttt_b200.ops import embed as E
+    net = make_engine().net(train=False)
+    seen, plain = [], E.embedding
+    monkeypatch.setattr(E, "embedding", lambda table, ids, *a, **k: seen.append(ids.clone()) or plain(table, ids, *a, **k))
+    with torch.no_grad():
+        net.p("final_norm.weight").fill_(float("nan"))
+    with pytest.raises(FloatingPointError, match="distribution"):
+        run(net, opts, temperature=1.0, **kw)
+    assert seen and all(((ids >= 0) & (ids < 128)).all() for ids in seen)
