@@ -5,9 +5,10 @@
 the inner step (reference ``src/ttt/inner_loop.py:350-397``, which runs two iterations in bf16).  On a CUDA device the products
 run on the tensor cores with f16 operands and f32 sums (``csrc/newton_schulz.cu``); elsewhere in f32.
 
-The result is the linear map ``g -> M g / |g|`` with a symmetric polynomial ``M`` of the matrix; as in the reference, ``M`` (and the
-norm, which the rescaling of the direction cancels) is held constant by the derivative, so the backward applies the same map
-to the cotangent, and so does the backward's own backward.
+The result is the linear map ``g -> M g / |g|`` with a symmetric polynomial ``M`` of the matrix; as in the reference, ``M`` is held
+constant by the derivative, and so is the norm: the backward applies the same map to the cotangent, and so does the
+backward's own backward.  Along ``g`` itself that is not the slope of the result, which does not depend on the scale of ``g``; a use
+that needs it projects the component along ``g`` out of the backward's result (the write does, ``ttt.inner.direction``).
 """
 from __future__ import annotations
 

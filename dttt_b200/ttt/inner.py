@@ -313,6 +313,24 @@ def orthogonalise(g: torch.Tensor, iters: int = 2) -> torch.Tensor:
     return y.transpose(-1, -2) if tr else y
 
 
+class _ScaleFree(torch.autograd.Function):
+    """The matrices ``x [..., m, n]`` as they are, for a use that depends on each of them up to its scale only: the cotangent loses its
+    component along the matrix, which is what the derivative of the norm subtracts in ``f(x / |x|)``."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(x)
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, c):
+        x, = ctx.saved_tensors
+        size = x.detach().abs().amax((-2, -1), keepdim=True).float()
+        xs = x.float() / torch.where(size > 0, size, 1.0)           # squares of any finite matrix stay in range
+        along = (xs * c.float()).sum((-2, -1), keepdim=True) / xs.pow(2).sum((-2, -1), keepdim=True).clamp_min(1e-30)
+        return (c.float() - xs * along).to(c.dtype)
+
+
 def direction(g: List[torch.Tensor], rule: str) -> List[torch.Tensor]:
     if rule == "sgd":
         return g
@@ -321,7 +339,8 @@ def direction(g: List[torch.Tensor], rule: str) -> List[torch.Tensor]:
     elif rule == "muon2":
         u = [orthogonalise(x, 2) for x in g]
     elif rule == "muon5":
-        u = [newton_schulz(x, 5) for x in g]
+        # every matrix is normalised by itself and the scale below is one for all of a sequence: the norms have a derivative
+        u = [newton_schulz(_ScaleFree.apply(x), 5) for x in g]
     else:
         raise ValueError(f"inner_update {rule!r}")
     ratio = seq_norm(g) / seq_norm(u)

@@ -96,3 +96,28 @@ def test_the_first_call_on_a_device_is_not_captured(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(_lib.KernelError, match="before the capture"):
         kernels._status_word(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_write_rule_against_differences_of_itself(dtype):
+    """Scaling one of several matrices leaves its polynomial as it is, so holding that constant is exact along this direction: the
+    derivative has to be the slope of the rule itself.  The rule's values: the matrices' own directions y_j, which do not move,
+    times |g| / |y| over all of them; checked for scales of 2 and 1/2 (exact in every type), differenced in 64 bits.
+    The cotangents and, of bf16 matrices, the gradients round by 2^-8: at most that of the absolute sum of the terms each, and twice
+    as much of the gradient's own, which takes their differences."""
+    gen = torch.Generator().manual_seed(11)
+    g = [torch.randn(2, *s, generator=gen).to(dtype) for s in ((6, 9), (9, 6), (5, 5))]
+    c = [x.float() * a for x, a in zip(g, (1.0, -2.0, 0.5))]                # cotangents along the matrices: nothing cancels
+    norm = lambda ts: sum(t.double().pow(2).sum((-2, -1)) for t in ts).sqrt()[:, None, None]
+    y = [newton_schulz(x, 5).double() for x in g]
+    for j in range(3):
+        scaled = lambda t: [x.double() * t if i == j else x.double() for i, x in enumerate(g)]
+        for t in (0.5, 1.0, 2.0):
+            for a, b in zip(IN.direction([x.to(dtype) for x in scaled(t)], "muon5"), y):
+                assert torch.allclose(a.double(), b * norm(scaled(t)) / norm(y), rtol=1e-5, atol=0)
+        value = lambda t: sum((a * norm(scaled(t)) / norm(y) * b).sum() for a, b in zip(y, c))
+        slope = (value(1 + 1e-4) - value(1 - 1e-4)) / 2e-4
+        leaf = [x.clone().requires_grad_(True) for x in g]
+        got, = torch.autograd.grad(sum((a * b).sum() for a, b in zip(IN.direction(leaf, "muon5"), c)), leaf[j:j + 1])
+        terms = sum((a * norm(g) / norm(y) * b).abs().sum() for a, b in zip(y, c)) + (got.double() * g[j].double()).abs().sum()
+        assert abs((got.double() * g[j].double()).sum() - slope) <= 3 * 2.0 ** -8 * terms
