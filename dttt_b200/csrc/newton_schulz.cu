@@ -934,7 +934,9 @@ static int prepare_device(int* n_sm) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 301;
   static thread_local int bound_dev = -1;
-  if (bound_dev != dev) { cudaSetDevice(dev); cudaFree(0); bound_dev = dev; }      // the encoder needs a current context
+  // The encoder needs a current context, which cudaSetDevice makes.  (cudaFree(0) would too, but a thread's first call may lie inside a
+  // capture, autograd's for a captured backward say, and ends that.)
+  if (bound_dev != dev) { if (cudaSetDevice(dev) != cudaSuccess) return 301; bound_dev = dev; }
   std::lock_guard<std::mutex> lock(mu);
   if (!(attr_mask >> dev & 1ull)) {
     if (cudaFuncSetAttribute(ns_product_kernel<256, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||

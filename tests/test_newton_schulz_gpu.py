@@ -169,3 +169,26 @@ def test_the_write_rule_on_the_kernels():
     for t in u:
         s = torch.linalg.svdvals(t.float())
         assert (s.amax(-1) / s.amin(-1) < 2.5).all()
+
+
+@pytest.mark.parametrize("shape", [(4, 300, 200), (2, 64, 100)])
+def test_capture_on_a_thread_that_has_not_called_before(shape):
+    """Autograd's thread, or one of the user's, may meet the device for the first time inside a capture."""
+    import threading
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    g, _ = make(shape, torch.bfloat16, 8)
+    want, got = newton_schulz(g), []
+    torch.cuda.synchronize()
+
+    def work():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = newton_schulz(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        got.append(y.clone())
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert len(got) == 1 and got[0].equal(want)
