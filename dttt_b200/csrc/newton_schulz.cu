@@ -12,7 +12,8 @@
 // up to 3.4 each, and what the roundings of x and P leave in those directions grows with them: 1.2e-2 of the result with bf16
 // operands, 1.0e-3 to 1.5e-3 with f16 (Gaussian and gradient-like matrices; the bf16 result itself rounds by 1.7e-3).  Everything that
 // is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12 for
-// those, 2^5 for the cotangent, which may grow 3.4445-fold per iteration.  Sums are f32 (tensor memory), the norms f64.
+// those.  The cotangent, which grows 3.4445-fold per iteration where the matrix has no singular value, is scaled to norm 2^5 and stays
+// inside f16 for six products; the seventh leaves as f32, and further ones start again from that.  Sums are f32 (tensor memory), the norms f64.
 //
 // Every product is C = alpha A B + beta D (+ s I) on CTA pairs: tiles of 256 rows and 256 or 128 columns, tcgen05.mma.cta_group::2,
 // plain per-CTA TMA loads, symmetric results formed for the tiles on and below the diagonal and stored twice.  What bounds it:
@@ -55,6 +56,7 @@ constexpr int MAX_STEPS = 32;
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float X_SCALE = 4096.f;           // of x, G and P
 constexpr float R_SCALE = 32.f;             // of the cotangent
+constexpr int PART_STEPS = 7;               // of the derivative between two f32 results: 32 3.4445^6 < 65504
 
 enum { OUT_F16 = 0, OUT_BF16 = 1, OUT_F32 = 2 };
 
@@ -307,9 +309,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
       const int row0 = tm * 2 * BM + (int)rank * BM + quarter * 32, n0 = tn * BN + c0;
       const int rows = p.M - row0;                             // of this warp's 32 (may be negative)
       float alpha = p.alpha, beta = p.beta;
+      bool none = false;                                       // a zero matrix has a zero derivative, whatever the cotangent
       if (p.num || p.den) {
         const double den = p.den ? p.den[b] : 1.0;
-        const float f = den == 0.0 ? 0.f : (float)((p.num ? p.num[b] : 1.0) / den);      // a zero matrix has a zero derivative
+        const float f = (float)((p.num ? p.num[b] : 1.0) / den);
+        none = den == 0.0;
         alpha *= f; beta *= f;
       }
       const __half* d0 = p.D ? p.D + (long long)b * p.d_batch + (long long)row0 * p.ldd + n0 : nullptr;
@@ -363,6 +367,10 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
             }
           }
           __syncwarp();
+        }
+        if (none) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) r[e] = 0;
         }
         if (MODE != 0) {                                       // rows start at multiples of 32, columns of 64
           const int on = row0 - n0 - c;
@@ -515,7 +523,7 @@ struct SmallParams {
   float scale;                 // of the f16 copy
   __half* maps;                // [steps or 1, batch, d, ldd]
   long long map_stride;
-  double* norms;               // written by the forward, read by the derivative
+  double* norms;               // written by the forward, read by the derivative (null: 1)
   void* y;
   int* status;
   float alpha[MAX_STEPS];      // x' = alpha x + M x with M = P + (a - alpha) I
@@ -650,7 +658,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
     }
   }
   float last = 1.f / p.scale;                                  // brings the last product to the result's scale
-  if (p.apply) { const double n = p.norms[b]; last = n == 0.0 ? 0.f : (float)(whole / n / (double)p.scale); }
+  bool none = false;                                           // a zero matrix has a zero derivative, whatever the cotangent
+  if (p.apply) { const double n = p.norms ? p.norms[b] : 1.0; none = n == 0.0; last = (float)(whole / n / (double)p.scale); }
   tc_fence_before();
   fence_async_proxy();                                         // the tensor core reads what these threads wrote
   __syncthreads();
@@ -810,6 +819,10 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         const __half* h = reinterpret_cast<const __half*>(&o);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[8 * q + e] = fin * fmaf(alpha, __half2float(h[e]), __uint_as_float(r[8 * q + e]) * (1.f / X_SCALE));
+      }
+      if (none && end) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.f;
       }
       if (!end) {
         store_small(sx, row, col, v);
@@ -1168,30 +1181,45 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   return 0;
 }
 
-// r [batch, rows, cols] (f32 or bf16) -> out (f32 or bf16) = prod_k (alpha_k I + M_k) r / norms, the maps of a forward with keep.
-extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, int rows, int cols, int steps, void* scratch, const void* kept,
-                                        const double* norms, void* out, int out_f32, int* status, cudaStream_t stream) {
+// The derivative is applied in parts of at most PART_STEPS iterations, the last groups first, each a call with the result of the one
+// before (f32): the first group of the part that ends before group `upto`.
+extern "C" int dttt_newton_schulz_part(int rows, int cols, int steps, int upto) {
+  using namespace dttt::ns;
+  if (steps <= PART_STEPS || steps > MAX_STEPS) return 0;
+  Group plan[MAX_STEPS];
+  const int groups = make_plan(rows, cols, steps, plan);
+  int k = upto < groups ? upto : groups, sum = 0;
+  while (k > 0 && sum + plan[k - 1].steps <= PART_STEPS) sum += plan[--k].steps;
+  return k;
+}
+
+// r [batch, rows, cols] (f32 or bf16) -> out (f32 or bf16) = prod_{k in first .. upto - 1} (alpha_k I + M_k)^T r / norms (null: 1), the
+// maps of a forward with keep.
+extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, int rows, int cols, int steps, int first, int upto, void* scratch,
+                                        const void* kept, const double* norms, void* out, int out_f32, int* status, cudaStream_t stream) {
   using namespace dttt::ns;
   if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS || batch > 65535) return -2;
   int n_sm;
   if (int r = prepare_device(&n_sm)) return r;
   Group plan[MAX_STEPS];
-  const int groups = make_plan(rows, cols, steps, plan);
+  const int groups = make_plan(rows, cols, steps, plan), count = upto - first;
+  if (first < 0 || count <= 0 || upto > groups) return -2;
   if (is_small(batch, rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    SmallParams p = {r_in, rows, cols, steps, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, 1, 0, R_SCALE, (__half*)const_cast<void*>(kept),
-                           (long long)batch * small * ld, const_cast<double*>(norms), out, status};
-    for (int k = 0; k < steps; ++k) p.alpha[k] = plan[k].alpha;
+    const long long stride = (long long)batch * small * ld;
+    SmallParams p = {r_in, rows, cols, count, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, 1, 0, R_SCALE, (__half*)const_cast<void*>(kept) + first * stride,
+                     stride, const_cast<double*>(norms), out, status};
+    for (int k = 0; k < count; ++k) p.alpha[k] = plan[first + k].alpha;
     return launch_small(p, f32, batch, stream);
   }
   const Scratch s(scratch, batch, rows, cols);
   if (int r = cast(r_in, f32, batch, rows, cols, s.partial, R_SCALE, s.x[0], s.ld, s.norm, n_sm, stream)) return r;
   Maps maps;
-  for (int i = 0; i < groups; ++i) {
-    const int k = groups - 1 - i;
+  for (int i = 0; i < count; ++i) {
+    const int k = upto - 1 - i;
     const Mat X = {s.x[i & 1], rows, cols, s.ld};
     const Mat M = {(const uint8_t*)kept + (long long)k * batch * s.d * s.ldd * 2, s.d, s.d, s.ldd};
-    const bool last = k == 0;
+    const bool last = k == first;
     const float f = last ? 1.f / R_SCALE : 1.f;
     const Out o = {last ? out : s.x[(i + 1) & 1], last ? (out_f32 ? OUT_F32 : OUT_BF16) : OUT_F16, last ? cols : s.ld, last ? s.norm : nullptr,
                    last ? norms : nullptr};

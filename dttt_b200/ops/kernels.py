@@ -856,7 +856,8 @@ def unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure):
 _lib.register("dttt_newton_schulz_scratch", _ll, [_i, _i, _i])
 _lib.register("dttt_newton_schulz_groups", _i, [_i, _i, _i])
 _lib.register("dttt_newton_schulz", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp])
-_lib.register("dttt_newton_schulz_apply", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp])
+_lib.register("dttt_newton_schulz_part", _i, [_i, _i, _i, _i])
+_lib.register("dttt_newton_schulz_apply", _i, [_vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp])
 _SYMBOL.update(newton_schulz="dttt_newton_schulz")
 
 
@@ -890,17 +891,23 @@ def newton_schulz(g, steps, keep):
 
 
 def newton_schulz_apply(r, norms, polys, steps, out_dtype):
-    """The linear map of a kept forward applied to ``r [B, rows, cols]`` (f32 or bf16, contiguous)."""
+    """The linear map of a kept forward applied to ``r [B, rows, cols]`` (f32 or bf16, contiguous); from eight steps on in parts with
+    an f32 tensor in between (directions without a singular value grow 3.4445-fold a step, and inside a part ``r`` is held in f16)."""
     global LAUNCHES
     B, rows, cols = r.shape
-    dev = r.device
-    out = torch.empty_like(r, dtype=out_dtype)
+    dev, upto = r.device, polys.shape[0]
     l = _lib.lib()
     size = l.dttt_newton_schulz_scratch(B, rows, cols)
     scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), int(r.dtype == torch.float32), B, rows, cols, steps,
-            scratch.data_ptr() if size else None, polys.data_ptr(), norms.data_ptr(), out.data_ptr(), int(out_dtype == torch.float32),
-            _status_word(dev))
-    if size:
-        LAUNCHES += 1 + polys.shape[0]
-    return out
+    over = norms.data_ptr()
+    while True:
+        first = l.dttt_newton_schulz_part(rows, cols, steps, upto)
+        out = torch.empty_like(r, dtype=torch.float32 if first else out_dtype)
+        _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), int(r.dtype == torch.float32), B, rows, cols, steps,
+                first, upto, scratch.data_ptr() if size else None, polys.data_ptr(), over, out.data_ptr(), int(out.dtype == torch.float32),
+                _status_word(dev))
+        if size:
+            LAUNCHES += 1 + upto - first
+        if first == 0:
+            return out
+        r, upto, over = out, first, None

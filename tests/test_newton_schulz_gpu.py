@@ -192,3 +192,73 @@ def test_capture_on_a_thread_that_has_not_called_before(shape):
     t.start()
     t.join()
     assert len(got) == 1 and got[0].equal(want)
+
+
+# ------------------------------------------------------------------------------------------------------------ many steps
+def plan_of(rows, cols, steps):
+    """(iterations, alpha) of every group, as the launcher groups them: pairs at both ends of long large matrices."""
+    a, b, c = ref.NEWTON_SCHULZ
+    d, n = min(rows, cols), max(rows, cols)
+    q = lambda l: a + b * l + c * l * l
+    l, k, out = 1.0 / d, 0, []
+    while k < steps:
+        two = d >= 512 and n >= 2 * d and ((k == 0 and steps >= 2) or (k == steps - 2 and k >= 3))
+        l2 = l * q(l) ** 2
+        out.append((2, q(l) * q(l2)) if two else (1, q(l)))
+        l, k = (l2 * q(l2) ** 2, k + 2) if two else (l2, k + 1)
+    return out
+
+
+def maps_of(maps, shape, steps):
+    """The kept matrices of every group in 64 bits with their diagonal, and the largest growth in each."""
+    d = min(shape[-2:])
+    ms = [maps[k, :, :, :d].double() / 4096 + alpha * torch.eye(d, dtype=torch.float64, device=maps.device)
+          for k, (_, alpha) in enumerate(plan_of(*shape[-2:], steps))]
+    return ms, [torch.linalg.eigvalsh(m.mT @ m)[:, -1] for m in ms]
+
+
+def apply_of(ms, most, norms, r):
+    """What the kept matrices of a forward say the derivative is, in 64 bits, and the error that f16 roundings of the cotangent may
+    leave: a step rounds by 2^-11 over the square root of 3 in the mean square, and what it leaves grows like a part of the cotangent
+    in the direction that grows most."""
+    x = torch.where(norms[:, None, None] == 0, 0.0, r.double() / norms[:, None, None])
+    off2 = torch.zeros(r.shape[0], dtype=torch.float64, device=r.device)
+    for m, top in zip(reversed(ms), reversed(most)):
+        off2 = top * (off2 + (2.0 ** -11 / 3 ** 0.5) ** 2 * x.pow(2).sum((-2, -1)))
+        x = m.mT @ x if r.shape[-2] <= r.shape[-1] else x @ m.mT
+    return x, off2.sqrt()
+
+
+@pytest.mark.parametrize("shape", [(64, 200), (1, 48, 40), (2, 128, 1024), (512, 128), (2, 129, 300), (300, 200), (512, 1024), (1100, 520)])
+@pytest.mark.parametrize("steps", [7, 8, 12, 32])
+def test_derivative_of_many_steps(shape, steps):
+    """Directions without a singular value grow 3.4445-fold a step in the cotangent: 10^4 at eight steps, 10^17 at 32.  Against the kept
+    matrices themselves, so that what many steps do to the forward's roundings is not part of it.  The bound: that of the roundings,
+    in the norm (they are many and independent: a factor of two over the mean square is never met), and the result's own."""
+    from dttt_b200.ops import kernels
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    full, gy = make(shape if len(shape) == 3 else (1, *shape), torch.float32, 2)
+    d = min(shape[-2:])
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    lean = r(*full.shape[:-1], max(1, d // 3)) @ r(full.shape[0], max(1, d // 3), full.shape[-1])
+    gap = full.clone()
+    (gap[:, 3] if shape[-2] <= shape[-1] else gap[:, :, 3]).zero_()
+    one = torch.zeros_like(gy)
+    one[:, 3, 5] = 0.7
+    for g in (full, lean, gap, torch.zeros_like(full)):
+        _, norms, maps = kernels.newton_schulz(g, steps, True)
+        ms, growth = maps_of(maps, shape, steps)
+        for c in (gy, one, gy * 1e20):
+            want, off2 = apply_of(ms, growth, norms, c)
+            for dtype in (torch.float32, torch.bfloat16):
+                got = kernels.newton_schulz_apply(c, norms, maps, steps, dtype)
+                most = want.norm(dim=(-2, -1))
+                if most.max() > 1e37:                                       # (f32 itself ends)
+                    continue
+                assert got.isfinite().all()
+                lost = 2.0 ** -24 if dtype is torch.float32 else 2.0 ** -8
+                assert ((got.double() - want).norm(dim=(-2, -1)) <= 2 * off2 + lost * most).all()
+    leaf = torch.zeros_like(full).requires_grad_(True)
+    gx, = torch.autograd.grad(newton_schulz(leaf, steps), leaf, gy)
+    assert gx.eq(0).all()
