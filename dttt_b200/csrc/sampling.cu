@@ -15,7 +15,8 @@
 // Masses are integers: w in [0, 1] is rounded to a multiple of 2^-S with V 2^S <= 2^63, so sums are exact, independent of their
 // order, and every pass over the row that adds up a part of it sees the same numbers.  w itself is evaluated in 64 bits: the
 // draw and the top-p cut are comparisons of sums over up to V terms, and a 32-bit sum over 128k terms is off by more than the
-// gap between neighbouring borders of a flat row.
+// gap between neighbouring borders of a flat row.  A draw of fewer units than there are elements (u = 0; else u < 2^-24) may end
+// among tokens that have less than a unit: it is made again with masses in 64-bit floating point (`tiny_draw`).
 //
 // A row is spread over a cluster of 1 .. 8 CTAs, each of which keeps its slice (f32, after the bias) in shared memory, so the
 // logits are read from global memory once whatever the number of passes; the CTAs exchange maxima, histograms and masses
@@ -185,6 +186,8 @@ struct Shared {
   float scale, u, logz, pr;
   int top_k, greedy;
   u64 whole, goal, base, mine;
+  int tiny;                                 // the draw is made again by tiny_draw
+  double part[MAX_WARPS];                   // its masses, per warp
 };
 
 // exp((x - m) / T) as a mass of 2^S units, rounded to nearest.  Table-driven (Tang's scheme, from the mathematics): with
@@ -774,6 +777,55 @@ __device__ __noinline__ void few_candidates(const SampleParams& p, Shared& sh, c
   }
 }
 
+// The draw of a row whose goal is less than a unit of mass for every element: with masses as doubles, in order of the indices, over
+// all CTAs of the row.  `kept` as the caller has it.
+template <int WARPS>
+__device__ __noinline__ void tiny_draw(const SampleParams& p, Shared& sh, const float* xs, Segment seg, int first, unsigned int row, float m,
+                                       float least, float lo, float hi, int last_tie) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), me = (int)cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto mass = [&](int i) {
+    const float x = i < seg.b ? xs[i] : -INFINITY;
+    return i < seg.b && x >= least && (x > hi || (x >= lo && i <= last_tie)) ? exp(((double)x - (double)m) / sh.temp) : 0.0;
+  };
+  double s = 0;
+  for (int i = seg.a + lane; i < seg.b; i += 32) s += mass(i);
+  s = warp_sum(s);
+  if (lane == 0) sh.part[warp] = s;
+  cluster.sync();
+  double run = 0, total = 0;
+  for (int e = 0; e < ranks * WARPS; ++e) {
+    const double v = cluster.map_shared_rank(&sh, e / WARPS)->part[e % WARPS];
+    if (e < me * WARPS + warp) run += v;
+    total += v;
+  }
+  const double u = (double)sh.u, goal = u > 0 ? u * total : 0.0;
+  if (!(run <= goal && run + s > goal)) return;                    // one warp's, as the sums before it are the same for all
+  auto answer = [&](int i) {
+    p.tokens[row] = first + i;
+    p.logp[row] = (xs[i] - m) - sh.logz;
+    if (p.priority != PRI_LOGP) p.prio[row] = sh.pr;
+  };
+  int last = -1;                                                   // with a mass: the answer where only a rounding is missing
+  for (int i0 = seg.a; i0 < seg.b; i0 += 32) {
+    double inc = mass(i0 + lane);
+    if (inc > 0) last = i0 + lane;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    const unsigned int hit = __ballot_sync(0xffffffffu, run + inc > goal);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) answer(i0 + lane);
+      return;
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) answer(last);
+}
+
 static_assert(sizeof(Shared) <= 12600, "three CTAs with slices of 16032 elements (V = 128256) on an SM");
 
 template <class T, int WARPS>
@@ -988,6 +1040,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
         const double u = (double)sh.u;
         const u64 goal = u > 0 ? (u64)(fmin(u, 1.0) * (double)total) : 0;
         sh.goal = min(goal, total - 1);
+        sh.tiny = goal < (u64)p.V;
         sh.base = base; sh.mine = end - base;
       }
     }
@@ -1003,8 +1056,11 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
     }
   }
   __syncthreads();
+  const bool tiny = !greedy && sh.tiny;                            // the same in every CTA of the row
+  if (tiny) tiny_draw<WARPS>(p, sh, xs, seg, first, row, m, least, cut.lo, cut.hi, last_tie);
+  __syncwarp();
   cluster.barrier_arrive();                                        // nothing of a peer's memory is read any more
-  if (!greedy) {
+  if (!greedy && !tiny) {
     const u64 goal = sh.goal, base = sh.base;
     auto answer = [&](int tok, float x) {
       p.tokens[row] = tok;
@@ -1136,9 +1192,47 @@ __global__ void __launch_bounds__(STREAM_THREADS, 3) chunk_kernel(const SamplePa
   }
 }
 
+// The draw inside a chunk where less than a unit of mass for every element is left: masses as doubles, relative to the row's maximum,
+// in order of the indices.  By one warp.
+template <class T>
+__device__ __noinline__ void tiny_chunk_draw(const SampleParams& p, unsigned int row, int chunk, float m, double temp, double left, float logz,
+                                             float pr) {
+  const RowView<T> view(p, row);
+  const int lane = threadIdx.x & 31, start = max(0, chunk * CHUNK - view.mis), end = min(p.V, (chunk + 1) * CHUNK - view.mis);
+  auto value = [&](int i) {
+    if (i >= end) return -INFINITY;
+    const float x = to_f32(view.src[i]);
+    return view.bias ? x + view.bias[i] : x;
+  };
+  auto answer = [&](int i) {
+    p.tokens[row] = i;
+    p.logp[row] = (value(i) - m) - logz;
+    if (p.priority != PRI_LOGP) p.prio[row] = pr;
+  };
+  double run = 0;
+  int last = -1;                                                   // with a mass: the answer where only a rounding is missing
+  for (int i0 = start; i0 < end; i0 += 32) {
+    double inc = exp(((double)value(i0 + lane) - (double)m) / temp);
+    if (inc > 0) last = i0 + lane;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    const unsigned int hit = __ballot_sync(0xffffffffu, run + inc > left);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) answer(i0 + lane);
+      return;
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) answer(last);
+}
+
 // A warp per row.
 template <class T>
-__global__ void __launch_bounds__(32) chunk_draw_kernel(const SampleParams p, int most, const Chunk* __restrict__ in) {
+__global__ void __launch_bounds__(32) chunk_draw_kernel(const __grid_constant__ SampleParams p, int most, const Chunk* __restrict__ in) {
   __shared__ double tab[TAB * COPIES];
   const int lane = threadIdx.x;
   const unsigned int row = blockIdx.x;
@@ -1198,27 +1292,35 @@ __global__ void __launch_bounds__(32) chunk_draw_kernel(const SampleParams p, in
     const double t = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += t;
   }
+  // the sum before a lane comes from the lane before it: upto - mass would lose what is small beside the lane's own mass
+  const double up = __shfl_up_sync(0xffffffffu, upto, 1), before = lane ? up : 0.0;
   const double total = __shfl_sync(0xffffffffu, upto, 31), goal = u > 0 ? fmin(u, 1.0) * total : 0.0;
   // the first lane, and its first chunk, whose running mass exceeds the goal; rounding at the very end: the last chunk with a mass
   const unsigned int past = __ballot_sync(0xffffffffu, upto > goal), some = __ballot_sync(0xffffffffu, mass > 0);
   const int own = past & some ? __ffs(past & some) - 1 : 31 - __clz(some);
   int chunk = -1;
-  double rest = 0;
+  double rest = 0, left = 0;
   if (lane == own) {
-    double run = upto - mass;
+    double run = before;
     for (int c = c0; c < c1; ++c) {
       const Chunk q = r[c];
       if (q.m == -INFINITY || q.mass == 0) continue;
       const double f = exp(((double)q.m - (double)m) / temp), v = (double)q.mass * f;
       if (!(v > 0)) continue;
       chunk = c;
-      rest = (goal - run) / f;
+      left = goal - run;
+      rest = left / f;
       if (run + v > goal) break;
       run += v;
     }
   }
   chunk = __shfl_sync(0xffffffffu, chunk, own);
   rest = __shfl_sync(0xffffffffu, rest, own);
+  if (rest < CHUNK) {
+    left = __shfl_sync(0xffffffffu, left, own) * (1.0 / (double)(1ull << CHUNK_BITS));
+    tiny_chunk_draw<T>(p, row, chunk, m, temp, left, logz, pr);
+    return;
+  }
   const u64 held = r[chunk].mass;
   const u64 want = min(rest > 0 ? (u64)rest : 0, held - 1);
   const float mc = r[chunk].m;

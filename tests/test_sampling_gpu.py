@@ -233,6 +233,37 @@ def test_two_graphs_at_once(kw):
             assert all(a.equal(b) for a, b in zip(out, sample_tokens(x, u, **kw)))
 
 
+@pytest.mark.parametrize("V", [700, 5003, 128256, 390001])
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.4), dict(top_k=650), dict(top_p=1 - 1e-7, temperature=1.3), dict(min_p=1e-30),
+                                dict(temperature=0.5, top_k=699, min_p=1e-25), dict(temperature=1e-3), dict(top_k=4, top_p=0.9)])
+def test_draws_below_the_unit_of_mass(V, kw):
+    """Numbers near 0 draw the first tokens of a row however little mass they have: of 0 the first kept one that has any in 64
+    bits, of others the one where the running mass passes.  Rows that start with masses of e^-2000 to e^-20; many rows at once,
+    too, for the two-launch form.  (A border is met with the relative rounding of 64-bit sums only.)  Log-probabilities lie as low as
+    -2000 here, where the three roundings to f32 (x - m, the last subtraction, the oracle's result) are 2^-24 of them each."""
+    def far(x, priority, u, **kw):
+        from dttt_b200.ops.sampling import sample_tokens
+        got = sample_tokens(x, u, priority=priority, **kw)
+        par = [torch.full(u.shape, kw.get(k, v), dtype=torch.int64 if k == "top_k" else torch.float64, device="cuda")
+               for k, v in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))]
+        want = ref.sample_tokens(x, u, None, *par, priority)
+        assert got.tokens.equal(want[0]), (got.tokens != want[0]).nonzero()[:5].tolist()
+        for a, b, tol in ((got.logp, want[1], TOL["logp"]), (got.priority, want[2], TOL[priority])):
+            assert ((a - b).abs() <= tol + 3 * 2.0 ** -24 * b.abs()).all()
+
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    u = torch.tensor([0.0, 1e-44, 1e-38, 3e-30, 2e-22, 1e-17, 4e-14, 1e-11, 1e-9, -1.0, 2.0 ** -24], device="cuda")[None]
+    x, _ = logits((1, u.shape[1]), V, seed=V, kind="flat")
+    low = V // 2
+    x[..., :low] -= 20 + 100 * torch.rand(1, u.shape[1], low, generator=gen, device="cuda")
+    x[..., :low // 4] = -torch.linspace(800, 60, low // 4, device="cuda")[torch.randperm(low // 4, generator=gen, device="cuda")]
+    x[..., :3] = torch.tensor([-2000.0, float("-inf"), -760.0], device="cuda")
+    far(x, "logp", u, **kw)
+    far(x.to(torch.bfloat16), "entropy", u, **kw)
+    many = -(-(9 << 20) // V) // u.shape[1] + 1
+    far(x.repeat(1, many, 1)[:, :, 1:], "margin", u.repeat(1, many), **kw)
+
+
 # ------------------------------------------------------------------------------------------------------------ commit
 def commit_args(B, C, seed=0, special=False):
     gen = torch.Generator(device="cuda").manual_seed(seed)
