@@ -1104,9 +1104,15 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 9 : WARPS == 8 ? 3 : 
 // takes the chunk's own maximum, and leaves the chunk's sums relative to it (the masses as integers, as above).  A second launch, a
 // warp per row, brings them to the row's maximum in 64 bits, finds the chunk that holds the draw and reads it once more.
 constexpr int CHUNK_BITS = 50;                    // 1024 2^50 <= 2^62
-// Elements from which a draw takes two launches.  One / two, us: 8 x 128256 12.4 / 18.5, 16 x 128256 18.5 / 18.6, 32 x 128256 20.6 / 22.7,
-// 64 x 128256 33.0 / 28.8, 1024 x 128256 348 / 185; 1024 x 2048 16.5 / 20.6, 4096 x 1000 41 / 43.
-constexpr long long STREAM_LEAST = 2ll << 20;
+// A draw takes two launches from 6.2 million elements on, for vocabularies above 4096.  One / two, us (f32; bf16 within
+// 10 %; of 30 sizes in both types the form chosen here is at most 2 us slower than the other one):
+//   V = 128256: 8 rows 12.3 / 20.0, 32 rows 21.8 / 25.2, 48 rows (6.16 million) 26.4 / 28.7, 64 rows 37.1 / 30.8, 96 rows 45.4 / 35.7
+//   V = 390001: 8 rows 23.9 / 28.0, 16 rows (6.24 million) 55.3 / 32.8    V = 50257: 64 rows 19.2 / 22.0, 128 rows (6.43) 32.8 / 27.7
+//   V = 32000: 192 rows 26.4 / 26.7, 256 rows 36.5 / 28.7    V = 16384: 256 rows 20.5 / 23.3, 512 rows 37.1 / 28.7
+//   V = 8192: 512 rows 26.1 / 24.6, 1024 rows 39.0 / 30.8    V = 4096: 1024 rows 22.6 / 24.3, 2048 rows 39.0 / 39.2
+//   V = 2048: 4096 rows 49.2 / 58.9    V = 1000: 16384 rows 145.5 / 175.5 (a chunk of 1024 is mostly empty, and a row has its own second warp)
+constexpr long long STREAM_LEAST = 6200000;
+constexpr int STREAM_VOCAB = 4096;
 
 struct __align__(16) Chunk {
   float m, z, e;               // maximum (NaN or +inf if there is one), sum of exp(x - m), the priority's own value
@@ -1569,7 +1575,7 @@ extern "C" int dttt_sample_ranks(int V) {
 // Bytes of scratch that dttt_sample wants for `rows` rows whose draw no parameter truncates (0: none).
 extern "C" long long dttt_sample_scratch(long long rows, int V) {
   const long long most = (V + 7ll + CHUNK - 1) / CHUNK;
-  return rows * V >= STREAM_LEAST && rows * most <= 0x7fffffffll ? rows * most * (long long)sizeof(Chunk) : 0;
+  return V > STREAM_VOCAB && rows * V >= STREAM_LEAST && rows * most <= 0x7fffffffll ? rows * most * (long long)sizeof(Chunk) : 0;
 }
 
 // logits: rows [outer, inner] of V elements (dtype 0 f32, 1 bf16, 2 f16), element strides s_outer / s_inner, contiguous along V.

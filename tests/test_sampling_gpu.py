@@ -264,6 +264,51 @@ def test_draws_below_the_unit_of_mass(V, kw):
     far(x.repeat(1, many, 1)[:, :, 1:], "margin", u.repeat(1, many), **kw)
 
 
+@pytest.mark.parametrize("V", [1000, 4096, 4097, 8191, 32001, 128256, 390001])
+def test_one_launch_or_two(V):
+    """Untruncated draws on both sides of the rule: 6.2 million elements and V above 4096 take two launches over a scratch area."""
+    from dttt_b200.ops import _lib
+    size = _lib.lib().dttt_sample_scratch
+    edge = -(-6200000 // V)
+    assert size(edge - 1, V) == 0 and (size(edge, V) > 0) == (V > 4096) and (size(4 * edge, V) > 0) == (V > 4096)
+    for rows in (edge - 1, edge):
+        for dtype, priority, kind, kw in ((torch.float32, "entropy", "zipf", dict()), (torch.bfloat16, "margin", "ties", dict(temperature=0.6)),
+                                          (torch.float16, "logp", "few", dict(temperature=1e-6)), (torch.float32, "margin", "wide", dict(temperature=0.0)),
+                                          (torch.bfloat16, "entropy", "equal", dict(temperature=1e6))):
+            x, u = logits((1, rows), V + 3, dtype, seed=V, kind=kind)
+            x, u = x[:, :, 3:], u.clone()
+            x[0, 0] = float("-inf")
+            x[0, 1, V // 2] = float("nan")
+            x[0, 2, V - 1] = float("inf")
+            u[0, 3], u[0, 4], u[0, 5] = 0.0, 1.0, 1 - 2 ** -24
+            bias = torch.where(torch.rand(1, V, device="cuda") < 0.2, -2.0, 0.0)
+            out = check(x, u, priority, bias=bias if kind == "zipf" else None, **kw)
+            assert (out.tokens[0, :3] == -1).all() and (out.tokens[0, 3:] >= 0).all()
+
+
+def test_two_graphs_of_the_two_launch_form():
+    """Each graph has a scratch area of its own."""
+    from dttt_b200.ops.sampling import sample_tokens
+    sides, held = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for n in range(2):
+        x, u = logits((2, 90), 40001, seed=n)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = sample_tokens(x, u, temperature=0.9, priority="margin")
+        held.append((graph, x, u, out))
+    for turn in range(3):
+        for n, (graph, x, u, out) in enumerate(held):
+            x2, u2 = logits((2, 90), 40001, seed=10 * turn + n, kind=("zipf", "ties", "flat")[turn])
+            x.copy_(x2); u.copy_(u2)
+        torch.cuda.synchronize()
+        for side, (graph, *_) in zip(sides, held):
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, x, u, out in held:
+            assert all(a.equal(b) for a, b in zip(out, sample_tokens(x, u, temperature=0.9, priority="margin")))
+
+
 # ------------------------------------------------------------------------------------------------------------ commit
 def commit_args(B, C, seed=0, special=False):
     gen = torch.Generator(device="cuda").manual_seed(seed)
