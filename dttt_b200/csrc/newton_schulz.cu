@@ -8,12 +8,21 @@
 // y is a polynomial of the matrix times g / |g|; its derivative is taken with the polynomial and the norm held constant (the map
 // is then linear and self-adjoint), so the backward applies the same a r + P_k r in reverse order to the cotangent.
 //
-// Operands are f16, not bf16: the same tensor-core rate with three more bits.  Five iterations multiply small singular values by
-// up to 3.4 each, and what the roundings of x and P leave in those directions grows with them: 1.2e-2 of the result with bf16
-// operands, 1.0e-3 to 1.5e-3 with f16 (Gaussian and gradient-like matrices; the bf16 result itself rounds by 1.7e-3).  Everything that
-// is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12 for
-// those.  The cotangent, which grows 3.4445-fold per iteration where the matrix has no singular value, is scaled to norm 2^5 and stays
-// inside f16 for six products; the seventh leaves as f32, and further ones start again from that.  Sums are f32 (tensor memory), the norms f64.
+// Operands are f16, not bf16: the same tensor-core rate with three more bits.  Roundings of G, of P and of x inside P x stay within the
+// row or the column space of x: they turn singular vectors by about as much as they are, and nothing amplifies that.  What x loses when
+// it is stored lies mostly outside both, where an iteration multiplies by a = 3.4445 (five of them by 485), and the gradient of a
+// write, of as many tokens as a chunk has, fills at most a part of either space.  So x is kept in two f16 halves: the products take the
+// upper one, and the lower one is added with what the map does outside the spaces, alpha + s (below).  Only the last group does
+// without.  Five steps, off by (2-norm, the bf16 result's own 1.66e-3 included; in brackets with the upper half alone):
+//   512 x 2048 (paired iterations)  rank 1 3.9e-3 (0.145), rank 64 3.8e-3 (1.6e-2), rank 256 3.4e-3 (7.1e-3), full 2.06e-3 (2.06e-3)
+//   509 x 1283                      rank 1 2.3e-3 (0.147), rank 63 2.1e-3 (2.0e-2), rank 254 2.0e-3 (7.9e-3), full 1.9e-3 (1.9e-3)
+//   128 x 256                       rank 1 2.5e-3 (0.145), rank 16 2.1e-3 (3.5e-2), rank 64 2.1e-3 (1.3e-2), full 2.07e-3 (1.98e-3)
+// It costs 4 x 2048 x 8192 1807 -> 1834 us, 8192 x 2048 with its derivative 823 -> 839, 3 x 509 x 1283 likewise 221 -> 230, 128 x 512 in
+// one launch 53 -> 66.  Keeping G and P in two halves as well would leave the bf16 result's rounding alone, at three times the products.
+// Everything that is stored has singular values below 1.21 (x), 1.47 (G) and 2.82 (P), so fixed powers of two keep it inside f16: 2^12
+// for those (the lower half ends at 2^-25 of that scale).  The cotangent, which grows 3.4445-fold per iteration where the matrix has no
+// singular value, is scaled to norm 2^5 and stays inside f16 for six products; the seventh leaves as f32, and further ones start again
+// from that.  Sums are f32 (tensor memory), the norms f64.
 //
 // Every product is C = alpha A B + beta D (+ s I) on CTA pairs: tiles of 256 rows and 256 or 128 columns, tcgen05.mma.cta_group::2,
 // plain per-CTA TMA loads, symmetric results formed for the tiles on and below the diagonal and stored twice.  What bounds it:
@@ -42,13 +51,18 @@ constexpr int EPI_WARPS = 8;   // two per quarter of the accumulator's rows, hal
 constexpr int THREADS = (2 + EPI_WARPS) * 32;
 constexpr int STAGING_BYTES = EPI_WARPS * 4096;                // epilogue: 32 rows x 128 bytes per warp
 
-// BN: output columns per pair (256 or 128); each CTA loads BN / 2 of them.
-template <int BN>
+// What a product's epilogue does beside alpha A B + beta D: a kernel of its own each.
+enum { MODE_PLAIN = 0, MODE_SUM = 1, MODE_DIAG = 2, MODE_SPLIT = 3 };      // + beta2 D2 + diag I | + diag I | + beta2 D2, in two halves
+
+// BN: output columns per pair (256 or 128); each CTA loads BN / 2 of them.  With a second summand a second staging area takes the place
+// of one stage.
+template <int BN, int MODE>
 struct Tile {
   static constexpr int B_BYTES = (BN / 2) * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 6 : 8;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + STAGING_BYTES + 1024;
+  static constexpr bool TWO = MODE == MODE_SUM || MODE == MODE_SPLIT;
+  static constexpr int STAGES = (BN == 256 ? 6 : 8) - (TWO ? (STAGING_BYTES + STAGE_BYTES - 1) / STAGE_BYTES : 0);
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + (TWO ? 2 : 1) * STAGING_BYTES + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -65,9 +79,10 @@ struct Params {
   int a_mn_major, b_mn_major;
   float alpha, beta;
   const __half* D;             // or null; same shape as C
-  const __half* D2;            // MODE 1: a second one
+  const __half* D2;            // a second one
   long long ldd, d_batch;      // of both
-  float beta2, diag;           // MODE 1 and 2: `diag` is added on the diagonal
+  float beta2, diag;
+  __half* lo;                  // what the f16 rounding of C leaves, with the layout of C; may be D2
   void* C;
   int out;
   long long ldc, c_batch;
@@ -131,16 +146,18 @@ __device__ __forceinline__ void stage_in(uint8_t* stg, int lane, const uint4 (&v
 template <class T2> __device__ __forceinline__ T2 pack2(float a, float b);
 template <> __device__ __forceinline__ __half2 pack2<__half2>(float a, float b) { return __floats2half2_rn(a, b); }
 template <> __device__ __forceinline__ __nv_bfloat162 pack2<__nv_bfloat162>(float a, float b) { return __floats2bfloat162_rn(a, b); }
+// What is left of two values beside `h`, their f16 roundings.
+__device__ __forceinline__ __half2 left_over(__half2 h, float a, float b) {
+  const float2 f = __half22float2(h);
+  return __floats2half2_rn(a - f.x, b - f.y);
+}
 template <class T2>
-__device__ __forceinline__ void stage_out(uint8_t* stg, int lane, const uint32_t (&r)[64]) {
+__device__ __forceinline__ uint4 pack8(const uint32_t* r) {
+  uint4 v;
+  T2* h = reinterpret_cast<T2*>(&v);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    uint4 v;
-    T2* h = reinterpret_cast<T2*>(&v);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = pack2<T2>(__uint_as_float(r[8 * q + 2 * e]), __uint_as_float(r[8 * q + 2 * e + 1]));
-    *reinterpret_cast<uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16)) = v;
-  }
+  for (int e = 0; e < 4; ++e) h[e] = pack2<T2>(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+  return v;
 }
 __device__ __forceinline__ void flush_lines(const uint8_t* stg, int lane, uint16_t* out, long long ld, int rows, int cols) {
   const int piece = lane & 7;
@@ -163,27 +180,28 @@ __device__ __forceinline__ void flush_ragged(const uint8_t* stg, int lane, uint1
     }
   }
 }
-__device__ __forceinline__ void store_f32(float* out, long long ld, int rows, int cols, int lane, const uint32_t (&r)[64]) {
+// 32 columns
+__device__ __forceinline__ void store_f32(float* out, long long ld, int rows, int cols, int lane, const uint32_t (&r)[32]) {
   if (lane >= rows) return;
   float* o = out + lane * ld;
   if ((ld & 3) == 0) {
 #pragma unroll
-    for (int j = 0; j < 64; j += 4)
+    for (int j = 0; j < 32; j += 4)
       if (j < cols) *reinterpret_cast<float4*>(o + j) = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
                                                                     __uint_as_float(r[j + 3]));
   } else {
 #pragma unroll
-    for (int j = 0; j < 64; ++j)
+    for (int j = 0; j < 32; ++j)
       if (j < cols) o[j] = __uint_as_float(r[j]);
   }
 }
-// The piece's transpose: column j of the 64 becomes a row.  Neighbouring lanes (rows 2i, 2i + 1 of the piece) trade one value per
+// The transpose of 32 rows x 32 columns: column j becomes a row.  Neighbouring lanes (rows 2i, 2i + 1 of the piece) trade one value per
 // pair of columns, so that each stores two neighbours: an instruction writes 64 bytes of two rows.
-__device__ __forceinline__ void store_transposed(__half* out, long long ld, int rows, int cols, int lane, const uint32_t (&r)[64]) {
+__device__ __forceinline__ void store_transposed(__half* out, long long ld, int rows, int cols, int lane, const uint32_t (&r)[32]) {
   const bool odd = lane & 1;
   const int at = lane & ~1;
 #pragma unroll
-  for (int j = 0; j < 64; j += 2) {
+  for (int j = 0; j < 32; j += 2) {
     const float mine = __uint_as_float(odd ? r[j + 1] : r[j]);
     const float theirs = __shfl_xor_sync(0xffffffffu, __uint_as_float(odd ? r[j] : r[j + 1]), 1);
     const __half2 v = odd ? __floats2half2_rn(theirs, mine) : __floats2half2_rn(mine, theirs);
@@ -195,7 +213,8 @@ __device__ __forceinline__ void store_transposed(__half* out, long long ld, int 
 template <int BN, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, const Params p) {
-  constexpr int STAGES = Tile<BN>::STAGES, STAGE_BYTES = Tile<BN>::STAGE_BYTES;
+  constexpr int STAGES = Tile<BN, MODE>::STAGES, STAGE_BYTES = Tile<BN, MODE>::STAGE_BYTES;
+  constexpr bool TWO = Tile<BN, MODE>::TWO;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);      // the leader's count both CTAs' bytes
@@ -319,6 +338,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
       const __half* d0 = p.D ? p.D + (long long)b * p.d_batch + (long long)row0 * p.ldd + n0 : nullptr;
       uint4 dnext[8];                                          // 64 columns of D, eight lanes to a row's 128 bytes
       load_rows(d0, p.ldd, rows, (int)p.ldd - n0, lane, dnext);
+      uint4 lnext[8];                                          // and of D2
+      if (TWO) load_rows(p.D2 + (d0 - p.D), p.ldd, rows, (int)p.ldd - n0, lane, lnext);
       int got = 1;
       if (lane == 0) got = mbar_wait_bounded(&acc_full[acc], acc_ph, abort_word, p.status, ERR_WAIT_TMEM_FULL) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
@@ -326,75 +347,71 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
       tc_fence_after();
       const uint32_t taddr = tmem_base + acc * BN + c0 + ((uint32_t)(quarter * 32) << 16);
       uint8_t* stg = smem + STAGES * STAGE_BYTES + 1024 + (warp - 2) * 4096;
+      uint8_t* stg2 = stg + STAGING_BYTES;                     // of D2 and `lo`
 #pragma unroll 1
       for (int c = 0; c < BN / 2; c += 64) {
-        uint32_t r[64];
-        tmem_ld_32x32(taddr + c, reinterpret_cast<uint32_t(&)[32]>(r[0]));
-        tmem_ld_32x32(taddr + c + 32, reinterpret_cast<uint32_t(&)[32]>(r[32]));
         if (d0) {
           stage_in(stg, lane, dnext);
           if (c + 64 < BN / 2) load_rows(d0 + c + 64, p.ldd, rows, (int)p.ldd - n0 - c - 64, lane, dnext);
-          __syncwarp();
         }
-        tmem_ld_wait();
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          uint4 dv = make_uint4(0, 0, 0, 0);
-          if (d0) dv = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16));
-          const __half2* dh = reinterpret_cast<const __half2*>(&dv);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 df = __half22float2(dh[e]);
-            r[8 * q + 2 * e] = __float_as_uint(fmaf(beta, df.x, alpha * __uint_as_float(r[8 * q + 2 * e])));
-            r[8 * q + 2 * e + 1] = __float_as_uint(fmaf(beta, df.y, alpha * __uint_as_float(r[8 * q + 2 * e + 1])));
-          }
+        if (TWO) {
+          stage_in(stg2, lane, lnext);
+          if (c + 64 < BN / 2) load_rows(p.D2 + (d0 - p.D) + c + 64, p.ldd, rows, (int)p.ldd - n0 - c - 64, lane, lnext);
         }
         __syncwarp();
-        if (MODE == 1) {
-          uint4 v[8];
-          load_rows(p.D2 + (d0 - p.D) + c, p.ldd, rows, (int)p.ldd - n0 - c, lane, v);
-          stage_in(stg, lane, v);
-          __syncwarp();
+        // 32 columns at a time: 64 of them spill beside the rows that are on their way, and next to this much shared memory there is no L1
+        // for that (4 x 2048 x 8192 1826 instead of 1578 us); in narrow tiles they fit and are no gain (2 x 300 x 700 145 instead of 130 us).
+        // A lane's row of the staging areas is its own until the flush: results take the place of the summands that they were made of.
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + c + 32 * h, r);
+          tmem_ld_wait();
+          const int col = n0 + c + 32 * h;
+          const int on = MODE == MODE_SUM || MODE == MODE_DIAG ? row0 + lane - col : -1;      // the diagonal among the 32
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint4 dv = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16));
-            const __half2* dh = reinterpret_cast<const __half2*>(&dv);
+          for (int q = 0; q < 4; ++q) {
+            const int at = lane * 128 + (((4 * h + q) ^ (lane & 7)) * 16);
+            uint4 dv = make_uint4(0, 0, 0, 0), lv = make_uint4(0, 0, 0, 0);
+            if (d0) dv = *reinterpret_cast<const uint4*>(stg + at);
+            if (TWO) lv = *reinterpret_cast<const uint4*>(stg2 + at);
+            const __half2 *dh = reinterpret_cast<const __half2*>(&dv), *lh = reinterpret_cast<const __half2*>(&lv);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float2 df = __half22float2(dh[e >> 1]);
-              float& x = reinterpret_cast<float&>(r[8 * q + e]);
-              x = fmaf(p.beta2, e & 1 ? df.y : df.x, x);
+              const float2 df = __half22float2(dh[e >> 1]), lf = __half22float2(lh[e >> 1]);
+              float x = fmaf(beta, e & 1 ? df.y : df.x, alpha * __uint_as_float(r[8 * q + e]));
+              if (TWO) x = fmaf(p.beta2, e & 1 ? lf.y : lf.x, x);
+              if (MODE == MODE_SUM || MODE == MODE_DIAG) x += on == 8 * q + e ? p.diag : 0.f;
+              r[8 * q + e] = none ? 0u : __float_as_uint(x);
+            }
+            if (MODE == MODE_SPLIT) {
+              const uint4 o = pack8<__half2>(r + 8 * q);
+              const __half2* hi = reinterpret_cast<const __half2*>(&o);
+              uint4 w;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                reinterpret_cast<__half2*>(&w)[e] = left_over(hi[e], __uint_as_float(r[8 * q + 2 * e]), __uint_as_float(r[8 * q + 2 * e + 1]));
+              *reinterpret_cast<uint4*>(stg + at) = o;
+              *reinterpret_cast<uint4*>(stg2 + at) = w;
+            } else if (p.out == OUT_F16) {
+              *reinterpret_cast<uint4*>(stg + at) = pack8<__half2>(r + 8 * q);
+            } else if (p.out == OUT_BF16) {
+              *reinterpret_cast<uint4*>(stg + at) = pack8<__nv_bfloat162>(r + 8 * q);
             }
           }
-          __syncwarp();
-        }
-        if (none) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) r[e] = 0;
-        }
-        if (MODE != 0) {                                       // rows start at multiples of 32, columns of 64
-          const int on = row0 - n0 - c;
-          if (on == 0) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) if (e == lane) r[e] = __float_as_uint(__uint_as_float(r[e]) + p.diag);
-          } else if (on == 32) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) if (e == lane) r[32 + e] = __float_as_uint(__uint_as_float(r[32 + e]) + p.diag);
-          }
-        }
-        if (p.out == OUT_F32) {
-          store_f32(reinterpret_cast<float*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c, p.ldc, rows, p.N - n0 - c, lane, r);
+          if (p.out == OUT_F32)
+            store_f32(reinterpret_cast<float*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + col, p.ldc, rows, p.N - col, lane, r);
+          if (p.symmetric && tn < tm * (256 / BN))             // the result's other half
+            store_transposed(reinterpret_cast<__half*>(p.C) + (long long)b * p.c_batch + (long long)col * p.ldc + row0, p.ldc, p.N - col,
+                             (int)p.ldc - row0, lane, r);
           __syncwarp();                                        // the next load is one of the whole warp
-        } else {
-          if (p.out == OUT_F16) stage_out<__half2>(stg, lane, r);
-          else stage_out<__nv_bfloat162>(stg, lane, r);
-          __syncwarp();
-          uint16_t* out = reinterpret_cast<uint16_t*>(p.C) + (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c;
+        }
+        if (p.out != OUT_F32) {
+          const long long at = (long long)b * p.c_batch + (long long)row0 * p.ldc + n0 + c;
+          uint16_t* out = reinterpret_cast<uint16_t*>(p.C) + at;
           if ((p.ldc & 7) == 0) flush_lines(stg, lane, out, p.ldc, rows, (int)p.ldc - n0 - c);
           else flush_ragged(stg, lane, out, p.ldc, rows, p.N - n0 - c);
-          if (p.symmetric && tn < tm * (256 / BN))
-            store_transposed(reinterpret_cast<__half*>(p.C) + (long long)b * p.c_batch + (long long)(n0 + c) * p.ldc + row0, p.ldc, p.N - n0 - c,
-                             (int)p.ldc - row0, lane, r);
+          if (MODE == MODE_SPLIT) flush_lines(stg2, lane, reinterpret_cast<uint16_t*>(p.lo) + at, p.ldc, rows, (int)p.ldc - n0 - c);
           __syncwarp();
         }
       }
@@ -455,10 +472,11 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_squares_kernel(const T* __res
   if (threadIdx.x == 0) partial[(long long)blockIdx.y * NORM_BLOCKS + blockIdx.x] = sum;
 }
 
-// x [rows, ld] = f16(scale g / |g|), norm[b] = |g|
+// x [rows, ld] = f16(scale g / |g|), norm[b] = |g|; lo (or null): what the rounding leaves
 template <class T>
 __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restrict__ g, int rows, int cols, const double* __restrict__ partial,
-                                                              int parts, float scale, __half* __restrict__ x, int ld, double* __restrict__ norm) {
+                                                              int parts, float scale, __half* __restrict__ x, __half* __restrict__ lo, int ld,
+                                                              double* __restrict__ norm) {
   const int b = blockIdx.y;
   double v = 0;
   for (int i = threadIdx.x; i < parts; i += CAST_THREADS) v += partial[(long long)b * NORM_BLOCKS + i];
@@ -471,6 +489,7 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
   const float f0 = (float)ldexp(mant, e / 2), f1 = (float)ldexp(1.0, e - e / 2);
   const T* src = g + (long long)b * rows * cols;
   __half* dst = x + (long long)b * rows * ld;
+  __half* rest = lo ? lo + (long long)b * rows * ld : nullptr;
   const long long n = (long long)rows * cols, step = (long long)gridDim.x * CAST_THREADS;
   if (ld == cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {      // no padding: eight elements at a time
     constexpr int LOADS = 8 * (int)sizeof(T) / 16, UNROLL = sizeof(T) == 4 ? 2 : 4;
@@ -486,19 +505,28 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
       for (int k = 0; k < UNROLL; ++k) {
         if (i + k * step < nv) {
           const T* t = reinterpret_cast<const T*>(&raw[k][0]);
-          uint4 o;
-          __half2* h = reinterpret_cast<__half2*>(&o);
+          uint4 o, q;
+          __half2 *h = reinterpret_cast<__half2*>(&o), *l = reinterpret_cast<__half2*>(&q);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(to_f32(t[2 * j]) * f0 * f1, to_f32(t[2 * j + 1]) * f0 * f1);
+          for (int j = 0; j < 4; ++j) {
+            const float a = to_f32(t[2 * j]) * f0 * f1, c = to_f32(t[2 * j + 1]) * f0 * f1;
+            h[j] = __floats2half2_rn(a, c);
+            l[j] = left_over(h[j], a, c);
+          }
           reinterpret_cast<uint4*>(dst)[i + k * step] = o;
+          if (rest) reinterpret_cast<uint4*>(rest)[i + k * step] = q;
         }
       }
     }
     return;
   }
   for (int r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += CAST_THREADS)
-      dst[(long long)r * ld + c] = __float2half_rn(to_f32(src[(long long)r * cols + c]) * f0 * f1);
+    for (int c = threadIdx.x; c < cols; c += CAST_THREADS) {
+      const float v = to_f32(src[(long long)r * cols + c]) * f0 * f1;
+      const __half h = __float2half_rn(v);
+      dst[(long long)r * ld + c] = h;
+      if (rest) rest[(long long)r * ld + c] = __float2half_rn(v - __half2float(h));
+    }
 }
 
 // ------------------------------------------------------------------ few rows or columns: everything on chip
@@ -521,6 +549,7 @@ struct SmallParams {
   const void* in;
   int rows, cols, steps, apply, keep, out, ldd, ranks, slice;      // `slice`: columns of x per CTA, a multiple of 64
   float scale;                 // of the f16 copy
+  __half* lo;                  // what the f16 roundings of x leave, pieces of 8 columns with neighbouring rows side by side (null: not kept)
   __half* maps;                // [steps or 1, batch, d, ldd]
   long long map_stride;
   double* norms;               // written by the forward, read by the derivative (null: 1)
@@ -529,6 +558,8 @@ struct SmallParams {
   float alpha[MAX_STEPS];      // x' = alpha x + M x with M = P + (a - alpha) I
 };
 
+// elements of `lo` per CTA
+__host__ __device__ inline long long small_lo(int d, int slice) { return (long long)((d + 31) / 32 * 32) * slice; }
 __device__ __forceinline__ int small_offset(int row, int col) {      // bytes; of the 16-byte piece that starts at col
   return (col >> 6) * BLOCK_BYTES + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) * 16);
 }
@@ -620,6 +651,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   int ex = 0;
   const double mant = frexp(f, &ex);
   const float f0 = (float)ldexp(mant, ex / 2), f1 = (float)ldexp(1.0, ex - ex / 2);      // two factors: no finite norm leaves their range
+  uint4* lo = p.lo ? reinterpret_cast<uint4*>(p.lo + blockIdx.x * small_lo(d, p.slice)) : nullptr;
+  const int lo_rows = (d + 31) / 32 * 32;
   // pieces of 8 columns of x, neighbouring threads on neighbouring memory; four of them in flight
   const int pieces = Lp / 8, all = d * pieces;
   for (int i = all + tid; i < SMALL_D * pieces; i += SMALL_THREADS)      // rows beyond the matrix
@@ -650,11 +683,18 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + k * SMALL_THREADS;
       const int row = wide ? i / pieces : i % d, col = (wide ? i % pieces : i / d) * 8;
-      uint4 o;
-      __half2* h = reinterpret_cast<__half2*>(&o);
+      uint4 o, w;
+      __half2 *h = reinterpret_cast<__half2*>(&o), *l = reinterpret_cast<__half2*>(&w);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(x[k][2 * e] * f0 * f1, x[k][2 * e + 1] * f0 * f1);
-      if (i < all) *reinterpret_cast<uint4*>(sx + small_offset(row, col)) = o;
+      for (int e = 0; e < 4; ++e) {
+        const float a = x[k][2 * e] * f0 * f1, c = x[k][2 * e + 1] * f0 * f1;
+        h[e] = __floats2half2_rn(a, c);
+        l[e] = left_over(h[e], a, c);
+      }
+      if (i < all) {
+        *reinterpret_cast<uint4*>(sx + small_offset(row, col)) = o;
+        if (lo) lo[(col >> 3) * lo_rows + row] = w;
+      }
     }
   }
   float last = 1.f / p.scale;                                  // brings the last product to the result's scale
@@ -686,7 +726,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   constexpr int KEPT = SMALL_D * SMALL_D / 8 / SMALL_THREADS;
   const int kept_pieces = p.ldd / 8;
   auto map_of = [&](int k) { return p.maps + k * p.map_stride + (long long)b * d * p.ldd; };
-  uint4 next[KEPT];
+  uint4 next[KEPT];                                            // (or, in the forward, what the rounding of x left)
   auto fetch = [&](int k) {
     const __half* map = map_of(p.steps - 1 - k);
 #pragma unroll
@@ -805,9 +845,16 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
         const int r = i / kept_pieces, q = i % kept_pieces;
         reinterpret_cast<uint4*>(map_of(k) + r * p.ldd)[q] = *reinterpret_cast<const uint4*>(sp + small_offset(r, q * 8));
       }
+    // what the rounding of x left, of the columns that come first: this thread's own stores, or those before the first product
+    const bool end = k == p.steps - 1, has_lo = lo && row < d && !end;
+    static_assert(KEPT == 4, "32 columns of the low half");
+    auto fetch_lo = [&](int col) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) next[q] = has_lo ? lo[((col >> 3) + q) * lo_rows + row] : make_uint4(0, 0, 0, 0);
+    };
+    if (!p.apply && part * 32 < Lp) fetch_lo(part * 32);
     wait();
-    const bool end = k == p.steps - 1;
-    const float fin = end ? last : 1.f;
+    const float fx = (end ? last : 1.f) * alpha, fr = (end ? last : 1.f) / X_SCALE;
     for (int col = rows_here ? part * 32 : Lp; col < Lp; col += 128) {
       uint32_t r[32];
       tmem_ld_32x32(lanes + col, r);
@@ -816,15 +863,33 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint4 o = *reinterpret_cast<const uint4*>(sx + small_offset(row, col + 8 * q));
-        const __half* h = reinterpret_cast<const __half*>(&o);
+        const __half *h = reinterpret_cast<const __half*>(&o), *l = reinterpret_cast<const __half*>(&next[q]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * q + e] = fin * fmaf(alpha, __half2float(h[e]), __uint_as_float(r[8 * q + e]) * (1.f / X_SCALE));
+        for (int e = 0; e < 8; ++e) {
+          v[8 * q + e] = fmaf(fx, __half2float(h[e]), __uint_as_float(r[8 * q + e]) * fr);
+          if (!p.apply) v[8 * q + e] = fmaf(NS_A, __half2float(l[e]), v[8 * q + e]);
+        }
       }
+      if (!p.apply && col + 128 < Lp) fetch_lo(col + 128);
       if (none && end) {
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = 0.f;
       }
-      if (!end) {
+      if (!end && has_lo && k < p.steps - 2) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint4 o, w;
+          __half2 *h = reinterpret_cast<__half2*>(&o), *l = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = v[8 * q + 2 * e], c = v[8 * q + 2 * e + 1];
+            h[e] = __floats2half2_rn(a, c);
+            l[e] = left_over(h[e], a, c);
+          }
+          *reinterpret_cast<uint4*>(sx + small_offset(row, col + 8 * q)) = o;
+          lo[((col >> 3) + q) * lo_rows + row] = w;
+        }
+      } else if (!end) {
         store_small(sx, row, col, v);
       } else if (row < d && wide && p.out == OUT_BF16 && p.cols % 8 == 0) {
         uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.y) + (long long)b * n + row * p.cols + c0 + col);
@@ -867,11 +932,15 @@ static bool is_small(int batch, int rows, int cols) {
 static constexpr int small_smem(int slice, int ranks) { return (slice / 64 + (ranks > 1 ? 6 : 4)) * BLOCK_BYTES + 2048; }
 static_assert(small_smem(SMALL_L, SMALL_RANKS) + 256 <= 227 * 1024, "shared memory of an SM");
 
+static void small_split(int rows, int cols, int* ranks, int* slice) {
+  const int L = rows < cols ? cols : rows;
+  *ranks = 1;
+  while (*ranks * SMALL_L < L) *ranks *= 2;
+  *slice = ((L + *ranks - 1) / *ranks + 63) / 64 * 64;
+}
+
 static int launch_small(SmallParams p, int f32, int batch, cudaStream_t stream) {
-  const int L = p.rows < p.cols ? p.cols : p.rows;
-  p.ranks = 1;
-  while (p.ranks * SMALL_L < L) p.ranks *= 2;
-  p.slice = ((L + p.ranks - 1) / p.ranks + 63) / 64 * 64;
+  small_split(p.rows, p.cols, &p.ranks, &p.slice);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(batch * p.ranks);
   cfg.blockDim = dim3(SMALL_THREADS);
@@ -940,6 +1009,14 @@ struct Maps {
   }
 };
 
+struct ProductKernel {
+  void (*kernel)(const CUtensorMap, const CUtensorMap, const Params);
+  int smem;
+};
+template <int BN, int MODE> constexpr ProductKernel product_kernel() { return {ns_product_kernel<BN, MODE>, Tile<BN, MODE>::SMEM}; }
+static const ProductKernel wide_kernels[4] = {product_kernel<256, 0>(), product_kernel<256, 1>(), product_kernel<256, 2>(), product_kernel<256, 3>()};
+static const ProductKernel narrow_kernels[4] = {product_kernel<128, 0>(), product_kernel<128, 1>(), product_kernel<128, 2>(), product_kernel<128, 3>()};
+
 static int prepare_device(int* n_sm) {
   static std::mutex mu;
   static unsigned long long attr_mask = 0;
@@ -952,13 +1029,10 @@ static int prepare_device(int* n_sm) {
   if (bound_dev != dev) { if (cudaSetDevice(dev) != cudaSuccess) return 301; bound_dev = dev; }
   std::lock_guard<std::mutex> lock(mu);
   if (!(attr_mask >> dev & 1ull)) {
-    if (cudaFuncSetAttribute(ns_product_kernel<256, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<128, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<256, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<256, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<256>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_product_kernel<128, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<128>::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(ns_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_L, SMALL_RANKS)) != cudaSuccess ||
+    for (int k = 0; k < 4; ++k)
+      if (cudaFuncSetAttribute(wide_kernels[k].kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, wide_kernels[k].smem) != cudaSuccess ||
+          cudaFuncSetAttribute(narrow_kernels[k].kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, narrow_kernels[k].smem) != cudaSuccess) return 302;
+    if (cudaFuncSetAttribute(ns_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_L, SMALL_RANKS)) != cudaSuccess ||
         cudaFuncSetAttribute(ns_small_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_L, SMALL_RANKS)) != cudaSuccess) return 302;
     cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
     attr_mask |= 1ull << dev;
@@ -972,6 +1046,7 @@ struct Out {
   int kind;
   long long ld;
   const double *num, *den;
+  void* lo = nullptr;          // with D2: takes what the rounding of C leaves
 };
 
 // C [M, N] = alpha op(A) op(B) + beta D (+ beta2 D2, with the layout of D) + diag I over the batch (symmetric: C and D are, and only f16)
@@ -984,6 +1059,7 @@ static int product(Maps& maps, int batch, int M, int N, int K, const Mat& A, boo
   if (D) { p.D = (const __half*)D->ptr; p.ldd = D->ld; p.d_batch = D->ld * D->rows; }
   if (D2) { p.D2 = (const __half*)D2->ptr; p.beta2 = beta2; }
   p.diag = diag;
+  p.lo = (__half*)o.lo;
   p.C = o.C; p.out = o.kind; p.ldc = o.ld; p.c_batch = o.ld * M; p.num = o.num; p.den = o.den; p.status = status;
   p.symmetric = symmetric;
   p.tiles_m = (M + 2 * BM - 1) / (2 * BM);
@@ -1008,51 +1084,54 @@ static int product(Maps& maps, int batch, int M, int N, int K, const Mat& A, boo
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (int)(tiles[narrow] < pairs ? tiles[narrow] : pairs));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = narrow ? Tile<128>::SMEM : Tile<256>::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // the prologue overlaps the product before
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const int mode = D2 ? 1 : diag != 0.f ? 2 : 0;               // a kernel of its own each: with all of it the epilogue spills
-  auto* const kernel = narrow ? (mode == 0 ? ns_product_kernel<128, 0> : mode == 1 ? ns_product_kernel<128, 1> : ns_product_kernel<128, 2>)
-                              : (mode == 0 ? ns_product_kernel<256, 0> : mode == 1 ? ns_product_kernel<256, 1> : ns_product_kernel<256, 2>);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, copyA, *mapB, p);
+  const int mode = o.lo ? MODE_SPLIT : D2 ? MODE_SUM : diag != 0.f ? MODE_DIAG : MODE_PLAIN;
+  const ProductKernel& k = (narrow ? narrow_kernels : wide_kernels)[mode];
+  cfg.dynamicSmemBytes = k.smem;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k.kernel, copyA, *mapB, p);
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
-// r (f16) -> beta r + alpha M r (r M^T of a tall one), or with the transpose of M: into f16 or, at the end, into the caller's tensor
+// r (f16) -> beta r + alpha M r (r M^T of a tall one), or with the transpose of M, + beta2 D2: into f16 or, at the end, into the caller's
+// tensor
 static int apply(Maps& maps, int batch, int rows, int cols, const Mat& r, const Mat& M, bool transposed, float alpha, float beta, const Out& o, int* status,
-                 int n_sm, cudaStream_t stream) {
-  if (rows <= cols) return product(maps, batch, rows, cols, rows, M, transposed, r, true, alpha, beta, &r, o, false, status, n_sm, stream);
-  return product(maps, batch, rows, cols, cols, r, false, M, transposed, alpha, beta, &r, o, false, status, n_sm, stream);
+                 int n_sm, cudaStream_t stream, const Mat* D2 = nullptr, float beta2 = 0.f) {
+  if (rows <= cols) return product(maps, batch, rows, cols, rows, M, transposed, r, true, alpha, beta, &r, o, false, status, n_sm, stream, D2, beta2);
+  return product(maps, batch, rows, cols, cols, r, false, M, transposed, alpha, beta, &r, o, false, status, n_sm, stream, D2, beta2);
 }
 
+// Matrices of `bytes` each whose two passes run together: about 48 MB, so that the second reads them from L2 (126 MB) while the f16
+// copies are written.
+static int cast_group(long long bytes) { return (int)(bytes > (48ll << 20) ? 1 : (48ll << 20) / bytes); }
+
 template <class T>
-static int cast(const T* g, int batch, int rows, int cols, double* partial, float scale, __half* x, int ld, double* norm, int n_sm,
+static int cast(const T* g, int batch, int rows, int cols, double* partial, float scale, __half* x, __half* lo, int ld, double* norm, int n_sm,
                 cudaStream_t stream) {
   const long long n = (long long)rows * cols, bytes = n * (long long)sizeof(T);
   auto blocks = [](long long work, long long each, int most) { const long long w = (work + each - 1) / each; return (int)(w < most ? w : most); };
   const int parts = blocks(n, 8192, NORM_BLOCKS);
   const int casts = ld == cols ? blocks(n, 4096, 8 * n_sm) : blocks(rows, 1, 8 * n_sm);
-  // groups of about 48 MB: the second pass reads them from L2 (126 MB) while the f16 copies are written
-  const int group = (int)(bytes > (48ll << 20) ? 1 : (48ll << 20) / bytes);
+  const int group = cast_group(bytes);
   for (int b = 0; b < batch; b += group) {
     const int k = batch - b < group ? batch - b : group;
     double* part = partial + (long long)b * NORM_BLOCKS;
     ns_squares_kernel<T><<<dim3(parts, k), CAST_THREADS, 0, stream>>>(g + b * n, n, part);
-    ns_cast_kernel<T><<<dim3(casts, k), CAST_THREADS, 0, stream>>>(g + b * n, rows, cols, part, parts, scale, x + (long long)b * rows * ld, ld,
-                                                                  norm + b);
+    ns_cast_kernel<T><<<dim3(casts, k), CAST_THREADS, 0, stream>>>(g + b * n, rows, cols, part, parts, scale, x + (long long)b * rows * ld,
+                                                                  lo ? lo + (long long)b * rows * ld : nullptr, ld, norm + b);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
 
-static int cast(const void* g, int f32, int batch, int rows, int cols, double* partial, float scale, void* x, int ld, double* norm, int n_sm,
+static int cast(const void* g, int f32, int batch, int rows, int cols, double* partial, float scale, void* x, void* lo, int ld, double* norm, int n_sm,
                 cudaStream_t stream) {
-  if (f32) return cast<float>((const float*)g, batch, rows, cols, partial, scale, (__half*)x, ld, norm, n_sm, stream);
-  return cast<__nv_bfloat16>((const __nv_bfloat16*)g, batch, rows, cols, partial, scale, (__half*)x, ld, norm, n_sm, stream);
+  if (f32) return cast<float>((const float*)g, batch, rows, cols, partial, scale, (__half*)x, (__half*)lo, ld, norm, n_sm, stream);
+  return cast<__nv_bfloat16>((const __nv_bfloat16*)g, batch, rows, cols, partial, scale, (__half*)x, (__half*)lo, ld, norm, n_sm, stream);
 }
 
 }  // namespace ns
@@ -1100,7 +1179,7 @@ static int make_plan(int rows, int cols, int steps, Group* g) {
 }
 
 struct Scratch {
-  void *x[2], *gram, *h, *p;
+  void *x[2], *lo, *gram, *h, *p;
   double *partial, *norm;
   long long bytes;
   int ld, d, ldd;
@@ -1110,7 +1189,7 @@ struct Scratch {
     const long long xb = up((long long)batch * rows * ld * 2), gb = up((long long)batch * d * ldd * 2);
     uint8_t* s = (uint8_t*)base;
     auto take = [&](long long n) { uint8_t* r = s; s += n; return r; };
-    x[0] = take(xb); x[1] = take(xb);
+    x[0] = take(xb); x[1] = take(xb); lo = take(xb);
     gram = take(gb); h = take(gb); p = take(gb);
     partial = (double*)take(up((long long)batch * NORM_BLOCKS * 8));
     norm = (double*)take(up((long long)batch * 8));
@@ -1123,7 +1202,24 @@ struct Scratch {
 
 // Bytes of the scratch area for `batch` matrices [rows, cols] (256-byte aligned base).
 extern "C" long long dttt_newton_schulz_scratch(int batch, int rows, int cols) {
-  return dttt::ns::is_small(batch, rows, cols) ? 0 : dttt::ns::Scratch(nullptr, batch, rows, cols).bytes;
+  using namespace dttt::ns;
+  if (!is_small(batch, rows, cols)) return Scratch(nullptr, batch, rows, cols).bytes;
+  int ranks, slice;
+  small_split(rows, cols, &ranks, &slice);
+  return batch * (long long)ranks * small_lo(rows < cols ? rows : cols, slice) * 2;      // (of the forward)
+}
+
+// Kernels that a forward (`parts` 0) or a part of `parts` groups of the derivative launches.
+extern "C" int dttt_newton_schulz_launches(int f32, int batch, int rows, int cols, int steps, int parts) {
+  using namespace dttt::ns;
+  if (batch <= 0 || rows <= 0 || cols <= 0 || steps <= 0 || steps > MAX_STEPS) return 0;
+  if (is_small(batch, rows, cols)) return 1;
+  const int group = cast_group((long long)rows * cols * (f32 ? 4 : 2)), casts = 2 * ((batch + group - 1) / group);
+  if (parts) return casts + parts;
+  Group plan[MAX_STEPS];
+  int n = casts;
+  for (int k = make_plan(rows, cols, steps, plan) - 1; k >= 0; --k) n += plan[k].steps == 1 ? 3 : 7;
+  return n;
 }
 
 // Groups of iterations, each with one d x d matrix of the linear map.
@@ -1144,16 +1240,17 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   const int groups = make_plan(rows, cols, steps, plan);
   if (is_small(batch, rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, 1, 0, X_SCALE, (__half*)kept, (long long)batch * small * ld, norms, y, status};
+    SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, 1, 0, X_SCALE, steps > 1 ? (__half*)scratch : nullptr, (__half*)kept, (long long)batch * small * ld,
+                     norms, y, status};
     for (int k = 0; k < steps; ++k) p.alpha[k] = plan[k].alpha;
     return launch_small(p, f32, batch, stream);
   }
   const Scratch s(scratch, batch, rows, cols);
   const int d = s.d, ldd = s.ldd;
-  if (int r = cast(g, f32, batch, rows, cols, s.partial, X_SCALE, s.x[0], s.ld, norms, n_sm, stream)) return r;
+  if (int r = cast(g, f32, batch, rows, cols, s.partial, X_SCALE, s.x[0], groups > 1 ? s.lo : nullptr, s.ld, norms, n_sm, stream)) return r;
   const bool wide = rows <= cols;
   Maps maps;
-  const Mat G = {s.gram, d, d, ldd}, H = {s.h, d, d, ldd}, P1 = {s.p, d, d, ldd};
+  const Mat G = {s.gram, d, d, ldd}, H = {s.h, d, d, ldd}, P1 = {s.p, d, d, ldd}, Lo = {s.lo, rows, cols, s.ld};
   auto square = [&](const Mat& A, const Mat& B, float alpha, float beta, const Mat& D, const Mat& C, const Mat* D2 = nullptr, float beta2 = 0.f,
                     float diag = 0.f) {
     const Out o = {const_cast<void*>(C.ptr), OUT_F16, ldd, nullptr, nullptr};
@@ -1175,8 +1272,11 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
     }
     const bool last = k == groups - 1;
     const float f = last ? 1.f / X_SCALE : 1.f;
-    const Out ox = {last ? y : s.x[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : s.ld, nullptr, nullptr};
-    if (int r = apply(maps, batch, rows, cols, X, M, false, f / X_SCALE, f * plan[k].alpha, ox, status, n_sm, stream)) return r;
+    // The last group goes without the low half: what x_k lost grows only by this group's factor there (3.4445, or 11.9 of a pair, times
+    // 2.8e-4), and a third of the traffic is saved.
+    const Out ox = {last ? y : s.x[(k + 1) & 1], last ? OUT_BF16 : OUT_F16, last ? cols : s.ld, nullptr, nullptr, k < groups - 2 ? s.lo : nullptr};
+    const float beta2 = plan[k].alpha + plan[k].shift;
+    if (int r = apply(maps, batch, rows, cols, X, M, false, f / X_SCALE, f * plan[k].alpha, ox, status, n_sm, stream, last ? nullptr : &Lo, beta2)) return r;
   }
   return 0;
 }
@@ -1207,13 +1307,13 @@ extern "C" int dttt_newton_schulz_apply(const void* r_in, int f32, int batch, in
   if (is_small(batch, rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
     const long long stride = (long long)batch * small * ld;
-    SmallParams p = {r_in, rows, cols, count, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, 1, 0, R_SCALE, (__half*)const_cast<void*>(kept) + first * stride,
-                     stride, const_cast<double*>(norms), out, status};
+    SmallParams p = {r_in, rows, cols, count, 1, 1, out_f32 ? OUT_F32 : OUT_BF16, ld, 1, 0, R_SCALE, nullptr,
+                     (__half*)const_cast<void*>(kept) + first * stride, stride, const_cast<double*>(norms), out, status};
     for (int k = 0; k < count; ++k) p.alpha[k] = plan[first + k].alpha;
     return launch_small(p, f32, batch, stream);
   }
   const Scratch s(scratch, batch, rows, cols);
-  if (int r = cast(r_in, f32, batch, rows, cols, s.partial, R_SCALE, s.x[0], s.ld, s.norm, n_sm, stream)) return r;
+  if (int r = cast(r_in, f32, batch, rows, cols, s.partial, R_SCALE, s.x[0], nullptr, s.ld, s.norm, n_sm, stream)) return r;
   Maps maps;
   for (int i = 0; i < count; ++i) {
     const int k = upto - 1 - i;

@@ -855,6 +855,7 @@ def unmask(ids, known, held, tokens, logp, priority, quota, allowed, sure):
 # =============================================================================== Newton-Schulz family
 _lib.register("dttt_newton_schulz_scratch", _ll, [_i, _i, _i])
 _lib.register("dttt_newton_schulz_groups", _i, [_i, _i, _i])
+_lib.register("dttt_newton_schulz_launches", _i, [_i, _i, _i, _i, _i, _i])
 _lib.register("dttt_newton_schulz", _i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp])
 _lib.register("dttt_newton_schulz_part", _i, [_i, _i, _i, _i])
 _lib.register("dttt_newton_schulz_apply", _i, [_vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp])
@@ -873,20 +874,19 @@ def newton_schulz(g, steps, keep):
     holds the matrix of every group of iterations with ``keep``, else it is scratch."""
     global LAUNCHES
     B, rows, cols = g.shape
-    d, dev = min(rows, cols), g.device
+    d, dev, f32 = min(rows, cols), g.device, int(g.dtype == torch.float32)
     y = torch.empty_like(g, dtype=torch.bfloat16)
     norms = torch.empty(B, dtype=torch.float64, device=dev)
     l = _lib.lib()
-    size = l.dttt_newton_schulz_scratch(B, rows, cols)                   # 0: small matrices, one launch that needs none
+    launches = l.dttt_newton_schulz_launches(f32, B, rows, cols, steps, 0)
+    size = l.dttt_newton_schulz_scratch(B, rows, cols)
     scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     polys = None
-    if keep or size:
+    if keep or launches > 1:                                             # (small matrices take one launch and hold theirs on chip)
         polys = torch.empty((l.dttt_newton_schulz_groups(rows, cols, steps) if keep else 1, B, d, -(-d // 8) * 8), dtype=torch.float16, device=dev)
-    _launch("newton_schulz", l.dttt_newton_schulz, dev, g.data_ptr(), int(g.dtype == torch.float32), B, rows, cols, steps,
-            scratch.data_ptr() if size else None, None if polys is None else polys.data_ptr(), int(keep), norms.data_ptr(), y.data_ptr(),
-            _status_word(dev))
-    if size:
-        LAUNCHES += 1 + 3 * steps
+    _launch("newton_schulz", l.dttt_newton_schulz, dev, g.data_ptr(), f32, B, rows, cols, steps, None if scratch is None else scratch.data_ptr(),
+            None if polys is None else polys.data_ptr(), int(keep), norms.data_ptr(), y.data_ptr(), _status_word(dev))
+    LAUNCHES += launches - 1
     return y, norms, polys
 
 
@@ -897,17 +897,17 @@ def newton_schulz_apply(r, norms, polys, steps, out_dtype):
     B, rows, cols = r.shape
     dev, upto = r.device, polys.shape[0]
     l = _lib.lib()
-    size = l.dttt_newton_schulz_scratch(B, rows, cols)
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    over = norms.data_ptr()
+    scratch, over = None, norms.data_ptr()
     while True:
-        first = l.dttt_newton_schulz_part(rows, cols, steps, upto)
+        first, f32 = l.dttt_newton_schulz_part(rows, cols, steps, upto), int(r.dtype == torch.float32)
+        launches = l.dttt_newton_schulz_launches(f32, B, rows, cols, steps, upto - first)
+        if launches > 1 and scratch is None:
+            scratch = torch.empty(l.dttt_newton_schulz_scratch(B, rows, cols), dtype=torch.uint8, device=dev)
         out = torch.empty_like(r, dtype=torch.float32 if first else out_dtype)
-        _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), int(r.dtype == torch.float32), B, rows, cols, steps,
-                first, upto, scratch.data_ptr() if size else None, polys.data_ptr(), over, out.data_ptr(), int(out.dtype == torch.float32),
+        _launch("newton_schulz_apply", l.dttt_newton_schulz_apply, dev, r.data_ptr(), f32, B, rows, cols, steps, first, upto,
+                None if scratch is None else scratch.data_ptr(), polys.data_ptr(), over, out.data_ptr(), int(out.dtype == torch.float32),
                 _status_word(dev))
-        if size:
-            LAUNCHES += 1 + upto - first
+        LAUNCHES += launches - 1
         if first == 0:
             return out
         r, upto, over = out, first, None

@@ -11,6 +11,8 @@ alike, takes it up.
   2^-8 + 15 * 3.4445 * 2^-11 = 2.9e-2.
 
 The derivative applies the steps' products with the same P and f16 roundings: the same bounds."""
+import math
+
 import pytest
 import torch
 
@@ -262,3 +264,51 @@ def test_derivative_of_many_steps(shape, steps):
     leaf = torch.zeros_like(full).requires_grad_(True)
     gx, = torch.autograd.grad(newton_schulz(leaf, steps), leaf, gy)
     assert gx.eq(0).all()
+
+
+# ------------------------------------------------------------------------------------------------- fewer tokens than rows
+@pytest.mark.parametrize("shape", [(64, 100), (2, 128, 256), (256, 128), (3, 100, 900), (1024, 64), (128, 2048), (260, 300), (2, 509, 1283), (1283, 509),
+                                   (512, 2048), (1200, 600)])
+@pytest.mark.parametrize("tokens", [1, 8, 0.25, 0.5, 1.0])
+@pytest.mark.parametrize("steps", [2, 5, 8])
+def test_matrices_of_low_rank(shape, tokens, steps):
+    """The gradient of a write has at most the rank of its chunk's tokens.  Roundings of G, of P and of x inside P x stay in the row or
+    the column space of x: they turn singular vectors, by at most |P| / |a + P| <= 4.4 of themselves a step, and nothing amplifies
+    that: the bound above.  What lies outside both spaces grows 3.4445-fold a step, and that is only what x loses when it is
+    stored: half a step of 2^-11 of what a step of 2^-11 leaves, evenly spread both (2^-22 / 3), and the few 2^-24 of f32 arithmetic,
+    1e-7 of |x_0| = 1 together, relative to a result of at least 0.68 (one singular value); a factor of two over the mean square.
+    The last group takes x in one half: 2.8e-4 of it, 3.4445-fold (11.9-fold by a pair), independent of the rest."""
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    d = min(shape[-2:])
+    t = tokens if isinstance(tokens, int) else int(tokens * d)
+    gen = torch.Generator(device="cuda").manual_seed(sum(shape) + t)
+    h = torch.randn(*shape[:-2], t, shape[-2], generator=gen, device="cuda")
+    e = torch.randn(*shape[:-2], t, shape[-1], generator=gen, device="cuda") * torch.rand(*shape[:-2], t, 1, generator=gen, device="cuda")
+    gy = torch.randn(*shape, generator=gen, device="cuda").to(torch.bfloat16)
+    lost = plan_of(*shape[-2:], steps)[-1][0]
+    for g in (h.mT @ e * 1e-3, (h.mT @ e * 1e-3).to(torch.bfloat16)):
+        want, norms, polys = ref.newton_schulz(g, steps, torch.float64)
+        before = (ref.newton_schulz(g, steps - lost, torch.float64)[0].norm() / want.norm()).item()
+        bound = math.hypot(BOUND, 2.0 ** -11 / 3 ** 0.5 * 3.4445 ** lost * before) + 2 * 1e-7 * 3.4445 ** steps / 0.68
+        leaf = g.clone().requires_grad_(True)
+        y = newton_schulz(leaf, steps)
+        assert newton_schulz(g, steps).equal(y) and off(y, want) <= bound
+        got, = torch.autograd.grad(y, leaf, gy)
+        assert off(got, ref.newton_schulz_apply(gy, norms, polys)) <= bound
+
+
+def test_launches_are_counted():
+    """What the calls say they launch, against the profiler."""
+    from dttt_b200.ops import kernels
+    from torch.profiler import ProfilerActivity, profile
+    for shape in [(2, 64, 100), (3, 129, 300), (1, 512, 1100), (2, 2048, 3100)]:
+        g, gy = make(shape, torch.float32, 1)
+        for steps in (1, 5, 9):
+            y, norms, maps = kernels.newton_schulz(g, steps, True)
+            for call in (lambda: kernels.newton_schulz(g, steps, False), lambda: kernels.newton_schulz_apply(gy, norms, maps, steps, torch.float32)):
+                n = kernels.LAUNCHES
+                with profile(activities=[ProfilerActivity.CUDA]) as prof:
+                    call()
+                    torch.cuda.synchronize()
+                seen = sum(e.count for e in prof.key_averages() if "ns_" in e.key and "kernel" in e.key)
+                assert kernels.LAUNCHES - n == seen, (shape, steps)
