@@ -31,7 +31,7 @@
 //   * middle ones: the chain of products, each of which is one round of tiles whose first loads, store and mirrored store are
 //     not hidden: 3 x 509 x 1283, five steps 167 us and its derivative 53 us, 8 to 11 us a product; programmatic launches start a
 //     product's prologue under the one before (263 -> 230 us).  All of them in one cooperative launch gained nothing.
-//   * d <= 128 and L <= 4096: one CTA or cluster and one launch (below), 21 us for 2 x 128 x 256 and two steps.
+//   * d <= 128 and L <= 4096, most of them (`is_small`): one CTA or cluster and one launch, 23 us for 2 x 128 x 256 and two steps.
 #include "host_check.h"
 #include "ptx_sm100.cuh"
 
@@ -530,17 +530,24 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
 }
 
 // ------------------------------------------------------------------ few rows or columns: everything on chip
-// d <= 128 and L <= 4096: one CTA, or a cluster of up to eight with 512 columns each, holds x [128, L] (transposed when rows > cols), G
+// d <= 128 and L <= 4096 (not all of them: `is_small`): one CTA, or a cluster of up to eight with 512 columns each, holds x [128, L] (transposed when rows > cols), G
 // and P in shared memory and runs all iterations in one launch; what such sizes cost otherwise is launches.  x lies as blocks of 128
 // rows x 64 columns with 128-byte swizzle, which is the K-major operand of G = x x^T and, read with its columns as N, the MN-major
 // one of P x.  Rows and columns beyond the matrix are zero and stay so.  In a cluster each CTA adds up a share of the partial G of
 // all, rounds it and hands it round; P is then formed by everyone.  Also the derivative (`apply`): the kept P of every iteration is
 // read back.  A wait that runs out sets the status word and the kernel goes on to its end, so that no CTA waits for one that left.
-// Five steps with keep and their derivative, here / as products of their own, in us (one matrix; 300 of them):
-//   16 x 64      23 + 15 / 73 + 30                             64 x 256   31 + 21 / 77 + 32
-//   128 x 512    53 + 39 / 89 + 35                             512 x 128  64 + 49 / 89 + 35
-//   64 x 1024    62 + 33 / 96 + 35 (304 + 160 / 824 + 485)     128 x 4096 96 + 41 / 155 + 37 (1985 + 878 / 2600 + 1964)
-//   1024 x 64    70 + 42 / 95 + 33 (348 + 208 / 610 + 265)     4096 x 128 136 + 64 / 158 + 37 (2823 + 1339 / 1869 + 1212)
+// Five steps with keep and their derivative, here / as products of their own, in us (* : where `is_small` sends them to the products):
+//   one matrix                                                                     300 of them
+//   16 x 64      23 + 14 / 65 + 23      64 x 256    35 + 22 / 76 + 27               16 x 64     66 + 39 / 330 + 78
+//   128 x 256    42 + 25 / 81 + 28      128 x 512   65 + 42 / 86 + 29               128 x 512   209 + 135 / 735 + 306
+//   512 x 128    70 + 52 / 86 + 29      64 x 1024   72 + 35 / 91 + 28               64 x 1024   373 + 176 / 1020 + 526
+//   128 x 1024   88 + 44 / 97 + 30      128 x 4096  109 + 44 / 149 + 31             128 x 4096  2374 + 953 / 3554 + 1857
+//   1024 x 64    78 + 44 / 90 + 28      2048 x 128  103 + 53 / 115 + 30             1024 x 64   400 + 221 / 701 + 282
+//   4096 x 16    79 + 40 / 142 + 29     4095 x 127  113 + 53 / 155 + 35             4096 x 128  2425 + 1130 / 2493 + 1246
+//   16 x 601     58 + 31 / 83 + 28      30 x 2049   71 + 36 / 112 + 32              30 x 2049   1463 + 719 / 1871 + 1160
+//   84 x 915   * 124 + 82 / 102 + 34    100 x 701 * 115 + 73 / 95 + 33              84 x 915    648 + 436 / 1286 + 680
+//   127 x 2049 * 136 + 74 / 130 + 35    (16 of 84 x 915 * 126 + 84 / 133 + 58, 32 of them 126 + 85 / 185 + 95)
+//                                                                                  127 x 2049 * 2965 + 1645 / 2637 + 1476
 // Bound by the latency of its three dependent products a step and, with many matrices, by loading x and by the epilogues.
 constexpr int SMALL_D = 128, SMALL_L = 512, SMALL_RANKS = 8, SMALL_THREADS = 512;
 constexpr int BLOCK_BYTES = SMALL_D * 128;                     // 128 rows x 64 f16
@@ -923,11 +930,14 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) ns_small_kernel(const SmallP
   }
 }
 
-// Matrices whose elements come one by one (tall ones, rows that do not start at 16 bytes) take a cluster only where that is made up
-// for: 84 x 915 191 us as against 146 of the products, 17 of them 195 / 196, 300 993 / 1624; tall ones above.
+// Which matrices take one launch: all up to 128 x 512 or 512 x 128, all tall ones up to 4096 x 128, and wide ones up to 128 x 4096 whose
+// rows start at 16 bytes.  The rows of other wide ones beyond 512 columns come element by element into every CTA of a cluster, which is
+// made up for where there are few of them (d <= 64) or where many matrices of at most two CTAs each share the device; so the same
+// matrix may take either way, and round differently, by the size of its batch.
 static bool is_small(int batch, int rows, int cols) {
   const int d = rows < cols ? rows : cols, L = rows < cols ? cols : rows;
-  return d <= SMALL_D && L <= SMALL_L * SMALL_RANKS && (L <= SMALL_L || (rows < cols && (cols % 8 == 0 || batch >= 16)) || (cols < rows && d * L <= SMALL_D * SMALL_L));
+  if (d > SMALL_D || L > SMALL_L * SMALL_RANKS) return false;
+  return L <= SMALL_L || rows > cols || cols % 8 == 0 || d <= 64 || (batch >= 24 && L <= 2 * SMALL_L);
 }
 static constexpr int small_smem(int slice, int ranks) { return (slice / 64 + (ranks > 1 ? 6 : 4)) * BLOCK_BYTES + 2048; }
 static_assert(small_smem(SMALL_L, SMALL_RANKS) + 256 <= 227 * 1024, "shared memory of an SM");

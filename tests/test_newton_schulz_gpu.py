@@ -311,4 +311,18 @@ def test_launches_are_counted():
                     call()
                     torch.cuda.synchronize()
                 seen = sum(e.count for e in prof.key_averages() if "ns_" in e.key and "kernel" in e.key)
+                if not seen:
+                    pytest.skip("no device events from the profiler here")
                 assert kernels.LAUNCHES - n == seen, (shape, steps)
+
+
+@pytest.mark.parametrize("shape,one", [((24, 84, 915), True), ((23, 84, 915), False), ((25, 100, 701), True), ((2, 127, 2049), False), ((40, 3001), True),
+                                       ((2, 65, 601), False), ((3, 64, 601), True), ((4096, 128), True), ((2, 4095, 127), True), ((1500, 128), True),
+                                       ((2, 3000, 50), True), ((4097, 16), False), ((129, 129), False), ((128, 4104), False), ((3, 1, 4095), True)])
+def test_both_sides_of_the_one_launch_rule(shape, one):
+    from dttt_b200.ops import kernels
+    n = kernels.LAUNCHES
+    kernels.newton_schulz(make(shape, torch.float32)[0].reshape(-1, *shape[-2:]), 2, False)
+    assert (kernels.LAUNCHES - n == 1) == one
+    for dtype in (torch.float32, torch.bfloat16):
+        test_direction_and_derivative(shape, dtype, 5)
