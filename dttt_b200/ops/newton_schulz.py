@@ -31,29 +31,41 @@ def _linear(r: torch.Tensor, norms, maps, steps: int, dtype: torch.dtype) -> tor
     return kernels.newton_schulz_apply(_flat(r), norms, maps, steps, dtype).view(r.shape)
 
 
+def _maps(saved, listed: bool):
+    """Norms and maps as ``_run`` gave them, from what a context saved."""
+    norms, *maps = saved
+    return norms, (maps if listed else maps[0])
+
+
 class _Apply(torch.autograd.Function):
     """``_linear`` as a differentiable operation: linear and self-adjoint."""
 
     @staticmethod
-    def forward(ctx, r, norms, maps, steps, dtype):
-        ctx.kept, ctx.dtype = (norms, maps, steps), r.dtype
-        return _linear(r, norms, maps, steps, dtype)
+    def forward(ctx, r, steps, dtype, listed, *kept):
+        ctx.save_for_backward(*kept)
+        ctx.steps, ctx.listed, ctx.dtype = steps, listed, r.dtype
+        return _linear(r, *_maps(kept, listed), steps, dtype)
 
     @staticmethod
     def backward(ctx, c):
-        return _Apply.apply(c, *ctx.kept, ctx.dtype), None, None, None, None
+        kept = ctx.saved_tensors
+        return (_Apply.apply(c, ctx.steps, ctx.dtype, ctx.listed, *kept), None, None, None, *[None] * len(kept))
 
 
 class _NewtonSchulz(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, steps):
         y, norms, maps = _run(g, steps, True)
-        ctx.kept, ctx.dtype = (norms, maps, steps), g.dtype
+        ctx.steps, ctx.listed, ctx.dtype = steps, isinstance(maps, list), g.dtype
+        ctx.save_for_backward(norms, *(maps if ctx.listed else (maps,)))
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        return (_Apply.apply if torch.is_grad_enabled() else _linear)(gy, *ctx.kept, ctx.dtype), None
+        kept = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            return _Apply.apply(gy, ctx.steps, ctx.dtype, ctx.listed, *kept), None
+        return _linear(gy, *_maps(kept, ctx.listed), ctx.steps, ctx.dtype), None
 
 
 def _run(g: torch.Tensor, steps: int, keep: bool):

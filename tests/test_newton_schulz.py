@@ -121,3 +121,22 @@ def test_the_write_rule_against_differences_of_itself(dtype):
         got, = torch.autograd.grad(sum((a * b).sum() for a, b in zip(IN.direction(leaf, "muon5"), c)), leaf[j:j + 1])
         terms = sum((a * norm(g) / norm(y) * b).abs().sum() for a, b in zip(y, c)) + (got.double() * g[j].double()).abs().sum()
         assert abs((got.double() * g[j].double()).sum() - slope) <= 3 * 2.0 ** -8 * terms
+
+
+def test_what_the_derivative_keeps_are_saved_tensors():
+    """Hooks on saved tensors see the norms and every step's matrix, and a graph that has been walked holds neither."""
+    g = torch.randn(2, 4, 6, generator=torch.Generator().manual_seed(5)).requires_grad_(True)
+    gy = torch.ones(2, 4, 6, dtype=torch.bfloat16)
+    want, = torch.autograd.grad(newton_schulz(g, 3), g, gy)
+    packed = []
+
+    def pack(t):
+        packed.append(tuple(t.shape))
+        return t.clone()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = newton_schulz(g, 3)
+    assert packed == [(2, 1, 1)] + 3 * [(2, 4, 4)]
+    assert torch.autograd.grad(y, g, gy)[0].equal(want)
+    with pytest.raises(RuntimeError, match="second time|freed"):
+        torch.autograd.grad(y, g, gy)

@@ -326,3 +326,14 @@ def test_both_sides_of_the_one_launch_rule(shape, one):
     assert (kernels.LAUNCHES - n == 1) == one
     for dtype in (torch.float32, torch.bfloat16):
         test_direction_and_derivative(shape, dtype, 5)
+
+
+@pytest.mark.parametrize("shape", [(2, 64, 100), (2, 300, 200)])
+def test_kept_matrices_move_with_saved_tensor_hooks(shape):
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    g, gy = make(shape, torch.float32, 3)
+    leaf = g.requires_grad_(True)
+    want, = torch.autograd.grad(newton_schulz(leaf), leaf, gy)
+    with torch.autograd.graph.save_on_cpu():
+        y = newton_schulz(leaf)
+    assert torch.autograd.grad(y, leaf, gy)[0].equal(want)
