@@ -13,6 +13,7 @@ that needs it projects the component along ``g`` out of the backward's result (t
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import reference as ref
 
@@ -86,7 +87,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5) -> torch.Tensor:
     ``g``; where a matrix has no singular value a step multiplies what it holds there by 3.4445, in any arithmetic, so that the 2^-22
     left of ``x`` come to a tenth of the result after twelve steps (an f32 computation's 2^-24 after thirteen).  The derivative has the
     accuracy of bf16 whatever the type of ``g``.  The same matrix may come out with other last bits in a batch of another size.
-    At most 65535 matrices a call; the first call on a device cannot be captured into a graph."""
+    At most 65535 matrices a call; no forward-mode derivative; the first call on a device cannot be captured into a graph."""
     if g.dim() < 2 or g.shape[-1] == 0 or g.shape[-2] == 0:
         raise ValueError(f"newton_schulz: g {tuple(g.shape)}, [..., rows, cols] with non-empty matrices is wanted")
     if g.dtype not in (torch.float32, torch.bfloat16):
@@ -95,6 +96,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5) -> torch.Tensor:
         raise ValueError(f"newton_schulz: steps = {steps!r}, a number from 1 to 32 is wanted")
     if g.numel() // (g.shape[-1] * g.shape[-2]) > 65535:
         raise ValueError(f"newton_schulz: {g.numel() // (g.shape[-1] * g.shape[-2])} matrices, at most 65535 are taken in one call")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(g).tangent is not None:
+        raise NotImplementedError("newton_schulz: there is no forward-mode derivative (a dual tensor would lose its tangent)")
     if g.numel() == 0:
         return g.to(torch.bfloat16)
     if torch.is_grad_enabled() and g.requires_grad:

@@ -140,3 +140,14 @@ def test_what_the_derivative_keeps_are_saved_tensors():
     assert torch.autograd.grad(y, g, gy)[0].equal(want)
     with pytest.raises(RuntimeError, match="second time|freed"):
         torch.autograd.grad(y, g, gy)
+
+
+def test_a_dual_tensor_is_refused():
+    from torch.autograd import forward_ad
+    g = torch.randn(3, 4)
+    with forward_ad.dual_level():
+        assert newton_schulz(g, 2).shape == (3, 4)
+        for x in (g, g.clone().requires_grad_(True)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                newton_schulz(forward_ad.make_dual(x, torch.ones(3, 4)), 2)
+    assert newton_schulz(g, 2).shape == (3, 4)
