@@ -30,6 +30,7 @@ import torch
 from .ckpt import store as ckpt
 from .engine import Engine
 from .models.blocks import Net
+from .ops import _lib
 from .ops import attention as A
 from .ops import functional as Fn
 from .ops import sampling
@@ -392,6 +393,8 @@ def generate(net: Net, prompt: torch.Tensor, max_new_tokens: int, key: torch.Ten
                                         device=dev)[None]
         state = commit_block(net, ids, pos, state, k_inner, inner_lr, inner_clip, inner_mask_ratio, fused_ce_block, inner_views,
                              inner_mask_span, inner_update_rule, host_mask, inner_task, host_perm, 1.0 - inner_target_frac, wc)
+        if dev.type == "cuda":
+            _lib.check_status(dev)                                  # a kernel whose wait ran out left its result incomplete
         out.append(ids[0])
     return torch.cat(out)[:total]
 

@@ -80,3 +80,30 @@ def test_a_diverged_model_is_refused():
                        opts=G.DecodeOpts(top_p=0.9, presence_penalty=0.5))
     finally:
         E.embedding = plain
+
+
+def test_a_kernel_that_gave_up_is_reported(monkeypatch):
+    """A block whose kernels recorded an error (here: put into the status word by the test, before the block's write) does not become
+    context of the next one in silence."""
+    from dttt_b200 import generate as G
+    from dttt_b200.engine import Engine
+    from dttt_b200.ops import _lib
+    from dttt_b200.schema import ModelConfig
+    from dttt_b200.utils import rng
+    mc = ModelConfig(vocab_size=4096, hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2,
+                     head_dim=64, suffix_len=2, chunk_size=128, window_chunks=2, qk_norm=True, mask_token_id=4095, pad_token_id=4094,
+                     eos_token_id=4094)
+    eng = Engine(mc, tiny_train(compute_dtype="bfloat16", fused_ce_block=2048, seq_len=512), device=torch.device("cuda", 0))
+    net, blocks, plain = eng.net(train=False), [], G.commit_block
+
+    def commit(*a, **k):
+        blocks.append(1)
+        if len(blocks) == 2:
+            _lib.status_tensor(torch.device("cuda", 0))[0] = 3
+        return plain(*a, **k)
+
+    monkeypatch.setattr(G, "commit_block", commit)
+    with pytest.raises(_lib.KernelError, match="accumulator"):
+        G.generate(net, torch.arange(20), 400, rng.key(1), steps=2, outer_shift=True, inner_task="causal", inner_update_rule="muon5")
+    assert len(blocks) == 2
+    _lib.check_status()                                                     # the report has reset the word
