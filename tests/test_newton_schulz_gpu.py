@@ -337,3 +337,66 @@ def test_kept_matrices_move_with_saved_tensor_hooks(shape):
     with torch.autograd.graph.save_on_cpu():
         y = newton_schulz(leaf)
     assert torch.autograd.grad(y, leaf, gy)[0].equal(want)
+
+
+# ------------------------------------------------------------------------------------------------------------ the write
+def write_rule(g, steps=5):
+    """``ttt.inner.direction(g, "muon5")`` of 64-bit leaves, differentiable in all but the polynomials."""
+    y = []
+    for x in g:
+        with torch.no_grad():
+            _, _, polys = ref.newton_schulz(x, steps, torch.float64)
+        y.append(ref.newton_schulz_apply(x, torch.linalg.matrix_norm(x, keepdim=True), polys))
+    size = lambda ts: torch.sqrt(sum(t.pow(2).sum((-2, -1)) for t in ts) + 1e-8)[:, None, None]
+    return [t * size(g) / size(y) for t in y]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shapes,tokens", [(((64, 128), (64, 128), (128, 64)), 20), (((300, 700), (300, 700), (700, 300)), 90), (((128, 1000), (1000, 128)), 500)])
+def test_the_write_rule_and_its_derivative(shapes, tokens, dtype):
+    """Several matrices with one scale between them, against the rule in 64 bits with the derivative of every norm.  u is off as the
+    directions are; a gradient as the held map's result, of which the norm's share is taken away: the bound of each relative to
+    what is subtracted, and 2^-8 of the cotangent's rounding to bf16 besides."""
+    from dttt_b200.ttt import inner as IN
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    g = [(r(2, tokens, s[0]).mT @ r(2, tokens, s[1]) * 10.0 ** -i).to(dtype) for i, s in enumerate(shapes)]
+    c = [r(*x.shape) + x.float() / x.float().std() for x in g]              # some of it along the matrices
+    leaf, exact = [x.clone().requires_grad_(True) for x in g], [x.double().requires_grad_(True) for x in g]
+    u, want = IN.direction(leaf, "muon5"), write_rule(exact)
+    bound = math.hypot(BOUND, 2.0 ** -11 / 3 ** 0.5 * 3.4445 * 1.8)         # (the last step takes x in one half; values 0.68 to 1.21)
+    assert all(off(a, b) <= bound for a, b in zip(u, want))
+    got = torch.autograd.grad(sum((a * b).sum() for a, b in zip(u, c)), leaf)
+    grad = torch.autograd.grad(sum((a * b.double()).sum() for a, b in zip(want, c)), exact)
+    scale = [x.detach().norm(dim=(-2, -1), keepdim=True) for x in want]
+    for a, b, x, k, w, t in zip(got, grad, exact, c, want, scale):
+        with torch.no_grad():                                               # the held map's result, before the norms' share goes
+            y, n, polys = ref.newton_schulz(x.detach(), 5, torch.float64)
+            held = ref.newton_schulz_apply(k.double() * t / y.norm(dim=(-2, -1), keepdim=True), n, polys).norm()
+        assert a.dtype == dtype and (a.double() - b).norm() <= (bound + 2.0 ** -7) * (b.norm() + held)
+
+
+def test_training_gradients_with_the_kernel_and_without(monkeypatch):
+    """One step's outer gradients through the five-step write, with the direction and its derivative on the kernels and as statements.
+    Everything between is bf16: some thirty roundings of 2^-8 on the way, independent (2e-2 together, and as much between two runs, whose
+    sums differ in order); a factor of ten over that is still far below a term that is left out or counted twice."""
+    from dttt_b200.engine import Engine
+    from dttt_b200.ops import kernels
+    from dttt_b200.schema import ModelConfig, TrainConfig
+    from util import loss_and_grads, loss_config
+    mc = ModelConfig(vocab_size=4096, hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2,
+                     head_dim=64, suffix_len=2, chunk_size=128, window_chunks=2, qk_norm=True, mask_token_id=4095, pad_token_id=4094,
+                     eos_token_id=4094)
+    tc = TrainConfig(seq_len=512, batch_size=2, steps=10, warmup_steps=2, inner_lr_warmup_steps=0, inner_task="causal", outer_shift=True,
+                     cart_window=64, fused_ce_block=2048, inner_update="muon5")
+    eng = Engine(mc, tc, device=torch.device("cuda", 0))
+    ids = torch.randint(0, 4000, (2, 512), device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    n = kernels.LAUNCHES
+    loss, grads, _ = loss_and_grads(eng, ids, loss_config(tc))
+    assert kernels.LAUNCHES > n
+    monkeypatch.setattr(kernels, "_DISABLED", kernels._DISABLED | {"newton_schulz"})
+    loss2, plain, _ = loss_and_grads(eng, ids, loss_config(tc))
+    assert abs(loss - loss2) <= 2.0 ** -8 * abs(loss2)
+    for k in plain:
+        if plain[k].norm() > 0:
+            assert off(grads[k], plain[k]) <= 0.2, k
