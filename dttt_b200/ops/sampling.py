@@ -46,8 +46,9 @@ def _param(name: str, value: Param, rows, dtype: torch.dtype, device, lo: float,
         except RuntimeError:
             raise ValueError(f"sample_tokens: {name} {tuple(value.shape)} does not broadcast to the rows {tuple(rows)}") from None
     v = value.item() if isinstance(value, torch.Tensor) else value
-    if not ((lo < v if open_lo else lo <= v) and v <= hi):
-        raise ValueError(f"sample_tokens: {name} = {v!r} is outside {'(' if open_lo else '['}{lo}, {hi}]")
+    if not ((lo < v if open_lo else lo <= v) and v <= hi) or (dtype == torch.int32 and v != int(v)):
+        whole = " whole numbers of" if dtype == torch.int32 else ""
+        raise ValueError(f"sample_tokens: {name} = {v!r} is outside{whole} {'(' if open_lo else '['}{lo}, {hi}]")
     return int(v) if dtype == torch.int32 else float(v)
 
 

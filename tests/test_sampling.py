@@ -139,3 +139,10 @@ def test_unmask_refusals(at, bad):
         unmask(*args)
     with pytest.raises(ValueError, match="sure"):
         unmask(*commit_args(), sure=float("nan"))
+
+
+@pytest.mark.parametrize("k", [5.5, torch.tensor(2.25), float("inf"), float("nan")])
+def test_a_part_of_a_token_is_not_a_top_k(k):
+    with pytest.raises(ValueError, match="top_k"):
+        sample_tokens(torch.zeros(2, 9), torch.zeros(2), top_k=k)
+    assert sample_tokens(torch.zeros(2, 9), torch.zeros(2), top_k=5.0).tokens.tolist() == [0, 0]
