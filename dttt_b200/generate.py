@@ -13,7 +13,8 @@ Sampler options (``DecodeOpts``): confidence or random commit order, Gumbel samp
 (parallel decoding), presence penalty, a re-masking corrector loop, sub-block (semi-autoregressive) filling,
 and the priority measure (log-probability, top-2 margin or negative entropy) - reference ``generate.py:196-355``.
 ``sampler = "inverse"``, and any of ``top_k`` / ``top_p`` / ``min_p``, draws by the inverse distribution function from one
-uniform number per slot (``ops.sampling.sample_tokens``: one or two kernel launches instead of a Gumbel number per token).
+uniform number per slot (``ops.sampling.sample_tokens``: one or two kernel launches a call instead of a Gumbel number per token; a
+round is one call, or under the outer shift two, slot 0 by itself).
 With the outer shift slot ``i`` predicts token ``i+1`` and the first token of a block comes from the previous
 block's tail logit.
 """

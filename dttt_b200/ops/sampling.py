@@ -3,8 +3,8 @@
 ``sample_tokens`` draws one token per row of logits from given uniform numbers (temperature, top-k, top-p, min-p) and returns
 with it what a denoising round ranks its slots by; ``unmask`` commits the best-ranked open slots of every sequence
 (reference ``src/ttt/generate.py:227-355``: the proposals and the commit of one round; the reference draws by Gumbel noise and
-has no truncation).  On a CUDA device both are one launch of ``csrc/sampling.cu``; elsewhere the statements of
-``ops.reference`` run.  Neither is differentiable.
+has no truncation).  On a CUDA device both are kernels of ``csrc/sampling.cu``, one launch a call, or two and a scratch area for
+untruncated draws from 6.2 million elements on; elsewhere the statements of ``ops.reference`` run.  Neither is differentiable.
 """
 from __future__ import annotations
 
@@ -22,7 +22,7 @@ Param = Union[float, int, torch.Tensor]
 class Drawn(NamedTuple):
     tokens: torch.Tensor          # int64 [...]
     logp: torch.Tensor            # f32: log-probability of the token under the untempered, untruncated distribution
-    priority: torch.Tensor        # f32: larger means surer
+    priority: torch.Tensor        # f32: larger means surer (ranked by logp, it may be the same tensor)
 
 
 class Committed(NamedTuple):
