@@ -314,8 +314,8 @@ def orthogonalise(g: torch.Tensor, iters: int = 2) -> torch.Tensor:
 
 
 class _ScaleFree(torch.autograd.Function):
-    """The matrices ``x [..., m, n]`` as they are, for a use that depends on each of them up to its scale only: the cotangent loses its
-    component along the matrix, which is what the derivative of the norm subtracts in ``f(x / |x|)``."""
+    """The f32 matrices ``x [..., m, n]`` as they are, for a use that depends on each of them up to its scale only: the cotangent loses
+    its component along the matrix, which is what the derivative of the norm subtracts in ``f(x / |x|)``."""
 
     @staticmethod
     def forward(ctx, x):
@@ -325,10 +325,9 @@ class _ScaleFree(torch.autograd.Function):
     @staticmethod
     def backward(ctx, c):
         x, = ctx.saved_tensors
-        size = x.detach().abs().amax((-2, -1), keepdim=True).float()
-        xs = x.float() / torch.where(size > 0, size, 1.0)           # squares of any finite matrix stay in range
-        along = (xs * c.float()).sum((-2, -1), keepdim=True) / xs.pow(2).sum((-2, -1), keepdim=True).clamp_min(1e-30)
-        return (c.float() - xs * along).to(c.dtype)
+        size = x.detach().abs().amax((-2, -1), keepdim=True)
+        xs = x / torch.where(size > 0, size, 1.0)                   # squares of any finite matrix stay in range
+        return c - xs * ((xs * c).sum((-2, -1), keepdim=True) / xs.pow(2).sum((-2, -1), keepdim=True).clamp_min(1e-30))
 
 
 def direction(g: List[torch.Tensor], rule: str) -> List[torch.Tensor]:
@@ -339,8 +338,14 @@ def direction(g: List[torch.Tensor], rule: str) -> List[torch.Tensor]:
     elif rule == "muon2":
         u = [orthogonalise(x, 2) for x in g]
     elif rule == "muon5":
-        # every matrix is normalised by itself and the scale below is one for all of a sequence: the norms have a derivative
-        u = [newton_schulz(_ScaleFree.apply(x), 5) for x in g]
+        # Every matrix is normalised by itself and the scale below is one for all of a sequence, so the norms have a derivative.  It is
+        # taken, and summed with that of the scale, in f32: what it takes off an entry is less than half a step of a bf16 gradient,
+        # which is large where the matrix has no singular value, and a rounding in between would put it back.
+        if torch.is_grad_enabled() and any(x.requires_grad for x in g):
+            g = [x.float() for x in g]
+            u = [newton_schulz(_ScaleFree.apply(x), 5) for x in g]
+        else:
+            u = [newton_schulz(x, 5) for x in g]
     else:
         raise ValueError(f"inner_update {rule!r}")
     ratio = seq_norm(g) / seq_norm(u)

@@ -151,3 +151,21 @@ def test_a_dual_tensor_is_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 newton_schulz(forward_ad.make_dual(x, torch.ones(3, 4)), 2)
     assert newton_schulz(g, 2).shape == (3, 4)
+
+
+def test_the_write_rule_rounds_behind_the_projection():
+    """bf16 gradients of low rank: the held map's result is large where the matrix has no singular value, and what the norm's
+    derivative takes off each entry is less than half a step of that.  Rounded once, behind it, the roundings (2^-8, evenly spread)
+    are independent of the matrix: a factor of four over their mean square; rounded before as well they put all of it back."""
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen)
+    dots = lambda a, b: (a.double() * b.double()).sum((-2, -1))
+    g = [(r(2, 20, m).mT @ r(2, 20, n) * s).to(torch.bfloat16) for m, n, s in ((64, 128, 1.0), (64, 128, 0.1), (128, 64, 0.01))]
+    c = [r(*x.shape) + x.float() / x.float().std() for x in g]
+    leaf = [x.clone().requires_grad_(True) for x in g]
+    u = IN.direction(leaf, "muon5")
+    got = torch.autograd.grad(sum((a * b).sum() for a, b in zip(u, c)), leaf)
+    for a, x in zip(got, g):
+        common = sum(dots(v, w.detach()) for v, w in zip(c, u)) * dots(x, x) / sum(dots(z, z) for z in g)
+        lost = 2.0 ** -8 * 4 / 3 ** 0.5 * dots(a.double() ** 2, x.double() ** 2).sqrt()
+        assert a.dtype == torch.bfloat16 and ((dots(a, x) - common).abs() <= 2.0 ** -8 * common.abs() + lost).all()

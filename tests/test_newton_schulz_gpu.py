@@ -369,11 +369,17 @@ def test_the_write_rule_and_its_derivative(shapes, tokens, dtype):
     got = torch.autograd.grad(sum((a * b).sum() for a, b in zip(u, c)), leaf)
     grad = torch.autograd.grad(sum((a * b.double()).sum() for a, b in zip(want, c)), exact)
     scale = [x.detach().norm(dim=(-2, -1), keepdim=True) for x in want]
-    for a, b, x, k, w, t in zip(got, grad, exact, c, want, scale):
+    for a, b, x, k, t in zip(got, grad, exact, c, scale):
         with torch.no_grad():                                               # the held map's result, before the norms' share goes
             y, n, polys = ref.newton_schulz(x.detach(), 5, torch.float64)
             held = ref.newton_schulz_apply(k.double() * t / y.norm(dim=(-2, -1), keepdim=True), n, polys).norm()
         assert a.dtype == dtype and (a.double() - b).norm() <= (bound + 2.0 ** -7) * (b.norm() + held)
+        # along the matrix by itself: what is left there is the common scale's, (c u) |g_j|^2 / |g|^2, and the gradient's own roundings
+        # (half a step each, evenly spread; f32: of some products on the way; a factor of four over the mean square)
+        dots = lambda p, q: (p.double() * q.double()).sum((-2, -1))
+        common = sum(dots(v, w) for v, w in zip(c, want)) * dots(x, x) / sum(dots(z, z) for z in exact)
+        lost = (2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -22) * 4 / 3 ** 0.5 * dots(a.double() ** 2, x * x).sqrt()
+        assert torch.allclose(dots(b, x), common, rtol=1e-6) and ((dots(a, x) - common).abs() <= 2 * bound * common.abs() + lost).all()
 
 
 def test_training_gradients_with_the_kernel_and_without(monkeypatch):
