@@ -26,10 +26,11 @@
 //
 // Every product is C = alpha A B + beta D (+ s I) on CTA pairs: tiles of 256 rows and 256 or 128 columns, tcgen05.mma.cta_group::2,
 // plain per-CTA TMA loads, symmetric results formed for the tiles on and below the diagonal and stored twice.  What bounds it:
-//   * large matrices: the tensor cores.  4 x 2048 x 8192 f32, five steps: 1.83 ms for 2.23 TFLOP (symmetric halves counted once) =
-//     1220 TFLOP/s, tensor pipe 91 % busy in a product with x; 8192 x 2048 with its derivative 0.84 ms = 1075 TFLOP/s.
+//   * large matrices: the tensor cores.  4 x 2048 x 8192 f32, five steps: 1.84 ms for 2.23 TFLOP (symmetric halves counted once) =
+//     1210 TFLOP/s; tensor pipe 92 % busy in a product with x alone, 86 % and 78 % where the lower half is read, and read and written;
+//     8192 x 2048 with its derivative 0.84 ms = 1075 TFLOP/s.
 //   * middle ones: the chain of products, each of which is one round of tiles whose first loads, store and mirrored store are
-//     not hidden: 3 x 509 x 1283, five steps 167 us and its derivative 53 us, 8 to 11 us a product; programmatic launches start a
+//     not hidden: 3 x 509 x 1283, five steps 177 us and its derivative 53 us, 8 to 11 us a product; programmatic launches start a
 //     product's prologue under the one before (263 -> 230 us).  All of them in one cooperative launch gained nothing.
 //   * d <= 128 and L <= 4096, most of them (`is_small`): one CTA or cluster and one launch, 23 us for 2 x 128 x 256 and two steps.
 #include "host_check.h"
@@ -360,7 +361,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
         }
         __syncwarp();
         // 32 columns at a time: 64 of them spill beside the rows that are on their way, and next to this much shared memory there is no L1
-        // for that (4 x 2048 x 8192 1826 instead of 1578 us); in narrow tiles they fit and are no gain (2 x 300 x 700 145 instead of 130 us).
+        // for that (4 x 2048 x 8192 1826 instead of 1578 us, both at the burst clock); in narrow tiles they fit and are no gain (2 x 300 x 700 145 instead of 130 us).
         // A lane's row of the staging areas is its own until the flush: results take the place of the summands that they were made of.
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {

@@ -27,11 +27,11 @@
 //
 // What bounds it, at V = 128256 (f32, 525 MB for 1024 rows, 81 us at the copy rate):
 //   one row, top-p: 16 us.  Latency: load 1.5 us, three exchanges over the cluster, ranking the list 3.4 us.
-//   1024 rows, top-p 0.9: 440 us = 1.2 TB/s.  A CTA takes 17 us, of which loading 4.5, its pass 4, looking for candidates 1.4 and the
+//   1024 rows, top-p 0.9: 465 us = 1.1 TB/s.  A CTA takes 17 us, of which loading 4.5, its pass 4, looking for candidates 1.4 and the
 //     exchanges 6.5; three to an SM hide each other's waits only in part (issue slots 42 % busy).
 //   1024 rows, untruncated: 203 + 12 us = 2.5 TB/s, bound by issue: 38 instructions an element, of which the 64-bit exponential
 //     (FP64 pipe 36 % busy, issue slots 68 %) is most.
-//   252 rows bf16 with bias, top-k 50 and min-p: 114 us for 67 MB: 4.5 rounds of CTAs as above.
+//   252 rows bf16 with bias, top-k 50 and min-p: 115 us for 67 MB: 4.5 rounds of CTAs as above, whose slices are f32.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
