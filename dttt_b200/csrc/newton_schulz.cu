@@ -361,8 +361,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constan
         }
         __syncwarp();
         // 32 columns at a time: 64 of them spill beside the rows that are on their way, and next to this much shared memory there is no L1
-        // for that (4 x 2048 x 8192 1826 instead of 1578 us, both at the burst clock); in narrow tiles they fit and are no gain (2 x 300 x 700 145 instead of 130 us).
-        // A lane's row of the staging areas is its own until the flush: results take the place of the summands that they were made of.
+        // for that (4 x 2048 x 8192 1826 instead of 1578 us, both at the burst clock); in narrow tiles they fit and are no gain (2 x 300 x
+        // 700 145 instead of 130 us).  A lane's row of the staging areas is its own until the flush: results take the place of the summands
+        // that they were made of.
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           uint32_t r[32];
@@ -531,8 +532,9 @@ __global__ void __launch_bounds__(CAST_THREADS) ns_cast_kernel(const T* __restri
 }
 
 // ------------------------------------------------------------------ few rows or columns: everything on chip
-// d <= 128 and L <= 4096 (not all of them: `is_small`): one CTA, or a cluster of up to eight with 512 columns each, holds x [128, L] (transposed when rows > cols), G
-// and P in shared memory and runs all iterations in one launch; what such sizes cost otherwise is launches.  x lies as blocks of 128
+// d <= 128 and L <= 4096 (not all of them: `is_small`): one CTA, or a cluster of up to eight with 512 columns each, holds x [128, L]
+// (transposed when rows > cols), G and P in shared memory and runs all iterations in one launch; what such sizes cost otherwise is
+// launches.  The lower half of x goes through L2: on chip, up to 256 columns a CTA, it was no faster.  x lies as blocks of 128
 // rows x 64 columns with 128-byte swizzle, which is the K-major operand of G = x x^T and, read with its columns as N, the MN-major
 // one of P x.  Rows and columns beyond the matrix are zero and stay so.  In a cluster each CTA adds up a share of the partial G of
 // all, rounds it and hands it round; P is then formed by everyone.  Also the derivative (`apply`): the kept P of every iteration is
@@ -1251,8 +1253,8 @@ extern "C" int dttt_newton_schulz(const void* g, int f32, int batch, int rows, i
   const int groups = make_plan(rows, cols, steps, plan);
   if (is_small(batch, rows, cols)) {
     const int small = rows < cols ? rows : cols, ld = (small + 7) / 8 * 8;
-    SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, 1, 0, X_SCALE, steps > 1 ? (__half*)scratch : nullptr, (__half*)kept, (long long)batch * small * ld,
-                     norms, y, status};
+    SmallParams p = {g, rows, cols, steps, 0, keep, OUT_BF16, ld, 1, 0, X_SCALE, steps > 1 ? (__half*)scratch : nullptr, (__half*)kept,
+                     (long long)batch * small * ld, norms, y, status};
     for (int k = 0; k < steps; ++k) p.alpha[k] = plan[k].alpha;
     return launch_small(p, f32, batch, stream);
   }

@@ -224,7 +224,7 @@ class BlockUnmasker:
         logits = block_forward(self.net, x, self.pos, self.state, pos_q=self.pos_q, own_kv=own_kv)[0]
         logits[..., self.mask_id] = float("-inf")
         if o.inverse:
-            return self.draw(logits, x, key)
+            return self.draw(logits, x, key, visible)
         if self.outer_shift:                                        # slot i is predicted at slot i - 1; slot 0 by the previous block's tail
             lead = self.prev_tail.clone() if self.prev_tail is not None else torch.zeros(self.B, self.V, device=self.dev)
             lead[..., self.mask_id] = float("-inf")
@@ -241,10 +241,10 @@ class BlockUnmasker:
         chosen = logp.gather(-1, tokens[..., None])[..., 0]
         return tokens, chosen, _PRIORITY[o.priority](logp, chosen)
 
-    def draw(self, logits: torch.Tensor, x: torch.Tensor, key: torch.Tensor):
+    def draw(self, logits: torch.Tensor, x: torch.Tensor, key: torch.Tensor, visible: torch.Tensor):
         """Proposals from one uniform number per slot; under the outer shift slot 0 is drawn from the previous block's tail and
-        the others in place, from the rows before them.  A row without a distribution has no token: the block is refused when it
-        is complete (``check``), and until then token 0 stands in, because what is proposed is committed, embedded and scattered by."""
+        the others in place, from the rows before them.  A row without a distribution has no token: if its slot is open the block is
+        refused (``check``), and until then token 0 stands in, because what is proposed is committed, embedded and scattered by."""
         o = self.opts
         u = rng.uniform(key.to("cpu"), (self.B, self.C)).to(self.dev)
         bias = None
@@ -260,7 +260,7 @@ class BlockUnmasker:
             lead[..., self.mask_id] = float("-inf")
             parts = zip(sampling.sample_tokens(lead[:, None], u[:, :1], **kw), sampling.sample_tokens(logits[:, :-1], u[:, 1:], **kw))
             tokens, logp, priority = (torch.cat(p, 1) for p in parts)
-        self.void |= (tokens < 0).any()
+        self.void |= ((tokens < 0) & ~visible).any()
         return tokens.clamp_(min=0), logp, priority
 
     def check(self) -> None:
@@ -295,6 +295,7 @@ class BlockUnmasker:
         while (~self.known).any() and rounds < self.C:
             key = self.keys.take()
             tokens, logp, priority = self.propose(self.known, key)
+            self.check()
             self.commit(tokens, logp, self.order(priority, key), one, sure=float(np.log(threshold)))
             rounds += 1
 

@@ -69,3 +69,32 @@ def test_logits_without_a_distribution_are_an_error_and_never_an_index(opts, kw,
     with pytest.raises(FloatingPointError, match="distribution"):
         run(net, opts, temperature=1.0, **kw)
     assert seen and all(((ids >= 0) & (ids < 128)).all() for ids in seen)
+
+
+def test_only_rows_that_are_drawn_need_a_distribution(monkeypatch):
+    """A slot whose token is known is not drawn: what its logits hold does not matter.  A slot that is open does, and rounds that end by
+    confidence end with the first of it."""
+    net = make_engine().net(train=False)
+    plain, rounds = G.block_forward, []
+
+    def broken(where):
+        def forward(net, ids, pos, state, *a, **k):
+            rounds.append(1)
+            out = plain(net, ids, pos, state, *a, **k)
+            for slot in where:
+                out[0][:, slot] = float("nan")
+            return out
+        return forward
+
+    decode = lambda opts: G.decode_block(net, ids, known, pos, G.init_state(net), rng.key(3), 3, 1.0, opts=opts)
+    ids = torch.tensor([[5, 6, 7, 127, 127, 127, 127, 127]])
+    known, pos = ids != 127, torch.arange(8)[None]
+    monkeypatch.setattr(G, "block_forward", broken([0, 2]))
+    out, _ = decode(G.DecodeOpts(top_p=0.9))
+    assert torch.equal(out[:, :3], ids[:, :3]) and ((out >= 0) & (out < 127)).all()
+    monkeypatch.setattr(G, "block_forward", broken([4]))
+    for opts in (G.DecodeOpts(top_p=0.9), G.DecodeOpts(top_p=0.9, threshold=0.999)):
+        rounds.clear()
+        with pytest.raises(FloatingPointError):
+            decode(opts)
+    assert len(rounds) == 1
