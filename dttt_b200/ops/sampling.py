@@ -67,7 +67,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Param =
     not read by the host and are taken as ``temperature <= 0``: greedy, else clamped to [1e-6, 1e6]; ``top_k <= 0`` or ``>= V``:
     off; ``top_p >= 1``: off, ``<= 0``: the best token alone; ``min_p <= 0``: off, above 1: as 1; NaN: as off (``temperature``:
     greedy).  ``u`` outside [0, 1) is clamped, NaN taken as 0.  A row without a distribution (NaN or +inf in it, or every token
-    at -inf) gives token -1 and NaN: no index, so look for it before the tokens are embedded or scattered by.  On a CUDA device ``V`` goes up to 393216."""
+    at -inf) gives token -1 and NaN: no index, so look for it before the tokens are embedded or scattered by.  On a CUDA device
+    ``V`` goes up to 393216."""
     rows, dev = logits.shape[:-1], logits.device
     if not rows or logits.shape[-1] == 0:
         raise ValueError(f"sample_tokens: logits {tuple(logits.shape)}, at least [rows, V] are wanted")
@@ -111,7 +112,8 @@ def unmask(ids: torch.Tensor, known: torch.Tensor, held: torch.Tensor, tokens: t
     (not ``known``, and ``allowed`` where given), and with ``sure`` also every slot that is not known and whose ``logp`` reaches
     it.  ``ids``, ``known`` and ``held`` (the log-probability a slot was committed with) come back with ``tokens`` / True /
     ``logp`` at the committed slots.  Slots of equal priority rank by position, NaN ranks last; a slot that is not open ranks as
-    one of priority ``-inf``.  Tokens are copied as they are (a -1 of ``sample_tokens`` too).  One launch for ``C`` up to 32768 on a CUDA device, the statement of ``ops.reference`` beyond."""
+    one of priority ``-inf``.  Tokens are copied as they are (a -1 of ``sample_tokens`` too).  One launch for
+    ``C`` up to 32768 on a CUDA device, the statement of ``ops.reference`` beyond."""
     shape, dev = ids.shape, ids.device
     if len(shape) != 2:
         raise ValueError(f"unmask: ids {tuple(shape)}, [B, C] is wanted")
