@@ -406,3 +406,44 @@ def test_training_gradients_with_the_kernel_and_without(monkeypatch):
     for k in plain:
         if plain[k].norm() > 0:
             assert off(grads[k], plain[k]) <= 0.2, k
+
+
+@pytest.mark.parametrize("shapes", [((2, 300, 700), (2, 300, 700)), ((128, 2000), (3, 128, 512)), ((1, 512, 1100), (40, 100, 701))])
+def test_two_calls_at_once_and_two_graphs_at_once(shapes):
+    """Every call and every graph has its own workspaces: side by side on two streams, on inputs that change between replays."""
+    from dttt_b200.ops.newton_schulz import newton_schulz
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    data = [make(s, torch.float32, n) for n, s in enumerate(shapes)]
+
+    def both(g, gy):
+        leaf = g.detach().requires_grad_(True)
+        y = newton_schulz(leaf, 8)
+        return y.detach(), torch.autograd.grad(y, leaf, gy)[0]
+
+    want = [both(*d) for d in data]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for n in range(2):
+            with torch.cuda.stream(sides[n]):
+                got[n].append(both(*data[n]))
+    torch.cuda.synchronize()
+    for n in range(2):
+        assert all(a.equal(b) for out in got[n] for a, b in zip(out, want[n]))
+    held = []
+    for g, gy in data:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both(g, gy)
+        held.append((graph, out))
+    for turn in range(3):
+        for n, (g, gy) in enumerate(data):
+            g2, gy2 = make(shapes[n], torch.float32, 10 + 2 * turn + n)
+            g.copy_(g2); gy.copy_(gy2)
+        torch.cuda.synchronize()
+        for side, (graph, _) in zip(sides, held):
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (g, gy), (_, out) in zip(data, held):
+            assert all(a.equal(b) for a, b in zip(out, both(g, gy)))
